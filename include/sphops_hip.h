@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define SPHOPS_ABI_VERSION 24
+#define SPHOPS_ABI_VERSION 25
 
 #define SPHOPS_CLAMPED 0
 #define SPHOPS_PERIODIC 1
@@ -543,6 +543,63 @@ int sphops_mlp_weight_grad(const float* z, const float* a, const float* dy, cons
                            float* dw2, float* db2, int64_t rows, int in_features, int hidden, int out_features,
                            void* workspace, void* stream);
 
+/*
+ * Rows in 8 bits (no reference counterpart).  A row x of cols values, with
+ * m = max(max |x|, 2^-100), has the scale m / 127 and the codes
+ * rint(x * (127 / m)) (float32 steps, ties to even); a value is code * scale.
+ * A row that holds a NaN or an infinity has a NaN scale and zero codes.  Codes
+ * are int8, a row every ld >= cols bytes; ld is a multiple of 4, and what lies
+ * between cols and ld is written as zeros.
+ */
+#define SPHOPS_F32 0
+#define SPHOPS_BF16 1
+#define SPHOPS_F16 2
+
+/* x: rows of `type`, row_stride elements apart (each row contiguous).  relu:
+ * the rows kept are relu(x), and no positive value has the code 0, so that a
+ * code is positive exactly where x is (in rows that are finite). */
+int sphops_quantize_rows(const void* x, int type, int64_t row_stride, int8_t* codes, int64_t ld, float* scale,
+                         int64_t rows, int64_t cols, int relu, void* stream);
+/* out (rows x cols, dense, of `type`) = code * scale, rounded once. */
+int sphops_restore_rows(const int8_t* codes, int64_t ld, const float* scale, void* out, int type, int64_t rows,
+                        int64_t cols, void* stream);
+
+/* sphops_linear_weight_grad with x given as rows in 8 bits: dw = dy^T x and,
+ * unless NULL, db = the column sums of dy; in a fixed order of summation.
+ * workspace: sphops_rows8_weight_grad_workspace_bytes bytes (-1: shape not
+ * supported), 16-byte aligned. */
+int sphops_rows8_weight_grad(const int8_t* codes, int64_t ld, const float* scale, const float* dy, float* dw,
+                             float* db, int64_t rows, int in_features, int out_features, void* workspace,
+                             void* stream);
+int64_t sphops_rows8_weight_grad_workspace_bytes(int64_t rows, int in_features, int out_features);
+
+/* A linear layer in 8-bit integers: x (rows x in_features of `type`, rows
+ * row_stride elements apart) is put into 8 bits, y = (sums of code products in
+ * int32) * (row scale * channel scale) + b, rounded to `type`.  w_codes:
+ * out_features rows of w_ld codes, w_ld a multiple of 16, 16-byte aligned, with zeros from
+ * in_features on; b (out_features) may be NULL.  Inference only.  workspace:
+ * sphops_linear8_workspace_bytes bytes (-1: shape not supported), 16-byte aligned. */
+int sphops_linear8(const void* x, int type, int64_t row_stride, const int8_t* w_codes, int64_t w_ld,
+                   const float* w_scale, const float* b, void* y, int64_t rows, int in_features, int out_features,
+                   void* workspace, void* stream);
+int64_t sphops_linear8_workspace_bytes(int64_t rows, int in_features, int out_features);
+
+/* sphops_mlp_forward in 8-bit integers: z and then the hidden row relu(...)
+ * put into 8 bits, both layers as in sphops_linear8 (weights as there; b1 and
+ * b2 may be NULL).  Inference only. */
+int sphops_mlp8_forward(const float* z, const int8_t* w1_codes, int64_t w1_ld, const float* w1_scale, const float* b1,
+                        const int8_t* w2_codes, int64_t w2_ld, const float* w2_scale, const float* b2, float* y,
+                        int64_t rows, int in_features, int hidden, int out_features, void* stream);
+
+/* The gradients of sphops_mlp_forward at an input kept in 8 bits: the hidden
+ * values are computed again from the codes, so nothing else is kept.  dz, dw1,
+ * db1, dw2 and db2 may each be NULL.  workspace:
+ * sphops_mlp_rows8_workspace_bytes bytes (-1: shape not supported), 16-byte aligned. */
+int sphops_mlp_rows8_backward(const int8_t* codes, int64_t ld, const float* scale, const float* dy, const float* w1,
+                              const float* b1, const float* w2, float* dz, float* dw1, float* db1, float* dw2,
+                              float* db2, int64_t rows, int in_features, int hidden, int out_features,
+                              void* workspace, void* stream);
+int64_t sphops_mlp_rows8_workspace_bytes(int64_t rows, int in_features, int hidden, int out_features);
 
 /* sphops_neighbor_candidates, _fill and _schedule in one call and two
  * launches fewer (no reference counterpart): counts (8-byte aligned) receives

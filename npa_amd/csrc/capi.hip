@@ -1228,6 +1228,133 @@ int sphops_mlp_weight_grad(const float* z, const float* a, const float* dy, cons
 
 }  // extern "C"
 
+// ------------------------------------------------------- rows in 8 bits
+
+namespace {
+
+void require_rows8(int64_t rows, int64_t cols, int64_t ld) {
+  require(rows >= 0 && rows <= sphops::kMaxRows8Rows, "rows must be in [0, 2^30]");
+  require(cols >= 1 && cols <= sphops::kMaxRows8Cols, "a row must have 1 to 65536 values");
+  require(ld >= cols && ld % 4 == 0 && ld <= 2 * sphops::kMaxRows8Cols,
+          "ld must be a multiple of 4, at least the row's length and at most 131072");
+}
+void require_type(int type) {
+  require(type == SPHOPS_F32 || type == SPHOPS_BF16 || type == SPHOPS_F16, "unknown element type");
+}
+void require_weight8(const int8_t* codes, int64_t ld, int in_features) {
+  require(ld >= in_features && ld % 16 == 0 && ld <= 2 * sphops::kMaxRows8Cols,
+          "the weights' ld must be a multiple of 16 and at least in_features");
+  require(reinterpret_cast<uintptr_t>(codes) % 16 == 0, "the weights' codes must be 16-byte aligned");
+}
+bool linear8_fits(int64_t rows, int in_features, int out_features) {
+  return rows >= 0 && rows <= sphops::kMaxRows8Rows && in_features >= 1 && in_features <= sphops::kMaxRows8Cols &&
+         out_features >= 1 && out_features <= sphops::kMaxRows8Cols;
+}
+bool rows8_weight_grad_fits(int64_t rows, int in_features, int out_features) {
+  return rows >= 0 && rows <= sphops::kMaxLinearRows && in_features >= 1 && out_features >= 1 &&
+         in_features <= sphops::kMaxLinearFeatures && out_features <= sphops::kMaxLinearFeatures &&
+         sphops::linear_grad_fits(rows, in_features, out_features);
+}
+
+}  // namespace
+
+extern "C" {
+
+int sphops_quantize_rows(const void* x, int type, int64_t row_stride, int8_t* codes, int64_t ld, float* scale,
+                         int64_t rows, int64_t cols, int relu, void* stream) {
+  return guarded([&] {
+    require_type(type);
+    require_rows8(rows, cols, ld);
+    require(rows <= 1 || row_stride >= 0, "row_stride must be >= 0");
+    require(rows == 0 || (x && codes && scale), "null buffer");
+    require(reinterpret_cast<uintptr_t>(codes) % 4 == 0, "codes must be 4-byte aligned");
+    sphops::run_quantize_rows(x, type, row_stride, codes, ld, scale, rows, cols, relu != 0,
+                              sphops::as_stream(stream));
+  });
+}
+
+int sphops_restore_rows(const int8_t* codes, int64_t ld, const float* scale, void* out, int type, int64_t rows,
+                        int64_t cols, void* stream) {
+  return guarded([&] {
+    require_type(type);
+    require_rows8(rows, cols, ld);
+    require(rows == 0 || (codes && scale && out), "null buffer");
+    require(reinterpret_cast<uintptr_t>(codes) % 4 == 0, "codes must be 4-byte aligned");
+    sphops::run_restore_rows(codes, ld, scale, out, type, rows, cols, sphops::as_stream(stream));
+  });
+}
+
+int64_t sphops_rows8_weight_grad_workspace_bytes(int64_t rows, int in_features, int out_features) {
+  if (!rows8_weight_grad_fits(rows, in_features, out_features)) return -1;
+  return sphops::rows8_weight_grad_floats(rows, in_features, out_features) * (int64_t)sizeof(float);
+}
+
+int sphops_rows8_weight_grad(const int8_t* codes, int64_t ld, const float* scale, const float* dy, float* dw,
+                             float* db, int64_t rows, int in_features, int out_features, void* workspace,
+                             void* stream) {
+  return guarded([&] {
+    require(rows8_weight_grad_fits(rows, in_features, out_features), "layer not supported");
+    require_rows8(rows, in_features, ld);
+    require(dw != nullptr && (rows == 0 || (codes && scale && dy && workspace)), "null buffer");
+    require(reinterpret_cast<uintptr_t>(codes) % 4 == 0, "codes must be 4-byte aligned");
+    sphops::run_rows8_weight_grad(codes, ld, scale, dy, dw, db, rows, in_features, out_features,
+                                  static_cast<float*>(workspace), sphops::as_stream(stream));
+  });
+}
+
+int64_t sphops_linear8_workspace_bytes(int64_t rows, int in_features, int out_features) {
+  if (!linear8_fits(rows, in_features, out_features)) return -1;
+  return sphops::linear8_workspace_bytes(rows, in_features, out_features);
+}
+
+int sphops_linear8(const void* x, int type, int64_t row_stride, const int8_t* w_codes, int64_t w_ld,
+                   const float* w_scale, const float* b, void* y, int64_t rows, int in_features, int out_features,
+                   void* workspace, void* stream) {
+  return guarded([&] {
+    require_type(type);
+    require(linear8_fits(rows, in_features, out_features), "layer not supported");
+    require_weight8(w_codes, w_ld, in_features);
+    require(rows <= 1 || row_stride >= 0, "row_stride must be >= 0");
+    require(rows == 0 || (x && w_codes && w_scale && y && workspace), "null buffer");
+    sphops::run_linear8(x, type, row_stride, w_codes, w_ld, w_scale, b, y, rows, in_features, out_features, workspace,
+                        sphops::as_stream(stream));
+  });
+}
+
+int sphops_mlp8_forward(const float* z, const int8_t* w1_codes, int64_t w1_ld, const float* w1_scale, const float* b1,
+                        const int8_t* w2_codes, int64_t w2_ld, const float* w2_scale, const float* b2, float* y,
+                        int64_t rows, int in_features, int hidden, int out_features, void* stream) {
+  return guarded([&] {
+    require(sphops::mlp_fits(rows, in_features, hidden, out_features), "MLP shape not supported");
+    require_weight8(w1_codes, w1_ld, in_features);
+    require_weight8(w2_codes, w2_ld, hidden);
+    require(rows == 0 || (z && w1_codes && w1_scale && w2_codes && w2_scale && y), "null buffer");
+    sphops::run_mlp8(z, w1_codes, w1_ld, w1_scale, b1, w2_codes, w2_ld, w2_scale, b2, y, rows, in_features,
+                     out_features, sphops::as_stream(stream));
+  });
+}
+
+int64_t sphops_mlp_rows8_workspace_bytes(int64_t rows, int in_features, int hidden, int out_features) {
+  if (!sphops::mlp_fits(rows, in_features, hidden, out_features)) return -1;
+  return sphops::mlp_rows8_floats(rows, in_features, out_features) * (int64_t)sizeof(float);
+}
+
+int sphops_mlp_rows8_backward(const int8_t* codes, int64_t ld, const float* scale, const float* dy, const float* w1,
+                              const float* b1, const float* w2, float* dz, float* dw1, float* db1, float* dw2,
+                              float* db2, int64_t rows, int in_features, int hidden, int out_features,
+                              void* workspace, void* stream) {
+  return guarded([&] {
+    require(sphops::mlp_fits(rows, in_features, hidden, out_features), "MLP shape not supported");
+    require_rows8(rows, in_features, ld);
+    require(rows == 0 || (codes && scale && dy && w1 && w2 && workspace), "null buffer");
+    require(reinterpret_cast<uintptr_t>(codes) % 4 == 0, "codes must be 4-byte aligned");
+    sphops::run_mlp_rows8_backward(codes, ld, scale, dy, w1, b1, w2, dz, dw1, db1, dw2, db2, rows, in_features,
+                                   out_features, static_cast<float*>(workspace), sphops::as_stream(stream));
+  });
+}
+
+}  // extern "C"
+
 // ------------------------------------------------ binning without allocation
 //
 // sphops_initialize_noalloc runs sphops_initialize's kernels with their

@@ -1,0 +1,83 @@
+// Rows in 8 bits: one float32 scale and one int8 code a value (see rows8.hip).
+#pragma once
+
+#include "sphops_internal.hpp"
+#include "sphops_device.hpp"
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+namespace sphops {
+
+// Rows whose largest value is smaller are held against this one: 127 / m and
+// m / 127 stay normal numbers, and a row of zeros needs no case of its own.
+constexpr float kRowFloor = 0x1p-100f;
+
+struct RowScale {
+  float inv;    // 127 / m: code = rint(x * inv)
+  float scale;  // m / 127: value = code * scale; NaN for a row that is not finite
+  bool finite;
+};
+
+// From the largest |x| of a row as the bits of the float: as unsigned integers
+// they order like the values, with infinity and then NaN above all of them, so
+// a maximum of bits keeps what a maximum of floats may drop.
+__device__ __forceinline__ RowScale row_scale(uint32_t max_bits) {
+#pragma clang fp contract(off)
+  RowScale r;
+  r.finite = max_bits < 0x7f800000u;
+  const float m = fmaxf(__builtin_bit_cast(float, r.finite ? max_bits : 0u), kRowFloor);
+  r.inv = r.finite ? 127.0f / m : 0.0f;
+  r.scale = r.finite ? m / 127.0f : __builtin_nanf("");
+  return r;
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
+
+// Codes of finite rows lie in [-127, 127]: |x| * fl(127 / m) < 127.5.  A row
+// that is not finite has inv = 0 and NaN products, which convert to 0.
+__device__ __forceinline__ int row_code(float v, float inv) { return (int)rintf(v * inv); }
+
+// The four low bytes, first value lowest.
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+  return __builtin_amdgcn_perm((uint32_t)__builtin_amdgcn_perm((uint32_t)d, (uint32_t)c, 0x0c0c0400u),
+                               (uint32_t)__builtin_amdgcn_perm((uint32_t)b, (uint32_t)a, 0x0c0c0400u), 0x05040100u);
+}
+
+// Element types of the rows (SPHOPS_F32, SPHOPS_BF16, SPHOPS_F16).
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__hip_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __hip_bfloat16 from_f32<__hip_bfloat16>(float v) { return __float2bfloat16(v); }
+// The empty asm keeps a product before it a float: the compiler else takes both
+// in one mixed-precision instruction, which rounds once where the definition
+// rounds to float32 first.
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) {
+  asm("" : "+v"(v));
+  return __float2half(v);
+}
+
+// One value of an integer layer: each step rounds by itself, so every kernel
+// gives the same bits, whatever its tiles.
+__device__ __forceinline__ float linear8_value(int sum, float row_scale, float channel_scale, float bias) {
+#pragma clang fp contract(off)
+  const float unit = row_scale * channel_scale;
+  const float v = (float)sum * unit;
+  return v + bias;
+}
+
+// f(T{}) for a type code; the caller has checked the code.
+template <class F>
+void with_type(int type, F&& f) {
+  if (type == SPHOPS_F32) f(float{});
+  else if (type == SPHOPS_BF16) f(__hip_bfloat16{});
+  else f(__half{});
+}
+
+}  // namespace sphops

@@ -368,6 +368,29 @@ void run_mlp_input_grad(const float* dy, const float* w1, const float* w2, const
 void run_mlp_weight_grad(const float* z, const float* a, const float* dy, const float* w2, float* dw1, float* db1,
                          float* dw2, float* db2, int64_t rows, int nin, int nout, float* work, hipStream_t st);
 
+// rows8.hip: rows of up to kMaxRows8Cols values in 8 bits, a scale a row
+constexpr int64_t kMaxRows8Cols = 65536;  // the integer sums of a product stay below 2^31
+constexpr int64_t kMaxRows8Rows = int64_t(1) << 30;
+void run_quantize_rows(const void* x, int type, int64_t stride, int8_t* codes, int64_t ld, float* scale, int64_t rows,
+                       int64_t cols, bool relu, hipStream_t st);
+void run_restore_rows(const int8_t* codes, int64_t ld, const float* scale, void* out, int type, int64_t rows,
+                      int64_t cols, hipStream_t st);
+int64_t rows8_weight_grad_floats(int64_t rows, int nin, int nout);
+void run_rows8_weight_grad(const int8_t* codes, int64_t ld, const float* scale, const float* dy, float* dw, float* db,
+                           int64_t rows, int nin, int nout, float* work, hipStream_t st);
+// linear8.hip
+int64_t linear8_workspace_bytes(int64_t rows, int64_t cols, int outs);
+void run_linear8(const void* x, int type, int64_t stride, const int8_t* wq, int64_t wld, const float* ws,
+                 const float* b, void* y, int64_t rows, int64_t cols, int outs, void* work, hipStream_t st);
+// mlp8.hip
+void run_mlp8(const float* z, const int8_t* w1, int64_t ld1, const float* s1, const float* b1, const int8_t* w2,
+              int64_t ld2, const float* s2, const float* b2, float* y, int64_t rows, int nin, int nout,
+              hipStream_t st);
+int64_t mlp_rows8_floats(int64_t rows, int nin, int nout);
+void run_mlp_rows8_backward(const int8_t* codes, int64_t ld, const float* scale, const float* dy, const float* w1,
+                            const float* b1, const float* w2, float* dz, float* dw1, float* db1, float* dw2,
+                            float* db2, int64_t rows, int nin, int nout, float* work, hipStream_t st);
+
 constexpr uint32_t kMaxChannels = 64;
 constexpr int kRadixBins = 1024;  // digit values per radix-sort pass (10 bits)
 // Words of the radix histograms: kRadixBins tile counts per tile of 4096

@@ -20,6 +20,7 @@ import ctypes
 import torch
 import torch.nn.functional as F
 
+from . import int8
 from .sphops import _native
 
 _lib = _native.lib
@@ -210,23 +211,147 @@ RELU_LINEAR_MAX_OUT = 64
 RELU_LINEAR_MAX_IN = 256
 
 
-def linear(x, layer):
+class LinearRows8(torch.autograd.Function):
+    """``LinearRows`` that keeps x in 8 bits (``npa_amd.int8``): dW comes from
+    the codes.  Nothing is kept of x where no dW is wanted."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        kept = int8.quantize_rows(x) if ctx.needs_input_grad[1] else None
+        ctx.shape, ctx.has_bias = tuple(x.shape), bias is not None
+        ctx.save_for_backward(weight, *(() if kept is None else (kept.codes, kept.scale)))
+        return F.linear(x, weight, bias)
+
+    @staticmethod
+    def backward(ctx, dy):
+        weight, *kept = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad
+        dx = dw = db = None
+        if need_x:
+            dx = (dy.reshape(-1, weight.shape[0]) @ weight).reshape(ctx.shape)
+        if need_w:
+            dw, db = int8.weight_grad(int8.Rows8(*kept, ctx.shape), dy, need_b and ctx.has_bias)
+        elif need_b and ctx.has_bias:
+            db = dy.reshape(-1, weight.shape[0]).sum(0)
+        return dx, dw, db
+
+
+class ReluLinear8(torch.autograd.Function):
+    """``ReluLinear`` that keeps relu(a) in 8 bits, whose codes are positive
+    exactly where a is: the ReLU's mask is exact."""
+
+    @staticmethod
+    def forward(ctx, a, weight, bias):
+        kept = int8.quantize_rows(a, relu=True)
+        ctx.shape, ctx.has_bias = tuple(a.shape), bias is not None
+        ctx.save_for_backward(weight, kept.codes, kept.scale)
+        return F.linear(torch.relu(a), weight, bias)
+
+    @staticmethod
+    def backward(ctx, dy):
+        weight, codes, scale = ctx.saved_tensors
+        need_a, need_w, need_b = ctx.needs_input_grad
+        kept = int8.Rows8(codes, scale, ctx.shape)
+        da = dw = db = None
+        if need_a:
+            # a row that was not finite is restored as NaN: its upstream passes, as torch's does
+            g = (dy.reshape(-1, weight.shape[0]) @ weight).reshape(ctx.shape)
+            da = torch.where(int8.restore_rows(kept) <= 0, torch.zeros_like(g), g)
+        if need_w or (need_b and ctx.has_bias):
+            dw, db = int8.weight_grad(kept, dy, ctx.has_bias)
+        return da, (dw if need_w else None), (db if need_b else None)
+
+
+class MlpRows8(torch.autograd.Function):
+    """``MlpRows`` that keeps z in 8 bits and nothing else: y is computed from z
+    itself, and the backward computes the hidden values of the kept rows again
+    (``sphops_mlp_rows8_backward``).  The gradients are those of the MLP at the
+    kept rows, passed straight through the rounding of z."""
+
+    @staticmethod
+    def forward(ctx, z, w1, b1, w2, b2):
+        hidden, in_f = w1.shape
+        out_f = w2.shape[0]
+        z2 = z.reshape(-1, in_f).contiguous()
+        rows = z2.shape[0]
+        kept = int8.quantize_rows(z2)
+        dense = [None if t is None else t.detach().contiguous() for t in (w1, b1, w2, b2)]
+        ctx.shape, ctx.has_b2 = (rows, in_f, hidden, out_f), b2 is not None
+        y = torch.empty(rows, out_f, device=z.device)
+        _native.check(_lib.sphops_mlp_forward(_ptr(z2), *(_ptr(t) for t in dense), _ptr(None), _ptr(y), rows, in_f,
+                                              hidden, out_f, _stream(z)))
+        ctx.save_for_backward(kept.codes, kept.scale, w1, b1, w2)
+        return y.reshape(*z.shape[:-1], out_f)
+
+    @staticmethod
+    def backward(ctx, dy):
+        codes, scale, w1, b1, w2 = ctx.saved_tensors
+        need_z, need_w1, need_b1, need_w2, need_b2 = ctx.needs_input_grad
+        rows, in_f, hidden, out_f = ctx.shape
+        lead = dy.shape[:-1]
+        dy = dy.reshape(-1, out_f).contiguous()
+        if dy.dtype != torch.float32 or not dy.is_cuda:
+            raise TypeError("the MLP kernels take float32 GPU tensors")
+        dev = dy.device
+        dz = torch.empty(rows, in_f, device=dev) if need_z else None
+        dw1 = torch.empty(hidden, in_f, device=dev) if need_w1 else None
+        db1 = torch.empty(hidden, device=dev) if need_b1 and b1 is not None else None
+        dw2 = torch.empty(out_f, hidden, device=dev) if need_w2 else None
+        db2 = torch.empty(out_f, device=dev) if need_b2 and ctx.has_b2 else None
+        dense = [None if t is None else t.detach().contiguous() for t in (w1, b1, w2)]
+        nbytes = _lib.sphops_mlp_rows8_workspace_bytes(rows, in_f, hidden, out_f)
+        work = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+        _native.check(_lib.sphops_mlp_rows8_backward(_ptr(codes), codes.shape[1], _ptr(scale), _ptr(dy),
+                                                     *(_ptr(t) for t in dense), _ptr(dz), _ptr(dw1), _ptr(db1),
+                                                     _ptr(dw2), _ptr(db2), rows, in_f, hidden, out_f, _ptr(work),
+                                                     _stream(dy)))
+        return None if dz is None else dz.reshape(*lead, in_f), dw1, db1, dw2, db2
+
+
+def _rows8_ok(x, layer):
+    """What ``LinearRows8`` and ``ReluLinear8`` keep in 8 bits; any other input
+    keeps the layer's own function."""
+    tensors = [t for t in (x, layer.weight, layer.bias) if t is not None]
+    return (torch.is_grad_enabled() and any(t.requires_grad for t in tensors) and x.dim() >= 1
+            and all(t.is_cuda and t.dtype == torch.float32 and t.device == x.device for t in tensors)
+            and not torch.is_autocast_enabled())
+
+
+def _check_checkpoint(checkpoint):
+    if checkpoint not in (None, "int8"):
+        raise ValueError(f"checkpoint must be None or 'int8', got {checkpoint!r}")
+
+
+def linear(x, layer, checkpoint=None):
+    """``layer(x)``; with checkpoint="int8" x is kept in 8 bits for dW."""
+    _check_checkpoint(checkpoint)
+    if checkpoint and _rows8_ok(x, layer):
+        return LinearRows8.apply(x, layer.weight, layer.bias)
     return LinearRows.apply(x, layer.weight, layer.bias)
 
 
-def relu_linear(a, layer):
-    """``layer(torch.relu(a))`` with the fused backward."""
+def relu_linear(a, layer, checkpoint=None):
+    """``layer(torch.relu(a))`` with the fused backward; with checkpoint="int8"
+    relu(a) is kept in 8 bits and its mask exactly."""
+    _check_checkpoint(checkpoint)
+    if checkpoint and _rows8_ok(a, layer):
+        return ReluLinear8.apply(a, layer.weight, layer.bias)
     return ReluLinear.apply(a, layer.weight, layer.bias)
 
 
-def mlp(module, z):
+def mlp(module, z, checkpoint=None):
     """``module(z)`` for a ``torch.nn.Linear`` or a ``torch.nn.Sequential`` of
     layers (the shapes NPA's _get_mlp builds): a Linear, ReLU, Linear that
     ``MlpRows`` takes through it, a ReLU followed by a Linear of at most
     RELU_LINEAR_MAX_OUT outputs through ``ReluLinear``, every other Linear
-    through ``LinearRows``; any other module runs as it is."""
+    through ``LinearRows``; any other module runs as it is.
+
+    ``checkpoint="int8"``: what the layers keep for the backward is kept in 8
+    bits (``MlpRows8``, ``ReluLinear8``, ``LinearRows8``): y is the same, the
+    weight gradients are those of inputs rounded to their codes."""
+    _check_checkpoint(checkpoint)
     if isinstance(module, torch.nn.Linear):
-        return linear(z, module)
+        return linear(z, module, checkpoint)
     if isinstance(module, torch.nn.Sequential):
         layers = list(module)
         i = 0
@@ -238,15 +363,15 @@ def mlp(module, z):
                     and _mlp_rows_ok(z, layer, last)):
                 inputs = (z, layer.weight, layer.bias, last.weight, last.bias)
                 keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)
-                z = MlpRows.apply(*inputs, keep)
+                z = MlpRows8.apply(*inputs) if checkpoint and keep else MlpRows.apply(*inputs, keep)
                 i += 3
                 continue
             if (type(layer) is torch.nn.ReLU and isinstance(nxt, torch.nn.Linear)
-                    and nxt.out_features <= RELU_LINEAR_MAX_OUT):
-                z = relu_linear(z, nxt)
+                    and (nxt.out_features <= RELU_LINEAR_MAX_OUT or (checkpoint and _rows8_ok(z, nxt)))):
+                z = relu_linear(z, nxt, checkpoint)
                 i += 2
                 continue
-            z = linear(z, layer) if isinstance(layer, torch.nn.Linear) else layer(z)
+            z = linear(z, layer, checkpoint) if isinstance(layer, torch.nn.Linear) else layer(z)
             i += 1
         return z
     return module(z)

@@ -99,10 +99,10 @@ def _draws(x, update_prob, noise_std):
     return mask, noise
 
 
-def _step(model, x, s, grid, dt, update_prob, noise_std):
+def _step(model, x, s, grid, dt, update_prob, noise_std, checkpoint):
     z, x_bin, s_bin, snapshot = _perceive(model, x, s, grid)
     model.last_snapshot = snapshot
-    y = mlp(model.model, z).contiguous()
+    y = mlp(model.model, z, checkpoint).contiguous()
     mask, noise = _draws(x, update_prob, noise_std)
     alpha = buffer_value(model.alpha)
     x_new, s_new, dx_norm = EulerUpdate.apply(y, x_bin.contiguous(), s_bin.contiguous(), mask, noise,
@@ -111,10 +111,12 @@ def _step(model, x, s, grid, dt, update_prob, noise_std):
     return x_new, s_new, dx_norm, y, alpha
 
 
-def step_euler(model, x, s, grid, dt=1.0, update_prob=0.5, intermediate=False, noise_std=0.0):
+def step_euler(model, x, s, grid, dt=1.0, update_prob=0.5, intermediate=False, noise_std=0.0, checkpoint=None):
     """step_euler (models/npa.py:154-204): returns (x, s, stats) in binned
-    order; stats = {"dx_norm": mean |dx|} when intermediate, else None."""
-    x_new, s_new, dx_norm, _, _ = _step(model, x, s, grid, dt, update_prob, noise_std)
+    order; stats = {"dx_norm": mean |dx|} when intermediate, else None.
+    ``checkpoint="int8"`` keeps the MLP's input in 8 bits for the backward
+    (``npa_amd.mlp.mlp``): the same step, longer rollouts in the same memory."""
+    x_new, s_new, dx_norm, _, _ = _step(model, x, s, grid, dt, update_prob, noise_std, checkpoint)
     stats = {"dx_norm": dx_norm.mean()} if intermediate else None
     return x_new, s_new, stats
 
@@ -165,15 +167,16 @@ def step_euler_trace(model, x, s, grid, dt=1.0, update_prob=0.5, noise_std=0.0, 
     return x_trace, s_trace, dx_trace, ds_trace
 
 
-def step_euler_static(model, x, s, grid, dt=1.0, update_prob=0.5, channel_mask=None):
+def step_euler_static(model, x, s, grid, dt=1.0, update_prob=0.5, channel_mask=None, checkpoint=None):
     """step_euler of the state-only model (models/static_npa.py:15-38):
     fused perception, the model's MLP giving ds only, positions unchanged
     (x_bin + 0), s = s_bin + dt * ds * mask; returns (x, s) in binned order.
-    The update is a single elementwise expression, left to torch."""
+    The update is a single elementwise expression, left to torch.
+    ``checkpoint`` as in ``step_euler``."""
     B, N, C = s.shape
     z, x_bin, s_bin, snapshot = _perceive(model, x, s, grid)
     model.last_snapshot = snapshot
-    ds = mlp(model.model, z)
+    ds = mlp(model.model, z, checkpoint)
     mask = 1.0
     if update_prob < 1.0:
         mask = (torch.rand(B, N, 1, device=x.device) < update_prob).float()
