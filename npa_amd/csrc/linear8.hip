@@ -1,7 +1,10 @@
 // A linear layer in 8-bit integers, for gfx950: y = (cx cw^T) * (sx sw) + b
 // with a scale for each row of the input and each output channel, the sums in
-// int32 on the integer matrix cores (v_mfma_i32_32x32x32_i8).
+// int32 on the integer matrix cores.  The sums are exact and each later step
+// rounds by itself, so every kernel here gives the same bits.
 #include "rows8.hpp"
+
+#include <type_traits>
 
 namespace sphops {
 
@@ -10,43 +13,202 @@ namespace {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
-// One wave a tile of 32 rows and 32 channels.  Lane l supplies 16 codes of
-// input row l % 32 and 16 of channel l % 32, at k = 16 (l / 32) of a step of
-// 32; result register r of lane l is row 8 (r / 4) + 4 (l / 32) + r % 4,
-// channel l % 32.  xq's rows end in zeros up to a multiple of 32, so what a
-// channel's last step reads past its row (the next channel's codes) counts
-// nothing; the last channel's is not read past the end.
-template <class T>
-__global__ __launch_bounds__(256) void k_linear8(const int8_t* __restrict__ xq, int64_t xld,
-                                                 const float* __restrict__ xs, const int8_t* __restrict__ wq,
-                                                 int64_t wld, const float* __restrict__ ws,
-                                                 const float* __restrict__ b, T* __restrict__ y, int64_t rows,
-                                                 int outs, int row_tiles, int out_tiles) {
-  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
-  const int64_t job = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-  if (job >= (int64_t)row_tiles * out_tiles) return;
-  const int64_t r0 = job / out_tiles * 32;
-  const int o0 = (int)(job % out_tiles) * 32;
-  const int64_t row = min<int64_t>(r0 + c, rows - 1);
-  const int out = min(o0 + c, outs - 1);
-  const int8_t* __restrict__ xp = xq + row * xld + 16 * h;
-  const int8_t* __restrict__ wp = wq + (int64_t)out * wld + 16 * h;
-  i32x16 acc = i32x16{};
-  for (int64_t k = 0; k < xld; k += 32) {
-    const i32x4 a = *reinterpret_cast<const i32x4*>(xp + k);
-    const i32x4 w = k + 16 * h < wld ? *reinterpret_cast<const i32x4*>(wp + k) : i32x4{};
-    acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, w, acc, 0, 0, 0);
-  }
-  if (o0 + c >= outs) return;
-  const float s = ws[out], bias = b != nullptr ? b[out] : 0.0f;
+constexpr int kStep = 128;  // bytes of a row a step of the tile kernel takes
+
+__device__ __forceinline__ i32x16 mma8(i32x4 a, i32x4 b, i32x16 c) {
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
+}
+
+// 64 lanes' 16 bytes from memory to LDS, lane l's to lds + 16 l, past the
+// registers; done once the wave's vector memory count says so.
+__device__ __forceinline__ void load_to_lds(const int8_t* src, int8_t* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+
+// Output tiles in an order that keeps the tiles an XCD works on at a time in a
+// block of 8 row tiles by a few column tiles, whose panels its L2 holds.
+__device__ __forceinline__ void tile_of(uint32_t id, int mt, int nt, int& m, int& n) {
+  constexpr uint32_t kGroup = 8;
+  const uint32_t per = kGroup * (uint32_t)nt, g = id / per, first = g * kGroup;
+  const uint32_t size = min(kGroup, (uint32_t)mt - first), at = id - g * per;
+  m = (int)(first + at % size);
+  n = (int)(at / size);
+}
+
+// Workgroup = a tile of BM rows by BN channels, WM x WN waves of BM / WM by BN
+// / WN each.  A step of 128 bytes of both panels goes from memory straight to
+// LDS under the products of the step before.  In LDS a row's eight 16-byte
+// pieces are exchanged by the row's low bits (piece p stands at p ^ (row % 8)):
+// the 8 rows that a quarter of a wave's operand read takes then lie in
+// different banks.  For 32 x 32 x 32, lane l supplies 16 bytes of row l % 32 at
+// k = 16 (l / 32), and result register r of lane l is row 8 (r / 4) + 4 (l /
+// 32) + r % 4, channel l % 32.
+//
+// xq's rows end in zeros up to a multiple of the step, so what a channel's last
+// step holds past its codes counts nothing; its address is kept inside the row.
+template <class T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void k_linear8_tile(const int8_t* __restrict__ xq, int64_t xld,
+                                                               const float* __restrict__ xs,
+                                                               const int8_t* __restrict__ wq, int64_t wld,
+                                                               const float* __restrict__ ws,
+                                                               const float* __restrict__ b, T* __restrict__ y,
+                                                               int64_t rows, int outs, int mt, int nt) {
+  constexpr int kWaves = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+  constexpr int kLoadsA = BM / 8 / kWaves, kLoadsB = BN / 8 / kWaves;  // a wave's loads of 8 rows a step
+  static_assert(kLoadsA * 8 * kWaves == BM && kLoadsB * 8 * kWaves == BN, "whole loads");
+  // separate arrays: a load into one is no reason to wait before a read of the other
+  __shared__ __attribute__((aligned(16))) int8_t a0[BM * kStep], b0[BN * kStep], a1[BM * kStep], b1[BN * kStep];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+  const int c = lane & 31, h = lane >> 5;
+  int mi, ni;
+  tile_of(xcd_block_id(), mt, nt, mi, ni);
+  const int64_t m0 = (int64_t)mi * BM;
+  const int n0 = ni * BN;
+
+  const int piece = 16 * ((lane & 7) ^ (lane >> 3));  // of the step's 128 bytes
+  // 32-bit offsets from the panels' first rows
+  const int8_t* __restrict__ ap = xq + m0 * xld;
+  const int8_t* __restrict__ bp = wq + (int64_t)n0 * wld;
+  const int rows_here = (int)min<int64_t>(BM, rows - m0), outs_here = min(BN, outs - n0);
+  uint32_t oa[kLoadsA], ob[kLoadsB];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int64_t at = r0 + 8 * (r / 4) + 4 * h + r % 4;
-    if (at < rows) y[at * outs + out] = from_f32<T>(linear8_value(acc[r], xs[at], s, bias));
+  for (int i = 0; i < kLoadsA; ++i)
+    oa[i] = (uint32_t)min((i * kWaves + wave) * 8 + (lane >> 3), rows_here - 1) * (uint32_t)xld + (uint32_t)piece;
+#pragma unroll
+  for (int i = 0; i < kLoadsB; ++i)
+    ob[i] = (uint32_t)min((i * kWaves + wave) * 8 + (lane >> 3), outs_here - 1) * (uint32_t)wld;
+  const int last = (int)wld - 16, end = (int)xld;
+  // past the last step: the last one again, which nothing reads
+  auto load = [&](int k, int8_t* as, int8_t* bs) {
+    k = min(k, end - kStep);
+    const int8_t* __restrict__ ak = ap + k;
+#pragma unroll
+    for (int i = 0; i < kLoadsA; ++i) load_to_lds(ak + oa[i], as + (i * kWaves + wave) * 1024);
+    const uint32_t kb = (uint32_t)min(k + piece, last);
+#pragma unroll
+    for (int i = 0; i < kLoadsB; ++i) load_to_lds(bp + (ob[i] + kb), bs + (i * kWaves + wave) * 1024);
+    __builtin_amdgcn_sched_barrier(0);  // the loads go out before the products, not after them
+  };
+  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  i32x16 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = i32x16{};
+  }
+  auto compute = [&](const int8_t* as, const int8_t* bs) {
+#pragma unroll
+    for (int s = 0; s < kStep / 32; ++s) {
+      const int at = c * kStep + 16 * ((2 * s + h) ^ (c & 7));
+      i32x4 a[TM], w[TN];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) a[i] = *reinterpret_cast<const i32x4*>(as + (wm + 32 * i) * kStep + at);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) w[j] = *reinterpret_cast<const i32x4*>(bs + (wn + 32 * j) * kStep + at);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = mma8(a[i], w[j], acc[i][j]);
+      }
+    }
+  };
+  // every wave's loads of a step have landed, and every wave has read the step before
+  auto turn = [&] {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    __syncthreads();
+  };
+  load(0, a0, b0);
+  turn();
+  for (int k = 0; k + kStep < end; k += 2 * kStep) {
+    load(k + kStep, a1, b1);
+    compute(a0, b0);
+    turn();
+    load(k + 2 * kStep, a0, b0);
+    compute(a1, b1);
+    turn();
+  }
+  if (end / kStep % 2 != 0) compute(a0, b0);
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+    const int out = n0 + wn + 32 * j + c;
+    if (out >= outs) continue;
+    const float s = ws[out], bias = b != nullptr ? b[out] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int64_t at = m0 + wm + 32 * i + 8 * (r / 4) + 4 * h + r % 4;
+        if (at < rows) y[at * outs + out] = from_f32<T>(linear8_value(acc[i][j][r], xs[at], s, bias));
+      }
+    }
   }
 }
 
-int64_t padded_cols(int64_t cols) { return (cols + 31) / 32 * 32; }
+// Few rows: workgroup = 32 channels and all the rows (RT tiles of 32), its
+// eight waves a share of the row's length each; both operands come straight
+// from memory in the matrix instruction's layout (the weights once, the rows
+// from L2), and the waves' sums meet in LDS.  Integer sums: any order gives the
+// same value.
+constexpr int kFewWaves = 8;
+template <class T, int RT>
+__global__ __launch_bounds__(64 * kFewWaves) void k_linear8_few(const int8_t* __restrict__ xq, int64_t xld,
+                                                                const float* __restrict__ xs,
+                                                                const int8_t* __restrict__ wq, int64_t wld,
+                                                                const float* __restrict__ ws,
+                                                                const float* __restrict__ b, T* __restrict__ y,
+                                                                int rows, int outs, int share) {
+  __shared__ int sums[RT][16][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+  const int c = lane & 31, h = lane >> 5;
+  const int out = (int)blockIdx.x * 32 + c;
+  for (int i = threadIdx.x; i < RT * 16 * 64; i += 64 * kFewWaves) (&sums[0][0][0])[i] = 0;
+  const int8_t* __restrict__ wp = wq + (int64_t)min(out, outs - 1) * wld;
+  const int8_t* xp[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) xp[t] = xq + (int64_t)min(32 * t + c, rows - 1) * xld + 16 * h;
+  const int k0 = wave * share, k1 = min(k0 + share, (int)xld), last = (int)wld - 16;
+  i32x16 acc[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) acc[t] = i32x16{};
+  constexpr int kAhead = 8;  // steps of 32 bytes in flight
+  for (int k = k0; k < k1; k += 32 * kAhead) {
+    i32x4 w[kAhead], a[kAhead][RT];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) w[u] = *reinterpret_cast<const i32x4*>(wp + min(k + 32 * u + 16 * h, last));
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      // past the wave's share: zeros, whatever the weights are
+      const bool on = k + 32 * u < k1;
+#pragma unroll
+      for (int t = 0; t < RT; ++t) a[u][t] = on ? *reinterpret_cast<const i32x4*>(xp[t] + k + 32 * u) : i32x4{};
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) acc[t] = mma8(a[u][t], w[u], acc[t]);
+    }
+  }
+  __syncthreads();
+  if (k0 < k1) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) atomicAdd(&sums[t][r][lane], acc[t][r]);
+    }
+  }
+  __syncthreads();
+  if (out >= outs) return;
+  const float s = ws[out], bias = b != nullptr ? b[out] : 0.0f;
+#pragma unroll
+  for (int i = 0; i < RT * 16 / kFewWaves; ++i) {
+    const int e = i * kFewWaves + wave, t = e / 16, r = e % 16, at = 32 * t + 8 * (r / 4) + 4 * h + r % 4;
+    if (at < rows) y[(int64_t)at * outs + out] = from_f32<T>(linear8_value(sums[t][r][lane], xs[at], s, bias));
+  }
+}
+
+int64_t padded_cols(int64_t cols) { return (cols + kStep - 1) / kStep * kStep; }
+int64_t tiles_of(int64_t n, int tile) { return (n + tile - 1) / tile; }
 
 }  // namespace
 
@@ -60,12 +222,33 @@ void run_linear8(const void* x, int type, int64_t stride, const int8_t* wq, int6
   int8_t* xq = static_cast<int8_t*>(work);
   float* xs = reinterpret_cast<float*>(xq + rows * xld);
   run_quantize_rows(x, type, stride, xq, xld, xs, rows, cols, false, st);
-  const int row_tiles = (int)((rows + 31) / 32), out_tiles = (outs + 31) / 32;
-  const int64_t jobs = (int64_t)row_tiles * out_tiles;
   with_type(type, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL((k_linear8<T>), dim3((uint32_t)((jobs + 3) / 4)), dim3(256), 0, st, xq, xld, xs, wq, wld, ws,
-                       b, static_cast<T*>(y), rows, outs, row_tiles, out_tiles);
+    T* out = static_cast<T*>(y);
+    if (rows <= 128) {
+      const int share = (int)(((xld + kFewWaves - 1) / kFewWaves + 31) / 32 * 32);
+      auto few = [&](auto rt) {
+        hipLaunchKernelGGL((k_linear8_few<T, decltype(rt)::value>), dim3((uint32_t)tiles_of(outs, 32)),
+                           dim3(64 * kFewWaves), 0, st, xq, xld, xs, wq, wld, ws, b, out, (int)rows, outs, share);
+      };
+      if (rows <= 32) few(std::integral_constant<int, 1>{});
+      else if (rows <= 64) few(std::integral_constant<int, 2>{});
+      else few(std::integral_constant<int, 4>{});
+      return;
+    }
+    auto tile = [&](auto bm, auto bn, auto wm, auto wn) {
+      constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value,
+                    WN = decltype(wn)::value;
+      const int64_t mt = tiles_of(rows, BM), nt = tiles_of(outs, BN);
+      hipLaunchKernelGGL((k_linear8_tile<T, BM, BN, WM, WN>), dim3((uint32_t)(mt * nt)), dim3(64 * WM * WN), 0, st,
+                         xq, xld, xs, wq, wld, ws, b, out, rows, outs, (int)mt, (int)nt);
+    };
+#define SPHOPS_N(n) std::integral_constant<int, n>{}
+    if (tiles_of(rows, 256) * tiles_of(outs, 256) >= 192) tile(SPHOPS_N(256), SPHOPS_N(256), SPHOPS_N(2), SPHOPS_N(4));
+    else if (tiles_of(rows, 128) * tiles_of(outs, 128) >= 192)
+      tile(SPHOPS_N(128), SPHOPS_N(128), SPHOPS_N(2), SPHOPS_N(2));
+    else tile(SPHOPS_N(64), SPHOPS_N(64), SPHOPS_N(2), SPHOPS_N(2));
+#undef SPHOPS_N
   });
   SPHOPS_LAUNCHED();
 }

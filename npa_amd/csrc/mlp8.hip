@@ -94,8 +94,7 @@ __global__ __launch_bounds__(kServeThreads, 2) void k_mlp8(
       i32x4 cz;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        cz[i] = (int)pack4(row_code(zv[s][i][0], qz.inv), row_code(zv[s][i][1], qz.inv),
-                           row_code(zv[s][i][2], qz.inv), row_code(zv[s][i][3], qz.inv));
+        cz[i] = (int)row_codes4(zv[s][i][0], zv[s][i][1], zv[s][i][2], zv[s][i][3], qz);
 #pragma unroll
       for (int t = 0; t < kHT; ++t)
         acc[t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w1img[s][t][lane], cz, acc[t], 0, 0, 0);
@@ -125,8 +124,7 @@ __global__ __launch_bounds__(kServeThreads, 2) void k_mlp8(
       i32x4 ch;
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        ch[q] = (int)pack4(row_code(hv[t][4 * q], qh.inv), row_code(hv[t][4 * q + 1], qh.inv),
-                           row_code(hv[t][4 * q + 2], qh.inv), row_code(hv[t][4 * q + 3], qh.inv));
+        ch[q] = (int)row_codes4(hv[t][4 * q], hv[t][4 * q + 1], hv[t][4 * q + 2], hv[t][4 * q + 3], qh);
 #pragma unroll
       for (int o = 0; o < OT; ++o)
         out[o] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w2img[t][o][lane], ch, out[o], 0, 0, 0);

@@ -34,14 +34,26 @@ __device__ __forceinline__ RowScale row_scale(uint32_t max_bits) {
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
-// Codes of finite rows lie in [-127, 127]: |x| * fl(127 / m) < 127.5.  A row
-// that is not finite has inv = 0 and NaN products, which convert to 0.
-__device__ __forceinline__ int row_code(float v, float inv) { return (int)rintf(v * inv); }
+// A code in the low byte of a word: added to 1.5 * 2^23, whose last place is 1,
+// the product is rounded to the nearest whole number, ties to the even one, and
+// stands in the low bits.  Codes of finite rows lie in [-127, 127]: |x| * fl(127
+// / m) < 127.5.
+__device__ __forceinline__ uint32_t row_code(float v, float inv) {
+#pragma clang fp contract(off)
+  const float p = v * inv;
+  return __builtin_bit_cast(uint32_t, p + 12582912.0f);
+}
 
-// The four low bytes, first value lowest.
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
-  return __builtin_amdgcn_perm((uint32_t)__builtin_amdgcn_perm((uint32_t)d, (uint32_t)c, 0x0c0c0400u),
-                               (uint32_t)__builtin_amdgcn_perm((uint32_t)b, (uint32_t)a, 0x0c0c0400u), 0x05040100u);
+// The low bytes of four words, first value lowest.
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u),
+                               0x05040100u);
+}
+
+// Four codes of a row: zeros in a row that is not finite.
+__device__ __forceinline__ uint32_t row_codes4(float a, float b, float c, float d, const RowScale& q) {
+  const uint32_t w = pack4(row_code(a, q.inv), row_code(b, q.inv), row_code(c, q.inv), row_code(d, q.inv));
+  return q.finite ? w : 0u;
 }
 
 // Element types of the rows (SPHOPS_F32, SPHOPS_BF16, SPHOPS_F16).
