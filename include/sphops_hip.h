@@ -591,6 +591,12 @@ int sphops_mlp8_forward(const float* z, const int8_t* w1_codes, int64_t w1_ld, c
                         const int8_t* w2_codes, int64_t w2_ld, const float* w2_scale, const float* b2, float* y,
                         int64_t rows, int in_features, int hidden, int out_features, void* stream);
 
+/* sphops_mlp_forward that also writes z in 8 bits (codes, scale; ld at most
+ * in_features rounded up to 16), in one pass over z. */
+int sphops_mlp_rows8_forward(const float* z, const float* w1, const float* b1, const float* w2, const float* b2,
+                             int8_t* codes, int64_t ld, float* scale, float* y, int64_t rows, int in_features,
+                             int hidden, int out_features, void* stream);
+
 /* The gradients of sphops_mlp_forward at an input kept in 8 bits: the hidden
  * values are computed again from the codes, so nothing else is kept.  dz, dw1,
  * db1, dw2 and db2 may each be NULL.  workspace:

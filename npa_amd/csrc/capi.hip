@@ -1334,6 +1334,20 @@ int sphops_mlp8_forward(const float* z, const int8_t* w1_codes, int64_t w1_ld, c
   });
 }
 
+int sphops_mlp_rows8_forward(const float* z, const float* w1, const float* b1, const float* w2, const float* b2,
+                             int8_t* codes, int64_t ld, float* scale, float* y, int64_t rows, int in_features,
+                             int hidden, int out_features, void* stream) {
+  return guarded([&] {
+    require(sphops::mlp_fits(rows, in_features, hidden, out_features), "MLP shape not supported");
+    require_rows8(rows, in_features, ld);
+    require(ld <= (in_features + 15) / 16 * 16, "ld must be at most in_features rounded up to 16");
+    require(rows == 0 || (z && w1 && w2 && codes && scale && y), "null buffer");
+    require(reinterpret_cast<uintptr_t>(codes) % 4 == 0, "codes must be 4-byte aligned");
+    sphops::run_mlp_rows8_forward(z, w1, b1, w2, b2, codes, ld, scale, y, rows, in_features, out_features,
+                                  sphops::as_stream(stream));
+  });
+}
+
 int64_t sphops_mlp_rows8_workspace_bytes(int64_t rows, int in_features, int hidden, int out_features) {
   if (!sphops::mlp_fits(rows, in_features, hidden, out_features)) return -1;
   return sphops::mlp_rows8_floats(rows, in_features, out_features) * (int64_t)sizeof(float);

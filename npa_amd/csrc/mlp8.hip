@@ -60,6 +60,7 @@ __global__ __launch_bounds__(kServeThreads, 2) void k_mlp8(
   const int64_t step = (int64_t)gridDim.x * (kServeThreads / 64);
   int64_t tile = (int64_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * (kServeThreads / 64) + threadIdx.x / 64));
   for (; tile < tiles; tile += step) {
+    asm volatile("" ::: "memory");  // the images stay in LDS: read ahead of the loop they spill
     const int64_t r0 = tile * kT, nr = min<int64_t>(kT, rows - r0);
     const __amdgpu_buffer_rsrc_t rz = rows_rsrc(z + r0 * nin, nr * nin * 4);
     f32x4 zv[KS][4];
@@ -160,21 +161,722 @@ void run_mlp8(const float* z, const int8_t* w1, int64_t ld1, const float* s1, co
   SPHOPS_LAUNCHED();
 }
 
-// The backward from codes: the rows and the hidden values again in 32 bits,
-// then the gradients of mlp_rows.hip.
+namespace {
+
+
+// ---------------------------------------------------------------- training
+//
+// Products of float32 factors on the 16-bit matrix cores (a 32 x 32 x 16
+// instruction takes 32 cycles, eight float32 ones of 32 x 32 x 2 take 512):
+// * a factor is scaled by a power of two and split into two halves, hi = v to
+//   11 bits and lo = v - hi to 11 more, and a product is hi hi + hi lo + lo hi
+//   with float32 sums (the splitting that H. Ootomo and R. Yokota published,
+//   2022).  What it leaves out is at most 2^-22 of |a b|, and half the smallest
+//   subnormal of a factor, 2^-40 of the largest value that shares its scale;
+// * where no scale serves (sums over rows of any size) three bfloat16 pieces
+//   hold all 24 bits at float32's range, and six products are taken;
+// * a code is exact in either type, so its products need one factor split.
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// A power of two p with m p in [2^14, 2^15) for the largest magnitude m (as
+// bits), kept where p and 1 / p are normal, and 1 / p.
+struct Pow2 {
+  float p, ip;
+};
+__device__ __forceinline__ Pow2 pow2_for(uint32_t max_bits) {
+  const int e = min(268 - (int)(max_bits >> 23), 253);
+  return {__builtin_bit_cast(float, (uint32_t)e << 23), __builtin_bit_cast(float, (uint32_t)(254 - e) << 23)};
+}
+
+struct Halves {
+  f16x8 hi, lo;
+};
+__device__ __forceinline__ Halves split(f32x8 v) {
+  Halves r;
+  r.hi = __builtin_convertvector(v, f16x8);
+  r.lo = __builtin_convertvector(v - __builtin_convertvector(r.hi, f32x8), f16x8);
+  return r;
+}
+// + a b for factors in halves, the small products first
+__device__ __forceinline__ f32x16 mma(const Halves& a, const Halves& b, f32x16 c) {
+  return mma(a.hi, b.hi, mma(a.hi, b.lo, mma(a.lo, b.hi, c)));
+}
+
+struct Thirds {
+  bf16x8 v[3];
+};
+__device__ __forceinline__ Thirds split3(f32x8 v) {
+  Thirds r;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    r.v[i] = __builtin_convertvector(v, bf16x8);
+    if (i < 2) v -= __builtin_convertvector(r.v[i], f32x8);
+  }
+  return r;
+}
+__device__ __forceinline__ f32x16 mma(const Thirds& a, const Thirds& b, f32x16 c) {
+  c = mma(a.v[1], b.v[1], mma(a.v[2], b.v[0], mma(a.v[0], b.v[2], c)));
+  return mma(a.v[0], b.v[0], mma(a.v[1], b.v[0], mma(a.v[0], b.v[1], c)));
+}
+
+// Eight codes as halves: as unsigned numbers code + 128 they are the low bits
+// of the halves 1024 + code + 128.
+__device__ __forceinline__ f16x8 codes_f16(u32x2 w) {
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t u = w[i] ^ 0x80808080u;
+    r[2 * i] = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
+    r[2 * i + 1] = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+  }
+  return __builtin_bit_cast(f16x8, r) - (_Float16)1152.0f;
+}
+__device__ __forceinline__ bf16x4 codes_bf16(uint32_t w) {
+  const uint32_t u = w ^ 0x80808080u;
+  f32x4 v = {(float)(u & 0xffu), (float)((u >> 8) & 0xffu), (float)((u >> 16) & 0xffu), (float)(u >> 24)};
+  return __builtin_convertvector(v - 128.0f, bf16x4);
+}
+
+// Four 16-bit values down a column: of each 16 lanes, lane i gives the address
+// of four values of row i / 4 of a block of 4 rows by 16 columns, columns 4 (i %
+// 4) .. + 3, and receives column i.  (A plain LDS read moves rows.)
+__device__ __forceinline__ s16x4 read_column(const void* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s16x4*)const_cast<void*>(p));
+}
+__device__ __forceinline__ s16x8 join(s16x4 a, s16x4 b) {
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t bytes_rsrc(const int8_t* base, int64_t bytes) {
+  return rows_rsrc(reinterpret_cast<const float*>(base), bytes);
+}
+__device__ __forceinline__ u32x2 load2(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+}
+
+// Eight values of a row of n from column k (zeros past it), through a resource
+// over all rows.
+__device__ __forceinline__ f32x8 load8(__amdgpu_buffer_rsrc_t r, int row, int n, int k) {
+  f32x8 v;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = load1(r, k + j < n ? (uint32_t)(row * n + k + j) * 4u : kPast);
+  return v;
+}
+
+// W1 in halves as an operand image: lane l of entry (s, t) holds W1[32 t + l %
+// 32][16 s + 8 (l / 32) .. + 7] times the hidden unit's own power of two, whose
+// inverse is left in inv.  All threads; ends with a barrier.  `top` is scratch.
+template <int KS, int kThreads>
+__device__ __forceinline__ void w1_image(const float* __restrict__ w1, int nin, f16x8 (&hi)[KS][kHT][64],
+                                         f16x8 (&lo)[KS][kHT][64], uint32_t (&top)[kHid], float (&inv)[kHid]) {
+  constexpr int kEntries = KS * kHT * 64, kOwn = (kEntries + kThreads - 1) / kThreads;
+  const __amdgpu_buffer_rsrc_t r = rows_rsrc(w1, kHid * nin * 4);
+  f32x8 v[kOwn];
+  if (threadIdx.x < kHid) top[threadIdx.x] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kOwn; ++u) {
+    const int i = u * kThreads + (int)threadIdx.x, l = i & 63, t = (i >> 6) % kHT, s = (i >> 6) / kHT;
+    v[u] = f32x8{};
+    if (i < kEntries) v[u] = load8(r, kT * t + (l & 31), nin, 16 * s + 8 * (l >> 5));
+  }
+#pragma unroll
+  for (int u = 0; u < kOwn; ++u) {
+    const int i = u * kThreads + (int)threadIdx.x, l = i & 63, t = (i >> 6) % kHT;
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[u][j]));
+    if (i < kEntries) atomicMax(&top[kT * t + (l & 31)], m);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kOwn; ++u) {
+    const int i = u * kThreads + (int)threadIdx.x, l = i & 63, t = (i >> 6) % kHT, s = (i >> 6) / kHT;
+    if (i >= kEntries) continue;
+    const Halves h = split(v[u] * pow2_for(top[kT * t + (l & 31)]).p);
+    hi[s][t][l] = h.hi;
+    lo[s][t][l] = h.lo;
+  }
+  if (threadIdx.x < kHid) inv[threadIdx.x] = pow2_for(top[threadIdx.x]).ip;
+  __syncthreads();
+}
+
+// ------------------------------------------------------ training: forward
+
+// y = relu(z W1^T + b1) W2^T + b2 and z in 8 bits.  One wave a tile of 32 rows
+// (rows as the columns n): z's row and then the hidden row are scaled by their
+// own powers of two and split.  The hidden tile's result registers 8 j .. 8 j +
+// 7 of lane l are hidden units 16 j + 4 (l / 32) + 0..3 and 8 more of its row:
+// as they stand they are an operand with W2's image in the same order.
+template <int KS, int OT, int kThreads>
+__global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
+    const float* __restrict__ z, const float* __restrict__ w1, const float* __restrict__ b1,
+    const float* __restrict__ w2, const float* __restrict__ b2, int8_t* __restrict__ codes, int64_t ld,
+    float* __restrict__ scale, float* __restrict__ y, int64_t rows, int nin, int nout, int64_t tiles) {
+  __shared__ f16x8 w1hi[KS][kHT][64], w1lo[KS][kHT][64];
+  __shared__ f16x8 w2hi[kHT][2][OT][64], w2lo[kHT][2][OT][64];
+  __shared__ uint32_t top[kHid];
+  __shared__ __attribute__((aligned(16))) float i1s[kHid], b1s[kHid], i2s[OT * kT], b2s[OT * kT];
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  w1_image<KS, kThreads>(w1, nin, w1hi, w1lo, top, i1s);
+  {
+    constexpr int kEntries = kHT * 2 * OT * 64, kOwn = (kEntries + kThreads - 1) / kThreads;
+    const __amdgpu_buffer_rsrc_t r2 = rows_rsrc(w2, nout * kHid * 4);
+    f32x8 v[kOwn];
+    if (threadIdx.x < OT * kT) top[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kOwn; ++u) {
+      const int i = u * kThreads + (int)threadIdx.x, l = i & 63, o = (i >> 6) % OT, p = (i >> 6) / OT, n = kT * o + (l & 31);
+      const uint32_t at = n < nout ? (uint32_t)(n * kHid + 16 * p + 4 * (l >> 5)) * 4u : kPast;
+      const f32x4 x0 = load4(r2, at), x1 = load4(r2, at + 32u);
+      v[u] = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[u][j]));
+      if (i < kEntries) atomicMax(&top[n], m);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kOwn; ++u) {
+      const int i = u * kThreads + (int)threadIdx.x, l = i & 63, o = (i >> 6) % OT, p = (i >> 6) / OT;
+      if (i >= kEntries) continue;
+      const Halves x = split(v[u] * pow2_for(top[kT * o + (l & 31)]).p);
+      w2hi[p / 2][p % 2][o][l] = x.hi;
+      w2lo[p / 2][p % 2][o][l] = x.lo;
+    }
+    if (threadIdx.x < OT * kT) {
+      i2s[threadIdx.x] = pow2_for(top[threadIdx.x]).ip;
+      b2s[threadIdx.x] = b2 != nullptr && (int)threadIdx.x < nout ? b2[threadIdx.x] : 0.0f;
+    }
+    if (threadIdx.x < kHid) b1s[threadIdx.x] = b1 != nullptr ? b1[threadIdx.x] : 0.0f;
+  }
+  __syncthreads();
+
+  const int64_t step = (int64_t)gridDim.x * (kThreads / 64);
+  int64_t tile = (int64_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64 * gridDim.x + blockIdx.x));
+  f32x4 zn[KS][2];
+  auto load = [&](int64_t t) {
+    const int64_t r0 = t * kT, nr = t < tiles ? min<int64_t>(kT, rows - r0) : 0;
+    const __amdgpu_buffer_rsrc_t rz = rows_rsrc(z + (nr > 0 ? r0 * nin : 0), nr * nin * 4);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) zn[s][i] = load4(rz, (uint32_t)(c * nin + 16 * s + 8 * h + 4 * i) * 4u);
+    }
+  };
+  load(tile);
+  for (; tile < tiles; tile += step) {
+    asm volatile("" ::: "memory");  // the images stay in LDS: read ahead of the loop they spill
+    const int64_t r0 = tile * kT, nr = min<int64_t>(kT, rows - r0);
+    f32x8 zv[KS];
+    uint32_t zt = 0;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      zv[s] = __builtin_shufflevector(zn[s][0], zn[s][1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (s == KS - 1 && 16 * s + 8 * h + j >= nin) zv[s][j] = 0.0f;  // the next row's
+        zt = max(zt, abs_bits(zv[s][j]));
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load(tile + step);  // in flight until the next tile
+    __builtin_amdgcn_sched_barrier(0);
+    zt = max(zt, (uint32_t)__shfl_xor((int)zt, 32));
+    const RowScale q = row_scale(zt);
+    const __amdgpu_buffer_rsrc_t rc = bytes_rsrc(codes + r0 * ld, nr * ld);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int k = 16 * s + 8 * h;
+      const u32x2 w = {row_codes4(zv[s][0], zv[s][1], zv[s][2], zv[s][3], q),
+                       row_codes4(zv[s][4], zv[s][5], zv[s][6], zv[s][7], q)};
+      if (s < KS - 1) {
+        __builtin_amdgcn_raw_buffer_store_b64(w, rc, (uint32_t)(c * (int)ld + k), 0, 0);
+      } else {
+        __builtin_amdgcn_raw_buffer_store_b32(w[0], rc, k < (int)ld ? (uint32_t)(c * (int)ld + k) : kPast, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b32(w[1], rc, k + 4 < (int)ld ? (uint32_t)(c * (int)ld + k + 4) : kPast, 0, 0);
+      }
+    }
+    if (h == 0 && c < nr) scale[r0 + c] = q.scale;
+    const Pow2 pz = pow2_for(zt);
+    Halves zs[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) zs[s] = split(zv[s] * pz.p);
+    float hv[kHT][16];
+    uint32_t ht = 0;
+#pragma unroll
+    for (int t = 0; t < kHT; ++t) {
+      f32x16 acc = f32x16{};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) acc = mma(Halves{w1hi[s][t][lane], w1lo[s][t][lane]}, zs[s], acc);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int at = kT * t + 8 * g + 4 * h;
+        const f32x4 iv = *reinterpret_cast<const f32x4*>(i1s + at), bv = *reinterpret_cast<const f32x4*>(b1s + at);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float v = relu(acc[4 * g + j] * pz.ip * iv[j] + bv[j]);
+          hv[t][4 * g + j] = v;
+          ht = max(ht, abs_bits(v));
+        }
+      }
+    }
+    ht = max(ht, (uint32_t)__shfl_xor((int)ht, 32));
+    const Pow2 ph = pow2_for(ht);
+    f32x16 out[OT];
+#pragma unroll
+    for (int o = 0; o < OT; ++o) out[o] = f32x16{};
+#pragma unroll
+    for (int t = 0; t < kHT; ++t) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        f32x8 v;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = hv[t][8 * p + j] * ph.p;
+        const Halves hs = split(v);
+#pragma unroll
+        for (int o = 0; o < OT; ++o) out[o] = mma(Halves{w2hi[t][p][o][lane], w2lo[t][p][o][lane]}, hs, out[o]);
+      }
+    }
+    const __amdgpu_buffer_rsrc_t ry = rows_rsrc(y + r0 * nout, nr * nout * 4);
+#pragma unroll
+    for (int o = 0; o < OT; ++o) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int at = kT * o + 8 * g + 4 * h;
+        const f32x4 iv = *reinterpret_cast<const f32x4*>(i2s + at), bv = *reinterpret_cast<const f32x4*>(b2s + at);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[o][4 * g + j] = out[o][4 * g + j] * ph.ip * iv[j] + bv[j];
+      }
+      store_row(ry, nout, kT * o, c, h, out[o]);
+    }
+  }
+}
+
+// ------------------------------------------------- training: input gradient
+
+// dz from codes and dy.  One wave a tile of 32 rows, rows as the columns n:
+// hidden tile by hidden tile, a (for its sign) from the codes and dh = W2^T dy
+// masked by it; then dz^T += W1^T dh^T with W1's image read down its columns.
+// A hidden unit's power of two is taken out of W2's image, so that W1's stands
+// in for W1; the row's own power of two keeps dy and dh in range: |dy| <= 2^15,
+// |W2| <= 2^15 in the image, so |dh| <= 2^30 nout, and `shrink` brings it to
+// 2^15.
+template <int KS, int OS, int kThreads>
+__global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
+    const int8_t* __restrict__ codes, int64_t ld, const float* __restrict__ scale, const float* __restrict__ dy,
+    const float* __restrict__ w1, const float* __restrict__ b1, const float* __restrict__ w2, float* __restrict__ dz,
+    int64_t rows, int nin, int nout, float shrink, int64_t tiles) {
+  constexpr int CT = (KS + 1) / 2;
+  __shared__ f16x8 w1hi[2 * CT][kHT][64], w1lo[2 * CT][kHT][64];
+  __shared__ f16x8 w2hi[OS][kHT][64], w2lo[OS][kHT][64];
+  __shared__ uint32_t top[kHid], top2;
+  __shared__ __attribute__((aligned(16))) float i1s[kHid], nbs[kHid];
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  if (threadIdx.x == 0) top2 = 0;
+  w1_image<2 * CT, kThreads>(w1, nin, w1hi, w1lo, top, i1s);
+  float ip2;
+  {
+    constexpr int kEntries = OS * kHT * 64, kOwn = (kEntries + kThreads - 1) / kThreads;
+    const __amdgpu_buffer_rsrc_t r2 = rows_rsrc(w2, nout * kHid * 4);
+    f32x8 v[kOwn];
+#pragma unroll
+    for (int u = 0; u < kOwn; ++u) {
+      const int i = u * kThreads + (int)threadIdx.x, l = i & 63, t = (i >> 6) % kHT, s = (i >> 6) / kHT;
+      const int k = 16 * s + 8 * (l >> 5), n = kT * t + (l & 31);
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[u][j] = load1(r2, i < kEntries && k + j < nout ? (uint32_t)((k + j) * kHid + n) * 4u : kPast) * i1s[n];
+        m = max(m, abs_bits(v[u][j]));
+      }
+      if (i < kEntries) atomicMax(&top2, m);
+    }
+    __syncthreads();
+    const Pow2 p2 = pow2_for(top2);
+    ip2 = p2.ip / shrink;
+#pragma unroll
+    for (int u = 0; u < kOwn; ++u) {
+      const int i = u * kThreads + (int)threadIdx.x, l = i & 63, t = (i >> 6) % kHT, s = (i >> 6) / kHT;
+      if (i >= kEntries) continue;
+      const Halves x = split(v[u] * p2.p);
+      w2hi[s][t][l] = x.hi;
+      w2lo[s][t][l] = x.lo;
+    }
+    // a > 0 where the scaled product exceeds this
+    if (threadIdx.x < kHid) nbs[threadIdx.x] = b1 != nullptr ? -b1[threadIdx.x] / i1s[threadIdx.x] : 0.0f;
+  }
+  __syncthreads();
+
+  // a column read of W1's image: columns 32 ct + 16 (lane / 16 % 2) + .., hidden
+  // rows 4 h + lane % 16 / 4 from a multiple of 8
+  const int i16 = lane & 15, g2 = (lane >> 4) & 1;
+  const int wcol = (g2 * kHT * 64 + ((i16 >> 1) & 1) * 32 + 4 * h + (i16 >> 2)) * 16 + (i16 & 1) * 8;
+  const int64_t step = (int64_t)gridDim.x * (kThreads / 64);
+  int64_t tile = (int64_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64 * gridDim.x + blockIdx.x));
+  u32x2 cn[KS];
+  f32x4 dn[OS][2];
+  float sn;
+  auto load = [&](int64_t t) {
+    const int64_t r0 = t < tiles ? t * kT : 0, nr = t < tiles ? min<int64_t>(kT, rows - r0) : 0;
+    const __amdgpu_buffer_rsrc_t rc = bytes_rsrc(codes + r0 * ld, nr * ld), rs = rows_rsrc(scale + r0, nr * 4);
+    const __amdgpu_buffer_rsrc_t rd = rows_rsrc(dy + r0 * nout, nr * nout * 4);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) cn[s] = load2(rc, (uint32_t)(c * (int)ld + 16 * s + 8 * h));
+#pragma unroll
+    for (int s = 0; s < OS; ++s) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) dn[s][i] = load4(rd, (uint32_t)(c * nout + 16 * s + 8 * h + 4 * i) * 4u);
+    }
+    sn = load1(rs, (uint32_t)c * 4u);
+  };
+  load(tile);
+  for (; tile < tiles; tile += step) {
+    asm volatile("" ::: "memory");  // the images stay in LDS: read ahead of the loop they spill
+    const int64_t r0 = tile * kT, nr = min<int64_t>(kT, rows - r0);
+    // codes past the row's end meet zeros in W1's image
+    f16x8 cz[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) cz[s] = codes_f16(cn[s]);
+    const float sc = sn;
+    f32x8 dv[OS];
+    uint32_t dt = 0;
+#pragma unroll
+    for (int s = 0; s < OS; ++s) {
+      dv[s] = __builtin_shufflevector(dn[s][0], dn[s][1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (s == OS - 1 && 16 * s + 8 * h + j >= nout) dv[s][j] = 0.0f;
+        dt = max(dt, abs_bits(dv[s][j]));
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load(tile + step);
+    __builtin_amdgcn_sched_barrier(0);
+    dt = max(dt, (uint32_t)__shfl_xor((int)dt, 32));
+    const Pow2 pd = pow2_for(dt);
+    Halves ds[OS];
+#pragma unroll
+    for (int s = 0; s < OS; ++s) ds[s] = split(dv[s] * pd.p);
+    f32x16 out[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) out[ct] = f32x16{};
+#pragma unroll
+    for (int t = 0; t < kHT; ++t) {
+      f32x16 a = f32x16{}, dh = f32x16{};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) a = mma(w1hi[s][t][lane], cz[s], mma(w1lo[s][t][lane], cz[s], a));
+#pragma unroll
+      for (int s = 0; s < OS; ++s) dh = mma(Halves{w2hi[s][t][lane], w2lo[s][t][lane]}, ds[s], dh);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 nb = *reinterpret_cast<const f32x4*>(nbs + kT * t + 8 * g + 4 * h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          // as torch: 0 where relu(a) <= 0, so a NaN lets the upstream pass
+          const float v = dh[4 * g + j] * shrink;
+          dh[4 * g + j] = a[4 * g + j] * sc <= nb[j] ? 0.0f : v;
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        f32x8 v;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = dh[8 * p + j];
+        const Halves hs = split(v);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          const char* ph = reinterpret_cast<const char*>(&w1hi[2 * ct][t][0]) + wcol + 16 * 16 * p;
+          const char* pl = reinterpret_cast<const char*>(&w1lo[2 * ct][t][0]) + wcol + 16 * 16 * p;
+          const Halves w = {__builtin_bit_cast(f16x8, join(read_column(ph), read_column(ph + 8 * 16))),
+                            __builtin_bit_cast(f16x8, join(read_column(pl), read_column(pl + 8 * 16)))};
+          out[ct] = mma(w, hs, out[ct]);
+        }
+      }
+    }
+    const __amdgpu_buffer_rsrc_t rz = rows_rsrc(dz + r0 * nin, nr * nin * 4);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) out[ct][r] = out[ct][r] * pd.ip * ip2;
+      store_row(rz, nin, kT * ct, c, h, out[ct]);
+    }
+  }
+}
+
+// ------------------------------------------------ training: weight gradients
+
+constexpr int kGradThreads = 256;
+constexpr int weight_grad8_waves(int ks, int os) { return ks > 7 || os > 2 ? 1 : 2; }
+
+// Workgroup = one chunk of rows, wave t the hidden units 32 t .. 32 t + 31 with
+// their weights' pieces in registers.  A row tile's codes (as bfloat16) and
+// dy's pieces stand in LDS by rows: read along rows they are the operands of a
+// = z W1^T and dh = dy W2, read down columns those of dW1 = (dh s)^T codes and
+// dW2 = dy^T relu(a), whose other operands come in a's and dh's result layout.
+// The next tile is loaded under this one's products.  The chunk's partial sums:
+// dW1 (128 x nin), db1 (128), dW2 (nout x 128), db2 (nout).
+template <int KS, int OS>
+__global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_mlp_weight_grad8(
+    const int8_t* __restrict__ codes, int64_t ld, const float* __restrict__ scale, const float* __restrict__ dy,
+    const float* __restrict__ w1, const float* __restrict__ b1, const float* __restrict__ w2,
+    float* __restrict__ part, int64_t rows, int nin, int nout, int64_t chunk_rows) {
+  constexpr int CT = (KS + 1) / 2, OT = (OS + 1) / 2;
+  constexpr int kZ = CT * kT + 8, kD = OT * kT + 8;      // 16-bit values a row of LDS
+  constexpr int kZG = CT * 8, kDG = OT * 8;              // groups of 4 columns a row
+  constexpr int kLZ = kT * kZG / kGradThreads, kLD = kT * kDG / kGradThreads;
+  __shared__ __attribute__((aligned(16))) __bf16 zs[2][kT][kZ], ds[2][3][kT][kD];
+  __shared__ __attribute__((aligned(16))) float ss[2][kT];
+  __shared__ f32x4 sums[kGradThreads];
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  const int band = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64) * kT;
+  const int64_t r0 = (int64_t)blockIdx.x * chunk_rows, nr = min<int64_t>(chunk_rows, rows - r0);
+
+  Thirds w1v[KS], w2v[OS];  // W1[band + c][16 s + 8 h ..], W2[16 s + 8 h + j][band + c]
+  {
+    const __amdgpu_buffer_rsrc_t rw1 = rows_rsrc(w1, kHid * nin * 4), rw2 = rows_rsrc(w2, nout * kHid * 4);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) w1v[s] = split3(load8(rw1, band + c, nin, 16 * s + 8 * h));
+#pragma unroll
+    for (int s = 0; s < OS; ++s) {
+      f32x8 v;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int k = 16 * s + 8 * h + j;
+        v[j] = load1(rw2, k < nout ? (uint32_t)(k * kHid + band + c) * 4u : kPast);
+      }
+      w2v[s] = split3(v);
+    }
+  }
+  const float bias = b1 != nullptr ? b1[band + c] : 0.0f;
+  f32x16 acc1[CT], acc2[OT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) acc1[ct] = f32x16{};
+#pragma unroll
+  for (int o = 0; o < OT; ++o) acc2[o] = f32x16{};
+  float sb1 = 0.0f;
+  f32x4 sb2[kLD];
+#pragma unroll
+  for (int u = 0; u < kLD; ++u) sb2[u] = f32x4{};
+
+  // rows past the chunk load zeros: dy's add nothing
+  uint32_t zst[kLZ];
+  f32x4 dst[kLD];
+  float sst;
+  auto load = [&](int64_t t0) {
+    const int64_t left = t0 < nr ? nr - t0 : 0, at = left > 0 ? r0 + t0 : 0;
+    const __amdgpu_buffer_rsrc_t rz = bytes_rsrc(codes + at * ld, min<int64_t>(left, kT) * ld);
+    const __amdgpu_buffer_rsrc_t rs = rows_rsrc(scale + at, min<int64_t>(left, kT) * 4);
+    const __amdgpu_buffer_rsrc_t rd = rows_rsrc(dy + at * nout, min<int64_t>(left, kT) * nout * 4);
+#pragma unroll
+    for (int u = 0; u < kLZ; ++u) {
+      const int i = u * kGradThreads + (int)threadIdx.x, row = i / kZG, k = 4 * (i % kZG);
+      zst[u] = __builtin_amdgcn_raw_buffer_load_b32(rz, k < (int)ld ? (uint32_t)(row * (int)ld + k) : kPast, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < kLD; ++u) {
+      const int i = u * kGradThreads + (int)threadIdx.x, row = i / kDG, k = 4 * (i % kDG);
+      dst[u] = load4(rd, k < nout ? (uint32_t)(row * nout + k) * 4u : kPast);
+    }
+    sst = load1(rs, threadIdx.x < kT ? threadIdx.x * 4u : kPast);
+  };
+  // column reads of a tile's rows: lane i of 16 gives row 4 h + i / 4 and columns 16 (lane / 16 % 2) + 4 (i % 4)
+  const int i16 = lane & 15, rrow = 4 * h + (i16 >> 2), rcol = 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+  load(0);
+  int buf = 0;
+  for (int64_t t0 = 0; t0 < nr; t0 += kT, buf ^= 1) {
+#pragma unroll
+    for (int u = 0; u < kLZ; ++u) {
+      const int i = u * kGradThreads + (int)threadIdx.x;
+      *reinterpret_cast<bf16x4*>(&zs[buf][i / kZG][4 * (i % kZG)]) = codes_bf16(zst[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kLD; ++u) {
+      const int i = u * kGradThreads + (int)threadIdx.x, row = i / kDG, k = 4 * (i % kDG);
+      f32x4 v = dst[u];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (k + j >= nout) v[j] = 0.0f;  // the next row's
+      sb2[u] += v;
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        const bf16x4 x = __builtin_convertvector(v, bf16x4);
+        *reinterpret_cast<bf16x4*>(&ds[buf][p][row][k]) = x;
+        if (p < 2) v -= __builtin_convertvector(x, f32x4);
+      }
+    }
+    if (threadIdx.x < kT) ss[buf][threadIdx.x] = sst;
+    // one barrier a tile: a wave writes a buffer again only after the next
+    // barrier, which every wave reaches after its reads of this one
+    __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+    load(t0 + kT);
+    __builtin_amdgcn_sched_barrier(0);
+    f32x16 a = f32x16{}, dh = f32x16{};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const bf16x8 z8 = *reinterpret_cast<const bf16x8*>(&zs[buf][c][16 * s + 8 * h]);
+      a = mma(z8, w1v[s].v[0], mma(z8, w1v[s].v[1], mma(z8, w1v[s].v[2], a)));
+    }
+#pragma unroll
+    for (int s = 0; s < OS; ++s) {
+      Thirds d;
+#pragma unroll
+      for (int p = 0; p < 3; ++p) d.v[p] = *reinterpret_cast<const bf16x8*>(&ds[buf][p][c][16 * s + 8 * h]);
+      dh = mma(d, w2v[s], dh);
+    }
+    f32x8 hv[2], gv[2];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 sv = *reinterpret_cast<const f32x4*>(&ss[buf][8 * g + 4 * h]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float av = a[4 * g + j] * sv[j] + bias;
+        const float d = av <= 0.0f ? 0.0f : dh[4 * g + j];
+        sb1 += d;
+        hv[g / 2][4 * (g % 2) + j] = relu(av);
+        gv[g / 2][4 * (g % 2) + j] = d * sv[j];
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const Thirds hs = split3(hv[p]), gs = split3(gv[p]);
+#pragma unroll
+      for (int o = 0; o < OT; ++o) {
+        Thirds d;
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+          d.v[q] = __builtin_bit_cast(bf16x8, join(read_column(&ds[buf][q][16 * p + rrow][kT * o + rcol]),
+                                                   read_column(&ds[buf][q][16 * p + 8 + rrow][kT * o + rcol])));
+        acc2[o] = mma(d, hs, acc2[o]);
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const bf16x8 z8 = __builtin_bit_cast(bf16x8, join(read_column(&zs[buf][16 * p + rrow][kT * ct + rcol]),
+                                                          read_column(&zs[buf][16 * p + 8 + rrow][kT * ct + rcol])));
+        acc1[ct] = mma(gs.v[0], z8, mma(gs.v[1], z8, mma(gs.v[2], z8, acc1[ct])));
+      }
+    }
+  }
+
+  const int64_t n1 = (int64_t)kHid * nin, n2 = (int64_t)nout * kHid;
+  float* __restrict__ p = part + (int64_t)blockIdx.x * (n1 + kHid + n2 + nout);
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int col = kT * ct + c;
+    if (col < nin) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) p[(int64_t)(band + 8 * (r / 4) + 4 * h + r % 4) * nin + col] = acc1[ct][r];
+    }
+  }
+  sb1 += __shfl_xor(sb1, 32);
+  if (h == 0) p[n1 + band + c] = sb1;
+#pragma unroll
+  for (int o = 0; o < OT; ++o) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int m = kT * o + 8 * (r / 4) + 4 * h + r % 4;
+      if (m < nout) p[n1 + kHid + (int64_t)m * kHid + band + c] = acc2[o][r];
+    }
+  }
+  // db2: thread i has summed rows i / kDG (and, with several pieces a thread,
+  // that many more rows) of columns 4 (i % kDG) ..
+#pragma unroll
+  for (int u = 1; u < kLD; ++u) sb2[0] += sb2[u];
+  sums[threadIdx.x] = sb2[0];
+  __syncthreads();
+  if ((int)threadIdx.x < nout) {
+    float t = 0.0f;
+    for (int i = 0; i < kGradThreads / kDG; ++i) t += sums[i * kDG + threadIdx.x / 4][threadIdx.x % 4];
+    p[n1 + kHid + n2 + threadIdx.x] = t;
+  }
+}
+
+// A chunk for every workgroup the chip holds at once, at least two row tiles
+// and at most kMaxChunkRows.
+int64_t grad8_chunk_rows(int64_t rows, int nin, int nout) {
+  const int64_t want = 256 * weight_grad8_waves((nin + 15) / 16, (nout + 15) / 16);
+  const int64_t c = (rows + want - 1) / want;
+  return std::min<int64_t>(kMaxChunkRows, std::max<int64_t>(64, (c + kT - 1) / kT * kT));
+}
+int64_t grad8_chunks(int64_t rows, int nin, int nout) {
+  const int64_t c = grad8_chunk_rows(rows, nin, nout);
+  return rows > 0 ? (rows + c - 1) / c : 0;
+}
+
+constexpr int kMaxKS = (kMaxMlpIn + 15) / 16, kMaxOS = kMaxMlpOut / 16;
+
+// Workgroups of the row tile kernels: one a CU, a row tile for each where there
+// are fewer than the waves.
+inline dim3 spread_grid(int64_t tiles) { return dim3((uint32_t)std::min<int64_t>(256, tiles)); }
+
+}  // namespace
+
+void run_mlp_rows8_forward(const float* z, const float* w1, const float* b1, const float* w2, const float* b2,
+                           int8_t* codes, int64_t ld, float* scale, float* y, int64_t rows, int nin, int nout,
+                           hipStream_t st) {
+  if (rows == 0) return;
+  const int64_t tiles = (rows + kT - 1) / kT;
+  with_groups<kMaxKS>((nin + 15) / 16, [&](auto ks) {
+    with_groups<2>(nout <= kT ? 1 : 2, [&](auto ot) {
+      constexpr int KS = decltype(ks)::value, T = KS > 7 ? 256 : 512;
+      hipLaunchKernelGGL((k_mlp_forward8<KS, decltype(ot)::value, T>), spread_grid(tiles), dim3(T), 0, st, z, w1, b1,
+                         w2, b2, codes, ld, scale, y, rows, nin, nout, tiles);
+    });
+  });
+  SPHOPS_LAUNCHED();
+}
+
 int64_t mlp_rows8_floats(int64_t rows, int nin, int nout) {
-  return rows * (nin + kHid + nout) + mlp_weight_grad_floats(rows, nin, nout);
+  return grad8_chunks(rows, nin, nout) * ((int64_t)kHid * nin + kHid + (int64_t)nout * kHid + nout);
 }
 
 void run_mlp_rows8_backward(const int8_t* codes, int64_t ld, const float* scale, const float* dy, const float* w1,
                             const float* b1, const float* w2, float* dz, float* dw1, float* db1, float* dw2,
                             float* db2, int64_t rows, int nin, int nout, float* work, hipStream_t st) {
-  float *zr = work, *a = zr + rows * nin, *y = a + rows * kHid, *part = y + rows * nout;
-  run_restore_rows(codes, ld, scale, zr, SPHOPS_F32, rows, nin, st);
-  run_mlp_forward(zr, w1, b1, w2, nullptr, a, y, rows, nin, nout, st);
-  if (dz != nullptr) run_mlp_input_grad(dy, w1, w2, a, dz, rows, nin, nout, st);
-  if (dw1 != nullptr || db1 != nullptr || dw2 != nullptr || db2 != nullptr)
-    run_mlp_weight_grad(zr, a, dy, w2, dw1, db1, dw2, db2, rows, nin, nout, part, st);
+  const int64_t tiles = (rows + kT - 1) / kT;
+  if (dz != nullptr && rows > 0) {
+    float shrink = 0x1p-15f;
+    for (int n = 1; n < nout; n *= 2) shrink *= 0.5f;
+    with_groups<kMaxKS>((nin + 15) / 16, [&](auto ks) {
+      with_groups<kMaxOS>((nout + 15) / 16, [&](auto os) {
+        constexpr int KS = decltype(ks)::value, T = KS > 7 ? 256 : 512;
+        hipLaunchKernelGGL((k_mlp_input_grad8<KS, decltype(os)::value, T>), spread_grid(tiles), dim3(T), 0, st,
+                           codes, ld, scale, dy, w1, b1, w2, dz, rows, nin, nout, shrink, tiles);
+      });
+    });
+    SPHOPS_LAUNCHED();
+  }
+  if (dw1 == nullptr && db1 == nullptr && dw2 == nullptr && db2 == nullptr) return;
+  const int64_t chunks = grad8_chunks(rows, nin, nout);
+  if (chunks > 0) {
+    with_groups<kMaxKS>((nin + 15) / 16, [&](auto ks) {
+      with_groups<kMaxOS>((nout + 15) / 16, [&](auto os) {
+        hipLaunchKernelGGL((k_mlp_weight_grad8<decltype(ks)::value, decltype(os)::value>), dim3((uint32_t)chunks),
+                           dim3(kGradThreads), 0, st, codes, ld, scale, dy, w1, b1, w2, work, rows, nin, nout,
+                           grad8_chunk_rows(rows, nin, nout));
+      });
+    });
+    SPHOPS_LAUNCHED();
+  }
+  run_mlp_chunk_sum(work, dw1, db1, dw2, db2, nin, nout, chunks, st);
 }
 
 }  // namespace sphops

@@ -549,8 +549,13 @@ void run_mlp_weight_grad(const float* z, const float* a, const float* dy, const 
     });
     SPHOPS_LAUNCHED();
   }
+  run_mlp_chunk_sum(work, dw1, db1, dw2, db2, nin, nout, chunks, st);
+}
+
+void run_mlp_chunk_sum(const float* part, float* dw1, float* db1, float* dw2, float* db2, int nin, int nout,
+                       int64_t chunks, hipStream_t st) {
   const int n1 = kHid * nin, n2 = nout * kHid, n = n1 + kHid + n2 + nout;
-  hipLaunchKernelGGL(k_mlp_chunk_sum, dim3((uint32_t)((n + 63) / 64)), dim3(64 * kSumWaves), 0, st, work, dw1, db1,
+  hipLaunchKernelGGL(k_mlp_chunk_sum, dim3((uint32_t)((n + 63) / 64)), dim3(64 * kSumWaves), 0, st, part, dw1, db1,
                      dw2, db2, n1, n2, n, chunks);
   SPHOPS_LAUNCHED();
 }

@@ -367,6 +367,9 @@ void run_mlp_input_grad(const float* dy, const float* w1, const float* w2, const
                         int nin, int nout, hipStream_t st);
 void run_mlp_weight_grad(const float* z, const float* a, const float* dy, const float* w2, float* dw1, float* db1,
                          float* dw2, float* db2, int64_t rows, int nin, int nout, float* work, hipStream_t st);
+// dW1, db1, dW2 and db2 from the chunks' partial sums, in a fixed order
+void run_mlp_chunk_sum(const float* part, float* dw1, float* db1, float* dw2, float* db2, int nin, int nout,
+                       int64_t chunks, hipStream_t st);
 
 // rows8.hip: rows of up to kMaxRows8Cols values in 8 bits, a scale a row
 constexpr int64_t kMaxRows8Cols = 65536;  // the integer sums of a product stay below 2^31
@@ -386,6 +389,9 @@ void run_linear8(const void* x, int type, int64_t stride, const int8_t* wq, int6
 void run_mlp8(const float* z, const int8_t* w1, int64_t ld1, const float* s1, const float* b1, const int8_t* w2,
               int64_t ld2, const float* s2, const float* b2, float* y, int64_t rows, int nin, int nout,
               hipStream_t st);
+void run_mlp_rows8_forward(const float* z, const float* w1, const float* b1, const float* w2, const float* b2,
+                           int8_t* codes, int64_t ld, float* scale, float* y, int64_t rows, int nin, int nout,
+                           hipStream_t st);
 int64_t mlp_rows8_floats(int64_t rows, int nin, int nout);
 void run_mlp_rows8_backward(const int8_t* codes, int64_t ld, const float* scale, const float* dy, const float* w1,
                             const float* b1, const float* w2, float* dz, float* dw1, float* db1, float* dw2,

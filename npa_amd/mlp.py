@@ -274,13 +274,14 @@ class MlpRows8(torch.autograd.Function):
         out_f = w2.shape[0]
         z2 = z.reshape(-1, in_f).contiguous()
         rows = z2.shape[0]
-        kept = int8.quantize_rows(z2)
         dense = [None if t is None else t.detach().contiguous() for t in (w1, b1, w2, b2)]
         ctx.shape, ctx.has_b2 = (rows, in_f, hidden, out_f), b2 is not None
+        codes = torch.empty(rows, -(-in_f // 4) * 4, dtype=torch.int8, device=z.device)
+        scale = torch.empty(rows, device=z.device)
         y = torch.empty(rows, out_f, device=z.device)
-        _native.check(_lib.sphops_mlp_forward(_ptr(z2), *(_ptr(t) for t in dense), _ptr(None), _ptr(y), rows, in_f,
-                                              hidden, out_f, _stream(z)))
-        ctx.save_for_backward(kept.codes, kept.scale, w1, b1, w2)
+        _native.check(_lib.sphops_mlp_rows8_forward(_ptr(z2), *(_ptr(t) for t in dense), _ptr(codes), codes.shape[1],
+                                                    _ptr(scale), _ptr(y), rows, in_f, hidden, out_f, _stream(z)))
+        ctx.save_for_backward(codes, scale, w1, b1, w2)
         return y.reshape(*z.shape[:-1], out_f)
 
     @staticmethod

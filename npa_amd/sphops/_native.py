@@ -87,6 +87,7 @@ _SIGNATURES = {
     "sphops_linear8": ([_p, _i32, _i64, _p, _i64, _p, _p, _p, _i64, _i32, _i32, _p, _p], _i32),
     "sphops_linear8_workspace_bytes": ([_i64, _i32, _i32], _i64),
     "sphops_mlp8_forward": ([_p, _p, _i64, _p, _p, _p, _i64, _p, _p, _p, _i64, _i32, _i32, _i32, _p], _i32),
+    "sphops_mlp_rows8_forward": ([_p, _p, _p, _p, _p, _p, _i64, _p, _p, _i64, _i32, _i32, _i32, _p], _i32),
     "sphops_mlp_rows8_backward": ([_p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _p, _p],
                                   _i32),
     "sphops_mlp_rows8_workspace_bytes": ([_i64, _i32, _i32, _i32], _i64),
