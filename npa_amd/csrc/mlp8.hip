@@ -209,7 +209,10 @@ struct Halves {
 __device__ __forceinline__ Halves split(f32x8 v) {
   Halves r;
   r.hi = __builtin_convertvector(v, f16x8);
-  r.lo = __builtin_convertvector(v - __builtin_convertvector(r.hi, f32x8), f16x8);
+  f32x8 rest;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) rest[j] = __builtin_fmaf((float)r.hi[j], -1.0f, v[j]);  // one mixed-precision instruction
+  r.lo = __builtin_convertvector(rest, f16x8);
   return r;
 }
 // + a b for factors in halves, the small products first
@@ -220,12 +223,28 @@ __device__ __forceinline__ f32x16 mma(const Halves& a, const Halves& b, f32x16 c
 struct Thirds {
   bf16x8 v[3];
 };
+// Two values at a time: a pair's pieces back in float32 are its word's halves.
+__device__ __forceinline__ uint32_t bf16_pair(float& a, float& b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+  a -= __builtin_bit_cast(float, w << 16);
+  b -= __builtin_bit_cast(float, w & 0xffff0000u);
+  return w;
+}
 __device__ __forceinline__ Thirds split3(f32x8 v) {
   Thirds r;
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
-    r.v[i] = __builtin_convertvector(v, bf16x8);
-    if (i < 2) v -= __builtin_convertvector(r.v[i], f32x8);
+    u32x4 w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float x = v[2 * j], y = v[2 * j + 1];
+      w[j] = bf16_pair(x, y);
+      v[2 * j] = x;
+      v[2 * j + 1] = y;
+    }
+    r.v[i] = __builtin_bit_cast(bf16x8, w);
   }
   return r;
 }
@@ -279,16 +298,26 @@ __device__ __forceinline__ f32x8 load8(__amdgpu_buffer_rsrc_t r, int row, int n,
   return v;
 }
 
-// W1 in halves as an operand image: lane l of entry (s, t) holds W1[32 t + l %
-// 32][16 s + 8 (l / 32) .. + 7] times the hidden unit's own power of two, whose
-// inverse is left in inv.  All threads; ends with a barrier.  `top` is scratch.
+// W1 in halves as an operand image: lane l's 16 bytes of entry (s, t), at
+// image_lane(s, l), are W1[32 t + l % 32][16 s + 8 (l / 32) .. + 7] times the
+// hidden unit's own power of two, whose inverse is left in inv.  The scale
+// covers 2^-16 of the bias too, so that a bias over it stays in range where
+// W1's row is small or zero.  All threads; ends with a barrier.  `top` is
+// scratch.
+//
+// image_lane exchanges hidden rows so that the 32 lanes of half a column read
+// (read_column: 4 rows by 32 columns, 8 bytes a lane) lie in different banks;
+// as the rows stand, four of them meet in each.
+__device__ __forceinline__ int image_lane(int s, int l) { return l ^ ((l >> 5) << 3) ^ ((s & 1) << 2); }
+
 template <int KS, int kThreads>
-__device__ __forceinline__ void w1_image(const float* __restrict__ w1, int nin, f16x8 (&hi)[KS][kHT][64],
-                                         f16x8 (&lo)[KS][kHT][64], uint32_t (&top)[kHid], float (&inv)[kHid]) {
+__device__ __forceinline__ void w1_image(const float* __restrict__ w1, const float* __restrict__ b1, int nin,
+                                         f16x8 (&hi)[KS][kHT][64], f16x8 (&lo)[KS][kHT][64], uint32_t (&top)[kHid],
+                                         float (&inv)[kHid]) {
   constexpr int kEntries = KS * kHT * 64, kOwn = (kEntries + kThreads - 1) / kThreads;
   const __amdgpu_buffer_rsrc_t r = rows_rsrc(w1, kHid * nin * 4);
   f32x8 v[kOwn];
-  if (threadIdx.x < kHid) top[threadIdx.x] = 0;
+  if (threadIdx.x < kHid) top[threadIdx.x] = b1 != nullptr ? abs_bits(b1[threadIdx.x] * 0x1p-16f) : 0u;
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < kOwn; ++u) {
@@ -310,8 +339,8 @@ __device__ __forceinline__ void w1_image(const float* __restrict__ w1, int nin, 
     const int i = u * kThreads + (int)threadIdx.x, l = i & 63, t = (i >> 6) % kHT, s = (i >> 6) / kHT;
     if (i >= kEntries) continue;
     const Halves h = split(v[u] * pow2_for(top[kT * t + (l & 31)]).p);
-    hi[s][t][l] = h.hi;
-    lo[s][t][l] = h.lo;
+    hi[s][t][image_lane(s, l)] = h.hi;
+    lo[s][t][image_lane(s, l)] = h.lo;
   }
   if (threadIdx.x < kHid) inv[threadIdx.x] = pow2_for(top[threadIdx.x]).ip;
   __syncthreads();
@@ -321,7 +350,8 @@ __device__ __forceinline__ void w1_image(const float* __restrict__ w1, int nin, 
 
 // y = relu(z W1^T + b1) W2^T + b2 and z in 8 bits.  One wave a tile of 32 rows
 // (rows as the columns n): z's row and then the hidden row are scaled by their
-// own powers of two and split.  The hidden tile's result registers 8 j .. 8 j +
+// own powers of two and split.  A hidden unit's power of two stays in its hidden
+// value (relu(p a) = p relu(a)) and is taken out of W2's image.  The hidden tile's result registers 8 j .. 8 j +
 // 7 of lane l are hidden units 16 j + 4 (l / 32) + 0..3 and 8 more of its row:
 // as they stand they are an operand with W2's image in the same order.
 template <int KS, int OT, int kThreads>
@@ -334,7 +364,8 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
   __shared__ uint32_t top[kHid];
   __shared__ __attribute__((aligned(16))) float i1s[kHid], b1s[kHid], i2s[OT * kT], b2s[OT * kT];
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
-  w1_image<KS, kThreads>(w1, nin, w1hi, w1lo, top, i1s);
+  const int lane0 = image_lane(0, lane), lane1 = image_lane(1, lane);
+  w1_image<KS, kThreads>(w1, b1, nin, w1hi, w1lo, top, i1s);
   {
     constexpr int kEntries = kHT * 2 * OT * 64, kOwn = (kEntries + kThreads - 1) / kThreads;
     const __amdgpu_buffer_rsrc_t r2 = rows_rsrc(w2, nout * kHid * 4);
@@ -346,7 +377,9 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
       const int i = u * kThreads + (int)threadIdx.x, l = i & 63, o = (i >> 6) % OT, p = (i >> 6) / OT, n = kT * o + (l & 31);
       const uint32_t at = n < nout ? (uint32_t)(n * kHid + 16 * p + 4 * (l >> 5)) * 4u : kPast;
       const f32x4 x0 = load4(r2, at), x1 = load4(r2, at + 32u);
-      v[u] = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+      const f32x4 q0 = *reinterpret_cast<const f32x4*>(i1s + 16 * p + 4 * (l >> 5));
+      const f32x4 q1 = *reinterpret_cast<const f32x4*>(i1s + 16 * p + 4 * (l >> 5) + 8);
+      v[u] = __builtin_shufflevector(x0 * q0, x1 * q1, 0, 1, 2, 3, 4, 5, 6, 7);
       uint32_t m = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[u][j]));
@@ -365,7 +398,7 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
       i2s[threadIdx.x] = pow2_for(top[threadIdx.x]).ip;
       b2s[threadIdx.x] = b2 != nullptr && (int)threadIdx.x < nout ? b2[threadIdx.x] : 0.0f;
     }
-    if (threadIdx.x < kHid) b1s[threadIdx.x] = b1 != nullptr ? b1[threadIdx.x] : 0.0f;
+    if (threadIdx.x < kHid) b1s[threadIdx.x] = b1 != nullptr ? b1[threadIdx.x] / i1s[threadIdx.x] : 0.0f;
   }
   __syncthreads();
 
@@ -425,20 +458,22 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
     for (int t = 0; t < kHT; ++t) {
       f32x16 acc = f32x16{};
 #pragma unroll
-      for (int s = 0; s < KS; ++s) acc = mma(Halves{w1hi[s][t][lane], w1lo[s][t][lane]}, zs[s], acc);
+      for (int s = 0; s < KS; ++s) {
+        const int l = s % 2 == 0 ? lane0 : lane1;
+        acc = mma(Halves{w1hi[s][t][l], w1lo[s][t][l]}, zs[s], acc);
+      }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int at = kT * t + 8 * g + 4 * h;
-        const f32x4 iv = *reinterpret_cast<const f32x4*>(i1s + at), bv = *reinterpret_cast<const f32x4*>(b1s + at);
+        const f32x4 bv = *reinterpret_cast<const f32x4*>(b1s + kT * t + 8 * g + 4 * h);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float v = relu(acc[4 * g + j] * pz.ip * iv[j] + bv[j]);
+          const float v = relu(acc[4 * g + j] * pz.ip + bv[j]);
           hv[t][4 * g + j] = v;
-          ht = max(ht, abs_bits(v));
+          ht = max(ht, __builtin_bit_cast(uint32_t, v));  // no value below zero; a NaN of either sign is above all
         }
       }
     }
-    ht = max(ht, (uint32_t)__shfl_xor((int)ht, 32));
+    ht = max(ht, (uint32_t)__shfl_xor((int)ht, 32)) & 0x7fffffffu;
     const Pow2 ph = pow2_for(ht);
     f32x16 out[OT];
 #pragma unroll
@@ -477,13 +512,13 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
 // masked by it; then dz^T += W1^T dh^T with W1's image read down its columns.
 // A hidden unit's power of two is taken out of W2's image, so that W1's stands
 // in for W1; the row's own power of two keeps dy and dh in range: |dy| <= 2^15,
-// |W2| <= 2^15 in the image, so |dh| <= 2^30 nout, and `shrink` brings it to
+// |W2| <= 2^15 in the image, so |dh| <= 2^30 nout, and 2^-drop brings it to
 // 2^15.
 template <int KS, int OS, int kThreads>
 __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
     const int8_t* __restrict__ codes, int64_t ld, const float* __restrict__ scale, const float* __restrict__ dy,
     const float* __restrict__ w1, const float* __restrict__ b1, const float* __restrict__ w2, float* __restrict__ dz,
-    int64_t rows, int nin, int nout, float shrink, int64_t tiles) {
+    int64_t rows, int nin, int nout, int drop, int64_t tiles) {
   constexpr int CT = (KS + 1) / 2;
   __shared__ f16x8 w1hi[2 * CT][kHT][64], w1lo[2 * CT][kHT][64];
   __shared__ f16x8 w2hi[OS][kHT][64], w2lo[OS][kHT][64];
@@ -491,8 +526,8 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
   __shared__ __attribute__((aligned(16))) float i1s[kHid], nbs[kHid];
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   if (threadIdx.x == 0) top2 = 0;
-  w1_image<2 * CT, kThreads>(w1, nin, w1hi, w1lo, top, i1s);
-  float ip2;
+  w1_image<2 * CT, kThreads>(w1, b1, nin, w1hi, w1lo, top, i1s);
+  int e2;
   {
     constexpr int kEntries = OS * kHT * 64, kOwn = (kEntries + kThreads - 1) / kThreads;
     const __amdgpu_buffer_rsrc_t r2 = rows_rsrc(w2, nout * kHid * 4);
@@ -511,7 +546,7 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
     }
     __syncthreads();
     const Pow2 p2 = pow2_for(top2);
-    ip2 = p2.ip / shrink;
+    e2 = (int)(__builtin_bit_cast(uint32_t, p2.ip) >> 23) - 127 + drop;
 #pragma unroll
     for (int u = 0; u < kOwn; ++u) {
       const int i = u * kThreads + (int)threadIdx.x, l = i & 63, t = (i >> 6) % kHT, s = (i >> 6) / kHT;
@@ -528,7 +563,11 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
   // a column read of W1's image: columns 32 ct + 16 (lane / 16 % 2) + .., hidden
   // rows 4 h + lane % 16 / 4 from a multiple of 8
   const int i16 = lane & 15, g2 = (lane >> 4) & 1;
-  const int wcol = (g2 * kHT * 64 + ((i16 >> 1) & 1) * 32 + 4 * h + (i16 >> 2)) * 16 + (i16 & 1) * 8;
+  const int half = (i16 >> 1) & 1, wrow = (4 * h + (i16 >> 2)) ^ (4 * g2);
+  const int wcol = (g2 * kHT * 64 + half * 32 + wrow) * 16 + (i16 & 1) * 8;
+  const int wcol0 = wcol + 8 * 16 * half, wcol1 = wcol + 8 * 16 * (1 - half);  // the first and second eight rows
+  const int lane0 = image_lane(0, lane), lane1 = image_lane(1, lane);
+  const float shrink = __builtin_bit_cast(float, (uint32_t)(127 - drop) << 23);
   const int64_t step = (int64_t)gridDim.x * (kThreads / 64);
   int64_t tile = (int64_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64 * gridDim.x + blockIdx.x));
   u32x2 cn[KS];
@@ -582,7 +621,10 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
     for (int t = 0; t < kHT; ++t) {
       f32x16 a = f32x16{}, dh = f32x16{};
 #pragma unroll
-      for (int s = 0; s < KS; ++s) a = mma(w1hi[s][t][lane], cz[s], mma(w1lo[s][t][lane], cz[s], a));
+      for (int s = 0; s < KS; ++s) {
+        const int l = s % 2 == 0 ? lane0 : lane1;
+        a = mma(w1hi[s][t][l], cz[s], mma(w1lo[s][t][l], cz[s], a));
+      }
 #pragma unroll
       for (int s = 0; s < OS; ++s) dh = mma(Halves{w2hi[s][t][lane], w2lo[s][t][lane]}, ds[s], dh);
 #pragma unroll
@@ -603,19 +645,20 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
         const Halves hs = split(v);
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-          const char* ph = reinterpret_cast<const char*>(&w1hi[2 * ct][t][0]) + wcol + 16 * 16 * p;
-          const char* pl = reinterpret_cast<const char*>(&w1lo[2 * ct][t][0]) + wcol + 16 * 16 * p;
-          const Halves w = {__builtin_bit_cast(f16x8, join(read_column(ph), read_column(ph + 8 * 16))),
-                            __builtin_bit_cast(f16x8, join(read_column(pl), read_column(pl + 8 * 16)))};
+          const char* ph = reinterpret_cast<const char*>(&w1hi[2 * ct][t][16 * p]);
+          const char* pl = reinterpret_cast<const char*>(&w1lo[2 * ct][t][16 * p]);
+          const Halves w = {__builtin_bit_cast(f16x8, join(read_column(ph + wcol0), read_column(ph + wcol1))),
+                            __builtin_bit_cast(f16x8, join(read_column(pl + wcol0), read_column(pl + wcol1)))};
           out[ct] = mma(w, hs, out[ct]);
         }
       }
     }
     const __amdgpu_buffer_rsrc_t rz = rows_rsrc(dz + r0 * nin, nr * nin * 4);
+    const int e = (int)(__builtin_bit_cast(uint32_t, pd.ip) >> 23) - 127 + e2;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) out[ct][r] = out[ct][r] * pd.ip * ip2;
+      for (int r = 0; r < 16; ++r) out[ct][r] = __builtin_ldexpf(out[ct][r], e);
       store_row(rz, nin, kT * ct, c, h, out[ct]);
     }
   }
@@ -624,7 +667,7 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
 // ------------------------------------------------ training: weight gradients
 
 constexpr int kGradThreads = 256;
-constexpr int weight_grad8_waves(int ks, int os) { return ks > 7 || os > 2 ? 1 : 2; }
+constexpr int weight_grad8_waves(int ks, int os) { return ks > 6 || os > 2 ? 1 : 2; }
 
 // Workgroup = one chunk of rows, wave t the hidden units 32 t .. 32 t + 31 with
 // their weights' pieces in registers.  A row tile's codes (as bfloat16) and
@@ -639,17 +682,22 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
     const float* __restrict__ w1, const float* __restrict__ b1, const float* __restrict__ w2,
     float* __restrict__ part, int64_t rows, int nin, int nout, int64_t chunk_rows) {
   constexpr int CT = (KS + 1) / 2, OT = (OS + 1) / 2;
-  constexpr int kZ = CT * kT + 8, kD = OT * kT + 8;      // 16-bit values a row of LDS
+  // 16-bit values a row of LDS: an odd number of 64 bytes, and each 16 bytes of
+  // rows 4 to 7 of eight exchanged with its neighbour (at), so that neither the
+  // reads along rows nor those down columns meet in a bank
+  constexpr int kZ = (CT | 1) * kT, kD = (OT | 1) * kT;
   constexpr int kZG = CT * 8, kDG = OT * 8;              // groups of 4 columns a row
   constexpr int kLZ = kT * kZG / kGradThreads, kLD = kT * kDG / kGradThreads;
   __shared__ __attribute__((aligned(16))) __bf16 zs[2][kT][kZ], ds[2][3][kT][kD];
   __shared__ __attribute__((aligned(16))) float ss[2][kT];
+  __shared__ bf16x8 w2img[OS][3][4][64];
   __shared__ f32x4 sums[kGradThreads];
+  auto at = [](int row, int k) { return k ^ (row & 4 ? 8 : 0); };
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int band = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64) * kT;
   const int64_t r0 = (int64_t)blockIdx.x * chunk_rows, nr = min<int64_t>(chunk_rows, rows - r0);
 
-  Thirds w1v[KS], w2v[OS];  // W1[band + c][16 s + 8 h ..], W2[16 s + 8 h + j][band + c]
+  Thirds w1v[KS];  // W1[band + c][16 s + 8 h ..]; W2[16 s + 8 h + j][band + c] in LDS, each wave its own
   {
     const __amdgpu_buffer_rsrc_t rw1 = rows_rsrc(w1, kHid * nin * 4), rw2 = rows_rsrc(w2, nout * kHid * 4);
 #pragma unroll
@@ -662,7 +710,9 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
         const int k = 16 * s + 8 * h + j;
         v[j] = load1(rw2, k < nout ? (uint32_t)(k * kHid + band + c) * 4u : kPast);
       }
-      w2v[s] = split3(v);
+      const Thirds x = split3(v);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) w2img[s][p][threadIdx.x / 64][lane] = x.v[p];
     }
   }
   const float bias = b1 != nullptr ? b1[band + c] : 0.0f;
@@ -681,10 +731,10 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
   f32x4 dst[kLD];
   float sst;
   auto load = [&](int64_t t0) {
-    const int64_t left = t0 < nr ? nr - t0 : 0, at = left > 0 ? r0 + t0 : 0;
-    const __amdgpu_buffer_rsrc_t rz = bytes_rsrc(codes + at * ld, min<int64_t>(left, kT) * ld);
-    const __amdgpu_buffer_rsrc_t rs = rows_rsrc(scale + at, min<int64_t>(left, kT) * 4);
-    const __amdgpu_buffer_rsrc_t rd = rows_rsrc(dy + at * nout, min<int64_t>(left, kT) * nout * 4);
+    const int64_t left = t0 < nr ? nr - t0 : 0, at = left > 0 ? r0 + t0 : 0, n = left < kT ? left : (int64_t)kT;
+    const __amdgpu_buffer_rsrc_t rz = bytes_rsrc(codes + at * ld, n * ld);
+    const __amdgpu_buffer_rsrc_t rs = rows_rsrc(scale + at, n * 4);
+    const __amdgpu_buffer_rsrc_t rd = rows_rsrc(dy + at * nout, n * nout * 4);
 #pragma unroll
     for (int u = 0; u < kLZ; ++u) {
       const int i = u * kGradThreads + (int)threadIdx.x, row = i / kZG, k = 4 * (i % kZG);
@@ -698,14 +748,15 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
     sst = load1(rs, threadIdx.x < kT ? threadIdx.x * 4u : kPast);
   };
   // column reads of a tile's rows: lane i of 16 gives row 4 h + i / 4 and columns 16 (lane / 16 % 2) + 4 (i % 4)
-  const int i16 = lane & 15, rrow = 4 * h + (i16 >> 2), rcol = 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+  const int i16 = lane & 15, rrow = 4 * h + (i16 >> 2);
+  const int rcol = at(rrow, 16 * ((lane >> 4) & 1) + 4 * (i16 & 3));
   load(0);
   int buf = 0;
   for (int64_t t0 = 0; t0 < nr; t0 += kT, buf ^= 1) {
 #pragma unroll
     for (int u = 0; u < kLZ; ++u) {
       const int i = u * kGradThreads + (int)threadIdx.x;
-      *reinterpret_cast<bf16x4*>(&zs[buf][i / kZG][4 * (i % kZG)]) = codes_bf16(zst[u]);
+      *reinterpret_cast<bf16x4*>(&zs[buf][i / kZG][at(i / kZG, 4 * (i % kZG))]) = codes_bf16(zst[u]);
     }
 #pragma unroll
     for (int u = 0; u < kLD; ++u) {
@@ -717,9 +768,10 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
       sb2[u] += v;
 #pragma unroll
       for (int p = 0; p < 3; ++p) {
-        const bf16x4 x = __builtin_convertvector(v, bf16x4);
-        *reinterpret_cast<bf16x4*>(&ds[buf][p][row][k]) = x;
-        if (p < 2) v -= __builtin_convertvector(x, f32x4);
+        float x0 = v[0], x1 = v[1], x2 = v[2], x3 = v[3];
+        const u32x2 x = {bf16_pair(x0, x1), bf16_pair(x2, x3)};
+        v = f32x4{x0, x1, x2, x3};
+        *reinterpret_cast<u32x2*>(&ds[buf][p][row][at(row, k)]) = x;
       }
     }
     if (threadIdx.x < kT) ss[buf][threadIdx.x] = sst;
@@ -732,15 +784,18 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
     f32x16 a = f32x16{}, dh = f32x16{};
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const bf16x8 z8 = *reinterpret_cast<const bf16x8*>(&zs[buf][c][16 * s + 8 * h]);
+      const bf16x8 z8 = *reinterpret_cast<const bf16x8*>(&zs[buf][c][at(c, 16 * s + 8 * h)]);
       a = mma(z8, w1v[s].v[0], mma(z8, w1v[s].v[1], mma(z8, w1v[s].v[2], a)));
     }
 #pragma unroll
     for (int s = 0; s < OS; ++s) {
-      Thirds d;
+      Thirds d, w;
 #pragma unroll
-      for (int p = 0; p < 3; ++p) d.v[p] = *reinterpret_cast<const bf16x8*>(&ds[buf][p][c][16 * s + 8 * h]);
-      dh = mma(d, w2v[s], dh);
+      for (int p = 0; p < 3; ++p) {
+        d.v[p] = *reinterpret_cast<const bf16x8*>(&ds[buf][p][c][at(c, 16 * s + 8 * h)]);
+        w.v[p] = w2img[s][p][threadIdx.x / 64][lane];
+      }
+      dh = mma(d, w, dh);
     }
     f32x8 hv[2], gv[2];
 #pragma unroll
@@ -825,6 +880,8 @@ constexpr int kMaxKS = (kMaxMlpIn + 15) / 16, kMaxOS = kMaxMlpOut / 16;
 
 // Workgroups of the row tile kernels: one a CU, a row tile for each where there
 // are fewer than the waves.
+// Their threads: two waves a SIMD, or one where two would spill.
+constexpr int tile_threads(bool wide) { return wide ? 256 : 512; }
 inline dim3 spread_grid(int64_t tiles) { return dim3((uint32_t)std::min<int64_t>(256, tiles)); }
 
 }  // namespace
@@ -836,8 +893,8 @@ void run_mlp_rows8_forward(const float* z, const float* w1, const float* b1, con
   const int64_t tiles = (rows + kT - 1) / kT;
   with_groups<kMaxKS>((nin + 15) / 16, [&](auto ks) {
     with_groups<2>(nout <= kT ? 1 : 2, [&](auto ot) {
-      constexpr int KS = decltype(ks)::value, T = KS > 7 ? 256 : 512;
-      hipLaunchKernelGGL((k_mlp_forward8<KS, decltype(ot)::value, T>), spread_grid(tiles), dim3(T), 0, st, z, w1, b1,
+      constexpr int KS = decltype(ks)::value, OT = decltype(ot)::value, T = tile_threads(KS > 6 || KS * OT > 6);
+      hipLaunchKernelGGL((k_mlp_forward8<KS, OT, T>), spread_grid(tiles), dim3(T), 0, st, z, w1, b1,
                          w2, b2, codes, ld, scale, y, rows, nin, nout, tiles);
     });
   });
@@ -853,13 +910,13 @@ void run_mlp_rows8_backward(const int8_t* codes, int64_t ld, const float* scale,
                             float* db2, int64_t rows, int nin, int nout, float* work, hipStream_t st) {
   const int64_t tiles = (rows + kT - 1) / kT;
   if (dz != nullptr && rows > 0) {
-    float shrink = 0x1p-15f;
-    for (int n = 1; n < nout; n *= 2) shrink *= 0.5f;
+    int drop = 15;
+    for (int n = 1; n < nout; n *= 2) ++drop;
     with_groups<kMaxKS>((nin + 15) / 16, [&](auto ks) {
       with_groups<kMaxOS>((nout + 15) / 16, [&](auto os) {
-        constexpr int KS = decltype(ks)::value, T = KS > 7 ? 256 : 512;
-        hipLaunchKernelGGL((k_mlp_input_grad8<KS, decltype(os)::value, T>), spread_grid(tiles), dim3(T), 0, st,
-                           codes, ld, scale, dy, w1, b1, w2, dz, rows, nin, nout, shrink, tiles);
+        constexpr int KS = decltype(ks)::value, OS = decltype(os)::value, T = tile_threads(KS > 6 || KS * OS > 18);
+        hipLaunchKernelGGL((k_mlp_input_grad8<KS, OS, T>), spread_grid(tiles), dim3(T), 0, st,
+                           codes, ld, scale, dy, w1, b1, w2, dz, rows, nin, nout, drop, tiles);
       });
     });
     SPHOPS_LAUNCHED();
