@@ -1253,7 +1253,7 @@ bool linear8_fits(int64_t rows, int in_features, int out_features) {
 bool rows8_weight_grad_fits(int64_t rows, int in_features, int out_features) {
   return rows >= 0 && rows <= sphops::kMaxLinearRows && in_features >= 1 && out_features >= 1 &&
          in_features <= sphops::kMaxLinearFeatures && out_features <= sphops::kMaxLinearFeatures &&
-         sphops::linear_grad_fits(rows, in_features, out_features);
+         sphops::rows8_weight_grad_fits(rows, in_features, out_features);
 }
 
 }  // namespace

@@ -440,9 +440,13 @@ void run_linear_weight_grad(const float* x, const float* dy, float* dw, float* d
       default: launch_mfma<4>(p, x, dy, work, rows, nin, nout, relu_x, st); break;
     }
   }
-  const int64_t nw = (int64_t)nout * nin;
-  hipLaunchKernelGGL(k_chunk_reduce, dim3((uint32_t)((nw + nout + 63) / 64)), dim3(64 * kReduceWaves), 0, st, work,
-                     dw, db, nw, nout, p.chunks);
+  run_linear_chunk_sum(work, dw, db, (int64_t)nout * nin, nout, p.chunks, st);
+}
+
+void run_linear_chunk_sum(const float* part, float* dw, float* db, int64_t nw, int nout, int64_t chunks,
+                          hipStream_t st) {
+  hipLaunchKernelGGL(k_chunk_reduce, dim3((uint32_t)((nw + nout + 63) / 64)), dim3(64 * kReduceWaves), 0, st, part,
+                     dw, db, nw, nout, chunks);
   SPHOPS_LAUNCHED();
 }
 

@@ -7,6 +7,7 @@
 // in float32 steps, ties to the even code.  A row that holds a NaN or an
 // infinity has a NaN scale and zero codes: whatever is computed from it is NaN.
 #include "rows8.hpp"
+#include "split16.hpp"
 
 #include <type_traits>
 
@@ -252,15 +253,227 @@ void run_restore_rows(const int8_t* codes, int64_t ld, const float* scale, void*
   SPHOPS_LAUNCHED();
 }
 
-// The rows again in 32 bits, then the weight gradient of linear_grad.hip.
+namespace {
+
+// Weight gradient from rows in 8 bits: dW = dy^T (codes * scale), db = column
+// sums of dy.  A row's scale is put into dy, whose three bfloat16 pieces hold
+// 24 bits at float32's range; a code is exact in bfloat16, so three matrix
+// instructions of 32 x 32 x 16 (96 cycles) do what float32 ones take 512 for.
+//
+// Workgroup = a chunk of rows and a block of dW, WO x WI waves of 32 outputs by
+// NI tiles of 32 inputs each.  32 rows a step stand in LDS by rows, dy's pieces
+// and the codes as bfloat16, and both operands (whose k are the rows) are read
+// down their columns.  A row of LDS is an odd number of 64 bytes: the four rows
+// of a column read then lie in different banks.  The next step's rows are
+// loaded under this one's products.
+struct Grad8Plan {
+  int wo, wi, ni, o_blocks, i_blocks;
+  int64_t chunk_rows, chunks;
+};
+
+template <int WO, int WI, int NI>
+__global__ __launch_bounds__(64 * WO * WI, 2) void k_rows8_weight_grad(
+    const int8_t* __restrict__ codes, int64_t ld, const float* __restrict__ scale, const float* __restrict__ dy,
+    float* __restrict__ part, int64_t rows, int nin, int nout, int i_blocks, int64_t chunk_rows, int64_t part_stride) {
+  constexpr int kThreads = 64 * WO * WI, kStepRows = 32, kIT = WI * NI;
+  constexpr int kC = (kIT | 1) * 32, kD = (WO | 1) * 32;          // 16-bit values a row of LDS
+  constexpr int kCG = kIT * 8, kDG = WO * 8;                      // groups of 4 columns a row
+  constexpr int kLC = (kStepRows * kCG + kThreads - 1) / kThreads, kLD = (kStepRows * kDG + kThreads - 1) / kThreads;
+  static_assert(kThreads % kDG == 0, "a thread keeps its columns of dy");
+  __shared__ __attribute__((aligned(16))) __bf16 cs[2][kStepRows][kC], ds[2][3][kStepRows][kD];
+  __shared__ f32x4 sums[kThreads];
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64), wo = wave % WO, wi = wave / WO;
+  const int block = (int)blockIdx.y, o0 = block / i_blocks * WO * 32, i0 = block % i_blocks * kIT * 32;
+  const int64_t r0 = (int64_t)blockIdx.x * chunk_rows, left = rows - r0, nr = left < chunk_rows ? left : chunk_rows;
+  // dy's rows are `nout` apart at any alignment of 4 bytes; codes' are ld apart
+  uint32_t cst[kLC];
+  f32x4 dst[kLD];
+  float sst[kLD];
+  f32x4 sb[kLD];
+#pragma unroll
+  for (int u = 0; u < kLD; ++u) sb[u] = f32x4{};
+  f32x16 acc[NI];
+#pragma unroll
+  for (int t = 0; t < NI; ++t) acc[t] = f32x16{};
+
+  auto buffer = [](const void* base, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
+  };
+  constexpr uint32_t kPast = 0x80000000u;
+  // rows past the chunk load zeros, which add nothing
+  auto load = [&](int64_t t0) {
+    const int64_t rest = t0 < nr ? nr - t0 : 0, at = rest > 0 ? r0 + t0 : 0, n = rest < kStepRows ? rest : (int64_t)kStepRows;
+    const __amdgpu_buffer_rsrc_t rc = buffer(codes + at * ld, n * ld), rs = buffer(scale + at, n * 4);
+    const __amdgpu_buffer_rsrc_t rd = buffer(dy + at * nout, n * nout * 4);
+#pragma unroll
+    for (int u = 0; u < kLC; ++u) {
+      const int i = u * kThreads + (int)threadIdx.x, row = i / kCG, k = i0 + 4 * (i % kCG);
+      cst[u] = __builtin_amdgcn_raw_buffer_load_b32(
+          rc, row < kStepRows && k < (int)ld ? (uint32_t)(row * (int)ld + k) : kPast, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < kLD; ++u) {
+      const int i = u * kThreads + (int)threadIdx.x, row = i / kDG, k = o0 + 4 * (i % kDG);
+      dst[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+          rd, row < kStepRows && k < nout ? (uint32_t)(row * nout + k) * 4u : kPast, 0, 0));
+      sst[u] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+          rs, row < kStepRows ? (uint32_t)row * 4u : kPast, 0, 0));
+    }
+  };
+  const int i16 = lane & 15, rrow = 4 * h + (i16 >> 2), rcol = 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+  load(0);
+  int buf = 0;
+  for (int64_t t0 = 0; t0 < nr; t0 += kStepRows, buf ^= 1) {
+#pragma unroll
+    for (int u = 0; u < kLC; ++u) {
+      const int i = u * kThreads + (int)threadIdx.x;
+      if (kStepRows * kCG % kThreads == 0 || i < kStepRows * kCG)
+        *reinterpret_cast<bf16x4*>(&cs[buf][i / kCG][4 * (i % kCG)]) = codes_bf16(cst[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kLD; ++u) {
+      const int i = u * kThreads + (int)threadIdx.x, row = i / kDG, k = 4 * (i % kDG);
+      if (kStepRows * kDG % kThreads != 0 && i >= kStepRows * kDG) continue;
+      f32x4 v = dst[u];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (o0 + k + j >= nout) v[j] = 0.0f;  // the next row's
+      sb[u] += v;
+      v *= sst[u];
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        float x0 = v[0], x1 = v[1], x2 = v[2], x3 = v[3];
+        const u32x2 x = {bf16_pair(x0, x1), bf16_pair(x2, x3)};
+        v = f32x4{x0, x1, x2, x3};
+        *reinterpret_cast<u32x2*>(&ds[buf][p][row][k]) = x;
+      }
+    }
+    // one barrier a step: a wave writes a buffer again only after the next
+    // barrier, which every wave reaches after its reads of this one
+    __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+    load(t0 + kStepRows);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int p = 0; p < kStepRows / 16; ++p) {
+      Thirds d;
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+        d.v[q] = __builtin_bit_cast(bf16x8, join(read_column(&ds[buf][q][16 * p + rrow][32 * wo + rcol]),
+                                                 read_column(&ds[buf][q][16 * p + 8 + rrow][32 * wo + rcol])));
+#pragma unroll
+      for (int t = 0; t < NI; ++t) {
+        const int col = 32 * (wi * NI + t) + rcol;
+        const bf16x8 z = __builtin_bit_cast(
+            bf16x8, join(read_column(&cs[buf][16 * p + rrow][col]), read_column(&cs[buf][16 * p + 8 + rrow][col])));
+        acc[t] = mma(d.v[0], z, mma(d.v[1], z, mma(d.v[2], z, acc[t])));
+      }
+    }
+  }
+  float* __restrict__ p = part + (int64_t)blockIdx.x * part_stride;
+#pragma unroll
+  for (int t = 0; t < NI; ++t) {
+    const int col = i0 + 32 * (wi * NI + t) + c;
+    if (col >= nin) continue;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int m = o0 + 32 * wo + 8 * (r / 4) + 4 * h + r % 4;
+      if (m < nout) p[(int64_t)m * nin + col] = acc[t][r];
+    }
+  }
+  if (i0 != 0) return;
+#pragma unroll
+  for (int u = 1; u < kLD; ++u) sb[0] += sb[u];
+  sums[threadIdx.x] = sb[0];
+  __syncthreads();
+  for (int k = threadIdx.x; k < WO * 32; k += kThreads) {
+    if (o0 + k >= nout) continue;
+    float t = 0.0f;
+    for (int i = 0; i < kThreads / kDG; ++i) t += sums[i * kDG + k / 4][k % 4];
+    p[(int64_t)nout * nin + o0 + k] = t;
+  }
+}
+
+// The chunks' sums of element e, dW then db, in the chunks' order.
+__global__ __launch_bounds__(256) void k_rows8_sum(const float* __restrict__ part, float* __restrict__ dw,
+                                                   float* __restrict__ db, int64_t nw, int nout, int64_t chunks) {
+  const int64_t n = nw + nout, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= n) return;
+  float t = 0.0f;
+#pragma unroll 4
+  for (int64_t k = 0; k < chunks; ++k) t += part[k * n + e];
+  if (e < nw) dw[e] = t;
+  else if (db != nullptr) db[e - nw] = t;
+}
+
+// f(integral_constants WO, WI, NI) of a plan
+template <class F>
+void with_block(const Grad8Plan& p, F&& f) {
+  auto ni = [&](auto wo, auto wi) {
+    switch (p.ni) {
+      case 1: return f(wo, wi, std::integral_constant<int, 1>{});
+      case 2: return f(wo, wi, std::integral_constant<int, 2>{});
+      case 3: return f(wo, wi, std::integral_constant<int, 3>{});
+      default: return f(wo, wi, std::integral_constant<int, 4>{});
+    }
+  };
+  const std::integral_constant<int, 1> c1{};
+  const std::integral_constant<int, 2> c2{};
+  const std::integral_constant<int, 4> c4{};
+  if (p.wo == 1) ni(c1, c4);
+  else if (p.wo == 2) ni(c2, c2);
+  else if (p.wi == 1) ni(c4, c1);
+  else ni(c4, c2);
+}
+
+Grad8Plan grad8_plan(int64_t rows, int nin, int nout) {
+  Grad8Plan p;
+  const int ot = (nout + 31) / 32, it = (nin + 31) / 32;
+  p.wo = ot >= 3 ? 4 : ot;
+  p.wi = p.wo == 1 ? 4 : p.wo == 2 ? 2 : it > 4 ? 2 : 1;
+  p.o_blocks = (ot + p.wo - 1) / p.wo;
+  p.i_blocks = (it + 4 * p.wi - 1) / (4 * p.wi);
+  p.ni = (it + p.i_blocks * p.wi - 1) / (p.i_blocks * p.wi);
+  const int64_t blocks = (int64_t)p.o_blocks * p.i_blocks, want = (p.wo * p.wi == 8 ? 256 : 512) / blocks;
+  const int64_t c = (rows + std::max<int64_t>(1, want) - 1) / std::max<int64_t>(1, want);
+  p.chunk_rows = std::min<int64_t>(kMaxChunkRows, std::max<int64_t>(64, (c + 31) / 32 * 32));
+  p.chunks = rows > 0 ? (rows + p.chunk_rows - 1) / p.chunk_rows : 0;
+  return p;
+}
+
+}  // namespace
+
+bool rows8_weight_grad_fits(int64_t rows, int nin, int nout) {
+  const Grad8Plan p = grad8_plan(rows, nin, nout);
+  return (int64_t)p.o_blocks * p.i_blocks <= 65535 && p.chunks < (int64_t(1) << 31);
+}
+
 int64_t rows8_weight_grad_floats(int64_t rows, int nin, int nout) {
-  return rows * nin + linear_grad_chunks(rows, nin, nout) * ((int64_t)nin * nout + nout);
+  const int64_t chunks = grad8_plan(rows, nin, nout).chunks;
+  return chunks * ((int64_t)nin * nout + nout);
 }
 
 void run_rows8_weight_grad(const int8_t* codes, int64_t ld, const float* scale, const float* dy, float* dw, float* db,
                            int64_t rows, int nin, int nout, float* work, hipStream_t st) {
-  run_restore_rows(codes, ld, scale, work, SPHOPS_F32, rows, nin, st);
-  run_linear_weight_grad(work, dy, dw, db, rows, nin, nout, work + rows * nin, false, st);
+  const Grad8Plan p = grad8_plan(rows, nin, nout);
+  const int64_t nw = (int64_t)nin * nout, n = nw + nout;
+  if (p.chunks > 0) {
+    with_block(p, [&](auto wo, auto wi, auto ni) {
+      constexpr int WO = decltype(wo)::value, WI = decltype(wi)::value;
+      hipLaunchKernelGGL((k_rows8_weight_grad<WO, WI, decltype(ni)::value>),
+                         dim3((uint32_t)p.chunks, (uint32_t)(p.o_blocks * p.i_blocks)), dim3(64 * WO * WI), 0, st,
+                         codes, ld, scale, dy, work, rows, nin, nout, p.i_blocks, p.chunk_rows, n);
+    });
+    SPHOPS_LAUNCHED();
+  }
+  // few chunks: a thread an element; many: the workgroups of linear_grad.hip share them out
+  if (p.chunks <= 16)
+    hipLaunchKernelGGL(k_rows8_sum, dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, work, dw, db, nw, nout,
+                       p.chunks);
+  else
+    run_linear_chunk_sum(work, dw, db, nw, nout, p.chunks, st);
+  SPHOPS_LAUNCHED();
 }
 
 }  // namespace sphops

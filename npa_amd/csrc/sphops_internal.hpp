@@ -378,6 +378,10 @@ void run_quantize_rows(const void* x, int type, int64_t stride, int8_t* codes, i
                        int64_t cols, bool relu, hipStream_t st);
 void run_restore_rows(const int8_t* codes, int64_t ld, const float* scale, void* out, int type, int64_t rows,
                       int64_t cols, hipStream_t st);
+// partial sums of dW (nw elements) then db (nout) a chunk, added in a fixed order (linear_grad.hip)
+void run_linear_chunk_sum(const float* part, float* dw, float* db, int64_t nw, int nout, int64_t chunks,
+                          hipStream_t st);
+bool rows8_weight_grad_fits(int64_t rows, int nin, int nout);
 int64_t rows8_weight_grad_floats(int64_t rows, int nin, int nout);
 void run_rows8_weight_grad(const int8_t* codes, int64_t ld, const float* scale, const float* dy, float* dw, float* db,
                            int64_t rows, int nin, int nout, float* work, hipStream_t st);
