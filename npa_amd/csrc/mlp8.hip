@@ -60,26 +60,30 @@ __global__ __launch_bounds__(kServeThreads, 2) void k_mlp8(
 
   const int64_t step = (int64_t)gridDim.x * (kServeThreads / 64);
   int64_t tile = (int64_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * (kServeThreads / 64) + threadIdx.x / 64));
+  f32x4 zn[KS][4];
+  auto load = [&](int64_t t) {
+    const int64_t r0 = t * kT, nr = t < tiles ? min<int64_t>(kT, rows - r0) : 0;
+    const __amdgpu_buffer_rsrc_t rz = rows_rsrc(z + (nr > 0 ? r0 * nin : 0), nr * nin * 4);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) zn[s][i] = load4(rz, (uint32_t)(c * nin + 32 * s + 16 * h + 4 * i) * 4u);
+    }
+  };
+  load(tile);
+  landed(zn);
   for (; tile < tiles; tile += step) {
     asm volatile("" ::: "memory");  // the images stay in LDS: read ahead of the loop they spill
     const int64_t r0 = tile * kT, nr = min<int64_t>(kT, rows - r0);
-    const __amdgpu_buffer_rsrc_t rz = rows_rsrc(z + r0 * nin, nr * nin * 4);
     f32x4 zv[KS][4];
     uint32_t top = 0;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int k = 32 * s + 16 * h + 4 * i;
-        zv[s][i] = load4(rz, (uint32_t)(c * nin + k) * 4u);
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+          zv[s][i][j] = zn[s][i][j];
           // past the row's end lies the next row
           if (s == KS - 1 && 32 * s + 16 * h + 4 * i + j >= nin) zv[s][i][j] = 0.0f;
           top = max(top, abs_bits(zv[s][i][j]));
@@ -101,6 +105,9 @@ __global__ __launch_bounds__(kServeThreads, 2) void k_mlp8(
       for (int t = 0; t < kHT; ++t)
         acc[t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w1img[s][t][lane], cz, acc[t], 0, 0, 0);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    load(tile + step);  // in flight until the row tile's stores
+    __builtin_amdgcn_sched_barrier(0);
     f32x16 hv[kHT];
     top = 0;
 #pragma unroll
@@ -131,6 +138,7 @@ __global__ __launch_bounds__(kServeThreads, 2) void k_mlp8(
       for (int o = 0; o < OT; ++o)
         out[o] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w2img[t][o][lane], ch, out[o], 0, 0, 0);
     }
+    landed(zn);
     const __amdgpu_buffer_rsrc_t ry = rows_rsrc(y + r0 * nout, nr * nout * 4);
 #pragma unroll
     for (int o = 0; o < OT; ++o) {
@@ -177,17 +185,31 @@ __device__ __forceinline__ u32x2 load2(__amdgpu_buffer_rsrc_t r, uint32_t off) {
 // Eight values of a row of n from column k (zeros past it), through a resource
 // over all rows.
 __device__ __forceinline__ f32x8 load8(__amdgpu_buffer_rsrc_t r, int row, int n, int k) {
-  f32x8 v;
+  const uint32_t at = (uint32_t)(row * n + k) * 4u;
+  f32x8 v = __builtin_shufflevector(load4(r, at), load4(r, at + 16u), 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = load1(r, k + j < n ? (uint32_t)(row * n + k + j) * 4u : kPast);
+  for (int j = 0; j < 8; ++j) v[j] = k + j < n ? v[j] : 0.0f;  // the next row's
   return v;
 }
 
+// Result columns 32 t + lane % 32 of a tile whose registers are rows 8 (r / 4) +
+// 4 (lane / 32) + r % 4: a store writes two runs of 128 bytes.
+__device__ __forceinline__ void store_columns(__amdgpu_buffer_rsrc_t r, int width, int col, int h, f32x16 v) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    store1(r, col < width ? (uint32_t)((8 * (i / 4) + 4 * h + i % 4) * width + col) * 4u : kPast, v[i]);
+}
+
+// The columns that a lane of half h holds of step s of a product over a row: two
+// steps take 16 neighbouring ones, so that a lane's loads of a row are whole
+// 64-byte pieces.  (With 8 columns a step and half, lines left L1 between the
+// four loads that share one.)
+__device__ __forceinline__ constexpr int step_column(int s, int h) { return 32 * (s / 2) + 16 * h + 8 * (s % 2); }
+
 // W1 in halves as an operand image: lane l's 16 bytes of entry (s, t), at
-// image_lane(s, l), are W1[32 t + l % 32][16 s + 8 (l / 32) .. + 7] times the
-// hidden unit's own power of two, whose inverse is left in inv.  The scale
-// covers 2^-16 of the bias too, so that a bias over it stays in range where
-// W1's row is small or zero.  All threads; ends with a barrier.  `top` is
+// image_lane(s, l), are W1[32 t + l % 32][step_column(s, l / 32) .. + 7] times
+// the hidden unit's own power of two, whose inverse is left in inv.  The scale
+// covers 2^-6 of the bias too, so that a bias over it is at most 2^21.  All threads; ends with a barrier.  `top` is
 // scratch.
 //
 // image_lane exchanges hidden rows so that the 32 lanes of half a column read
@@ -202,13 +224,13 @@ __device__ __forceinline__ void w1_image(const float* __restrict__ w1, const flo
   constexpr int kEntries = KS * kHT * 64, kOwn = (kEntries + kThreads - 1) / kThreads;
   const __amdgpu_buffer_rsrc_t r = rows_rsrc(w1, kHid * nin * 4);
   f32x8 v[kOwn];
-  if (threadIdx.x < kHid) top[threadIdx.x] = b1 != nullptr ? abs_bits(b1[threadIdx.x] * 0x1p-16f) : 0u;
+  if (threadIdx.x < kHid) top[threadIdx.x] = b1 != nullptr ? abs_bits(b1[threadIdx.x] * 0x1p-6f) : 0u;
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < kOwn; ++u) {
     const int i = u * kThreads + (int)threadIdx.x, l = i & 63, t = (i >> 6) % kHT, s = (i >> 6) / kHT;
     v[u] = f32x8{};
-    if (i < kEntries) v[u] = load8(r, kT * t + (l & 31), nin, 16 * s + 8 * (l >> 5));
+    if (i < kEntries) v[u] = load8(r, kT * t + (l & 31), nin, step_column(s, l >> 5));
   }
 #pragma unroll
   for (int u = 0; u < kOwn; ++u) {
@@ -238,18 +260,23 @@ __device__ __forceinline__ void w1_image(const float* __restrict__ w1, const flo
 // own powers of two and split.  A hidden unit's power of two stays in its hidden
 // value (relu(p a) = p relu(a)) and is taken out of W2's image.  The hidden tile's result registers 8 j .. 8 j +
 // 7 of lane l are hidden units 16 j + 4 (l / 32) + 0..3 and 8 more of its row:
-// as they stand they are an operand with W2's image in the same order.
-template <int KS, int OT, int kThreads>
+// as they stand they are an operand with W2's image in the same order, and as
+// the first operand they leave y's rows in registers and its columns in lanes,
+// whose stores are whole.
+template <int CT, int OT, int kThreads>
 __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
     const float* __restrict__ z, const float* __restrict__ w1, const float* __restrict__ b1,
     const float* __restrict__ w2, const float* __restrict__ b2, int8_t* __restrict__ codes, int64_t ld,
     float* __restrict__ scale, float* __restrict__ y, int64_t rows, int nin, int nout, int64_t tiles) {
+  constexpr int KS = 2 * CT;
   __shared__ f16x8 w1hi[KS][kHT][64], w1lo[KS][kHT][64];
   __shared__ f16x8 w2hi[kHT][2][OT][64], w2lo[kHT][2][OT][64];
-  __shared__ uint32_t top[kHid];
+  __shared__ uint32_t top[kHid], btop;
   __shared__ __attribute__((aligned(16))) float i1s[kHid], b1s[kHid], i2s[OT * kT], b2s[OT * kT];
+  __shared__ f32x4 unit[kThreads / 64][kT / 4];  // each wave's own: its rows' hidden scales
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int lane0 = image_lane(0, lane), lane1 = image_lane(1, lane);
+  if (threadIdx.x == 0) btop = 0;  // w1_image's barriers come before its use
   w1_image<KS, kThreads>(w1, b1, nin, w1hi, w1lo, top, i1s);
   {
     constexpr int kEntries = kHT * 2 * OT * 64, kOwn = (kEntries + kThreads - 1) / kThreads;
@@ -283,23 +310,28 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
       i2s[threadIdx.x] = pow2_for(top[threadIdx.x]).ip;
       b2s[threadIdx.x] = b2 != nullptr && (int)threadIdx.x < nout ? b2[threadIdx.x] : 0.0f;
     }
-    if (threadIdx.x < kHid) b1s[threadIdx.x] = b1 != nullptr ? b1[threadIdx.x] / i1s[threadIdx.x] : 0.0f;
+    if (threadIdx.x < kHid) {
+      const float v = b1 != nullptr ? b1[threadIdx.x] / i1s[threadIdx.x] : 0.0f;
+      b1s[threadIdx.x] = v;
+      atomicMax(&btop, abs_bits(v));
+    }
   }
   __syncthreads();
 
   const int64_t step = (int64_t)gridDim.x * (kThreads / 64);
   int64_t tile = (int64_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64 * gridDim.x + blockIdx.x));
-  f32x4 zn[KS][2];
+  f32x4 zn[CT][4];
   auto load = [&](int64_t t) {
     const int64_t r0 = t * kT, nr = t < tiles ? min<int64_t>(kT, rows - r0) : 0;
     const __amdgpu_buffer_rsrc_t rz = rows_rsrc(z + (nr > 0 ? r0 * nin : 0), nr * nin * 4);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
+    for (int s = 0; s < CT; ++s) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) zn[s][i] = load4(rz, (uint32_t)(c * nin + 16 * s + 8 * h + 4 * i) * 4u);
+      for (int i = 0; i < 4; ++i) zn[s][i] = load4(rz, (uint32_t)(c * nin + 32 * s + 16 * h + 4 * i) * 4u);
     }
   };
   load(tile);
+  landed(zn);
   for (; tile < tiles; tile += step) {
     asm volatile("" ::: "memory");  // the images stay in LDS: read ahead of the loop they spill
     const int64_t r0 = tile * kT, nr = min<int64_t>(kT, rows - r0);
@@ -307,10 +339,10 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
     uint32_t zt = 0;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      zv[s] = __builtin_shufflevector(zn[s][0], zn[s][1], 0, 1, 2, 3, 4, 5, 6, 7);
+      zv[s] = __builtin_shufflevector(zn[s / 2][s % 2 * 2], zn[s / 2][s % 2 * 2 + 1], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if (s == KS - 1 && 16 * s + 8 * h + j >= nin) zv[s][j] = 0.0f;  // the next row's
+        if (s / 2 == CT - 1 && step_column(s, h) + j >= nin) zv[s][j] = 0.0f;  // the next row's
         zt = max(zt, abs_bits(zv[s][j]));
       }
     }
@@ -321,15 +353,21 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
     const RowScale q = row_scale(zt);
     const __amdgpu_buffer_rsrc_t rc = bytes_rsrc(codes + r0 * ld, nr * ld);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int k = 16 * s + 8 * h;
-      const u32x2 w = {row_codes4(zv[s][0], zv[s][1], zv[s][2], zv[s][3], q),
-                       row_codes4(zv[s][4], zv[s][5], zv[s][6], zv[s][7], q)};
-      if (s < KS - 1) {
-        __builtin_amdgcn_raw_buffer_store_b64(w, rc, (uint32_t)(c * (int)ld + k), 0, 0);
+    for (int s = 0; s < CT; ++s) {
+      const int k = 32 * s + 16 * h;
+      u32x4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x8 v = zv[2 * s + i / 2];
+        w[i] = i % 2 == 0 ? row_codes4(v[0], v[1], v[2], v[3], q) : row_codes4(v[4], v[5], v[6], v[7], q);
+      }
+      if (s < CT - 1) {
+        __builtin_amdgcn_raw_buffer_store_b128(w, rc, (uint32_t)(c * (int)ld + k), 0, 0);
       } else {
-        __builtin_amdgcn_raw_buffer_store_b32(w[0], rc, k < (int)ld ? (uint32_t)(c * (int)ld + k) : kPast, 0, 0);
-        __builtin_amdgcn_raw_buffer_store_b32(w[1], rc, k + 4 < (int)ld ? (uint32_t)(c * (int)ld + k + 4) : kPast, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          __builtin_amdgcn_raw_buffer_store_b32(
+              w[i], rc, k + 4 * i < (int)ld ? (uint32_t)(c * (int)ld + k + 4 * i) : kPast, 0, 0);
       }
     }
     if (h == 0 && c < nr) scale[r0 + c] = q.scale;
@@ -337,56 +375,53 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
     Halves zs[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) zs[s] = split(zv[s] * pz.p);
-    float hv[kHT][16];
-    uint32_t ht = 0;
-#pragma unroll
-    for (int t = 0; t < kHT; ++t) {
-      f32x16 acc = f32x16{};
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int l = s % 2 == 0 ? lane0 : lane1;
-        acc = mma(Halves{w1hi[s][t][l], w1lo[s][t][l]}, zs[s], acc);
-      }
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 bv = *reinterpret_cast<const f32x4*>(b1s + kT * t + 8 * g + 4 * h);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float v = relu(acc[4 * g + j] * pz.ip + bv[j]);
-          hv[t][4 * g + j] = v;
-          ht = max(ht, __builtin_bit_cast(uint32_t, v));  // no value below zero; a NaN of either sign is above all
-        }
-      }
-    }
-    ht = max(ht, (uint32_t)__shfl_xor((int)ht, 32)) & 0x7fffffffu;
-    const Pow2 ph = pow2_for(ht);
+    // no hidden value exceeds this, and it is not far above the largest: W1's
+    // values are at most 2^15 in the image
+    const Pow2 ph = pow2_for(__builtin_bit_cast(uint32_t, __builtin_bit_cast(float, zt) * (32768.0f * (float)nin) +
+                                                              __builtin_bit_cast(float, btop)));
     f32x16 out[OT];
 #pragma unroll
     for (int o = 0; o < OT; ++o) out[o] = f32x16{};
 #pragma unroll
     for (int t = 0; t < kHT; ++t) {
+      f32x16 acc = f32x16{};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const int l = k % 2 == 0 ? lane0 : lane1;
+        acc = mma(Halves{w1hi[k][t][l], w1lo[k][t][l]}, zs[k], acc);
+      }
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         f32x8 v;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = hv[t][8 * p + j] * ph.p;
+        for (int g = 2 * p; g < 2 * p + 2; ++g) {
+          const f32x4 bv = *reinterpret_cast<const f32x4*>(b1s + kT * t + 8 * g + 4 * h);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[4 * (g - 2 * p) + j] = relu(acc[4 * g + j] * pz.ip + bv[j]) * ph.p;
+        }
         const Halves hs = split(v);
 #pragma unroll
-        for (int o = 0; o < OT; ++o) out[o] = mma(Halves{w2hi[t][p][o][lane], w2lo[t][p][o][lane]}, hs, out[o]);
+        for (int o = 0; o < OT; ++o) out[o] = mma(hs, Halves{w2hi[t][p][o][lane], w2lo[t][p][o][lane]}, out[o]);
       }
     }
+    landed(zn);
+    // rows are the registers now: their scales come from the lanes that hold them
+    float* __restrict__ us = reinterpret_cast<float*>(unit[threadIdx.x / 64]);
+    if (h == 0) us[c] = ph.ip;
+    __builtin_amdgcn_wave_barrier();
     const __amdgpu_buffer_rsrc_t ry = rows_rsrc(y + r0 * nout, nr * nout * 4);
 #pragma unroll
     for (int o = 0; o < OT; ++o) {
+      const float iv = i2s[kT * o + c], bv = b2s[kT * o + c];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int at = kT * o + 8 * g + 4 * h;
-        const f32x4 iv = *reinterpret_cast<const f32x4*>(i2s + at), bv = *reinterpret_cast<const f32x4*>(b2s + at);
+        const f32x4 rv = *reinterpret_cast<const f32x4*>(us + 8 * g + 4 * h);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) out[o][4 * g + j] = out[o][4 * g + j] * ph.ip * iv[j] + bv[j];
+        for (int j = 0; j < 4; ++j) out[o][4 * g + j] = out[o][4 * g + j] * rv[j] * iv + bv;
       }
-      store_row(ry, nout, kT * o, c, h, out[o]);
+      store_columns(ry, nout, kT * o + c, h, out[o]);
     }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -394,24 +429,26 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
 
 // dz from codes and dy.  One wave a tile of 32 rows, rows as the columns n:
 // hidden tile by hidden tile, a (for its sign) from the codes and dh = W2^T dy
-// masked by it; then dz^T += W1^T dh^T with W1's image read down its columns.
+// masked by it; then dz += dh W1 with W1's image read down its columns, dh's
+// result registers as they stand being the first operand.
 // A hidden unit's power of two is taken out of W2's image, so that W1's stands
 // in for W1; the row's own power of two keeps dy and dh in range: |dy| <= 2^15,
 // |W2| <= 2^15 in the image, so |dh| <= 2^30 nout, and 2^-drop brings it to
 // 2^15.
-template <int KS, int OS, int kThreads>
+template <int CT, int OT, int kThreads>
 __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
     const int8_t* __restrict__ codes, int64_t ld, const float* __restrict__ scale, const float* __restrict__ dy,
     const float* __restrict__ w1, const float* __restrict__ b1, const float* __restrict__ w2, float* __restrict__ dz,
     int64_t rows, int nin, int nout, int drop, int64_t tiles) {
-  constexpr int CT = (KS + 1) / 2;
-  __shared__ f16x8 w1hi[2 * CT][kHT][64], w1lo[2 * CT][kHT][64];
+  constexpr int KS = 2 * CT, OS = 2 * OT;
+  __shared__ f16x8 w1hi[KS][kHT][64], w1lo[KS][kHT][64];
   __shared__ f16x8 w2hi[OS][kHT][64], w2lo[OS][kHT][64];
   __shared__ uint32_t top[kHid], top2;
   __shared__ __attribute__((aligned(16))) float i1s[kHid], nbs[kHid];
+  __shared__ __attribute__((aligned(16))) int exps[kThreads / 64][kT];  // each wave's own: its rows' exponents
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   if (threadIdx.x == 0) top2 = 0;
-  w1_image<2 * CT, kThreads>(w1, b1, nin, w1hi, w1lo, top, i1s);
+  w1_image<KS, kThreads>(w1, b1, nin, w1hi, w1lo, top, i1s);
   int e2;
   {
     constexpr int kEntries = OS * kHT * 64, kOwn = (kEntries + kThreads - 1) / kThreads;
@@ -420,7 +457,7 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
 #pragma unroll
     for (int u = 0; u < kOwn; ++u) {
       const int i = u * kThreads + (int)threadIdx.x, l = i & 63, t = (i >> 6) % kHT, s = (i >> 6) / kHT;
-      const int k = 16 * s + 8 * (l >> 5), n = kT * t + (l & 31);
+      const int k = step_column(s, l >> 5), n = kT * t + (l & 31);
       uint32_t m = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -445,55 +482,61 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
   }
   __syncthreads();
 
-  // a column read of W1's image: columns 32 ct + 16 (lane / 16 % 2) + .., hidden
-  // rows 4 h + lane % 16 / 4 from a multiple of 8
-  const int i16 = lane & 15, g2 = (lane >> 4) & 1;
-  const int half = (i16 >> 1) & 1, wrow = (4 * h + (i16 >> 2)) ^ (4 * g2);
-  const int wcol = (g2 * kHT * 64 + half * 32 + wrow) * 16 + (i16 & 1) * 8;
+  // a column read of W1's image: columns 16 (lane / 16 % 2) + 4 (lane % 4) ..
+  // + 3 of a tile's 32, hidden rows 4 h + lane % 16 / 4 from a multiple of 8
+  const int i16 = lane & 15, half = (lane >> 4) & 1, odd = (i16 >> 1) & 1;
+  const int wcol = (odd * kHT * 64 + half * 32 + ((4 * h + (i16 >> 2)) ^ (4 * odd))) * 16 + (i16 & 1) * 8;
   const int wcol0 = wcol + 8 * 16 * half, wcol1 = wcol + 8 * 16 * (1 - half);  // the first and second eight rows
   const int lane0 = image_lane(0, lane), lane1 = image_lane(1, lane);
   const float shrink = __builtin_bit_cast(float, (uint32_t)(127 - drop) << 23);
   const int64_t step = (int64_t)gridDim.x * (kThreads / 64);
   int64_t tile = (int64_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64 * gridDim.x + blockIdx.x));
-  u32x2 cn[KS];
-  f32x4 dn[OS][2];
+  u32x4 cn[CT];
+  f32x4 dn[OT][4];
   float sn;
   auto load = [&](int64_t t) {
     const int64_t r0 = t < tiles ? t * kT : 0, nr = t < tiles ? min<int64_t>(kT, rows - r0) : 0;
     const __amdgpu_buffer_rsrc_t rc = bytes_rsrc(codes + r0 * ld, nr * ld), rs = rows_rsrc(scale + r0, nr * 4);
     const __amdgpu_buffer_rsrc_t rd = rows_rsrc(dy + r0 * nout, nr * nout * 4);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) cn[s] = load2(rc, (uint32_t)(c * (int)ld + 16 * s + 8 * h));
+    for (int s = 0; s < CT; ++s)
+      cn[s] = __builtin_amdgcn_raw_buffer_load_b128(rc, (uint32_t)(c * (int)ld + 32 * s + 16 * h), 0, 0);
 #pragma unroll
-    for (int s = 0; s < OS; ++s) {
+    for (int s = 0; s < OT; ++s) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) dn[s][i] = load4(rd, (uint32_t)(c * nout + 16 * s + 8 * h + 4 * i) * 4u);
+      for (int i = 0; i < 4; ++i) dn[s][i] = load4(rd, (uint32_t)(c * nout + 32 * s + 16 * h + 4 * i) * 4u);
     }
     sn = load1(rs, (uint32_t)c * 4u);
   };
   load(tile);
+  landed(cn);
+  landed(dn);
+  asm volatile("" : "+v"(sn));
+  auto column = [&](int t, int p, int ct) {
+    const char* ph = reinterpret_cast<const char*>(&w1hi[2 * ct][t][16 * p]);
+    const char* pl = reinterpret_cast<const char*>(&w1lo[2 * ct][t][16 * p]);
+    return Halves{__builtin_bit_cast(f16x8, join(read_column(ph + wcol0), read_column(ph + wcol1))),
+                  __builtin_bit_cast(f16x8, join(read_column(pl + wcol0), read_column(pl + wcol1)))};
+  };
   for (; tile < tiles; tile += step) {
     asm volatile("" ::: "memory");  // the images stay in LDS: read ahead of the loop they spill
     const int64_t r0 = tile * kT, nr = min<int64_t>(kT, rows - r0);
     // codes past the row's end meet zeros in W1's image
     f16x8 cz[KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) cz[s] = codes_f16(cn[s]);
+    for (int s = 0; s < KS; ++s) cz[s] = codes_f16(u32x2{cn[s / 2][s % 2 * 2], cn[s / 2][s % 2 * 2 + 1]});
     const float sc = sn;
     f32x8 dv[OS];
     uint32_t dt = 0;
 #pragma unroll
     for (int s = 0; s < OS; ++s) {
-      dv[s] = __builtin_shufflevector(dn[s][0], dn[s][1], 0, 1, 2, 3, 4, 5, 6, 7);
+      dv[s] = __builtin_shufflevector(dn[s / 2][s % 2 * 2], dn[s / 2][s % 2 * 2 + 1], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if (s == OS - 1 && 16 * s + 8 * h + j >= nout) dv[s][j] = 0.0f;
+        if (s / 2 == OT - 1 && step_column(s, h) + j >= nout) dv[s][j] = 0.0f;
         dt = max(dt, abs_bits(dv[s][j]));
       }
     }
-    __builtin_amdgcn_sched_barrier(0);
-    load(tile + step);
-    __builtin_amdgcn_sched_barrier(0);
     dt = max(dt, (uint32_t)__shfl_xor((int)dt, 32));
     const Pow2 pd = pow2_for(dt);
     Halves ds[OS];
@@ -506,46 +549,54 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
     for (int t = 0; t < kHT; ++t) {
       f32x16 a = f32x16{}, dh = f32x16{};
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int l = s % 2 == 0 ? lane0 : lane1;
-        a = mma(w1hi[s][t][l], cz[s], mma(w1lo[s][t][l], cz[s], a));
+      for (int k = 0; k < KS; ++k) {
+        const int l = k % 2 == 0 ? lane0 : lane1;
+        a = mma(w1hi[k][t][l], cz[k], mma(w1lo[k][t][l], cz[k], a));
       }
 #pragma unroll
-      for (int s = 0; s < OS; ++s) dh = mma(Halves{w2hi[s][t][lane], w2lo[s][t][lane]}, ds[s], dh);
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 nb = *reinterpret_cast<const f32x4*>(nbs + kT * t + 8 * g + 4 * h);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          // as torch: 0 where relu(a) <= 0, so a NaN lets the upstream pass
-          const float v = dh[4 * g + j] * shrink;
-          dh[4 * g + j] = a[4 * g + j] * sc <= nb[j] ? 0.0f : v;
-        }
+      for (int k = 0; k < OS; ++k) dh = mma(Halves{w2hi[k][t][lane], w2lo[k][t][lane]}, ds[k], dh);
+      if (t == kHT - 1) {  // into the registers that this tile's codes and dy leave
+        __builtin_amdgcn_sched_barrier(0);
+        load(tile + step);
+        __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         f32x8 v;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = dh[8 * p + j];
+        for (int g = 2 * p; g < 2 * p + 2; ++g) {
+          const f32x4 nb = *reinterpret_cast<const f32x4*>(nbs + kT * t + 8 * g + 4 * h);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            // as torch: 0 where relu(a) <= 0, so a NaN lets the upstream pass
+            const float d = dh[4 * g + j] * shrink;
+            v[4 * (g - 2 * p) + j] = a[4 * g + j] * sc <= nb[j] ? 0.0f : d;
+          }
+        }
         const Halves hs = split(v);
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          const char* ph = reinterpret_cast<const char*>(&w1hi[2 * ct][t][16 * p]);
-          const char* pl = reinterpret_cast<const char*>(&w1lo[2 * ct][t][16 * p]);
-          const Halves w = {__builtin_bit_cast(f16x8, join(read_column(ph + wcol0), read_column(ph + wcol1))),
-                            __builtin_bit_cast(f16x8, join(read_column(pl + wcol0), read_column(pl + wcol1)))};
-          out[ct] = mma(w, hs, out[ct]);
-        }
+        for (int ct = 0; ct < CT; ++ct) out[ct] = mma(hs, column(t, p, ct), out[ct]);
       }
     }
+    landed(cn);
+    landed(dn);
+    asm volatile("" : "+v"(sn));
+    // rows are the registers now: their exponents come from the lanes that hold them
+    int* __restrict__ es = exps[threadIdx.x / 64];
+    if (h == 0) es[c] = (int)(__builtin_bit_cast(uint32_t, pd.ip) >> 23) - 127 + e2;
+    __builtin_amdgcn_wave_barrier();
     const __amdgpu_buffer_rsrc_t rz = rows_rsrc(dz + r0 * nin, nr * nin * 4);
-    const int e = (int)(__builtin_bit_cast(uint32_t, pd.ip) >> 23) - 127 + e2;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) out[ct][r] = __builtin_ldexpf(out[ct][r], e);
-      store_row(rz, nin, kT * ct, c, h, out[ct]);
+      for (int g = 0; g < 4; ++g) {
+        const i32x4 ev = *reinterpret_cast<const i32x4*>(es + 8 * g + 4 * h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[ct][4 * g + j] = __builtin_ldexpf(out[ct][4 * g + j], ev[j]);
+      }
+      store_columns(rz, nin, kT * ct + c, h, out[ct]);
     }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -554,13 +605,39 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
 constexpr int kGradThreads = 256;
 constexpr int weight_grad8_waves(int ks, int os) { return ks > 6 || os > 2 ? 1 : 2; }
 
+// A lane's running power of two for sums over rows: where a value would leave a
+// half's range (32768), the scale falls to where 16 times the value still fits,
+// and the sums so far with it.  Both lanes of a column (l and l + 32) keep the
+// same one.
+struct Running {
+  float p = 0x1p126f, ip = 0x1p-126f;
+  // the factor that the lane's sums take, 1 if the scale stays
+  __device__ __forceinline__ float fit(float largest) {
+    largest = fmaxf(largest, __shfl_xor(largest, 32));
+    if (!(largest * p > 32768.0f)) return 1.0f;
+    const Pow2 q = pow2_for(abs_bits(largest));
+    const float old = ip;
+    p = fmaxf(q.p * 0x1p-4f, 0x1p-126f);
+    ip = 1.0f / p;
+    return p * old;
+  }
+};
+template <int N>
+__device__ __forceinline__ void scale_sums(f32x16 (&acc)[N], float f) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] *= f;
+}
+
 // Workgroup = one chunk of rows, wave t the hidden units 32 t .. 32 t + 31 with
-// their weights' pieces in registers.  A row tile's codes (as bfloat16) and
-// dy's pieces stand in LDS by rows: read along rows they are the operands of a
-// = z W1^T and dh = dy W2, read down columns those of dW1 = (dh s)^T codes and
-// dW2 = dy^T relu(a), whose other operands come in a's and dh's result layout.
-// The next tile is loaded under this one's products.  The chunk's partial sums:
-// dW1 (128 x nin), db1 (128), dW2 (nout x 128), db2 (nout).
+// W1's rows in registers (each by its own power of two, as in w1_image).  A row
+// tile's codes (as halves) and dy's halves (each row by its own power of two)
+// stand in LDS by rows: read along rows they are the operands of a = z W1^T and
+// dh = dy W2, read down columns those of dW1 = codes^T (dh s) and dW2 = dy^T
+// relu(a), whose other operands come in a's and dh's result layout, a hidden
+// unit to a lane.  Sums over rows take a lane's running power of two: what it
+// leaves out of a small row is small against the sums.  The next tile is loaded
+// under this one's products.  The chunk's partial sums: dW1 (128 x nin), db1
+// (128), dW2 (nout x 128), db2 (nout).
 template <int KS, int OS>
 __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_mlp_weight_grad8(
     const int8_t* __restrict__ codes, int64_t ld, const float* __restrict__ scale, const float* __restrict__ dy,
@@ -573,34 +650,51 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
   constexpr int kZ = (CT | 1) * kT, kD = (OT | 1) * kT;
   constexpr int kZG = CT * 8, kDG = OT * 8;              // groups of 4 columns a row
   constexpr int kLZ = kT * kZG / kGradThreads, kLD = kT * kDG / kGradThreads;
-  __shared__ __attribute__((aligned(16))) __bf16 zs[2][kT][kZ], ds[2][3][kT][kD];
-  __shared__ __attribute__((aligned(16))) float ss[2][kT];
-  __shared__ bf16x8 w2img[OS][3][4][64];
+  __shared__ __attribute__((aligned(16))) _Float16 zs[2][kT][kZ], ds[2][2][kT][kD];
+  // a row's scale, 1 / its dy's power of two, and the product of the two
+  __shared__ __attribute__((aligned(16))) float ss[2][kT], us[2][kT], qs[2][kT];
+  __shared__ f16x8 w2img[OS][2][4][64];
   __shared__ f32x4 sums[kGradThreads];
   auto at = [](int row, int k) { return k ^ (row & 4 ? 8 : 0); };
-  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
-  const int band = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64) * kT;
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, wave = threadIdx.x / 64;
+  const int band = __builtin_amdgcn_readfirstlane(wave) * kT;
   const int64_t r0 = (int64_t)blockIdx.x * chunk_rows, nr = min<int64_t>(chunk_rows, rows - r0);
 
-  Thirds w1v[KS];  // W1[band + c][16 s + 8 h ..]; W2[16 s + 8 h + j][band + c] in LDS, each wave its own
+  Halves w1v[KS];  // W1[band + c][16 s + 8 h ..] p1; W2[16 s + 8 h + j][band + c] p2 in LDS, each wave its own
+  const float bias = b1 != nullptr ? b1[band + c] : 0.0f;
+  Pow2 p1, p2;
   {
     const __amdgpu_buffer_rsrc_t rw1 = rows_rsrc(w1, kHid * nin * 4), rw2 = rows_rsrc(w2, nout * kHid * 4);
+    f32x8 v[KS], x[OS];
+    uint32_t m1 = abs_bits(bias * 0x1p-6f), m2 = 0;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) w1v[s] = split3(load8(rw1, band + c, nin, 16 * s + 8 * h));
+    for (int s = 0; s < KS; ++s) {
+      v[s] = load8(rw1, band + c, nin, 16 * s + 8 * h);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m1 = max(m1, abs_bits(v[s][j]));
+    }
 #pragma unroll
     for (int s = 0; s < OS; ++s) {
-      f32x8 v;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int k = 16 * s + 8 * h + j;
-        v[j] = load1(rw2, k < nout ? (uint32_t)(k * kHid + band + c) * 4u : kPast);
+        x[s][j] = load1(rw2, k < nout ? (uint32_t)(k * kHid + band + c) * 4u : kPast);
+        m2 = max(m2, abs_bits(x[s][j]));
       }
-      const Thirds x = split3(v);
+    }
+    p1 = pow2_for(max(m1, (uint32_t)__shfl_xor((int)m1, 32)));
+    p2 = pow2_for(max(m2, (uint32_t)__shfl_xor((int)m2, 32)));
 #pragma unroll
-      for (int p = 0; p < 3; ++p) w2img[s][p][threadIdx.x / 64][lane] = x.v[p];
+    for (int s = 0; s < KS; ++s) w1v[s] = split(v[s] * p1.p);
+#pragma unroll
+    for (int s = 0; s < OS; ++s) {
+      const Halves q = split(x[s] * p2.p);
+      w2img[s][0][wave][lane] = q.hi;
+      w2img[s][1][wave][lane] = q.lo;
     }
   }
-  const float bias = b1 != nullptr ? b1[band + c] : 0.0f;
+  const float bs = bias * p1.p;
+  Running pg, ph;
   f32x16 acc1[CT], acc2[OT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) acc1[ct] = f32x16{};
@@ -614,12 +708,12 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
   // rows past the chunk load zeros: dy's add nothing
   uint32_t zst[kLZ];
   f32x4 dst[kLD];
-  float sst;
+  float sst[kLD];
   auto load = [&](int64_t t0) {
-    const int64_t left = t0 < nr ? nr - t0 : 0, at = left > 0 ? r0 + t0 : 0, n = left < kT ? left : (int64_t)kT;
-    const __amdgpu_buffer_rsrc_t rz = bytes_rsrc(codes + at * ld, n * ld);
-    const __amdgpu_buffer_rsrc_t rs = rows_rsrc(scale + at, n * 4);
-    const __amdgpu_buffer_rsrc_t rd = rows_rsrc(dy + at * nout, n * nout * 4);
+    const int64_t left = t0 < nr ? nr - t0 : 0, from = left > 0 ? r0 + t0 : 0, n = left < kT ? left : (int64_t)kT;
+    const __amdgpu_buffer_rsrc_t rz = bytes_rsrc(codes + from * ld, n * ld);
+    const __amdgpu_buffer_rsrc_t rs = rows_rsrc(scale + from, n * 4);
+    const __amdgpu_buffer_rsrc_t rd = rows_rsrc(dy + from * nout, n * nout * 4);
 #pragma unroll
     for (int u = 0; u < kLZ; ++u) {
       const int i = u * kGradThreads + (int)threadIdx.x, row = i / kZG, k = 4 * (i % kZG);
@@ -629,37 +723,50 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
     for (int u = 0; u < kLD; ++u) {
       const int i = u * kGradThreads + (int)threadIdx.x, row = i / kDG, k = 4 * (i % kDG);
       dst[u] = load4(rd, k < nout ? (uint32_t)(row * nout + k) * 4u : kPast);
+      sst[u] = load1(rs, (uint32_t)row * 4u);
     }
-    sst = load1(rs, threadIdx.x < kT ? threadIdx.x * 4u : kPast);
   };
   // column reads of a tile's rows: lane i of 16 gives row 4 h + i / 4 and columns 16 (lane / 16 % 2) + 4 (i % 4)
   const int i16 = lane & 15, rrow = 4 * h + (i16 >> 2);
   const int rcol = at(rrow, 16 * ((lane >> 4) & 1) + 4 * (i16 & 3));
+  auto column = [&](const _Float16* tile, int width, int p, int col) {
+    const _Float16* q = tile + (16 * p + rrow) * width + col + rcol;
+    return __builtin_bit_cast(f16x8, join(read_column(q), read_column(q + 8 * width)));
+  };
   load(0);
   int buf = 0;
   for (int64_t t0 = 0; t0 < nr; t0 += kT, buf ^= 1) {
 #pragma unroll
     for (int u = 0; u < kLZ; ++u) {
       const int i = u * kGradThreads + (int)threadIdx.x;
-      *reinterpret_cast<bf16x4*>(&zs[buf][i / kZG][at(i / kZG, 4 * (i % kZG))]) = codes_bf16(zst[u]);
+      *reinterpret_cast<f16x4*>(&zs[buf][i / kZG][at(i / kZG, 4 * (i % kZG))]) = codes_f16(zst[u]);
     }
 #pragma unroll
     for (int u = 0; u < kLD; ++u) {
       const int i = u * kGradThreads + (int)threadIdx.x, row = i / kDG, k = 4 * (i % kDG);
       f32x4 v = dst[u];
+      uint32_t m = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < 4; ++j) {
         if (k + j >= nout) v[j] = 0.0f;  // the next row's
+        m = max(m, abs_bits(v[j]));
+      }
       sb2[u] += v;
+      // the row's lanes are neighbours
 #pragma unroll
-      for (int p = 0; p < 3; ++p) {
-        float x0 = v[0], x1 = v[1], x2 = v[2], x3 = v[3];
-        const u32x2 x = {bf16_pair(x0, x1), bf16_pair(x2, x3)};
-        v = f32x4{x0, x1, x2, x3};
-        *reinterpret_cast<u32x2*>(&ds[buf][p][row][at(row, k)]) = x;
+      for (int s = 1; s < kDG; s *= 2) m = max(m, (uint32_t)__shfl_xor((int)m, s));
+      const Pow2 pd = pow2_for(m);
+      v *= pd.p;
+      const f16x4 hi = __builtin_convertvector(v, f16x4);
+      *reinterpret_cast<f16x4*>(&ds[buf][0][row][at(row, k)]) = hi;
+      *reinterpret_cast<f16x4*>(&ds[buf][1][row][at(row, k)]) =
+          __builtin_convertvector(v - __builtin_convertvector(hi, f32x4), f16x4);
+      if (k == 0) {
+        ss[buf][row] = sst[u];
+        us[buf][row] = pd.ip;
+        qs[buf][row] = pd.ip * sst[u];
       }
     }
-    if (threadIdx.x < kT) ss[buf][threadIdx.x] = sst;
     // one barrier a tile: a wave writes a buffer again only after the next
     // barrier, which every wave reaches after its reads of this one
     __syncthreads();
@@ -669,61 +776,69 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
     f32x16 a = f32x16{}, dh = f32x16{};
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const bf16x8 z8 = *reinterpret_cast<const bf16x8*>(&zs[buf][c][at(c, 16 * s + 8 * h)]);
-      a = mma(z8, w1v[s].v[0], mma(z8, w1v[s].v[1], mma(z8, w1v[s].v[2], a)));
+      const f16x8 z8 = *reinterpret_cast<const f16x8*>(&zs[buf][c][at(c, 16 * s + 8 * h)]);
+      a = mma(z8, w1v[s].hi, mma(z8, w1v[s].lo, a));
     }
 #pragma unroll
     for (int s = 0; s < OS; ++s) {
-      Thirds d, w;
-#pragma unroll
-      for (int p = 0; p < 3; ++p) {
-        d.v[p] = *reinterpret_cast<const bf16x8*>(&ds[buf][p][c][at(c, 16 * s + 8 * h)]);
-        w.v[p] = w2img[s][p][threadIdx.x / 64][lane];
-      }
-      dh = mma(d, w, dh);
+      const int k = at(c, 16 * s + 8 * h);
+      const Halves d = {*reinterpret_cast<const f16x8*>(&ds[buf][0][c][k]),
+                        *reinterpret_cast<const f16x8*>(&ds[buf][1][c][k])};
+      dh = mma(d, Halves{w2img[s][0][wave][lane], w2img[s][1][wave][lane]}, dh);
     }
-    f32x8 hv[2], gv[2];
+    // a by p1, dh by dy's row and p2; then (dh s) and relu(a) / (dy's row)
+    float hv[16], gv[16], hm = 0.0f, gm = 0.0f;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const f32x4 sv = *reinterpret_cast<const f32x4*>(&ss[buf][8 * g + 4 * h]);
+      const f32x4 uv = *reinterpret_cast<const f32x4*>(&us[buf][8 * g + 4 * h]);
+      const f32x4 qv = *reinterpret_cast<const f32x4*>(&qs[buf][8 * g + 4 * h]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float av = a[4 * g + j] * sv[j] + bias;
-        const float d = av <= 0.0f ? 0.0f : dh[4 * g + j];
-        sb1 += d;
-        hv[g / 2][4 * (g % 2) + j] = relu(av);
-        gv[g / 2][4 * (g % 2) + j] = d * sv[j];
+        const float av = a[4 * g + j] * sv[j] + bs;
+        const bool off = av <= 0.0f;  // as torch: a NaN lets the upstream pass
+        const float d = off ? 0.0f : dh[4 * g + j] * p2.ip;
+        sb1 += d * uv[j];
+        gv[4 * g + j] = d * qv[j];
+        hv[4 * g + j] = (off ? 0.0f : av) * uv[j];
+        gm = fmaxf(gm, fabsf(gv[4 * g + j]));
+        hm = fmaxf(hm, fabsf(hv[4 * g + j]));
       }
+    }
+    if (__any(gm * pg.p > 32768.0f || hm * ph.p > 32768.0f)) {
+      scale_sums(acc1, pg.fit(gm));
+      scale_sums(acc2, ph.fit(hm));
     }
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const Thirds hs = split3(hv[p]), gs = split3(gv[p]);
+      f32x8 x, y;
 #pragma unroll
-      for (int o = 0; o < OT; ++o) {
-        Thirds d;
-#pragma unroll
-        for (int q = 0; q < 3; ++q)
-          d.v[q] = __builtin_bit_cast(bf16x8, join(read_column(&ds[buf][q][16 * p + rrow][kT * o + rcol]),
-                                                   read_column(&ds[buf][q][16 * p + 8 + rrow][kT * o + rcol])));
-        acc2[o] = mma(d, hs, acc2[o]);
+      for (int j = 0; j < 8; ++j) {
+        x[j] = hv[8 * p + j] * ph.p;
+        y[j] = gv[8 * p + j] * pg.p;
       }
+      const Halves hs = split(x), gs = split(y);
+#pragma unroll
+      for (int o = 0; o < OT; ++o)
+        acc2[o] = mma(Halves{column(&ds[buf][0][0][0], kD, p, kT * o), column(&ds[buf][1][0][0], kD, p, kT * o)}, hs,
+                      acc2[o]);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        const bf16x8 z8 = __builtin_bit_cast(bf16x8, join(read_column(&zs[buf][16 * p + rrow][kT * ct + rcol]),
-                                                          read_column(&zs[buf][16 * p + 8 + rrow][kT * ct + rcol])));
-        acc1[ct] = mma(gs.v[0], z8, mma(gs.v[1], z8, mma(gs.v[2], z8, acc1[ct])));
+        const f16x8 z = column(&zs[buf][0][0], kZ, p, kT * ct);
+        acc1[ct] = mma(z, gs.hi, mma(z, gs.lo, acc1[ct]));
       }
     }
   }
 
+  // lane l holds hidden unit band + l % 32; registers are inputs or outputs
   const int64_t n1 = (int64_t)kHid * nin, n2 = (int64_t)nout * kHid;
   float* __restrict__ p = part + (int64_t)blockIdx.x * (n1 + kHid + n2 + nout);
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    const int col = kT * ct + c;
-    if (col < nin) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) p[(int64_t)(band + 8 * (r / 4) + 4 * h + r % 4) * nin + col] = acc1[ct][r];
+    for (int r = 0; r < 16; ++r) {
+      const int col = kT * ct + 8 * (r / 4) + 4 * h + r % 4;
+      if (col < nin) p[(int64_t)(band + c) * nin + col] = acc1[ct][r] * pg.ip;
     }
   }
   sb1 += __shfl_xor(sb1, 32);
@@ -733,7 +848,7 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int m = kT * o + 8 * (r / 4) + 4 * h + r % 4;
-      if (m < nout) p[n1 + kHid + (int64_t)m * kHid + band + c] = acc2[o][r];
+      if (m < nout) p[n1 + kHid + (int64_t)m * kHid + band + c] = acc2[o][r] * ph.ip * p1.ip;
     }
   }
   // db2: thread i has summed rows i / kDG (and, with several pieces a thread,
@@ -761,7 +876,7 @@ int64_t grad8_chunks(int64_t rows, int nin, int nout) {
   return rows > 0 ? (rows + c - 1) / c : 0;
 }
 
-constexpr int kMaxKS = (kMaxMlpIn + 15) / 16, kMaxOS = kMaxMlpOut / 16;
+constexpr int kMaxKS = (kMaxMlpIn + 15) / 16, kMaxOS = kMaxMlpOut / 16, kMaxCT = (kMaxMlpIn + kT - 1) / kT;
 
 // Workgroups of the row tile kernels: one a CU, a row tile for each where there
 // are fewer than the waves.
@@ -776,10 +891,10 @@ void run_mlp_rows8_forward(const float* z, const float* w1, const float* b1, con
                            hipStream_t st) {
   if (rows == 0) return;
   const int64_t tiles = (rows + kT - 1) / kT;
-  with_groups<kMaxKS>((nin + 15) / 16, [&](auto ks) {
+  with_groups<kMaxCT>((nin + kT - 1) / kT, [&](auto ct) {
     with_groups<2>(nout <= kT ? 1 : 2, [&](auto ot) {
-      constexpr int KS = decltype(ks)::value, OT = decltype(ot)::value, T = tile_threads(KS > 6 || KS * OT > 6);
-      hipLaunchKernelGGL((k_mlp_forward8<KS, OT, T>), spread_grid(tiles), dim3(T), 0, st, z, w1, b1,
+      constexpr int CT = decltype(ct)::value, OT = decltype(ot)::value, T = tile_threads(CT * OT > 3);
+      hipLaunchKernelGGL((k_mlp_forward8<CT, OT, T>), spread_grid(tiles), dim3(T), 0, st, z, w1, b1,
                          w2, b2, codes, ld, scale, y, rows, nin, nout, tiles);
     });
   });
@@ -797,10 +912,10 @@ void run_mlp_rows8_backward(const int8_t* codes, int64_t ld, const float* scale,
   if (dz != nullptr && rows > 0) {
     int drop = 15;
     for (int n = 1; n < nout; n *= 2) ++drop;
-    with_groups<kMaxKS>((nin + 15) / 16, [&](auto ks) {
-      with_groups<kMaxOS>((nout + 15) / 16, [&](auto os) {
-        constexpr int KS = decltype(ks)::value, OS = decltype(os)::value, T = tile_threads(KS > 6 || KS * OS > 18);
-        hipLaunchKernelGGL((k_mlp_input_grad8<KS, OS, T>), spread_grid(tiles), dim3(T), 0, st,
+    with_groups<kMaxCT>((nin + kT - 1) / kT, [&](auto ct) {
+      with_groups<2>(nout <= kT ? 1 : 2, [&](auto ot) {
+        constexpr int CT = decltype(ct)::value, OT = decltype(ot)::value, T = tile_threads(CT * OT > 3);
+        hipLaunchKernelGGL((k_mlp_input_grad8<CT, OT, T>), spread_grid(tiles), dim3(T), 0, st,
                            codes, ld, scale, dy, w1, b1, w2, dz, rows, nin, nout, drop, tiles);
       });
     });

@@ -112,6 +112,12 @@ __device__ __forceinline__ f16x8 codes_f16(u32x2 w) {
   }
   return __builtin_bit_cast(f16x8, r) - (_Float16)1152.0f;
 }
+__device__ __forceinline__ f16x4 codes_f16(uint32_t w) {
+  const uint32_t u = w ^ 0x80808080u;
+  const u32x2 r = {__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u),
+                   __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)};
+  return __builtin_bit_cast(f16x4, r) - (_Float16)1152.0f;
+}
 __device__ __forceinline__ bf16x4 codes_bf16(uint32_t w) {
   const uint32_t u = w ^ 0x80808080u;
   f32x4 v = {(float)(u & 0xffu), (float)((u >> 8) & 0xffu), (float)((u >> 16) & 0xffu), (float)(u >> 24)};
