@@ -347,7 +347,7 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    load(tile + step);  // in flight until the next tile
+    load(tile + step);  // in flight until the row tile's last stores
     __builtin_amdgcn_sched_barrier(0);
     zt = max(zt, (uint32_t)__shfl_xor((int)zt, 32));
     const RowScale q = row_scale(zt);
@@ -605,39 +605,13 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
 constexpr int kGradThreads = 256;
 constexpr int weight_grad8_waves(int ks, int os) { return ks > 6 || os > 2 ? 1 : 2; }
 
-// A lane's running power of two for sums over rows: where a value would leave a
-// half's range (32768), the scale falls to where 16 times the value still fits,
-// and the sums so far with it.  Both lanes of a column (l and l + 32) keep the
-// same one.
-struct Running {
-  float p = 0x1p126f, ip = 0x1p-126f;
-  // the factor that the lane's sums take, 1 if the scale stays
-  __device__ __forceinline__ float fit(float largest) {
-    largest = fmaxf(largest, __shfl_xor(largest, 32));
-    if (!(largest * p > 32768.0f)) return 1.0f;
-    const Pow2 q = pow2_for(abs_bits(largest));
-    const float old = ip;
-    p = fmaxf(q.p * 0x1p-4f, 0x1p-126f);
-    ip = 1.0f / p;
-    return p * old;
-  }
-};
-template <int N>
-__device__ __forceinline__ void scale_sums(f32x16 (&acc)[N], float f) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] *= f;
-}
-
 // Workgroup = one chunk of rows, wave t the hidden units 32 t .. 32 t + 31 with
-// W1's rows in registers (each by its own power of two, as in w1_image).  A row
-// tile's codes (as halves) and dy's halves (each row by its own power of two)
-// stand in LDS by rows: read along rows they are the operands of a = z W1^T and
-// dh = dy W2, read down columns those of dW1 = codes^T (dh s) and dW2 = dy^T
-// relu(a), whose other operands come in a's and dh's result layout, a hidden
-// unit to a lane.  Sums over rows take a lane's running power of two: what it
-// leaves out of a small row is small against the sums.  The next tile is loaded
-// under this one's products.  The chunk's partial sums: dW1 (128 x nin), db1
-// (128), dW2 (nout x 128), db2 (nout).
+// their weights' pieces in registers.  A row tile's codes (as bfloat16) and
+// dy's pieces stand in LDS by rows: read along rows they are the operands of a
+// = z W1^T and dh = dy W2, read down columns those of dW1 = (dh s)^T codes and
+// dW2 = dy^T relu(a), whose other operands come in a's and dh's result layout.
+// The next tile is loaded under this one's products.  The chunk's partial sums:
+// dW1 (128 x nin), db1 (128), dW2 (nout x 128), db2 (nout).
 template <int KS, int OS>
 __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_mlp_weight_grad8(
     const int8_t* __restrict__ codes, int64_t ld, const float* __restrict__ scale, const float* __restrict__ dy,
@@ -650,51 +624,34 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
   constexpr int kZ = (CT | 1) * kT, kD = (OT | 1) * kT;
   constexpr int kZG = CT * 8, kDG = OT * 8;              // groups of 4 columns a row
   constexpr int kLZ = kT * kZG / kGradThreads, kLD = kT * kDG / kGradThreads;
-  __shared__ __attribute__((aligned(16))) _Float16 zs[2][kT][kZ], ds[2][2][kT][kD];
-  // a row's scale, 1 / its dy's power of two, and the product of the two
-  __shared__ __attribute__((aligned(16))) float ss[2][kT], us[2][kT], qs[2][kT];
-  __shared__ f16x8 w2img[OS][2][4][64];
+  __shared__ __attribute__((aligned(16))) __bf16 zs[2][kT][kZ], ds[2][3][kT][kD];
+  __shared__ __attribute__((aligned(16))) float ss[2][kT];
+  __shared__ bf16x8 w2img[OS][3][4][64];
   __shared__ f32x4 sums[kGradThreads];
   auto at = [](int row, int k) { return k ^ (row & 4 ? 8 : 0); };
-  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5, wave = threadIdx.x / 64;
-  const int band = __builtin_amdgcn_readfirstlane(wave) * kT;
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  const int band = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64) * kT;
   const int64_t r0 = (int64_t)blockIdx.x * chunk_rows, nr = min<int64_t>(chunk_rows, rows - r0);
 
-  Halves w1v[KS];  // W1[band + c][16 s + 8 h ..] p1; W2[16 s + 8 h + j][band + c] p2 in LDS, each wave its own
-  const float bias = b1 != nullptr ? b1[band + c] : 0.0f;
-  Pow2 p1, p2;
+  Thirds w1v[KS];  // W1[band + c][16 s + 8 h ..]; W2[16 s + 8 h + j][band + c] in LDS, each wave its own
   {
     const __amdgpu_buffer_rsrc_t rw1 = rows_rsrc(w1, kHid * nin * 4), rw2 = rows_rsrc(w2, nout * kHid * 4);
-    f32x8 v[KS], x[OS];
-    uint32_t m1 = abs_bits(bias * 0x1p-6f), m2 = 0;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      v[s] = load8(rw1, band + c, nin, 16 * s + 8 * h);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) m1 = max(m1, abs_bits(v[s][j]));
-    }
+    for (int s = 0; s < KS; ++s) w1v[s] = split3(load8(rw1, band + c, nin, 16 * s + 8 * h));
 #pragma unroll
     for (int s = 0; s < OS; ++s) {
+      f32x8 v;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int k = 16 * s + 8 * h + j;
-        x[s][j] = load1(rw2, k < nout ? (uint32_t)(k * kHid + band + c) * 4u : kPast);
-        m2 = max(m2, abs_bits(x[s][j]));
+        v[j] = load1(rw2, k < nout ? (uint32_t)(k * kHid + band + c) * 4u : kPast);
       }
-    }
-    p1 = pow2_for(max(m1, (uint32_t)__shfl_xor((int)m1, 32)));
-    p2 = pow2_for(max(m2, (uint32_t)__shfl_xor((int)m2, 32)));
+      const Thirds x = split3(v);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) w1v[s] = split(v[s] * p1.p);
-#pragma unroll
-    for (int s = 0; s < OS; ++s) {
-      const Halves q = split(x[s] * p2.p);
-      w2img[s][0][wave][lane] = q.hi;
-      w2img[s][1][wave][lane] = q.lo;
+      for (int p = 0; p < 3; ++p) w2img[s][p][threadIdx.x / 64][lane] = x.v[p];
     }
   }
-  const float bs = bias * p1.p;
-  Running pg, ph;
+  const float bias = b1 != nullptr ? b1[band + c] : 0.0f;
   f32x16 acc1[CT], acc2[OT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) acc1[ct] = f32x16{};
@@ -708,12 +665,12 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
   // rows past the chunk load zeros: dy's add nothing
   uint32_t zst[kLZ];
   f32x4 dst[kLD];
-  float sst[kLD];
+  float sst;
   auto load = [&](int64_t t0) {
-    const int64_t left = t0 < nr ? nr - t0 : 0, from = left > 0 ? r0 + t0 : 0, n = left < kT ? left : (int64_t)kT;
-    const __amdgpu_buffer_rsrc_t rz = bytes_rsrc(codes + from * ld, n * ld);
-    const __amdgpu_buffer_rsrc_t rs = rows_rsrc(scale + from, n * 4);
-    const __amdgpu_buffer_rsrc_t rd = rows_rsrc(dy + from * nout, n * nout * 4);
+    const int64_t left = t0 < nr ? nr - t0 : 0, at = left > 0 ? r0 + t0 : 0, n = left < kT ? left : (int64_t)kT;
+    const __amdgpu_buffer_rsrc_t rz = bytes_rsrc(codes + at * ld, n * ld);
+    const __amdgpu_buffer_rsrc_t rs = rows_rsrc(scale + at, n * 4);
+    const __amdgpu_buffer_rsrc_t rd = rows_rsrc(dy + at * nout, n * nout * 4);
 #pragma unroll
     for (int u = 0; u < kLZ; ++u) {
       const int i = u * kGradThreads + (int)threadIdx.x, row = i / kZG, k = 4 * (i % kZG);
@@ -723,50 +680,37 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
     for (int u = 0; u < kLD; ++u) {
       const int i = u * kGradThreads + (int)threadIdx.x, row = i / kDG, k = 4 * (i % kDG);
       dst[u] = load4(rd, k < nout ? (uint32_t)(row * nout + k) * 4u : kPast);
-      sst[u] = load1(rs, (uint32_t)row * 4u);
     }
+    sst = load1(rs, threadIdx.x < kT ? threadIdx.x * 4u : kPast);
   };
   // column reads of a tile's rows: lane i of 16 gives row 4 h + i / 4 and columns 16 (lane / 16 % 2) + 4 (i % 4)
   const int i16 = lane & 15, rrow = 4 * h + (i16 >> 2);
   const int rcol = at(rrow, 16 * ((lane >> 4) & 1) + 4 * (i16 & 3));
-  auto column = [&](const _Float16* tile, int width, int p, int col) {
-    const _Float16* q = tile + (16 * p + rrow) * width + col + rcol;
-    return __builtin_bit_cast(f16x8, join(read_column(q), read_column(q + 8 * width)));
-  };
   load(0);
   int buf = 0;
   for (int64_t t0 = 0; t0 < nr; t0 += kT, buf ^= 1) {
 #pragma unroll
     for (int u = 0; u < kLZ; ++u) {
       const int i = u * kGradThreads + (int)threadIdx.x;
-      *reinterpret_cast<f16x4*>(&zs[buf][i / kZG][at(i / kZG, 4 * (i % kZG))]) = codes_f16(zst[u]);
+      *reinterpret_cast<bf16x4*>(&zs[buf][i / kZG][at(i / kZG, 4 * (i % kZG))]) = codes_bf16(zst[u]);
     }
 #pragma unroll
     for (int u = 0; u < kLD; ++u) {
       const int i = u * kGradThreads + (int)threadIdx.x, row = i / kDG, k = 4 * (i % kDG);
       f32x4 v = dst[u];
-      uint32_t m = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 4; ++j)
         if (k + j >= nout) v[j] = 0.0f;  // the next row's
-        m = max(m, abs_bits(v[j]));
-      }
       sb2[u] += v;
-      // the row's lanes are neighbours
 #pragma unroll
-      for (int s = 1; s < kDG; s *= 2) m = max(m, (uint32_t)__shfl_xor((int)m, s));
-      const Pow2 pd = pow2_for(m);
-      v *= pd.p;
-      const f16x4 hi = __builtin_convertvector(v, f16x4);
-      *reinterpret_cast<f16x4*>(&ds[buf][0][row][at(row, k)]) = hi;
-      *reinterpret_cast<f16x4*>(&ds[buf][1][row][at(row, k)]) =
-          __builtin_convertvector(v - __builtin_convertvector(hi, f32x4), f16x4);
-      if (k == 0) {
-        ss[buf][row] = sst[u];
-        us[buf][row] = pd.ip;
-        qs[buf][row] = pd.ip * sst[u];
+      for (int p = 0; p < 3; ++p) {
+        float x0 = v[0], x1 = v[1], x2 = v[2], x3 = v[3];
+        const u32x2 x = {bf16_pair(x0, x1), bf16_pair(x2, x3)};
+        v = f32x4{x0, x1, x2, x3};
+        *reinterpret_cast<u32x2*>(&ds[buf][p][row][at(row, k)]) = x;
       }
     }
+    if (threadIdx.x < kT) ss[buf][threadIdx.x] = sst;
     // one barrier a tile: a wave writes a buffer again only after the next
     // barrier, which every wave reaches after its reads of this one
     __syncthreads();
@@ -776,69 +720,61 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
     f32x16 a = f32x16{}, dh = f32x16{};
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      const f16x8 z8 = *reinterpret_cast<const f16x8*>(&zs[buf][c][at(c, 16 * s + 8 * h)]);
-      a = mma(z8, w1v[s].hi, mma(z8, w1v[s].lo, a));
+      const bf16x8 z8 = *reinterpret_cast<const bf16x8*>(&zs[buf][c][at(c, 16 * s + 8 * h)]);
+      a = mma(z8, w1v[s].v[0], mma(z8, w1v[s].v[1], mma(z8, w1v[s].v[2], a)));
     }
 #pragma unroll
     for (int s = 0; s < OS; ++s) {
-      const int k = at(c, 16 * s + 8 * h);
-      const Halves d = {*reinterpret_cast<const f16x8*>(&ds[buf][0][c][k]),
-                        *reinterpret_cast<const f16x8*>(&ds[buf][1][c][k])};
-      dh = mma(d, Halves{w2img[s][0][wave][lane], w2img[s][1][wave][lane]}, dh);
+      Thirds d, w;
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        d.v[p] = *reinterpret_cast<const bf16x8*>(&ds[buf][p][c][at(c, 16 * s + 8 * h)]);
+        w.v[p] = w2img[s][p][threadIdx.x / 64][lane];
+      }
+      dh = mma(d, w, dh);
     }
-    // a by p1, dh by dy's row and p2; then (dh s) and relu(a) / (dy's row)
-    float hv[16], gv[16], hm = 0.0f, gm = 0.0f;
+    f32x8 hv[2], gv[2];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const f32x4 sv = *reinterpret_cast<const f32x4*>(&ss[buf][8 * g + 4 * h]);
-      const f32x4 uv = *reinterpret_cast<const f32x4*>(&us[buf][8 * g + 4 * h]);
-      const f32x4 qv = *reinterpret_cast<const f32x4*>(&qs[buf][8 * g + 4 * h]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float av = a[4 * g + j] * sv[j] + bs;
-        const bool off = av <= 0.0f;  // as torch: a NaN lets the upstream pass
-        const float d = off ? 0.0f : dh[4 * g + j] * p2.ip;
-        sb1 += d * uv[j];
-        gv[4 * g + j] = d * qv[j];
-        hv[4 * g + j] = (off ? 0.0f : av) * uv[j];
-        gm = fmaxf(gm, fabsf(gv[4 * g + j]));
-        hm = fmaxf(hm, fabsf(hv[4 * g + j]));
+        const float av = a[4 * g + j] * sv[j] + bias;
+        const float d = av <= 0.0f ? 0.0f : dh[4 * g + j];
+        sb1 += d;
+        hv[g / 2][4 * (g % 2) + j] = relu(av);
+        gv[g / 2][4 * (g % 2) + j] = d * sv[j];
       }
-    }
-    if (__any(gm * pg.p > 32768.0f || hm * ph.p > 32768.0f)) {
-      scale_sums(acc1, pg.fit(gm));
-      scale_sums(acc2, ph.fit(hm));
     }
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      f32x8 x, y;
+      const Thirds hs = split3(hv[p]), gs = split3(gv[p]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[j] = hv[8 * p + j] * ph.p;
-        y[j] = gv[8 * p + j] * pg.p;
+      for (int o = 0; o < OT; ++o) {
+        Thirds d;
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+          d.v[q] = __builtin_bit_cast(bf16x8, join(read_column(&ds[buf][q][16 * p + rrow][kT * o + rcol]),
+                                                   read_column(&ds[buf][q][16 * p + 8 + rrow][kT * o + rcol])));
+        acc2[o] = mma(d, hs, acc2[o]);
       }
-      const Halves hs = split(x), gs = split(y);
-#pragma unroll
-      for (int o = 0; o < OT; ++o)
-        acc2[o] = mma(Halves{column(&ds[buf][0][0][0], kD, p, kT * o), column(&ds[buf][1][0][0], kD, p, kT * o)}, hs,
-                      acc2[o]);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        const f16x8 z = column(&zs[buf][0][0], kZ, p, kT * ct);
-        acc1[ct] = mma(z, gs.hi, mma(z, gs.lo, acc1[ct]));
+        const bf16x8 z8 = __builtin_bit_cast(bf16x8, join(read_column(&zs[buf][16 * p + rrow][kT * ct + rcol]),
+                                                          read_column(&zs[buf][16 * p + 8 + rrow][kT * ct + rcol])));
+        acc1[ct] = mma(gs.v[0], z8, mma(gs.v[1], z8, mma(gs.v[2], z8, acc1[ct])));
       }
     }
   }
 
-  // lane l holds hidden unit band + l % 32; registers are inputs or outputs
   const int64_t n1 = (int64_t)kHid * nin, n2 = (int64_t)nout * kHid;
   float* __restrict__ p = part + (int64_t)blockIdx.x * (n1 + kHid + n2 + nout);
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
+    const int col = kT * ct + c;
+    if (col < nin) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int col = kT * ct + 8 * (r / 4) + 4 * h + r % 4;
-      if (col < nin) p[(int64_t)(band + c) * nin + col] = acc1[ct][r] * pg.ip;
+      for (int r = 0; r < 16; ++r) p[(int64_t)(band + 8 * (r / 4) + 4 * h + r % 4) * nin + col] = acc1[ct][r];
     }
   }
   sb1 += __shfl_xor(sb1, 32);
@@ -848,7 +784,7 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int m = kT * o + 8 * (r / 4) + 4 * h + r % 4;
-      if (m < nout) p[n1 + kHid + (int64_t)m * kHid + band + c] = acc2[o][r] * ph.ip * p1.ip;
+      if (m < nout) p[n1 + kHid + (int64_t)m * kHid + band + c] = acc2[o][r];
     }
   }
   // db2: thread i has summed rows i / kDG (and, with several pieces a thread,
@@ -894,8 +830,8 @@ void run_mlp_rows8_forward(const float* z, const float* w1, const float* b1, con
   with_groups<kMaxCT>((nin + kT - 1) / kT, [&](auto ct) {
     with_groups<2>(nout <= kT ? 1 : 2, [&](auto ot) {
       constexpr int CT = decltype(ct)::value, OT = decltype(ot)::value, T = tile_threads(CT * OT > 3);
-      hipLaunchKernelGGL((k_mlp_forward8<CT, OT, T>), spread_grid(tiles), dim3(T), 0, st, z, w1, b1,
-                         w2, b2, codes, ld, scale, y, rows, nin, nout, tiles);
+      hipLaunchKernelGGL((k_mlp_forward8<CT, OT, T>), spread_grid(tiles), dim3(T), 0, st, z, w1, b1, w2, b2, codes,
+                         ld, scale, y, rows, nin, nout, tiles);
     });
   });
   SPHOPS_LAUNCHED();
