@@ -207,6 +207,110 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_linear8_few(const int8_t* __
   }
 }
 
+// A few short rows (single tokens) in one launch: workgroup = 16 channels, its
+// eight waves a share of the length each, with 16 x 16 x 64 instructions.  Every
+// workgroup puts the rows into 8 bits for itself, into LDS (they come from L2;
+// a launch of their own costs more), while its first weights are on their way.
+// R: rows rounded up to a power of two; N: 16-byte pieces of x a thread holds.
+constexpr int kTokenThreads = 512, kTokenWaves = 8, kTokenCodes = 16384;
+template <class T, int R, int N>
+__global__ __launch_bounds__(kTokenThreads) void k_linear8_token(const T* __restrict__ x, int64_t stride, int cols,
+                                                                 const int8_t* __restrict__ wq, int64_t wld,
+                                                                 const float* __restrict__ ws,
+                                                                 const float* __restrict__ b, T* __restrict__ y,
+                                                                 int rows, int outs, int xld, int share) {
+  constexpr int V = Piece<T>::V, L = kTokenThreads / R;  // threads a row
+  __shared__ __attribute__((aligned(16))) int8_t codes[kTokenCodes + 16 * R];
+  __shared__ uint32_t tops[kTokenWaves];
+  __shared__ float scales[R];
+  __shared__ i32x4 sums[kTokenWaves][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+  const int l = threadIdx.x % L, row = threadIdx.x / L, ld = xld + 16;  // rows of LDS in different banks
+  const T* __restrict__ from = x + (int64_t)min(row, rows - 1) * stride;
+  Piece<T> p[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) p[n].load(from, (n * L + l) * V, cols);
+  const int c = lane & 15, h = lane >> 4, out = (int)blockIdx.x * 16 + c, last = (int)wld - 16;
+  const int8_t* __restrict__ wp = wq + (int64_t)min(out, outs - 1) * wld;
+  const int k0 = wave * share, k1 = min(k0 + share, xld);
+  constexpr int kAhead = 8;  // steps of 64 bytes in flight
+  i32x4 w[kAhead];
+  auto load = [&](int k) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) w[u] = *reinterpret_cast<const i32x4*>(wp + min(k + 64 * u + 16 * h, last));
+  };
+  __builtin_amdgcn_sched_barrier(0);
+  load(k0);
+  __builtin_amdgcn_sched_barrier(0);
+  uint32_t top = 0;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) top = top_of<false>(top, p[n].get(j));
+  }
+#pragma unroll
+  for (int s = 1; s < (L < 64 ? L : 64); s *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, s));
+  if constexpr (L > 64) {
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < L / 64; ++i) top = max(top, tops[row * (L / 64) + i]);
+  }
+  const RowScale q = row_scale(top);
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int k = (n * L + l) * V;
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i)
+      if (k + 4 * i < xld)
+        *reinterpret_cast<uint32_t*>(codes + row * ld + k + 4 * i) =
+            row_codes4(p[n].get(4 * i), p[n].get(4 * i + 1), p[n].get(4 * i + 2), p[n].get(4 * i + 3), q);
+  }
+  if (l == 0) scales[row] = q.scale;
+  __syncthreads();
+  const int8_t* __restrict__ xp = codes + (c & (R - 1)) * ld + 16 * h;  // rows past R again: their sums are not kept
+  i32x4 acc = i32x4{};
+  for (int k = k0; k < k1; k += 64 * kAhead) {
+    if (k != k0) load(k);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (k + 64 * u >= k1) break;
+      acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const i32x4*>(xp + k + 64 * u), w[u], acc, 0, 0, 0);
+    }
+  }
+  sums[wave][lane] = acc;
+  __syncthreads();
+  // result register r of lane l is row 4 (l / 16) + r, channel l % 16
+  if (threadIdx.x >= 16 * R) return;
+  const int at = threadIdx.x / 16, n = threadIdx.x % 16, channel = (int)blockIdx.x * 16 + n;
+  if (at >= rows || channel >= outs) return;
+  int total = 0;
+#pragma unroll
+  for (int i = 0; i < kTokenWaves; ++i) total += sums[i][16 * (at / 4) + n][at % 4];
+  y[(int64_t)at * outs + channel] =
+      from_f32<T>(linear8_value(total, scales[at], ws[channel], b != nullptr ? b[channel] : 0.0f));
+}
+
+// f(integral_constants R, N) if the rows suit k_linear8_token
+template <class T, class F>
+bool with_token(int64_t rows, int64_t cols, int64_t xld, F&& f) {
+  if (rows > 8) return false;
+  auto at = [&](auto r) {
+    constexpr int R = decltype(r)::value, L = kTokenThreads / R, V = Piece<T>::V, kMost = kTokenCodes / R / L / V;
+    if (rows > R || R * xld > kTokenCodes) return false;
+    const int64_t n = (xld / V + L - 1) / L;  // every code up to xld has a thread
+    if constexpr (kMost >= 8) {
+      if (n > 4) return f(r, std::integral_constant<int, 8>{}), true;
+    }
+    if (n > 2) f(r, std::integral_constant<int, 4>{});
+    else if (n > 1) f(r, std::integral_constant<int, 2>{});
+    else f(r, std::integral_constant<int, 1>{});
+    return true;
+  };
+  return at(std::integral_constant<int, 1>{}) || at(std::integral_constant<int, 2>{}) ||
+         at(std::integral_constant<int, 4>{}) || at(std::integral_constant<int, 8>{});
+}
+
 int64_t padded_cols(int64_t cols) { return (cols + kStep - 1) / kStep * kStep; }
 int64_t tiles_of(int64_t n, int tile) { return (n + tile - 1) / tile; }
 
@@ -219,6 +323,20 @@ void run_linear8(const void* x, int type, int64_t stride, const int8_t* wq, int6
                  const float* b, void* y, int64_t rows, int64_t cols, int outs, void* work, hipStream_t st) {
   if (rows == 0) return;
   const int64_t xld = padded_cols(cols);
+  bool done = false;
+  with_type(type, [&](auto t) {
+    using T = decltype(t);
+    done = with_token<T>(rows, cols, xld, [&](auto r, auto n) {
+      const int share = (int)((xld / kTokenWaves + 63) / 64 * 64);
+      hipLaunchKernelGGL((k_linear8_token<T, decltype(r)::value, decltype(n)::value>),
+                         dim3((uint32_t)tiles_of(outs, 16)), dim3(kTokenThreads), 0, st, static_cast<const T*>(x),
+                         stride, (int)cols, wq, wld, ws, b, static_cast<T*>(y), (int)rows, outs, (int)xld, share);
+    });
+  });
+  if (done) {
+    SPHOPS_LAUNCHED();
+    return;
+  }
   int8_t* xq = static_cast<int8_t*>(work);
   float* xs = reinterpret_cast<float*>(xq + rows * xld);
   run_quantize_rows(x, type, stride, xq, xld, xs, rows, cols, false, st);

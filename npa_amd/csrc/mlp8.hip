@@ -60,30 +60,26 @@ __global__ __launch_bounds__(kServeThreads, 2) void k_mlp8(
 
   const int64_t step = (int64_t)gridDim.x * (kServeThreads / 64);
   int64_t tile = (int64_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * (kServeThreads / 64) + threadIdx.x / 64));
-  f32x4 zn[KS][4];
-  auto load = [&](int64_t t) {
-    const int64_t r0 = t * kT, nr = t < tiles ? min<int64_t>(kT, rows - r0) : 0;
-    const __amdgpu_buffer_rsrc_t rz = rows_rsrc(z + (nr > 0 ? r0 * nin : 0), nr * nin * 4);
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) zn[s][i] = load4(rz, (uint32_t)(c * nin + 32 * s + 16 * h + 4 * i) * 4u);
-    }
-  };
-  load(tile);
-  landed(zn);
   for (; tile < tiles; tile += step) {
     asm volatile("" ::: "memory");  // the images stay in LDS: read ahead of the loop they spill
     const int64_t r0 = tile * kT, nr = min<int64_t>(kT, rows - r0);
+    const __amdgpu_buffer_rsrc_t rz = rows_rsrc(z + r0 * nin, nr * nin * 4);
     f32x4 zv[KS][4];
     uint32_t top = 0;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        const int k = 32 * s + 16 * h + 4 * i;
+        zv[s][i] = load4(rz, (uint32_t)(c * nin + k) * 4u);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          zv[s][i][j] = zn[s][i][j];
           // past the row's end lies the next row
           if (s == KS - 1 && 32 * s + 16 * h + 4 * i + j >= nin) zv[s][i][j] = 0.0f;
           top = max(top, abs_bits(zv[s][i][j]));
@@ -105,9 +101,6 @@ __global__ __launch_bounds__(kServeThreads, 2) void k_mlp8(
       for (int t = 0; t < kHT; ++t)
         acc[t] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w1img[s][t][lane], cz, acc[t], 0, 0, 0);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    load(tile + step);  // in flight until the row tile's stores
-    __builtin_amdgcn_sched_barrier(0);
     f32x16 hv[kHT];
     top = 0;
 #pragma unroll
@@ -138,7 +131,6 @@ __global__ __launch_bounds__(kServeThreads, 2) void k_mlp8(
       for (int o = 0; o < OT; ++o)
         out[o] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w2img[t][o][lane], ch, out[o], 0, 0, 0);
     }
-    landed(zn);
     const __amdgpu_buffer_rsrc_t ry = rows_rsrc(y + r0 * nout, nr * nout * 4);
 #pragma unroll
     for (int o = 0; o < OT; ++o) {
@@ -331,7 +323,6 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
     }
   };
   load(tile);
-  landed(zn);
   for (; tile < tiles; tile += step) {
     asm volatile("" ::: "memory");  // the images stay in LDS: read ahead of the loop they spill
     const int64_t r0 = tile * kT, nr = min<int64_t>(kT, rows - r0);
@@ -347,7 +338,7 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    load(tile + step);  // in flight until the row tile's last stores
+    load(tile + step);  // in flight until the next row tile
     __builtin_amdgcn_sched_barrier(0);
     zt = max(zt, (uint32_t)__shfl_xor((int)zt, 32));
     const RowScale q = row_scale(zt);
@@ -404,7 +395,6 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
         for (int o = 0; o < OT; ++o) out[o] = mma(hs, Halves{w2hi[t][p][o][lane], w2lo[t][p][o][lane]}, out[o]);
       }
     }
-    landed(zn);
     // rows are the registers now: their scales come from the lanes that hold them
     float* __restrict__ us = reinterpret_cast<float*>(unit[threadIdx.x / 64]);
     if (h == 0) us[c] = ph.ip;
@@ -509,9 +499,6 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
     sn = load1(rs, (uint32_t)c * 4u);
   };
   load(tile);
-  landed(cn);
-  landed(dn);
-  asm volatile("" : "+v"(sn));
   auto column = [&](int t, int p, int ct) {
     const char* ph = reinterpret_cast<const char*>(&w1hi[2 * ct][t][16 * p]);
     const char* pl = reinterpret_cast<const char*>(&w1lo[2 * ct][t][16 * p]);
@@ -578,9 +565,6 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
         for (int ct = 0; ct < CT; ++ct) out[ct] = mma(hs, column(t, p, ct), out[ct]);
       }
     }
-    landed(cn);
-    landed(dn);
-    asm volatile("" : "+v"(sn));
     // rows are the registers now: their exponents come from the lanes that hold them
     int* __restrict__ es = exps[threadIdx.x / 64];
     if (h == 0) es[c] = (int)(__builtin_bit_cast(uint32_t, pd.ip) >> 23) - 127 + e2;

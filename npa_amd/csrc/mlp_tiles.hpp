@@ -43,21 +43,6 @@ __device__ __forceinline__ f32x16 mma(float a, float b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
 }
 
-// Waits for loads into registers here: a row loop does so before its stores,
-// where the loads have had the row tile's products to land.  The memory counter
-// runs in order, so a wait after the stores, at the loop's head, waits for them
-// too (32 rows of 83 columns stored by each wave: a third of the loop's time).
-template <class T, int N>
-__device__ __forceinline__ void landed(T (&v)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
-}
-template <class T, int N, int M>
-__device__ __forceinline__ void landed(T (&v)[N][M]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) landed(v[i]);
-}
-
 // relu as torch computes it: NaN stays NaN
 __device__ __forceinline__ float relu(float v) { return v <= 0.0f ? 0.0f : v; }
 

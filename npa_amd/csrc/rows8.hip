@@ -17,54 +17,6 @@ namespace {
 
 constexpr int kRowThreads = 256;
 
-// 16 bytes of a row: V values, at any alignment a row can start at.
-template <class T>
-struct Piece {
-  static constexpr int V = 16 / sizeof(T);
-  struct __attribute__((packed, aligned(alignof(T)))) Raw {
-    uint32_t w[4];
-  };
-  Raw raw;
-  __device__ __forceinline__ float get(int j) const {
-    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, raw.w[j]);
-    else return to_f32(__builtin_bit_cast(T, (uint16_t)(raw.w[j / 2] >> (16 * (j % 2)))));
-  }
-  __device__ __forceinline__ void set(int j, T v) {
-    if constexpr (sizeof(T) == 4) raw.w[j] = __builtin_bit_cast(uint32_t, v);
-    else raw.w[j / 2] = (raw.w[j / 2] & (0xffffu << (16 - 16 * (j % 2)))) |
-                        ((uint32_t)__builtin_bit_cast(uint16_t, v) << (16 * (j % 2)));
-  }
-  // values k .. k + V - 1 of a row of `cols`, zeros past it
-  __device__ __forceinline__ void load(const T* __restrict__ row, int k, int cols) {
-    if (k + V <= cols) {
-      raw = *reinterpret_cast<const Raw*>(row + k);
-    } else {
-      raw = Raw{};
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (k + j < cols) set(j, row[k + j]);
-    }
-  }
-  __device__ __forceinline__ void store(T* __restrict__ row, int k, int cols) const {
-    if (k + V <= cols) {
-      *reinterpret_cast<Raw*>(row + k) = raw;
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (k + j < cols) {
-          if constexpr (sizeof(T) == 4) row[k + j] = __builtin_bit_cast(T, raw.w[j]);
-          else row[k + j] = __builtin_bit_cast(T, (uint16_t)(raw.w[j / 2] >> (16 * (j % 2))));
-        }
-      }
-    }
-  }
-};
-
-template <bool RELU>
-__device__ __forceinline__ uint32_t top_of(uint32_t top, float v) {
-  return RELU && v <= 0.0f ? top : max(top, abs_bits(v));
-}
-
 // The codes of one piece, written up to ld (a multiple of 4).
 template <class T, bool RELU>
 __device__ __forceinline__ void write_codes(int8_t* __restrict__ row, const Piece<T>& p, int k, int ld,

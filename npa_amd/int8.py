@@ -187,8 +187,10 @@ def linear(x, w, bias=None):
         raise RuntimeError(f"no integer product for {rows} rows of {cols} inputs and {outs} outputs")
     y = torch.empty(*x.shape[:-1], outs, dtype=x.dtype, device=x.device)
     work = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=x.device)
-    _native.check(_lib.sphops_linear8(_ptr(v), TYPES[x.dtype], stride, _ptr(w.codes), w.codes.shape[1], _ptr(w.scale),
-                                      _ptr(bias), _ptr(y), rows, cols, outs, _ptr(work), _stream(x)))
+    _native.check(_lib.sphops_linear8(
+        v.data_ptr(), TYPES[x.dtype], stride, w.codes.data_ptr(), w.codes.shape[1], w.scale.data_ptr(),
+        None if bias is None else bias.data_ptr(), y.data_ptr(), rows, cols, outs, work.data_ptr(),
+        torch._C._cuda_getCurrentRawStream(x.device.index)))
     return y
 
 
@@ -217,9 +219,11 @@ def mlp(z, w1, b1, w2, b2):
     if rows > MAX_ROWS:
         raise RuntimeError(f"z must have at most {MAX_ROWS} rows")
     y = torch.empty(*z.shape[:-1], nout, device=z.device)
-    _native.check(_lib.sphops_mlp8_forward(_ptr(zc), _ptr(w1.codes), w1.codes.shape[1], _ptr(w1.scale), _ptr(b1),
-                                           _ptr(w2.codes), w2.codes.shape[1], _ptr(w2.scale), _ptr(b2), _ptr(y), rows,
-                                           nin, hidden, nout, _stream(z)))
+    _native.check(_lib.sphops_mlp8_forward(
+        zc.data_ptr(), w1.codes.data_ptr(), w1.codes.shape[1], w1.scale.data_ptr(),
+        None if b1 is None else b1.data_ptr(), w2.codes.data_ptr(), w2.codes.shape[1], w2.scale.data_ptr(),
+        None if b2 is None else b2.data_ptr(), y.data_ptr(), rows, nin, hidden, nout,
+        torch._C._cuda_getCurrentRawStream(z.device.index)))
     return y
 
 

@@ -262,9 +262,18 @@ class ReluLinear8(torch.autograd.Function):
         return da, (dw if need_w else None), (db if need_b else None)
 
 
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
 class MlpRows8(torch.autograd.Function):
-    """``MlpRows`` that keeps z in 8 bits and nothing else: y is computed from z
-    itself, and the backward computes the hidden values of the kept rows again
+    """``MlpRows`` that keeps z in 8 bits and nothing else: one kernel computes y
+    from z itself and writes z's codes (``sphops_mlp_rows8_forward``), and the
+    backward computes the hidden values of the kept rows again
     (``sphops_mlp_rows8_backward``).  The gradients are those of the MLP at the
     kept rows, passed straight through the rounding of z."""
 
@@ -272,41 +281,41 @@ class MlpRows8(torch.autograd.Function):
     def forward(ctx, z, w1, b1, w2, b2):
         hidden, in_f = w1.shape
         out_f = w2.shape[0]
-        z2 = z.reshape(-1, in_f).contiguous()
-        rows = z2.shape[0]
-        dense = [None if t is None else t.detach().contiguous() for t in (w1, b1, w2, b2)]
+        z2 = _dense(z if z.dim() == 2 else z.reshape(-1, in_f))
+        rows, dev = z2.shape[0], z.device
+        dense = [_dense(t) for t in (w1, b1, w2, b2)]
         ctx.shape, ctx.has_b2 = (rows, in_f, hidden, out_f), b2 is not None
-        codes = torch.empty(rows, -(-in_f // 4) * 4, dtype=torch.int8, device=z.device)
-        scale = torch.empty(rows, device=z.device)
-        y = torch.empty(rows, out_f, device=z.device)
-        _native.check(_lib.sphops_mlp_rows8_forward(_ptr(z2), *(_ptr(t) for t in dense), _ptr(codes), codes.shape[1],
-                                                    _ptr(scale), _ptr(y), rows, in_f, hidden, out_f, _stream(z)))
+        codes = torch.empty(rows, -(-in_f // 4) * 4, dtype=torch.int8, device=dev)
+        scale = torch.empty(rows, device=dev)
+        y = torch.empty(rows, out_f, device=dev)
+        _native.check(_lib.sphops_mlp_rows8_forward(
+            z2.data_ptr(), *map(_address, dense), codes.data_ptr(), codes.shape[1], scale.data_ptr(), y.data_ptr(),
+            rows, in_f, hidden, out_f, torch._C._cuda_getCurrentRawStream(dev.index)))
         ctx.save_for_backward(codes, scale, w1, b1, w2)
-        return y.reshape(*z.shape[:-1], out_f)
+        return y if z.dim() == 2 else y.reshape(*z.shape[:-1], out_f)
 
     @staticmethod
     def backward(ctx, dy):
         codes, scale, w1, b1, w2 = ctx.saved_tensors
         need_z, need_w1, need_b1, need_w2, need_b2 = ctx.needs_input_grad
         rows, in_f, hidden, out_f = ctx.shape
-        lead = dy.shape[:-1]
-        dy = dy.reshape(-1, out_f).contiguous()
         if dy.dtype != torch.float32 or not dy.is_cuda:
             raise TypeError("the MLP kernels take float32 GPU tensors")
-        dev = dy.device
+        lead, dev = dy.shape[:-1], dy.device
+        dy = _dense(dy if dy.dim() == 2 else dy.reshape(-1, out_f))
         dz = torch.empty(rows, in_f, device=dev) if need_z else None
         dw1 = torch.empty(hidden, in_f, device=dev) if need_w1 else None
         db1 = torch.empty(hidden, device=dev) if need_b1 and b1 is not None else None
         dw2 = torch.empty(out_f, hidden, device=dev) if need_w2 else None
         db2 = torch.empty(out_f, device=dev) if need_b2 and ctx.has_b2 else None
-        dense = [None if t is None else t.detach().contiguous() for t in (w1, b1, w2)]
-        nbytes = _lib.sphops_mlp_rows8_workspace_bytes(rows, in_f, hidden, out_f)
-        work = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-        _native.check(_lib.sphops_mlp_rows8_backward(_ptr(codes), codes.shape[1], _ptr(scale), _ptr(dy),
-                                                     *(_ptr(t) for t in dense), _ptr(dz), _ptr(dw1), _ptr(db1),
-                                                     _ptr(dw2), _ptr(db2), rows, in_f, hidden, out_f, _ptr(work),
-                                                     _stream(dy)))
-        return None if dz is None else dz.reshape(*lead, in_f), dw1, db1, dw2, db2
+        dense = [_dense(t) for t in (w1, b1, w2)]
+        work = torch.empty(max(_lib.sphops_mlp_rows8_workspace_bytes(rows, in_f, hidden, out_f), 1),
+                           dtype=torch.uint8, device=dev)
+        _native.check(_lib.sphops_mlp_rows8_backward(
+            codes.data_ptr(), codes.shape[1], scale.data_ptr(), dy.data_ptr(), *map(_address, dense),
+            *map(_address, (dz, dw1, db1, dw2, db2)), rows, in_f, hidden, out_f, work.data_ptr(),
+            torch._C._cuda_getCurrentRawStream(dev.index)))
+        return (dz if dz is None or len(lead) == 1 else dz.reshape(*lead, in_f)), dw1, db1, dw2, db2
 
 
 def _rows8_ok(x, layer):
