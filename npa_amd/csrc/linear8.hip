@@ -42,8 +42,7 @@ __device__ __forceinline__ void tile_of(uint32_t id, int mt, int nt, int& m, int
 // pieces are exchanged by the row's low bits (piece p stands at p ^ (row % 8)):
 // the 8 rows that a quarter of a wave's operand read takes then lie in
 // different banks.  For 32 x 32 x 32, lane l supplies 16 bytes of row l % 32 at
-// k = 16 (l / 32), and result register r of lane l is row 8 (r / 4) + 4 (l /
-// 32) + r % 4, channel l % 32.
+// k = 16 (l / 32).
 //
 // xq's rows end in zeros up to a multiple of the step, so what a channel's last
 // step holds past its codes counts nothing; its address is kept inside the row.
@@ -109,7 +108,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear8_tile(const int8_t* __r
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = mma8(a[i], w[j], acc[i][j]);
+        for (int j = 0; j < TN; ++j) acc[i][j] = mma8(w[j], a[i], acc[i][j]);
       }
     }
   };
@@ -129,18 +128,55 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear8_tile(const int8_t* __r
     turn();
   }
   if (end / kStep % 2 != 0) compute(a0, b0);
+  // Result register r of lane l is channel 8 (r / 4) + 4 (l / 32) + r % 4 of row l
+  // % 32: four neighbours at a time go to the wave's own 4 KB of LDS, 32 rows of
+  // UC channels (16-byte pieces exchanged as above), and leave as whole lines.
+  // Stored from the registers, 64 bytes a row, they took 56 us of 370 at 8192 x
+  // 4096 -> 8192.
+  constexpr int V = Piece<T>::V, UC = 32 * TN < 128 / (int)sizeof(T) ? 32 * TN : 128 / (int)sizeof(T);
+  constexpr int kPieces = UC / V, kStores = 32 * kPieces / 64;
+  __syncthreads();  // the last step's panels have been read
+  typedef float f32x4 __attribute__((ext_vector_type(4)));
+  f32x4* const units = reinterpret_cast<f32x4*>(a1);  // the channels' scales, then their biases
+  for (int n = threadIdx.x; n < BN; n += 64 * kWaves) {
+    const int out = min(n0 + n, outs - 1);
+    reinterpret_cast<float*>(units)[n] = ws[out];
+    reinterpret_cast<float*>(units)[BN + n] = b != nullptr ? b[out] : 0.0f;
+  }
+  __syncthreads();
+  int8_t* const own = wave < kWaves / 2 ? a0 + wave * 4096 : b0 + (wave - kWaves / 2) * 4096;
 #pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int out = n0 + wn + 32 * j + c;
-    if (out >= outs) continue;
-    const float s = ws[out], bias = b != nullptr ? b[out] : 0.0f;
+  for (int i = 0; i < TM; ++i) {
+    asm volatile("" ::: "memory");  // the channels' scales stay in LDS
+    const float xscale = xs[min<int64_t>(m0 + wm + 32 * i + c, rows - 1)];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
+    for (int u = 0; u < 32 * TN / UC; ++u) {
+      const int col0 = n0 + wn + UC * u;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int64_t at = m0 + wm + 32 * i + 8 * (r / 4) + 4 * h + r % 4;
-        if (at < rows) y[at * outs + out] = from_f32<T>(linear8_value(acc[i][j][r], xs[at], s, bias));
+      for (int t = 0; t < UC / 32; ++t) {
+        const int j = u * UC / 32 + t;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int at = 32 * t + 8 * q + 4 * h;
+          const f32x4 s = units[(wn + UC * u + at) / 4], bias = units[(BN + wn + UC * u + at) / 4];
+          T v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[e] = from_f32<T>(linear8_value(acc[i][j][4 * q + e], xscale, s[e], bias[e]));
+          __builtin_memcpy(own + c * UC * sizeof(T) + 16 * ((at / V) ^ (c % kPieces)) + at % V * sizeof(T), v,
+                           sizeof(v));
+        }
       }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int n = 0; n < kStores; ++n) {
+        const int row = (64 * n + lane) / kPieces, piece16 = (64 * n + lane) % kPieces;
+        Piece<T> p;
+        __builtin_memcpy(&p.raw, own + row * UC * sizeof(T) + 16 * (piece16 ^ (row % kPieces)), 16);
+        const int64_t to = m0 + wm + 32 * i + row;
+        if (to < rows) p.store(y + to * outs, col0 + V * piece16, outs);
+      }
+      __builtin_amdgcn_wave_barrier();
     }
   }
 }
