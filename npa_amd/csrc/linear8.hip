@@ -202,27 +202,36 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_linear8_few(const int8_t* __
   const int8_t* __restrict__ wp = wq + (int64_t)min(out, outs - 1) * wld;
   const int8_t* xp[RT];
 #pragma unroll
-  for (int t = 0; t < RT; ++t) xp[t] = xq + (int64_t)min(32 * t + c, rows - 1) * xld + 16 * h;
+  for (int t = 0; t < RT; ++t) xp[t] = xq + (int64_t)min(32 * t + c, rows - 1) * xld;
   const int k0 = wave * share, k1 = min(k0 + share, (int)xld), last = (int)wld - 16;
   i32x16 acc[RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) acc[t] = i32x16{};
-  constexpr int kAhead = 8;  // steps of 32 bytes in flight
+  // two steps take 64 bytes of a row, 32 neighbouring ones a lane; up to kAhead
+  // steps of the weights are in flight, the rows' codes kGroup at a time
+  constexpr int kAhead = 16, kGroup = RT > 2 ? 2 : 4;
+  auto at = [&](int k, int u) { return k + 64 * (u / 2) + 32 * h + 16 * (u % 2); };
   for (int k = k0; k < k1; k += 32 * kAhead) {
-    i32x4 w[kAhead], a[kAhead][RT];
+    i32x4 w[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) w[u] = *reinterpret_cast<const i32x4*>(wp + min(k + 32 * u + 16 * h, last));
+    for (int u = 0; u < kAhead; ++u) w[u] = *reinterpret_cast<const i32x4*>(wp + min(at(k, u), last));
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      // past the wave's share: zeros, whatever the weights are
-      const bool on = k + 32 * u < k1;
+    for (int g = 0; g < kAhead; g += kGroup) {
+      if (k + 32 * g >= k1) break;  // uniform; a share is whole groups of 64 bytes
+      i32x4 a[kGroup][RT];
 #pragma unroll
-      for (int t = 0; t < RT; ++t) a[u][t] = on ? *reinterpret_cast<const i32x4*>(xp[t] + k + 32 * u) : i32x4{};
-    }
+      for (int u = 0; u < kGroup; ++u) {
+        // past the wave's share: zeros, whatever the weights are
+        const bool on = k + 64 * ((g + u) / 2) < k1;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
+        for (int t = 0; t < RT; ++t)
+          a[u][t] = on ? *reinterpret_cast<const i32x4*>(xp[t] + at(k, g + u)) : i32x4{};
+      }
 #pragma unroll
-      for (int t = 0; t < RT; ++t) acc[t] = mma8(a[u][t], w[u], acc[t]);
+      for (int u = 0; u < kGroup; ++u) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) acc[t] = mma8(a[u][t], w[g + u], acc[t]);
+      }
     }
   }
   __syncthreads();
@@ -380,7 +389,7 @@ void run_linear8(const void* x, int type, int64_t stride, const int8_t* wq, int6
     using T = decltype(t);
     T* out = static_cast<T*>(y);
     if (rows <= 128) {
-      const int share = (int)(((xld + kFewWaves - 1) / kFewWaves + 31) / 32 * 32);
+      const int share = (int)((xld / kFewWaves + 63) / 64 * 64);
       auto few = [&](auto rt) {
         hipLaunchKernelGGL((k_linear8_few<T, decltype(rt)::value>), dim3((uint32_t)tiles_of(outs, 32)),
                            dim3(64 * kFewWaves), 0, st, xq, xld, xs, wq, wld, ws, b, out, (int)rows, outs, share);
