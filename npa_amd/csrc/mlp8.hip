@@ -616,6 +616,8 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int band = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64) * kT;
   const int64_t r0 = (int64_t)blockIdx.x * chunk_rows, nr = min<int64_t>(chunk_rows, rows - r0);
+  // Every second chunk takes -dy, and its sums change sign at the end: see split16.hpp
+  const float sign = blockIdx.x & 1 ? -1.0f : 1.0f;
 
   Thirds w1v[KS];  // W1[band + c][16 s + 8 h ..]; W2[16 s + 8 h + j][band + c] in LDS, each wave its own
   {
@@ -686,6 +688,7 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
       for (int j = 0; j < 4; ++j)
         if (k + j >= nout) v[j] = 0.0f;  // the next row's
       sb2[u] += v;
+      v *= sign;
 #pragma unroll
       for (int p = 0; p < 3; ++p) {
         float x0 = v[0], x1 = v[1], x2 = v[2], x3 = v[3];
@@ -758,17 +761,17 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
     const int col = kT * ct + c;
     if (col < nin) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) p[(int64_t)(band + 8 * (r / 4) + 4 * h + r % 4) * nin + col] = acc1[ct][r];
+      for (int r = 0; r < 16; ++r) p[(int64_t)(band + 8 * (r / 4) + 4 * h + r % 4) * nin + col] = acc1[ct][r] * sign;
     }
   }
   sb1 += __shfl_xor(sb1, 32);
-  if (h == 0) p[n1 + band + c] = sb1;
+  if (h == 0) p[n1 + band + c] = sb1 * sign;
 #pragma unroll
   for (int o = 0; o < OT; ++o) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int m = kT * o + 8 * (r / 4) + 4 * h + r % 4;
-      if (m < nout) p[n1 + kHid + (int64_t)m * kHid + band + c] = acc2[o][r];
+      if (m < nout) p[n1 + kHid + (int64_t)m * kHid + band + c] = acc2[o][r] * sign;
     }
   }
   // db2: thread i has summed rows i / kDG (and, with several pieces a thread,

@@ -238,7 +238,8 @@ __global__ __launch_bounds__(64 * WO * WI, 2) void k_rows8_weight_grad(
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64), wo = wave % WO, wi = wave / WO;
   const int block = (int)blockIdx.y, o0 = block / i_blocks * WO * 32, i0 = block % i_blocks * kIT * 32;
   const int64_t r0 = (int64_t)blockIdx.x * chunk_rows, left = rows - r0, nr = left < chunk_rows ? left : chunk_rows;
-  // dy's rows are `nout` apart at any alignment of 4 bytes; codes' are ld apart
+  // every second chunk takes -dy, and its sums change sign at the end: see split16.hpp
+  const float sign = blockIdx.x & 1 ? -1.0f : 1.0f;
   uint32_t cst[kLC];
   f32x4 dst[kLD];
   float sst[kLD];
@@ -292,7 +293,7 @@ __global__ __launch_bounds__(64 * WO * WI, 2) void k_rows8_weight_grad(
       for (int j = 0; j < 4; ++j)
         if (o0 + k + j >= nout) v[j] = 0.0f;  // the next row's
       sb[u] += v;
-      v *= sst[u];
+      v *= sst[u] * sign;
 #pragma unroll
       for (int p = 0; p < 3; ++p) {
         float x0 = v[0], x1 = v[1], x2 = v[2], x3 = v[3];
@@ -331,7 +332,7 @@ __global__ __launch_bounds__(64 * WO * WI, 2) void k_rows8_weight_grad(
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int m = o0 + 32 * wo + 8 * (r / 4) + 4 * h + r % 4;
-      if (m < nout) p[(int64_t)m * nin + col] = acc[t][r];
+      if (m < nout) p[(int64_t)m * nin + col] = acc[t][r] * sign;
     }
   }
   if (i0 != 0) return;
