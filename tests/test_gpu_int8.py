@@ -148,6 +148,23 @@ def test_linear_at_larger_sizes(rows, cols, outs, dtype):
     _check_linear(rows, cols, outs, dtype)
 
 
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 8, 9])
+def test_linear_of_single_tokens(rows):
+    """Few rows of every length that shares out over a workgroup's threads and
+    waves, and lengths and row counts past that."""
+    for cols in (5, 64, 127, 129, 1000, 2048, 4095, 4097, 8192, 16383, 16384, 16385):
+        _check_linear(rows, cols, 35, (F32, BF16, F16)[cols % 3])
+    _check_linear(rows, 4096, 4096, BF16, ld=128)
+
+
+@pytest.mark.parametrize("rows,outs", [(4097, 3333), (1500, 2008), (700, 131), (65600, 33)])
+@pytest.mark.parametrize("cols", [70, 128, 200, 300, 400])
+def test_linear_tiles(rows, cols, outs):
+    """Ragged tiles of every size, channel counts that are no multiple of a
+    store's, and even and odd numbers of steps."""
+    _check_linear(rows, cols, outs, (F32, BF16, F16)[(rows + cols) % 3], bias=cols != 200)
+
+
 def test_linear_extremes():
     """The largest sums (all codes 127, both signs), padded weights, rows that are not finite, strides."""
     from npa_amd import int8
@@ -286,6 +303,26 @@ def test_weight_grad_of_many_rows(rows, cols, outs):
     dw, db = int8.weight_grad(r, dy)
     for got, ref in ((dw, dy.double().T @ kept), (db, dy.double().sum(0))):
         assert ((got.double() - ref).norm() <= 4e-6 * ref.norm()).item()
+
+
+def test_gradients_of_sums_that_cancel():
+    """Over 2^19 rows of random sign the errors of the matrix cores' sums, all of
+    one sign, would add up to 4e-6 of db1; rounding alone leaves under 1e-6."""
+    from npa_amd import int8
+    from npa_amd import mlp as M
+    net, g = _net(83, 19, True, 2)
+    z = torch.randn(1 << 19, 83, device="cuda", generator=g)
+    up = torch.randn(1 << 19, 19, device="cuda", generator=g)
+    w1, b1, w2 = (t.detach().double() for t in (net[0].weight, net[0].bias, net[2].weight))
+    zd = _kept(z)
+    a = zd @ w1.T + b1
+    up[(a.abs() < 1e-5).any(1)] = 0
+    M.mlp(net, z, checkpoint="int8").backward(up)
+    da = (up.double() @ w2) * (a > 0)
+    for got, ref in ((net[0].weight.grad, da.T @ zd), (net[0].bias.grad, da.sum(0)),
+                     (net[2].weight.grad, up.double().T @ a.clamp_min(0)),
+                     (int8.weight_grad(int8.quantize_rows(z), up)[0], up.double().T @ zd)):
+        assert ((got.double() - ref).norm() <= 1.5e-6 * ref.norm()).item()
 
 
 def test_weight_grad_ranges():
