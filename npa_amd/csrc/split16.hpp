@@ -63,8 +63,10 @@ __device__ __forceinline__ Halves split(f32x8 v) {
   Halves r;
   r.hi = __builtin_convertvector(v, f16x8);
   f32x8 rest;
+  float minus = -1.0f;
+  asm("" : "+v"(minus));  // keeps the subtraction one mixed-precision multiply-add
 #pragma unroll
-  for (int j = 0; j < 8; ++j) rest[j] = __builtin_fmaf((float)r.hi[j], -1.0f, v[j]);  // one mixed-precision instruction
+  for (int j = 0; j < 8; ++j) rest[j] = __builtin_fmaf((float)r.hi[j], minus, v[j]);
   r.lo = __builtin_convertvector(rest, f16x8);
   return r;
 }
