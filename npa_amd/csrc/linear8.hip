@@ -38,7 +38,7 @@ __device__ __forceinline__ void tile_of(uint32_t id, int mt, int nt, int& m, int
 
 // Workgroup = a tile of BM rows by BN channels, WM x WN waves of BM / WM by BN
 // / WN each.  A step of 128 bytes of both panels goes from memory straight to
-// LDS under the products of the step before.  In LDS a row's eight 16-byte
+// LDS, S - 1 steps ahead of its products.  In LDS a row's eight 16-byte
 // pieces are exchanged by the row's low bits (piece p stands at p ^ (row % 8)):
 // the 8 rows that a quarter of a wave's operand read takes then lie in
 // different banks.  For 32 x 32 x 32, lane l supplies 16 bytes of row l % 32 at
@@ -46,7 +46,7 @@ __device__ __forceinline__ void tile_of(uint32_t id, int mt, int nt, int& m, int
 //
 // xq's rows end in zeros up to a multiple of the step, so what a channel's last
 // step holds past its codes counts nothing; its address is kept inside the row.
-template <class T, int BM, int BN, int WM, int WN>
+template <class T, int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__(64 * WM * WN) void k_linear8_tile(const int8_t* __restrict__ xq, int64_t xld,
                                                                const float* __restrict__ xs,
                                                                const int8_t* __restrict__ wq, int64_t wld,
@@ -56,8 +56,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear8_tile(const int8_t* __r
   constexpr int kWaves = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
   constexpr int kLoadsA = BM / 8 / kWaves, kLoadsB = BN / 8 / kWaves;  // a wave's loads of 8 rows a step
   static_assert(kLoadsA * 8 * kWaves == BM && kLoadsB * 8 * kWaves == BN, "whole loads");
+  static_assert(S == 2 || S == 4, "stages");
   // separate arrays: a load into one is no reason to wait before a read of the other
-  __shared__ __attribute__((aligned(16))) int8_t a0[BM * kStep], b0[BN * kStep], a1[BM * kStep], b1[BN * kStep];
+  constexpr int kStage = (BM + BN) * kStep;  // the rows' panel, then the channels'
+  __shared__ __attribute__((aligned(16))) int8_t s0[kStage], s1[kStage], s2[S > 2 ? kStage : 16], s3[S > 2 ? kStage : 16];
+  auto stage = [&](int i) { return i == 0 ? s0 : i == 1 ? s1 : i == 2 ? s2 : s3; };
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
   const int c = lane & 31, h = lane >> 5;
   int mi, ni;
@@ -79,7 +82,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear8_tile(const int8_t* __r
     ob[i] = (uint32_t)min((i * kWaves + wave) * 8 + (lane >> 3), outs_here - 1) * (uint32_t)wld;
   const int last = (int)wld - 16, end = (int)xld;
   // past the last step: the last one again, which nothing reads
-  auto load = [&](int k, int8_t* as, int8_t* bs) {
+  auto load = [&](int k, int8_t* as) {
+    int8_t* const bs = as + BM * kStep;
     k = min(k, end - kStep);
     const int8_t* __restrict__ ak = ap + k;
 #pragma unroll
@@ -96,7 +100,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear8_tile(const int8_t* __r
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = i32x16{};
   }
-  auto compute = [&](const int8_t* as, const int8_t* bs) {
+  auto compute = [&](const int8_t* as) {
+    const int8_t* const bs = as + BM * kStep;
 #pragma unroll
     for (int s = 0; s < kStep / 32; ++s) {
       const int at = c * kStep + 16 * ((2 * s + h) ^ (c & 7));
@@ -112,22 +117,35 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear8_tile(const int8_t* __r
       }
     }
   };
-  // every wave's loads of a step have landed, and every wave has read the step before
-  auto turn = [&] {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-    __syncthreads();
-  };
-  load(0, a0, b0);
-  turn();
-  for (int k = 0; k + kStep < end; k += 2 * kStep) {
-    load(k + kStep, a1, b1);
-    compute(a0, b0);
-    turn();
-    load(k + 2 * kStep, a0, b0);
-    compute(a1, b1);
-    turn();
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) load(i * kStep, stage(i));
+  // every wave's loads of a step have landed (vmcnt: `later` may be in flight),
+  // and every wave has read the step before (lgkmcnt(0)), whose place the next
+  // load takes
+#define SPHOPS_TURN(later)                           \
+  asm volatile("" ::: "memory");                     \
+  __builtin_amdgcn_sched_barrier(0);                 \
+  __builtin_amdgcn_s_waitcnt(0x0070 | (later));      \
+  __builtin_amdgcn_s_barrier();                      \
+  __builtin_amdgcn_sched_barrier(0);                 \
+  asm volatile("" ::: "memory")
+  const int steps = end / kStep;
+  int k = 0;
+  for (int g = 0; g < steps / S; ++g) {
+#pragma unroll
+    for (int i = 0; i < S; ++i, k += kStep) {
+      SPHOPS_TURN((S - 2) * (kLoadsA + kLoadsB));
+      load(k + (S - 1) * kStep, stage((i + S - 1) % S));
+      compute(stage(i));
+    }
   }
-  if (end / kStep % 2 != 0) compute(a0, b0);
+  // the steps that are left, and no load in flight where LDS is used again below
+  SPHOPS_TURN(0);
+#undef SPHOPS_TURN
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) {
+    if (i < steps % S) compute(stage(i));
+  }
   // Result register r of lane l is channel 8 (r / 4) + 4 (l / 32) + r % 4 of row l
   // % 32: four neighbours at a time go to the wave's own 4 KB of LDS, 32 rows of
   // UC channels (16-byte pieces exchanged as above), and leave as whole lines.
@@ -137,14 +155,15 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear8_tile(const int8_t* __r
   constexpr int kPieces = UC / V, kStores = 32 * kPieces / 64;
   __syncthreads();  // the last step's panels have been read
   typedef float f32x4 __attribute__((ext_vector_type(4)));
-  f32x4* const units = reinterpret_cast<f32x4*>(a1);  // the channels' scales, then their biases
+  f32x4* const units = reinterpret_cast<f32x4*>(s1);  // the channels' scales, then their biases
   for (int n = threadIdx.x; n < BN; n += 64 * kWaves) {
     const int out = min(n0 + n, outs - 1);
     reinterpret_cast<float*>(units)[n] = ws[out];
     reinterpret_cast<float*>(units)[BN + n] = b != nullptr ? b[out] : 0.0f;
   }
   __syncthreads();
-  int8_t* const own = wave < kWaves / 2 ? a0 + wave * 4096 : b0 + (wave - kWaves / 2) * 4096;
+  static_assert(kWaves * 4096 <= kStage && 8 * BN <= kStage, "room");
+  int8_t* const own = s0 + wave * 4096;
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     asm volatile("" ::: "memory");  // the channels' scales stay in LDS
@@ -181,83 +200,12 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear8_tile(const int8_t* __r
   }
 }
 
-// Few rows: workgroup = 32 channels and all the rows (RT tiles of 32), its
-// eight waves a share of the row's length each; both operands come straight
-// from memory in the matrix instruction's layout (the weights once, the rows
-// from L2), and the waves' sums meet in LDS.  Integer sums: any order gives the
-// same value.
-constexpr int kFewWaves = 8;
-template <class T, int RT>
-__global__ __launch_bounds__(64 * kFewWaves) void k_linear8_few(const int8_t* __restrict__ xq, int64_t xld,
-                                                                const float* __restrict__ xs,
-                                                                const int8_t* __restrict__ wq, int64_t wld,
-                                                                const float* __restrict__ ws,
-                                                                const float* __restrict__ b, T* __restrict__ y,
-                                                                int rows, int outs, int share) {
-  __shared__ int sums[RT][16][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
-  const int c = lane & 31, h = lane >> 5;
-  const int out = (int)blockIdx.x * 32 + c;
-  for (int i = threadIdx.x; i < RT * 16 * 64; i += 64 * kFewWaves) (&sums[0][0][0])[i] = 0;
-  const int8_t* __restrict__ wp = wq + (int64_t)min(out, outs - 1) * wld;
-  const int8_t* xp[RT];
-#pragma unroll
-  for (int t = 0; t < RT; ++t) xp[t] = xq + (int64_t)min(32 * t + c, rows - 1) * xld;
-  const int k0 = wave * share, k1 = min(k0 + share, (int)xld), last = (int)wld - 16;
-  i32x16 acc[RT];
-#pragma unroll
-  for (int t = 0; t < RT; ++t) acc[t] = i32x16{};
-  // two steps take 64 bytes of a row, 32 neighbouring ones a lane; up to kAhead
-  // steps of the weights are in flight, the rows' codes kGroup at a time
-  constexpr int kAhead = 16, kGroup = RT > 2 ? 2 : 4;
-  auto at = [&](int k, int u) { return k + 64 * (u / 2) + 32 * h + 16 * (u % 2); };
-  for (int k = k0; k < k1; k += 32 * kAhead) {
-    i32x4 w[kAhead];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) w[u] = *reinterpret_cast<const i32x4*>(wp + min(at(k, u), last));
-#pragma unroll
-    for (int g = 0; g < kAhead; g += kGroup) {
-      if (k + 32 * g >= k1) break;  // uniform; a share is whole groups of 64 bytes
-      i32x4 a[kGroup][RT];
-#pragma unroll
-      for (int u = 0; u < kGroup; ++u) {
-        // past the wave's share: zeros, whatever the weights are
-        const bool on = k + 64 * ((g + u) / 2) < k1;
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-          a[u][t] = on ? *reinterpret_cast<const i32x4*>(xp[t] + at(k, g + u)) : i32x4{};
-      }
-#pragma unroll
-      for (int u = 0; u < kGroup; ++u) {
-#pragma unroll
-        for (int t = 0; t < RT; ++t) acc[t] = mma8(a[u][t], w[g + u], acc[t]);
-      }
-    }
-  }
-  __syncthreads();
-  if (k0 < k1) {
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) atomicAdd(&sums[t][r][lane], acc[t][r]);
-    }
-  }
-  __syncthreads();
-  if (out >= outs) return;
-  const float s = ws[out], bias = b != nullptr ? b[out] : 0.0f;
-#pragma unroll
-  for (int i = 0; i < RT * 16 / kFewWaves; ++i) {
-    const int e = i * kFewWaves + wave, t = e / 16, r = e % 16, at = 32 * t + 8 * (r / 4) + 4 * h + r % 4;
-    if (at < rows) y[(int64_t)at * outs + out] = from_f32<T>(linear8_value(sums[t][r][lane], xs[at], s, bias));
-  }
-}
-
 // A few short rows (single tokens) in one launch: workgroup = 16 channels, its
 // eight waves a share of the length each, with 16 x 16 x 64 instructions.  Every
 // workgroup puts the rows into 8 bits for itself, into LDS (they come from L2;
 // a launch of their own costs more), while its first weights are on their way.
 // R: rows rounded up to a power of two; N: 16-byte pieces of x a thread holds.
-constexpr int kTokenThreads = 512, kTokenWaves = 8, kTokenCodes = 16384;
+constexpr int kTokenThreads = 512, kTokenWaves = 8, kTokenRows = 16, kTokenCodes = 32768;
 template <class T, int R, int N>
 __global__ __launch_bounds__(kTokenThreads) void k_linear8_token(const T* __restrict__ x, int64_t stride, int cols,
                                                                  const int8_t* __restrict__ wq, int64_t wld,
@@ -339,21 +287,23 @@ __global__ __launch_bounds__(kTokenThreads) void k_linear8_token(const T* __rest
 // f(integral_constants R, N) if the rows suit k_linear8_token
 template <class T, class F>
 bool with_token(int64_t rows, int64_t cols, int64_t xld, F&& f) {
-  if (rows > 8) return false;
+  if (rows > kTokenRows) return false;
   auto at = [&](auto r) {
     constexpr int R = decltype(r)::value, L = kTokenThreads / R, V = Piece<T>::V, kMost = kTokenCodes / R / L / V;
     if (rows > R || R * xld > kTokenCodes) return false;
     const int64_t n = (xld / V + L - 1) / L;  // every code up to xld has a thread
-    if constexpr (kMost >= 8) {
-      if (n > 4) return f(r, std::integral_constant<int, 8>{}), true;
+    if constexpr (kMost >= 16) {
+      if (n > 8) return f(r, std::integral_constant<int, 16>{}), true;
     }
-    if (n > 2) f(r, std::integral_constant<int, 4>{});
+    if (n > 4) f(r, std::integral_constant<int, 8>{});
+    else if (n > 2) f(r, std::integral_constant<int, 4>{});
     else if (n > 1) f(r, std::integral_constant<int, 2>{});
     else f(r, std::integral_constant<int, 1>{});
     return true;
   };
   return at(std::integral_constant<int, 1>{}) || at(std::integral_constant<int, 2>{}) ||
-         at(std::integral_constant<int, 4>{}) || at(std::integral_constant<int, 8>{});
+         at(std::integral_constant<int, 4>{}) || at(std::integral_constant<int, 8>{}) ||
+         at(std::integral_constant<int, 16>{});
 }
 
 int64_t padded_cols(int64_t cols) { return (cols + kStep - 1) / kStep * kStep; }
@@ -388,29 +338,18 @@ void run_linear8(const void* x, int type, int64_t stride, const int8_t* wq, int6
   with_type(type, [&](auto t) {
     using T = decltype(t);
     T* out = static_cast<T*>(y);
-    if (rows <= 128) {
-      const int share = (int)((xld / kFewWaves + 63) / 64 * 64);
-      auto few = [&](auto rt) {
-        hipLaunchKernelGGL((k_linear8_few<T, decltype(rt)::value>), dim3((uint32_t)tiles_of(outs, 32)),
-                           dim3(64 * kFewWaves), 0, st, xq, xld, xs, wq, wld, ws, b, out, (int)rows, outs, share);
-      };
-      if (rows <= 32) few(std::integral_constant<int, 1>{});
-      else if (rows <= 64) few(std::integral_constant<int, 2>{});
-      else few(std::integral_constant<int, 4>{});
-      return;
-    }
-    auto tile = [&](auto bm, auto bn, auto wm, auto wn) {
+    auto tile = [&](auto bm, auto bn, auto wm, auto wn, auto stages) {
       constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value,
                     WN = decltype(wn)::value;
       const int64_t mt = tiles_of(rows, BM), nt = tiles_of(outs, BN);
-      hipLaunchKernelGGL((k_linear8_tile<T, BM, BN, WM, WN>), dim3((uint32_t)(mt * nt)), dim3(64 * WM * WN), 0, st,
+      hipLaunchKernelGGL((k_linear8_tile<T, BM, BN, WM, WN, decltype(stages)::value>), dim3((uint32_t)(mt * nt)), dim3(64 * WM * WN), 0, st,
                          xq, xld, xs, wq, wld, ws, b, out, rows, outs, (int)mt, (int)nt);
     };
 #define SPHOPS_N(n) std::integral_constant<int, n>{}
-    if (tiles_of(rows, 256) * tiles_of(outs, 256) >= 192) tile(SPHOPS_N(256), SPHOPS_N(256), SPHOPS_N(2), SPHOPS_N(4));
+    if (tiles_of(rows, 256) * tiles_of(outs, 256) >= 192) tile(SPHOPS_N(256), SPHOPS_N(256), SPHOPS_N(2), SPHOPS_N(4), SPHOPS_N(2));
     else if (tiles_of(rows, 128) * tiles_of(outs, 128) >= 192)
-      tile(SPHOPS_N(128), SPHOPS_N(128), SPHOPS_N(2), SPHOPS_N(2));
-    else tile(SPHOPS_N(64), SPHOPS_N(64), SPHOPS_N(2), SPHOPS_N(2));
+      tile(SPHOPS_N(128), SPHOPS_N(128), SPHOPS_N(2), SPHOPS_N(2), SPHOPS_N(2));
+    else tile(SPHOPS_N(64), SPHOPS_N(64), SPHOPS_N(2), SPHOPS_N(2), SPHOPS_N(4));
 #undef SPHOPS_N
   });
   SPHOPS_LAUNCHED();

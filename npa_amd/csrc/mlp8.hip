@@ -164,14 +164,10 @@ void run_mlp8(const float* z, const int8_t* w1, int64_t ld1, const float* s1, co
 
 namespace {
 
-
 // ---------------------------------------------------------------- training
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t bytes_rsrc(const int8_t* base, int64_t bytes) {
   return rows_rsrc(reinterpret_cast<const float*>(base), bytes);
-}
-__device__ __forceinline__ u32x2 load2(__amdgpu_buffer_rsrc_t r, uint32_t off) {
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
 }
 
 // Eight values of a row of n from column k (zeros past it), through a resource
@@ -803,8 +799,9 @@ constexpr int kMaxKS = (kMaxMlpIn + 15) / 16, kMaxOS = kMaxMlpOut / 16, kMaxCT =
 
 // Workgroups of the row tile kernels: one a CU, a row tile for each where there
 // are fewer than the waves.
-// Their threads: two waves a SIMD, or one where two would spill.
-constexpr int tile_threads(bool wide) { return wide ? 256 : 512; }
+// Their threads: two waves a SIMD where 256 registers hold a row tile (CT + OT
+// up to 6 forward and 5 backward: neither spills), else one.
+constexpr int tile_threads(int ct_ot, int most) { return ct_ot <= most ? 512 : 256; }
 inline dim3 spread_grid(int64_t tiles) { return dim3((uint32_t)std::min<int64_t>(256, tiles)); }
 
 }  // namespace
@@ -816,7 +813,7 @@ void run_mlp_rows8_forward(const float* z, const float* w1, const float* b1, con
   const int64_t tiles = (rows + kT - 1) / kT;
   with_groups<kMaxCT>((nin + kT - 1) / kT, [&](auto ct) {
     with_groups<2>(nout <= kT ? 1 : 2, [&](auto ot) {
-      constexpr int CT = decltype(ct)::value, OT = decltype(ot)::value, T = tile_threads(CT * OT > 3);
+      constexpr int CT = decltype(ct)::value, OT = decltype(ot)::value, T = tile_threads(CT + OT, 6);
       hipLaunchKernelGGL((k_mlp_forward8<CT, OT, T>), spread_grid(tiles), dim3(T), 0, st, z, w1, b1, w2, b2, codes,
                          ld, scale, y, rows, nin, nout, tiles);
     });
@@ -837,7 +834,7 @@ void run_mlp_rows8_backward(const int8_t* codes, int64_t ld, const float* scale,
     for (int n = 1; n < nout; n *= 2) ++drop;
     with_groups<kMaxCT>((nin + kT - 1) / kT, [&](auto ct) {
       with_groups<2>(nout <= kT ? 1 : 2, [&](auto ot) {
-        constexpr int CT = decltype(ct)::value, OT = decltype(ot)::value, T = tile_threads(CT * OT > 3);
+        constexpr int CT = decltype(ct)::value, OT = decltype(ot)::value, T = tile_threads(CT + OT, 5);
         hipLaunchKernelGGL((k_mlp_input_grad8<CT, OT, T>), spread_grid(tiles), dim3(T), 0, st,
                            codes, ld, scale, dy, w1, b1, w2, dz, rows, nin, nout, drop, tiles);
       });

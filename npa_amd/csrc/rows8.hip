@@ -420,8 +420,9 @@ void run_rows8_weight_grad(const int8_t* codes, int64_t ld, const float* scale, 
     });
     SPHOPS_LAUNCHED();
   }
-  // few chunks: a thread an element; many: the workgroups of linear_grad.hip share them out
-  if (p.chunks <= 16)
+  // few chunks, or enough elements to fill the card: a thread an element; else the
+  // workgroups of linear_grad.hip share an element's chunks out
+  if (p.chunks <= 16 || (p.chunks <= 64 && n >= 131072))
     hipLaunchKernelGGL(k_rows8_sum, dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, work, dw, db, nw, nout,
                        p.chunks);
   else

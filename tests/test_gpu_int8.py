@@ -165,6 +165,22 @@ def test_linear_tiles(rows, cols, outs):
     _check_linear(rows, cols, outs, (F32, BF16, F16)[(rows + cols) % 3], bias=cols != 200)
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 32768), (1, 32769), (2, 16385), (6, 4095), (8, 4096), (8, 4097), (9, 1),
+                                       (10, 83), (13, 1000), (15, 2047), (16, 2048), (16, 2049), (17, 64)])
+def test_linear_of_a_few_tokens(rows, cols):
+    """Rows that one launch holds and the first that it does not, in each type."""
+    for dtype in (F32, BF16, F16):
+        _check_linear(rows, cols, 37, dtype)
+
+
+@pytest.mark.parametrize("rows,outs", [(17, 5), (64, 64), (65, 130), (190, 600)])
+def test_linear_of_each_number_of_steps(rows, outs):
+    """1 to 10 steps of 128 columns, whole and begun ones."""
+    for steps in range(1, 11):
+        _check_linear(rows, 128 * steps, outs, BF16)
+        _check_linear(rows, 128 * steps - 127, outs, F32, bias=steps % 2 == 0)
+
+
 def test_linear_extremes():
     """The largest sums (all codes 127, both signs), padded weights, rows that are not finite, strides."""
     from npa_amd import int8
@@ -387,6 +403,12 @@ def test_mlp_with_checkpoint_matches_float64(shape, rows):
     _within("dW2", net[2].weight.grad, ud.T @ h, n * (ud.abs().T @ h) + ud.abs().T @ ea)
     if net[2].bias is not None:
         _within("db2", net[2].bias.grad, ud.sum(0), n * ud.abs().sum(0))
+
+
+@pytest.mark.parametrize("shape", [(150, 35), (165, 20), (112, 40)])
+def test_mlp_with_checkpoint_at_more_widths(shape):
+    test_mlp_with_checkpoint_matches_float64(shape, 65)
+    test_mlp_with_checkpoint_matches_float64(shape, 9000)
 
 
 @pytest.mark.parametrize("rows,shape", [(300001, (83, 19)), (300001, (163, 40)), (32769, (130, 32)), (100000, (66, 18))])
