@@ -124,10 +124,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear8_tile(const int8_t* __r
   // load takes
 #define SPHOPS_TURN(later)                           \
   asm volatile("" ::: "memory");                     \
-  __builtin_amdgcn_sched_barrier(0);                 \
   __builtin_amdgcn_s_waitcnt(0x0070 | (later));      \
   __builtin_amdgcn_s_barrier();                      \
-  __builtin_amdgcn_sched_barrier(0);                 \
   asm volatile("" ::: "memory")
   const int steps = end / kStep;
   int k = 0;

@@ -799,9 +799,11 @@ constexpr int kMaxKS = (kMaxMlpIn + 15) / 16, kMaxOS = kMaxMlpOut / 16, kMaxCT =
 
 // Workgroups of the row tile kernels: one a CU, a row tile for each where there
 // are fewer than the waves.
-// Their threads: two waves a SIMD where 256 registers hold a row tile (CT + OT
-// up to 6 forward and 5 backward: neither spills), else one.
-constexpr int tile_threads(int ct_ot, int most) { return ct_ot <= most ? 512 : 256; }
+// Their threads: two waves a SIMD where 256 registers hold a row tile, else one.
+// At 2^18 rows, us with two and one (the bounds' last and first past): forward
+// 112 -> 35 59 and 70, 150 -> 19 66 and 75, 163 -> 19 97 and 81, 130 -> 35 91 and 78;
+// input gradient with autograd's part 112 -> 35 163 and 171, 150 -> 19 205 and 177.
+constexpr int tile_threads(bool two) { return two ? 512 : 256; }
 inline dim3 spread_grid(int64_t tiles) { return dim3((uint32_t)std::min<int64_t>(256, tiles)); }
 
 }  // namespace
@@ -813,7 +815,7 @@ void run_mlp_rows8_forward(const float* z, const float* w1, const float* b1, con
   const int64_t tiles = (rows + kT - 1) / kT;
   with_groups<kMaxCT>((nin + kT - 1) / kT, [&](auto ct) {
     with_groups<2>(nout <= kT ? 1 : 2, [&](auto ot) {
-      constexpr int CT = decltype(ct)::value, OT = decltype(ot)::value, T = tile_threads(CT + OT, 6);
+      constexpr int CT = decltype(ct)::value, OT = decltype(ot)::value, T = tile_threads(CT + OT <= 6);
       hipLaunchKernelGGL((k_mlp_forward8<CT, OT, T>), spread_grid(tiles), dim3(T), 0, st, z, w1, b1, w2, b2, codes,
                          ld, scale, y, rows, nin, nout, tiles);
     });
@@ -834,7 +836,7 @@ void run_mlp_rows8_backward(const int8_t* codes, int64_t ld, const float* scale,
     for (int n = 1; n < nout; n *= 2) ++drop;
     with_groups<kMaxCT>((nin + kT - 1) / kT, [&](auto ct) {
       with_groups<2>(nout <= kT ? 1 : 2, [&](auto ot) {
-        constexpr int CT = decltype(ct)::value, OT = decltype(ot)::value, T = tile_threads(CT + OT, 5);
+        constexpr int CT = decltype(ct)::value, OT = decltype(ot)::value, T = tile_threads(CT <= 4);
         hipLaunchKernelGGL((k_mlp_input_grad8<CT, OT, T>), spread_grid(tiles), dim3(T), 0, st,
                            codes, ld, scale, dy, w1, b1, w2, dz, rows, nin, nout, drop, tiles);
       });
