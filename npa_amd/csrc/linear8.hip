@@ -44,6 +44,12 @@ __device__ __forceinline__ void tile_of(uint32_t id, int mt, int nt, int& m, int
 // different banks.  For 32 x 32 x 32, lane l supplies 16 bytes of row l % 32 at
 // k = 16 (l / 32).
 //
+// Bound: the matrix cores and the loads' latency under them: 8192 x 4096 -> 8192
+// in 266 us with the 19 of putting x into 8 bits (2.2 POP/s; the library's int8
+// product alone 255), 4096^3 80.  The 256 and 128 tiles take 2 stages (4 for the
+// 128: 1024 x 4096 -> 4096 34 us for 35, but 2048 rows 60 for 53), the 64 tile, whose
+// workgroups are few and wait on memory, 4 (128 x 4096 -> 4096 15 us, 2 stages 21).
+//
 // xq's rows end in zeros up to a multiple of the step, so what a channel's last
 // step holds past its codes counts nothing; its address is kept inside the row.
 template <class T, int BM, int BN, int WM, int WN, int S>
@@ -202,6 +208,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linear8_tile(const int8_t* __r
 // eight waves a share of the length each, with 16 x 16 x 64 instructions.  Every
 // workgroup puts the rows into 8 bits for itself, into LDS (they come from L2;
 // a launch of their own costs more), while its first weights are on their way.
+// Bound: latency, then the weights' bytes: 1 x 4096 -> 4096 in 4.7 us (a launch
+// takes 4.2), 1 x 8192 -> 8192 in 13.5 (5.0 TB/s).
 // R: rows rounded up to a power of two; N: 16-byte pieces of x a thread holds.
 constexpr int kTokenThreads = 512, kTokenWaves = 8, kTokenRows = 16, kTokenCodes = 32768;
 template <class T, int R, int N>
@@ -282,7 +290,10 @@ __global__ __launch_bounds__(kTokenThreads) void k_linear8_token(const T* __rest
       from_f32<T>(linear8_value(total, scales[at], ws[channel], b != nullptr ? b[channel] : 0.0f));
 }
 
-// f(integral_constants R, N) if the rows suit k_linear8_token
+// f(integral_constants R, N) if the rows suit k_linear8_token: their codes fit 32
+// KB.  Against two launches with the 64 tile: 1 x 4096 -> 4096 4.7 and 13.4 us, 16 x
+// 2048 -> 2048 float32 5.8 and 9.5, 16 x 2048 -> 8192 8.7 and 9.8, 8 x 4096 -> 16384
+// 17.2 and 17.6: every workgroup's own work on the rows has used up the gain there.
 template <class T, class F>
 bool with_token(int64_t rows, int64_t cols, int64_t xld, F&& f) {
   if (rows > kTokenRows) return false;
@@ -344,6 +355,9 @@ void run_linear8(const void* x, int type, int64_t stride, const int8_t* wq, int6
                          xq, xld, xs, wq, wld, ws, b, out, rows, outs, (int)mt, (int)nt);
     };
 #define SPHOPS_N(n) std::integral_constant<int, n>{}
+    // the largest tile of which there are three for every four CUs; us with tiles of
+    // 256, 128 and 64: 4096 x 4096 -> 4096 (256 of the first) 79, 89, 118; 2048 x 4096 ->
+    // 4096 (128; 512 of the second) 64, 51, 70; 512 x 4096 -> 4096 (32; 128) 58, 31, 24
     if (tiles_of(rows, 256) * tiles_of(outs, 256) >= 192) tile(SPHOPS_N(256), SPHOPS_N(256), SPHOPS_N(2), SPHOPS_N(4), SPHOPS_N(2));
     else if (tiles_of(rows, 128) * tiles_of(outs, 128) >= 192)
       tile(SPHOPS_N(128), SPHOPS_N(128), SPHOPS_N(2), SPHOPS_N(2), SPHOPS_N(2));

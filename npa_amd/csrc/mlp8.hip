@@ -22,6 +22,9 @@ constexpr int kServeThreads = 256;
 // units 8 q + 4 (l / 32) + 0..3 of its row: packed to one word each they are
 // the second product's operand, with W2's image in the same order, so hidden
 // codes never leave registers.  KS: steps of 32 input columns; OT: output tiles.
+//
+// Bound: HBM, 4 (nin + nout) bytes a row: 2^20 x 83 -> 19 in 93 us (4.6 TB/s); 4096
+// rows 7 us, the weights' images and one row tile's latency.
 template <int KS, int OT>
 __global__ __launch_bounds__(kServeThreads, 2) void k_mlp8(
     const float* __restrict__ z, const int8_t* __restrict__ w1, int64_t ld1, const float* __restrict__ s1,
@@ -190,8 +193,7 @@ __device__ __forceinline__ void store_columns(__amdgpu_buffer_rsrc_t r, int widt
 
 // The columns that a lane of half h holds of step s of a product over a row: two
 // steps take 16 neighbouring ones, so that a lane's loads of a row are whole
-// 64-byte pieces.  (With 8 columns a step and half, lines left L1 between the
-// four loads that share one.)
+// 64-byte pieces.
 __device__ __forceinline__ constexpr int step_column(int s, int h) { return 32 * (s / 2) + 16 * h + 8 * (s % 2); }
 
 // W1 in halves as an operand image: lane l's 16 bytes of entry (s, t), at
@@ -251,6 +253,11 @@ __device__ __forceinline__ void w1_image(const float* __restrict__ w1, const flo
 // as they stand they are an operand with W2's image in the same order, and as
 // the first operand they leave y's rows in registers and its columns in lanes,
 // whose stores are whole.
+//
+// Three products of halves each (split16.hpp).  2^20 rows, 83 -> 19: 150..170 us
+// (0.52 GB, 101 at the rate of a copy): matrix
+// instructions and the splits' vector ones overlap, at a clock that falls to 1.2
+// GHz under them.  More waves, operands read ahead or z through LDS gained nothing.
 template <int CT, int OT, int kThreads>
 __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
     const float* __restrict__ z, const float* __restrict__ w1, const float* __restrict__ b1,
@@ -421,6 +428,9 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
 // in for W1; the row's own power of two keeps dy and dh in range: |dy| <= 2^15,
 // |W2| <= 2^15 in the image, so |dh| <= 2^30 nout, and 2^-drop brings it to
 // 2^15.
+//
+// Bound: as the forward's; 2^20 rows, 83 -> 19 in 178 us.  dz's stores are whole
+// lines because rows are registers in its product.
 template <int CT, int OT, int kThreads>
 __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
     const int8_t* __restrict__ codes, int64_t ld, const float* __restrict__ scale, const float* __restrict__ dy,
@@ -583,6 +593,8 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
 // ------------------------------------------------ training: weight gradients
 
 constexpr int kGradThreads = 256;
+// Waves a SIMD: two where they do not spill.  us with one and two: 2^20 rows, 83 ->
+// 19 408 and 361 with the forward; 2^18, 112 -> 19 145 and 158, 83 -> 35 142 and 150.
 constexpr int weight_grad8_waves(int ks, int os) { return ks > 6 || os > 2 ? 1 : 2; }
 
 // Workgroup = one chunk of rows, wave t the hidden units 32 t .. 32 t + 31 with
@@ -592,6 +604,11 @@ constexpr int weight_grad8_waves(int ks, int os) { return ks > 6 || os > 2 ? 1 :
 // dW2 = dy^T relu(a), whose other operands come in a's and dh's result layout.
 // The next tile is loaded under this one's products.  The chunk's partial sums:
 // dW1 (128 x nin), db1 (128), dW2 (nout x 128), db2 (nout).
+//
+// Six products of bfloat16 pieces, three against codes: halves with a running
+// power of two were faster at 2^20 rows (205 us for 245) and slower at 65 K (62 for
+// 48).  Bound: matrix and vector work in one wave in turn, two waves a SIMD; 2^20
+// rows, 83 -> 19 in 190..260 us as the clock allows.
 template <int KS, int OS>
 __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_mlp_weight_grad8(
     const int8_t* __restrict__ codes, int64_t ld, const float* __restrict__ scale, const float* __restrict__ dy,

@@ -44,6 +44,10 @@ __device__ __forceinline__ void write_codes(int8_t* __restrict__ row, const Piec
 // RELU the row kept is relu(x), and no positive value has the code 0: a code is
 // positive exactly where x is.  L = 256: the workgroup's four waves share a
 // row.
+//
+// Bound: HBM, x read once and a quarter of it written: 2^20 x 83 float32 in 91
+// us (4.8 TB/s), 65536 x 163 in 11.  Rows of 2-byte values that start at odd
+// places lose a third: 8191 x 4097 bfloat16 32 us, 8192 x 4096 20.
 template <class T, bool RELU, int L, int N>
 __global__ __launch_bounds__(kRowThreads) void k_quantize_rows(const T* __restrict__ x, int64_t stride,
                                                                int8_t* __restrict__ codes, int64_t ld,
@@ -81,8 +85,9 @@ __global__ __launch_bounds__(kRowThreads) void k_quantize_rows(const T* __restri
   }
 }
 
-// Rows of any length: a workgroup a row, which is read twice (the second time
-// from cache).
+// Rows longer than a workgroup's registers hold: a workgroup a row, which is
+// read twice (the second time from cache).  4096 x 8192 float32: 44 us, 26 with
+// the row in registers.
 template <class T, bool RELU>
 __global__ __launch_bounds__(kRowThreads) void k_quantize_long_rows(const T* __restrict__ x, int64_t stride,
                                                                     int8_t* __restrict__ codes, int64_t ld,
@@ -116,6 +121,8 @@ __global__ __launch_bounds__(kRowThreads) void k_quantize_long_rows(const T* __r
 }
 
 // L lanes a row (256 / L rows a workgroup's turn), 16 bytes of the result a lane.
+// Bound: HBM, mostly the result's stores: 65536 x 163 float32 in 13.5 us (4.0
+// TB/s), 8191 x 4097 bfloat16, at odd places, in 17.4 (5.8 TB/s).
 template <class T, int L>
 __global__ __launch_bounds__(kRowThreads) void k_restore_rows(const int8_t* __restrict__ codes, int64_t ld,
                                                               const float* __restrict__ scale, T* __restrict__ out,
@@ -142,7 +149,10 @@ dim3 row_grid(int64_t rows, int rows_a_turn) {
   return dim3((uint32_t)std::min<int64_t>((rows + rows_a_turn - 1) / rows_a_turn, 16384));
 }
 
-// f(integral_constant L, integral_constant N) for rows of `pieces` 16-byte pieces; false: longer than all of them
+// f(integral_constant L, integral_constant N) for rows of `pieces` 16-byte pieces;
+// false: longer than all of them.  Few lanes with about four pieces
+// each: with 64 lanes for every row of up to 192 pieces 65536 rows of 16, 83,
+// 163, 200 and 600 float32 take 14, 16, 16, 15 and 28 us instead of 3, 5, 11, 11 and 28.
 template <class F>
 bool with_lanes(int64_t pieces, F&& f) {
   auto at = [&](auto l, auto n) {
@@ -196,6 +206,7 @@ void run_restore_rows(const int8_t* codes, int64_t ld, const float* scale, void*
       hipLaunchKernelGGL((k_restore_rows<T, L>), row_grid(rows, kRowThreads / L), dim3(kRowThreads), 0, st, codes, ld,
                          scale, static_cast<T*>(out), rows, (int)cols);
     };
+    // 65536 rows of 16 and of 83 float32: 3.4 and 8.5 us, with 64 lanes 7.2 and 10.6
     if (pieces <= 8) launch(std::integral_constant<int, 8>{});
     else if (pieces <= 16) launch(std::integral_constant<int, 16>{});
     else if (pieces <= 32) launch(std::integral_constant<int, 32>{});
@@ -218,6 +229,10 @@ namespace {
 // down their columns.  A row of LDS is an odd number of 64 bytes: the four rows
 // of a column read then lie in different banks.  The next step's rows are
 // loaded under this one's products.
+//
+// Bound: HBM where blocks are few (2^20 rows, 83 -> 128: 136 us, 4.7 TB/s of codes
+// and dy), the matrix cores where dW is wide (8192 rows, 2048 -> 2048: 190..220 us
+// with its sum, three products at 1.0 PFLOP/s; the library's float32 product 505).
 struct Grad8Plan {
   int wo, wi, ni, o_blocks, i_blocks;
   int64_t chunk_rows, chunks;
@@ -380,6 +395,12 @@ void with_block(const Grad8Plan& p, F&& f) {
   else ni(c4, c2);
 }
 
+// Waves: as many along the outputs as there are tiles, the rest along the inputs;
+// eight where both are many, which halves what a block reads (262144 rows, 256 ->
+// 256 123 us, four 182; 65536 rows, 163 -> 128 22 and 26).  Chunks: one for every
+// workgroup the card holds at once, two a CU or one of eight waves (2^20 rows, 83
+// -> 128 136 us, half as many chunks 179, twice 147; 8192 rows, 2048 -> 2048 191,
+// 332 and 198), of at least two steps.
 Grad8Plan grad8_plan(int64_t rows, int nin, int nout) {
   Grad8Plan p;
   const int ot = (nout + 31) / 32, it = (nin + 31) / 32;
@@ -421,7 +442,9 @@ void run_rows8_weight_grad(const int8_t* codes, int64_t ld, const float* scale, 
     SPHOPS_LAUNCHED();
   }
   // few chunks, or enough elements to fill the card: a thread an element; else the
-  // workgroups of linear_grad.hip share an element's chunks out
+  // workgroups of linear_grad.hip share an element's chunks out.  Whole gradient:
+  // 512 rows, 2048 -> 2048 (8 chunks) 34 and 142 us; 8192, 512 -> 512 (32) 27 and 34;
+  // 65536, 256 -> 256 (128 chunks, 65792 elements) 45 and 38.
   if (p.chunks <= 16 || (p.chunks <= 64 && n >= 131072))
     hipLaunchKernelGGL(k_rows8_sum, dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, work, dw, db, nw, nout,
                        p.chunks);
