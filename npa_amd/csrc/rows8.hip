@@ -47,7 +47,9 @@ __device__ __forceinline__ void write_codes(int8_t* __restrict__ row, const Piec
 //
 // Bound: HBM, x read once and a quarter of it written: 2^20 x 83 float32 in 91
 // us (4.8 TB/s), 65536 x 163 in 11.  Rows of 2-byte values that start at odd
-// places lose a third: 8191 x 4097 bfloat16 32 us, 8192 x 4096 20.
+// places lose a quarter where they come from memory: 8191 x 4097 bfloat16 23 us,
+// 8192 x 4096 19.  (Loads moved to even places, with the codes shifted between
+// lanes, took 20.6 there and 10% longer where x is in cache.)
 template <class T, bool RELU, int L, int N>
 __global__ __launch_bounds__(kRowThreads) void k_quantize_rows(const T* __restrict__ x, int64_t stride,
                                                                int8_t* __restrict__ codes, int64_t ld,
@@ -152,7 +154,9 @@ dim3 row_grid(int64_t rows, int rows_a_turn) {
 // f(integral_constant L, integral_constant N) for rows of `pieces` 16-byte pieces;
 // false: longer than all of them.  Few lanes with about four pieces
 // each: with 64 lanes for every row of up to 192 pieces 65536 rows of 16, 83,
-// 163, 200 and 600 float32 take 14, 16, 16, 15 and 28 us instead of 3, 5, 11, 11 and 28.
+// 163, 200 and 600 float32 take 14, 16, 16, 15 and 28 us instead of 3, 5, 11, 11 and
+// 28.  Long rows in steps of a lane's piece: 8191 x 4097 bfloat16, 513 pieces, 23 us
+// with nine a lane and 32 with twelve.
 template <class F>
 bool with_lanes(int64_t pieces, F&& f) {
   auto at = [&](auto l, auto n) {
@@ -163,8 +167,9 @@ bool with_lanes(int64_t pieces, F&& f) {
 #define SPHOPS_LANES(L, N) at(std::integral_constant<int, L>{}, std::integral_constant<int, N>{})
   return SPHOPS_LANES(4, 1) || SPHOPS_LANES(8, 1) || SPHOPS_LANES(8, 2) || SPHOPS_LANES(8, 3) ||
          SPHOPS_LANES(16, 2) || SPHOPS_LANES(16, 3) || SPHOPS_LANES(16, 4) || SPHOPS_LANES(32, 3) ||
-         SPHOPS_LANES(32, 4) || SPHOPS_LANES(64, 3) || SPHOPS_LANES(64, 4) || SPHOPS_LANES(64, 6) ||
-         SPHOPS_LANES(64, 8) || SPHOPS_LANES(64, 12) || SPHOPS_LANES(256, 4) || SPHOPS_LANES(256, 8);
+         SPHOPS_LANES(32, 4) || SPHOPS_LANES(64, 3) || SPHOPS_LANES(64, 4) || SPHOPS_LANES(64, 5) ||
+         SPHOPS_LANES(64, 6) || SPHOPS_LANES(64, 7) || SPHOPS_LANES(64, 8) || SPHOPS_LANES(64, 9) ||
+         SPHOPS_LANES(64, 10) || SPHOPS_LANES(64, 12) || SPHOPS_LANES(256, 4) || SPHOPS_LANES(256, 8);
 #undef SPHOPS_LANES
 }
 

@@ -102,6 +102,23 @@ def test_strides_alignments_and_leading_dimensions():
         _check_rows(x)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("cols", [63, 64, 65, 71, 72, 73, 95, 127, 128, 191, 255, 256, 383, 511, 767, 1023, 1535, 2047,
+                                  3000, 4095, 6143, 6144, 6145, 8193])
+def test_rows_at_odd_places(cols, dtype):
+    """Rows of 2-byte values that start between words: all of them, every second
+    one, a single one; the largest value first, last or not finite."""
+    flat = torch.randn(1 + 9 * (cols + 1), device="cuda", generator=_gen(cols)).to(dtype)
+    flat[0] = flat[-1] = 10000  # outside every row below
+    for start, stride in ((1, cols + cols % 2), (0, cols + 1 - cols % 2), (1, cols + 1 - cols % 2)):
+        x = torch.as_strided(flat, (8, cols), (stride, 1), start)
+        _check_rows(x, relu=cols % 4 == 3)
+        _check_rows(x[:1])
+    x[2, 0], x[3, -1], x[4, cols // 2], x[5, 0], x[6, -1] = 77, -88, float("nan"), float("inf"), float("nan")
+    _check_rows(x, align=16)
+    _check_rows(x, relu=True)
+
+
 def test_no_rows():
     from npa_amd import int8
     r = int8.quantize_rows(torch.empty(0, 83, device="cuda"))
