@@ -22,6 +22,7 @@ computed from it is NaN.
   with integer products, a scale for each row and each output channel.
 """
 import ctypes
+import functools
 from typing import NamedTuple, Tuple
 
 import torch
@@ -231,16 +232,19 @@ class _Checkpoint(torch.autograd.Function):
     @staticmethod
     def forward(ctx, function, x, *params):
         r = quantize_rows(x)
-        ctx.function, ctx.shape, ctx.dtype, ctx.params = function, r.shape, x.dtype, len(params)
+        ctx.function, ctx.shape, ctx.dtype = function, r.shape, x.dtype
+        # without its cache, which would keep casts of params made here without a graph
+        ctx.autocast = functools.partial(torch.autocast, "cuda", torch.get_autocast_dtype("cuda"),
+                                         torch.is_autocast_enabled("cuda"), cache_enabled=False)
         ctx.save_for_backward(r.codes, r.scale, *params)
-        with torch.no_grad():
+        with torch.no_grad(), ctx.autocast():
             return function(x, *params)
 
     @staticmethod
     def backward(ctx, dy):
         codes, scale, *params = ctx.saved_tensors
         needs = ctx.needs_input_grad[1:]
-        with torch.enable_grad():
+        with torch.enable_grad(), ctx.autocast():
             x = restore_rows(Rows8(codes, scale, ctx.shape), ctx.dtype).requires_grad_(needs[0])
             params = [p.detach().requires_grad_(n) for p, n in zip(params, needs[1:])]
             y = ctx.function(x, *params)
@@ -251,7 +255,8 @@ class _Checkpoint(torch.autograd.Function):
 
 def checkpoint(function, x, *params):
     """``function(x, *params)``, one tensor, that keeps x in 8 bits for its
-    backward: there x is restored and the function runs again with gradients.
+    backward: there x is restored and the function runs again with gradients,
+    under the forward's autocast; it must not draw random numbers.
     The rounding of x is passed straight through.  ``params``: the tensors
     besides x that gradients are wanted of."""
     _check_rows(x, "x")

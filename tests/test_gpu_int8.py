@@ -554,6 +554,23 @@ def test_checkpoint_of_a_function():
     assert not int8.checkpoint(f, fixed, w.detach()).requires_grad
 
 
+def test_checkpoint_of_a_function_under_autocast():
+    """The second run is under the forward's autocast: the same gradients as autograd's there."""
+    from npa_amd import int8
+    g = _gen(8)
+    x = torch.randn(40, 64, device="cuda", generator=g).requires_grad_(True)
+    m = torch.randn(64, 32, device="cuda", generator=g).requires_grad_(True)
+    up = torch.randn(40, 32, device="cuda", generator=g).to(BF16)
+    f = lambda v, w: torch.tanh(v @ w)
+    with torch.autocast("cuda", BF16):
+        y = int8.checkpoint(f, x, m)
+        kept = int8.restore_rows(int8.quantize_rows(x)).requires_grad_(True)
+        ref = f(kept, m)
+    assert y.dtype == BF16
+    for got, want in zip(torch.autograd.grad(y, [x, m], up), torch.autograd.grad(ref, [kept, m], up)):
+        assert got.dtype == F32 and torch.equal(got, want)
+
+
 def test_special_rows_with_checkpoint():
     """A row that is not finite gives NaN where it reaches: its own dz stays the
     upstream's product or NaN, no other row's changes."""
