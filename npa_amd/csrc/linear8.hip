@@ -357,8 +357,11 @@ void run_linear8(const void* x, int type, int64_t stride, const int8_t* wq, int6
 #define SPHOPS_N(n) std::integral_constant<int, n>{}
     // the largest tile of which there are three for every four CUs; us with tiles of
     // 256, 128 and 64: 4096 x 4096 -> 4096 (256 of the first) 79, 89, 118; 2048 x 4096 ->
-    // 4096 (128; 512 of the second) 64, 51, 70; 512 x 4096 -> 4096 (32; 128) 58, 31, 24
-    if (tiles_of(rows, 256) * tiles_of(outs, 256) >= 192) tile(SPHOPS_N(256), SPHOPS_N(256), SPHOPS_N(2), SPHOPS_N(4), SPHOPS_N(2));
+    // 4096 (128; 512 of the second) 64, 51, 70; 512 x 4096 -> 4096 (32; 128) 58, 31, 24.
+    // Up to 128 channels half of a 256 tile counts for nothing: 65536 x 1024 -> 100 56,
+    // 48, 55; 2^20 x 83 -> 128 float32 320, 268, 387; -> 160 56, 59, 63.
+    if (outs > 128 && tiles_of(rows, 256) * tiles_of(outs, 256) >= 192)
+      tile(SPHOPS_N(256), SPHOPS_N(256), SPHOPS_N(2), SPHOPS_N(4), SPHOPS_N(2));
     else if (tiles_of(rows, 128) * tiles_of(outs, 128) >= 192)
       tile(SPHOPS_N(128), SPHOPS_N(128), SPHOPS_N(2), SPHOPS_N(2), SPHOPS_N(2));
     else tile(SPHOPS_N(64), SPHOPS_N(64), SPHOPS_N(2), SPHOPS_N(2), SPHOPS_N(4));
