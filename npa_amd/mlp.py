@@ -357,8 +357,8 @@ def mlp(module, z, checkpoint=None):
     through ``LinearRows``; any other module runs as it is.
 
     ``checkpoint="int8"``: what the layers keep for the backward is kept in 8
-    bits (``MlpRows8``, ``ReluLinear8``, ``LinearRows8``): y is the same, the
-    weight gradients are those of inputs rounded to their codes."""
+    bits (``MlpRows8``, ``ReluLinear8``, ``LinearRows8``): y is computed from z
+    itself, to float32's rounding; the gradients are those at the kept rows."""
     _check_checkpoint(checkpoint)
     if isinstance(module, torch.nn.Linear):
         return linear(z, module, checkpoint)
