@@ -184,11 +184,14 @@ __device__ __forceinline__ f32x8 load8(__amdgpu_buffer_rsrc_t r, int row, int n,
 }
 
 // Result columns 32 t + lane % 32 of a tile whose registers are rows 8 (r / 4) +
-// 4 (lane / 32) + r % 4: a store writes two runs of 128 bytes.
+// 4 (lane / 32) + r % 4: a store writes two runs of 128 bytes.  The empty asm
+// keeps the 16 offsets of every tile from being held all along.
 __device__ __forceinline__ void store_columns(__amdgpu_buffer_rsrc_t r, int width, int col, int h, f32x16 v) {
+  uint32_t line = (uint32_t)width * 4u;
+  asm volatile("" : "+s"(line));
+  const uint32_t at = col < width ? 4u * (uint32_t)h * line + 4u * (uint32_t)col : kPast;
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
-    store1(r, col < width ? (uint32_t)((8 * (i / 4) + 4 * h + i % 4) * width + col) * 4u : kPast, v[i]);
+  for (int i = 0; i < 16; ++i) store1(r, at + (uint32_t)(8 * (i / 4) + i % 4) * line, v[i]);
 }
 
 // The columns that a lane of half h holds of step s of a product over a row: two
@@ -196,11 +199,9 @@ __device__ __forceinline__ void store_columns(__amdgpu_buffer_rsrc_t r, int widt
 // 64-byte pieces.
 __device__ __forceinline__ constexpr int step_column(int s, int h) { return 32 * (s / 2) + 16 * h + 8 * (s % 2); }
 
-// W1 in halves as an operand image: lane l's 16 bytes of entry (s, t), at
-// image_lane(s, l), are W1[32 t + l % 32][step_column(s, l / 32) .. + 7] times
-// the hidden unit's own power of two, whose inverse is left in inv.  The scale
-// covers 2^-6 of the bias too, so that a bias over it is at most 2^21.  All threads; ends with a barrier.  `top` is
-// scratch.
+// W1 in pieces as an operand image: lane l's 16 bytes of entry (s, t), at
+// image_lane(s, l), are W1[32 t + l % 32][step_column(s, l / 32) .. + 7].  All
+// threads; the caller's barrier ends it.
 //
 // image_lane exchanges hidden rows so that the 32 lanes of half a column read
 // (read_column: 4 rows by 32 columns, 8 bytes a lane) lie in different banks;
@@ -208,14 +209,10 @@ __device__ __forceinline__ constexpr int step_column(int s, int h) { return 32 *
 __device__ __forceinline__ int image_lane(int s, int l) { return l ^ ((l >> 5) << 3) ^ ((s & 1) << 2); }
 
 template <int KS, int kThreads>
-__device__ __forceinline__ void w1_image(const float* __restrict__ w1, const float* __restrict__ b1, int nin,
-                                         f16x8 (&hi)[KS][kHT][64], f16x8 (&lo)[KS][kHT][64], uint32_t (&top)[kHid],
-                                         float (&inv)[kHid]) {
+__device__ __forceinline__ void w1_image(const float* __restrict__ w1, int nin, bf16x8 (&image)[3][KS][kHT][64]) {
   constexpr int kEntries = KS * kHT * 64, kOwn = (kEntries + kThreads - 1) / kThreads;
   const __amdgpu_buffer_rsrc_t r = rows_rsrc(w1, kHid * nin * 4);
   f32x8 v[kOwn];
-  if (threadIdx.x < kHid) top[threadIdx.x] = b1 != nullptr ? abs_bits(b1[threadIdx.x] * 0x1p-6f) : 0u;
-  __syncthreads();
 #pragma unroll
   for (int u = 0; u < kOwn; ++u) {
     const int i = u * kThreads + (int)threadIdx.x, l = i & 63, t = (i >> 6) % kHT, s = (i >> 6) / kHT;
@@ -224,93 +221,90 @@ __device__ __forceinline__ void w1_image(const float* __restrict__ w1, const flo
   }
 #pragma unroll
   for (int u = 0; u < kOwn; ++u) {
-    const int i = u * kThreads + (int)threadIdx.x, l = i & 63, t = (i >> 6) % kHT;
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[u][j]));
-    if (i < kEntries) atomicMax(&top[kT * t + (l & 31)], m);
-  }
-  __syncthreads();
-#pragma unroll
-  for (int u = 0; u < kOwn; ++u) {
     const int i = u * kThreads + (int)threadIdx.x, l = i & 63, t = (i >> 6) % kHT, s = (i >> 6) / kHT;
     if (i >= kEntries) continue;
-    const Halves h = split(v[u] * pow2_for(top[kT * t + (l & 31)]).p);
-    hi[s][t][image_lane(s, l)] = h.hi;
-    lo[s][t][image_lane(s, l)] = h.lo;
+    const Thirds x = split3(v[u]);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) image[p][s][t][image_lane(s, l)] = x.v[p];
   }
-  if (threadIdx.x < kHid) inv[threadIdx.x] = pow2_for(top[threadIdx.x]).ip;
-  __syncthreads();
 }
+
+// Steps of 16 columns of an input of up to 32 CT: of the widest, 168, the
+// twelfth step's columns are all past the end.
+constexpr int image_steps(int ct) { return 32 * ct > kMaxMlpIn + 23 ? 2 * ct - 1 : 2 * ct; }
+static_assert(step_column(11, 0) >= kMaxMlpIn && image_steps(6) == 11 && image_steps(5) == 10, "nothing left out");
+
+// Pieces of W2 that stand in LDS beside W1's image (12 KB a step; W2 24 KB a
+// tile of outputs): all three, or the first one, and every wave keeps the other
+// two in registers.
+constexpr int lds_pieces(int ct, int ot) { return 12288 * image_steps(ct) + 24576 * ot + 2048 <= 163840 ? 3 : 1; }
 
 // ------------------------------------------------------ training: forward
 
 // y = relu(z W1^T + b1) W2^T + b2 and z in 8 bits.  One wave a tile of 32 rows
-// (rows as the columns n): z's row and then the hidden row are scaled by their
-// own powers of two and split.  A hidden unit's power of two stays in its hidden
-// value (relu(p a) = p relu(a)) and is taken out of W2's image.  The hidden tile's result registers 8 j .. 8 j +
-// 7 of lane l are hidden units 16 j + 4 (l / 32) + 0..3 and 8 more of its row:
-// as they stand they are an operand with W2's image in the same order, and as
-// the first operand they leave y's rows in registers and its columns in lanes,
-// whose stores are whole.
+// (rows as the columns n): z's rows, both weights and the hidden values are
+// split into three bfloat16 pieces (split16.hpp).  Every value keeps its 24
+// bits whatever else is in its row or matrix: with halves that shared a power of
+// two a row, a hidden unit or a matrix, a column 2^24 larger than the rest cost
+// y 13 of its bits and a hidden unit with a bias of -1e30 all of them.
+// The hidden tile's result registers 8 j .. 8 j + 7 of lane l are hidden units
+// 16 j + 4 (l / 32) + 0..3 and 8 more of its row: as they stand they are an
+// operand with W2's image in the same order, and as the first operand they leave
+// y's rows in registers and its columns in lanes, whose stores are whole.
+// The largest of a product's six parts have sums of their own: they are rounded
+// as often as there are steps, not six times as often.
 //
-// Three products of halves each (split16.hpp).  2^20 rows, 83 -> 19: 150..170 us
-// (0.52 GB, 101 at the rate of a copy): matrix
-// instructions and the splits' vector ones overlap, at a clock that falls to 1.2
-// GHz under them.  More waves, operands read ahead or z through LDS gained nothing.
+// Bound: matrix and vector work of the same SIMD; 2^20 rows, 83 -> 19 in 208 us
+// (192 matrix instructions of 32 cycles a row tile: 82 us of them at 2.4 GHz;
+// about 1300 vector ones, mostly splits; 0.52 GB, 101 us at the rate of a copy).
+// With shared powers of two and halves, half the matrix work: 146 us.
 template <int CT, int OT, int kThreads>
 __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
     const float* __restrict__ z, const float* __restrict__ w1, const float* __restrict__ b1,
     const float* __restrict__ w2, const float* __restrict__ b2, int8_t* __restrict__ codes, int64_t ld,
     float* __restrict__ scale, float* __restrict__ y, int64_t rows, int nin, int nout, int64_t tiles) {
-  constexpr int KS = 2 * CT;
-  __shared__ f16x8 w1hi[KS][kHT][64], w1lo[KS][kHT][64];
-  __shared__ f16x8 w2hi[kHT][2][OT][64], w2lo[kHT][2][OT][64];
-  __shared__ uint32_t top[kHid], btop;
-  __shared__ __attribute__((aligned(16))) float i1s[kHid], b1s[kHid], i2s[OT * kT], b2s[OT * kT];
-  __shared__ f32x4 unit[kThreads / 64][kT / 4];  // each wave's own: its rows' hidden scales
+  constexpr int KS = image_steps(CT), P = lds_pieces(CT, OT), kHeld = P < 3 ? OT : 0;
+  __shared__ bf16x8 w1img[3][KS][kHT][64];
+  __shared__ bf16x8 w2img[P][kHT][2][OT][64];
+  __shared__ __attribute__((aligned(16))) float b1s[kHid], b2s[OT * kT];
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int lane0 = image_lane(0, lane), lane1 = image_lane(1, lane);
-  if (threadIdx.x == 0) btop = 0;  // w1_image's barriers come before its use
-  w1_image<KS, kThreads>(w1, b1, nin, w1hi, w1lo, top, i1s);
-  {
-    constexpr int kEntries = kHT * 2 * OT * 64, kOwn = (kEntries + kThreads - 1) / kThreads;
-    const __amdgpu_buffer_rsrc_t r2 = rows_rsrc(w2, nout * kHid * 4);
-    f32x8 v[kOwn];
-    if (threadIdx.x < OT * kT) top[threadIdx.x] = 0;
-    __syncthreads();
+  w1_image<KS, kThreads>(w1, nin, w1img);
+  // entry (t, p, o) of W2: W2[32 o + l % 32][32 t + 16 p + 4 (l / 32) + 0..3, and 8 more]
+  const __amdgpu_buffer_rsrc_t r2 = rows_rsrc(w2, nout * kHid * 4);
+  auto w2_entry = [&](int tp, int o, int l) {
+    const int n = kT * o + (l & 31);
+    const uint32_t at = n < nout ? (uint32_t)(n * kHid + 16 * tp + 4 * (l >> 5)) * 4u : kPast;
+    return split3(__builtin_shufflevector(load4(r2, at), load4(r2, at + 32u), 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  bf16x8 w2r[kHT][2][kHeld + 1][2];
+  if constexpr (P == 3) {
+    constexpr int kEntries = kHT * 2 * OT * 64;
+    static_assert(kEntries % kThreads == 0, "whole turns");
 #pragma unroll
-    for (int u = 0; u < kOwn; ++u) {
-      const int i = u * kThreads + (int)threadIdx.x, l = i & 63, o = (i >> 6) % OT, p = (i >> 6) / OT, n = kT * o + (l & 31);
-      const uint32_t at = n < nout ? (uint32_t)(n * kHid + 16 * p + 4 * (l >> 5)) * 4u : kPast;
-      const f32x4 x0 = load4(r2, at), x1 = load4(r2, at + 32u);
-      const f32x4 q0 = *reinterpret_cast<const f32x4*>(i1s + 16 * p + 4 * (l >> 5));
-      const f32x4 q1 = *reinterpret_cast<const f32x4*>(i1s + 16 * p + 4 * (l >> 5) + 8);
-      v[u] = __builtin_shufflevector(x0 * q0, x1 * q1, 0, 1, 2, 3, 4, 5, 6, 7);
-      uint32_t m = 0;
+    for (int u = 0; u < kEntries / kThreads; ++u) {
+      const int i = u * kThreads + (int)threadIdx.x, l = i & 63, o = (i >> 6) % OT, tp = (i >> 6) / OT;
+      const Thirds x = w2_entry(tp, o, l);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[u][j]));
-      if (i < kEntries) atomicMax(&top[n], m);
+      for (int q = 0; q < 3; ++q) w2img[q][tp / 2][tp % 2][o][l] = x.v[q];
     }
-    __syncthreads();
+  } else {
 #pragma unroll
-    for (int u = 0; u < kOwn; ++u) {
-      const int i = u * kThreads + (int)threadIdx.x, l = i & 63, o = (i >> 6) % OT, p = (i >> 6) / OT;
-      if (i >= kEntries) continue;
-      const Halves x = split(v[u] * pow2_for(top[kT * o + (l & 31)]).p);
-      w2hi[p / 2][p % 2][o][l] = x.hi;
-      w2lo[p / 2][p % 2][o][l] = x.lo;
-    }
-    if (threadIdx.x < OT * kT) {
-      i2s[threadIdx.x] = pow2_for(top[threadIdx.x]).ip;
-      b2s[threadIdx.x] = b2 != nullptr && (int)threadIdx.x < nout ? b2[threadIdx.x] : 0.0f;
-    }
-    if (threadIdx.x < kHid) {
-      const float v = b1 != nullptr ? b1[threadIdx.x] / i1s[threadIdx.x] : 0.0f;
-      b1s[threadIdx.x] = v;
-      atomicMax(&btop, abs_bits(v));
+    for (int t = 0; t < kHT; ++t) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+#pragma unroll
+        for (int o = 0; o < OT; ++o) {
+          const Thirds x = w2_entry(2 * t + p, o, lane);
+          if (threadIdx.x < 64) w2img[0][t][p][o][lane] = x.v[0];
+          w2r[t][p][o][0] = x.v[1];
+          w2r[t][p][o][1] = x.v[2];
+        }
+      }
     }
   }
+  if (threadIdx.x < kHid) b1s[threadIdx.x] = b1 != nullptr ? b1[threadIdx.x] : 0.0f;
+  if (threadIdx.x < OT * kT) b2s[threadIdx.x] = b2 != nullptr && (int)threadIdx.x < nout ? b2[threadIdx.x] : 0.0f;
   __syncthreads();
 
   const int64_t step = (int64_t)gridDim.x * (kThreads / 64);
@@ -329,20 +323,18 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
   for (; tile < tiles; tile += step) {
     asm volatile("" ::: "memory");  // the images stay in LDS: read ahead of the loop they spill
     const int64_t r0 = tile * kT, nr = min<int64_t>(kT, rows - r0);
-    f32x8 zv[KS];
     uint32_t zt = 0;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      zv[s] = __builtin_shufflevector(zn[s / 2][s % 2 * 2], zn[s / 2][s % 2 * 2 + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+    for (int s = 0; s < CT; ++s) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (s / 2 == CT - 1 && step_column(s, h) + j >= nin) zv[s][j] = 0.0f;  // the next row's
-        zt = max(zt, abs_bits(zv[s][j]));
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (s == CT - 1 && 32 * s + 16 * h + 4 * i + j >= nin) zn[s][i][j] = 0.0f;  // the next row's
+          zt = max(zt, abs_bits(zn[s][i][j]));
+        }
       }
     }
-    __builtin_amdgcn_sched_barrier(0);
-    load(tile + step);  // in flight until the next row tile
-    __builtin_amdgcn_sched_barrier(0);
     zt = max(zt, (uint32_t)__shfl_xor((int)zt, 32));
     const RowScale q = row_scale(zt);
     const __amdgpu_buffer_rsrc_t rc = bytes_rsrc(codes + r0 * ld, nr * ld);
@@ -351,10 +343,7 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
       const int k = 32 * s + 16 * h;
       u32x4 w;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x8 v = zv[2 * s + i / 2];
-        w[i] = i % 2 == 0 ? row_codes4(v[0], v[1], v[2], v[3], q) : row_codes4(v[4], v[5], v[6], v[7], q);
-      }
+      for (int i = 0; i < 4; ++i) w[i] = row_codes4(zn[s][i][0], zn[s][i][1], zn[s][i][2], zn[s][i][3], q);
       if (s < CT - 1) {
         __builtin_amdgcn_raw_buffer_store_b128(w, rc, (uint32_t)(c * (int)ld + k), 0, 0);
       } else {
@@ -365,24 +354,23 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
       }
     }
     if (h == 0 && c < nr) scale[r0 + c] = q.scale;
-    const Pow2 pz = pow2_for(zt);
-    Halves zs[KS];
+    Thirds zs[KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) zs[s] = split(zv[s] * pz.p);
-    // no hidden value exceeds this, and it is not far above the largest: W1's
-    // values are at most 2^15 in the image
-    const Pow2 ph = pow2_for(__builtin_bit_cast(uint32_t, __builtin_bit_cast(float, zt) * (32768.0f * (float)nin) +
-                                                              __builtin_bit_cast(float, btop)));
-    f32x16 out[OT];
+    for (int s = 0; s < KS; ++s)
+      zs[s] = split3(__builtin_shufflevector(zn[s / 2][s % 2 * 2], zn[s / 2][s % 2 * 2 + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+    __builtin_amdgcn_sched_barrier(0);
+    load(tile + step);  // in flight until the next row tile
+    __builtin_amdgcn_sched_barrier(0);
+    f32x16 out[OT], rest[OT];
 #pragma unroll
-    for (int o = 0; o < OT; ++o) out[o] = f32x16{};
+    for (int o = 0; o < OT; ++o) out[o] = rest[o] = f32x16{};
 #pragma unroll
     for (int t = 0; t < kHT; ++t) {
-      f32x16 acc = f32x16{};
+      f32x16 acc = f32x16{}, low = f32x16{};
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const int l = k % 2 == 0 ? lane0 : lane1;
-        acc = mma(Halves{w1hi[k][t][l], w1lo[k][t][l]}, zs[k], acc);
+        mma(Thirds{w1img[0][k][t][l], w1img[1][k][t][l], w1img[2][k][t][l]}, zs[k], acc, low);
       }
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
@@ -391,30 +379,32 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
         for (int g = 2 * p; g < 2 * p + 2; ++g) {
           const f32x4 bv = *reinterpret_cast<const f32x4*>(b1s + kT * t + 8 * g + 4 * h);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[4 * (g - 2 * p) + j] = relu(acc[4 * g + j] * pz.ip + bv[j]) * ph.p;
+          for (int j = 0; j < 4; ++j) v[4 * (g - 2 * p) + j] = relu(acc[4 * g + j] + low[4 * g + j] + bv[j]);
         }
-        const Halves hs = split(v);
+        const Thirds hs = split3(v);
 #pragma unroll
-        for (int o = 0; o < OT; ++o) out[o] = mma(hs, Halves{w2hi[t][p][o][lane], w2lo[t][p][o][lane]}, out[o]);
+        for (int o = 0; o < OT; ++o) {
+          Thirds w;
+          w.v[0] = w2img[0][t][p][o][lane];
+          if constexpr (P == 3) {
+            w.v[1] = w2img[1][t][p][o][lane];
+            w.v[2] = w2img[2][t][p][o][lane];
+          } else {
+            w.v[1] = w2r[t][p][o][0];
+            w.v[2] = w2r[t][p][o][1];
+          }
+          mma(hs, w, out[o], rest[o]);
+        }
       }
     }
-    // rows are the registers now: their scales come from the lanes that hold them
-    float* __restrict__ us = reinterpret_cast<float*>(unit[threadIdx.x / 64]);
-    if (h == 0) us[c] = ph.ip;
-    __builtin_amdgcn_wave_barrier();
     const __amdgpu_buffer_rsrc_t ry = rows_rsrc(y + r0 * nout, nr * nout * 4);
 #pragma unroll
     for (int o = 0; o < OT; ++o) {
-      const float iv = i2s[kT * o + c], bv = b2s[kT * o + c];
+      const float bv = b2s[kT * o + c];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 rv = *reinterpret_cast<const f32x4*>(us + 8 * g + 4 * h);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) out[o][4 * g + j] = out[o][4 * g + j] * rv[j] * iv + bv;
-      }
+      for (int r = 0; r < 16; ++r) out[o][r] = out[o][r] + rest[o][r] + bv;
       store_columns(ry, nout, kT * o + c, h, out[o]);
     }
-    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -423,68 +413,65 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
 // dz from codes and dy.  One wave a tile of 32 rows, rows as the columns n:
 // hidden tile by hidden tile, a (for its sign) from the codes and dh = W2^T dy
 // masked by it; then dz += dh W1 with W1's image read down its columns, dh's
-// result registers as they stand being the first operand.
-// A hidden unit's power of two is taken out of W2's image, so that W1's stands
-// in for W1; the row's own power of two keeps dy and dh in range: |dy| <= 2^15,
-// |W2| <= 2^15 in the image, so |dh| <= 2^30 nout, and 2^-drop brings it to
-// 2^15.
+// result registers as they stand being the first operand.  All float32 factors
+// in three bfloat16 pieces, as in the forward.  dz's stores are whole lines
+// because rows are registers in its product.
 //
-// Bound: as the forward's; 2^20 rows, 83 -> 19 in 178 us.  dz's stores are whole
-// lines because rows are registers in its product.
+// Bound: as the forward's; 2^20 rows, 83 -> 19 in 240 us (264 matrix
+// instructions a row tile: 113 us at 2.4 GHz; 168 us with halves).
 template <int CT, int OT, int kThreads>
 __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
     const int8_t* __restrict__ codes, int64_t ld, const float* __restrict__ scale, const float* __restrict__ dy,
     const float* __restrict__ w1, const float* __restrict__ b1, const float* __restrict__ w2, float* __restrict__ dz,
-    int64_t rows, int nin, int nout, int drop, int64_t tiles) {
-  constexpr int KS = 2 * CT, OS = 2 * OT;
-  __shared__ f16x8 w1hi[KS][kHT][64], w1lo[KS][kHT][64];
-  __shared__ f16x8 w2hi[OS][kHT][64], w2lo[OS][kHT][64];
-  __shared__ uint32_t top[kHid], top2;
-  __shared__ __attribute__((aligned(16))) float i1s[kHid], nbs[kHid];
-  __shared__ __attribute__((aligned(16))) int exps[kThreads / 64][kT];  // each wave's own: its rows' exponents
+    int64_t rows, int nin, int nout, int64_t tiles) {
+  constexpr int KS = image_steps(CT), OS = 2 * OT, P = lds_pieces(CT, OT), kHeld = P < 3 ? OS : 0;
+  __shared__ bf16x8 w1img[3][KS][kHT][64];
+  __shared__ bf16x8 w2img[P][OS][kHT][64];
+  __shared__ __attribute__((aligned(16))) float b1s[kHid];
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
-  if (threadIdx.x == 0) top2 = 0;
-  w1_image<KS, kThreads>(w1, b1, nin, w1hi, w1lo, top, i1s);
-  int e2;
-  {
-    constexpr int kEntries = OS * kHT * 64, kOwn = (kEntries + kThreads - 1) / kThreads;
-    const __amdgpu_buffer_rsrc_t r2 = rows_rsrc(w2, nout * kHid * 4);
-    f32x8 v[kOwn];
+  w1_image<KS, kThreads>(w1, nin, w1img);
+  // entry (s, t) of W2: W2[step_column(s, l / 32) + 0..7][32 t + l % 32]
+  const __amdgpu_buffer_rsrc_t r2 = rows_rsrc(w2, nout * kHid * 4);
+  auto w2_entry = [&](int s, int t, int l) {
+    const int k = step_column(s, l >> 5), n = kT * t + (l & 31);
+    f32x8 v;
 #pragma unroll
-    for (int u = 0; u < kOwn; ++u) {
+    for (int j = 0; j < 8; ++j) v[j] = load1(r2, k + j < nout ? (uint32_t)((k + j) * kHid + n) * 4u : kPast);
+    return split3(v);
+  };
+  bf16x8 w2r[kHeld + 1][kHT][2];
+  if constexpr (P == 3) {
+    constexpr int kEntries = OS * kHT * 64;
+    static_assert(kEntries % kThreads == 0, "whole turns");
+#pragma unroll
+    for (int u = 0; u < kEntries / kThreads; ++u) {
       const int i = u * kThreads + (int)threadIdx.x, l = i & 63, t = (i >> 6) % kHT, s = (i >> 6) / kHT;
-      const int k = step_column(s, l >> 5), n = kT * t + (l & 31);
-      uint32_t m = 0;
+      const Thirds x = w2_entry(s, t, l);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[u][j] = load1(r2, i < kEntries && k + j < nout ? (uint32_t)((k + j) * kHid + n) * 4u : kPast) * i1s[n];
-        m = max(m, abs_bits(v[u][j]));
+      for (int q = 0; q < 3; ++q) w2img[q][s][t][l] = x.v[q];
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < OS; ++s) {
+#pragma unroll
+      for (int t = 0; t < kHT; ++t) {
+        const Thirds x = w2_entry(s, t, lane);
+        if (threadIdx.x < 64) w2img[0][s][t][lane] = x.v[0];
+        w2r[s][t][0] = x.v[1];
+        w2r[s][t][1] = x.v[2];
       }
-      if (i < kEntries) atomicMax(&top2, m);
     }
-    __syncthreads();
-    const Pow2 p2 = pow2_for(top2);
-    e2 = (int)(__builtin_bit_cast(uint32_t, p2.ip) >> 23) - 127 + drop;
-#pragma unroll
-    for (int u = 0; u < kOwn; ++u) {
-      const int i = u * kThreads + (int)threadIdx.x, l = i & 63, t = (i >> 6) % kHT, s = (i >> 6) / kHT;
-      if (i >= kEntries) continue;
-      const Halves x = split(v[u] * p2.p);
-      w2hi[s][t][l] = x.hi;
-      w2lo[s][t][l] = x.lo;
-    }
-    // a > 0 where the scaled product exceeds this
-    if (threadIdx.x < kHid) nbs[threadIdx.x] = b1 != nullptr ? -b1[threadIdx.x] / i1s[threadIdx.x] : 0.0f;
   }
+  if (threadIdx.x < kHid) b1s[threadIdx.x] = b1 != nullptr ? b1[threadIdx.x] : 0.0f;
   __syncthreads();
 
   // a column read of W1's image: columns 16 (lane / 16 % 2) + 4 (lane % 4) ..
   // + 3 of a tile's 32, hidden rows 4 h + lane % 16 / 4 from a multiple of 8
   const int i16 = lane & 15, half = (lane >> 4) & 1, odd = (i16 >> 1) & 1;
-  const int wcol = (odd * kHT * 64 + half * 32 + ((4 * h + (i16 >> 2)) ^ (4 * odd))) * 16 + (i16 & 1) * 8;
-  const int wcol0 = wcol + 8 * 16 * half, wcol1 = wcol + 8 * 16 * (1 - half);  // the first and second eight rows
+  const int even = (half * 32 + 4 * h + (i16 >> 2)) * 16 + (i16 & 1) * 8;
+  const int wcol = odd ? (kHT * 64 + half * 32 + ((4 * h + (i16 >> 2)) ^ 4)) * 16 + (i16 & 1) * 8 : even;
+  const int first8 = 8 * 16 * half, second8 = 8 * 16 * (1 - half);  // the first and second eight rows
   const int lane0 = image_lane(0, lane), lane1 = image_lane(1, lane);
-  const float shrink = __builtin_bit_cast(float, (uint32_t)(127 - drop) << 23);
   const int64_t step = (int64_t)gridDim.x * (kThreads / 64);
   int64_t tile = (int64_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64 * gridDim.x + blockIdx.x));
   u32x4 cn[CT];
@@ -505,88 +492,95 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
     sn = load1(rs, (uint32_t)c * 4u);
   };
   load(tile);
-  auto column = [&](int t, int p, int ct) {
-    const char* ph = reinterpret_cast<const char*>(&w1hi[2 * ct][t][16 * p]);
-    const char* pl = reinterpret_cast<const char*>(&w1lo[2 * ct][t][16 * p]);
-    return Halves{__builtin_bit_cast(f16x8, join(read_column(ph + wcol0), read_column(ph + wcol1))),
-                  __builtin_bit_cast(f16x8, join(read_column(pl + wcol0), read_column(pl + wcol1)))};
+  auto column = [&](int t, int p, int ct, int q) {
+    // the step that the widest input leaves out: its columns, which are not
+    // stored, read the one before it
+    const int at = 2 * ct + 1 < KS ? wcol : even;
+    const char* s = reinterpret_cast<const char*>(&w1img[q][2 * ct][t][16 * p]) + at;
+    return __builtin_bit_cast(bf16x8, join(read_column(s + first8), read_column(s + second8)));
   };
   for (; tile < tiles; tile += step) {
     asm volatile("" ::: "memory");  // the images stay in LDS: read ahead of the loop they spill
     const int64_t r0 = tile * kT, nr = min<int64_t>(kT, rows - r0);
     // codes past the row's end meet zeros in W1's image
-    f16x8 cz[KS];
+    bf16x8 cz[KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) cz[s] = codes_f16(u32x2{cn[s / 2][s % 2 * 2], cn[s / 2][s % 2 * 2 + 1]});
+    for (int s = 0; s < KS; ++s)
+      cz[s] = __builtin_shufflevector(codes_bf16(cn[s / 2][s % 2 * 2]), codes_bf16(cn[s / 2][s % 2 * 2 + 1]), 0, 1, 2,
+                                      3, 4, 5, 6, 7);
     const float sc = sn;
-    f32x8 dv[OS];
-    uint32_t dt = 0;
+    Thirds ds[OS];
 #pragma unroll
     for (int s = 0; s < OS; ++s) {
-      dv[s] = __builtin_shufflevector(dn[s / 2][s % 2 * 2], dn[s / 2][s % 2 * 2 + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+      f32x8 v = __builtin_shufflevector(dn[s / 2][s % 2 * 2], dn[s / 2][s % 2 * 2 + 1], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (s / 2 == OT - 1 && step_column(s, h) + j >= nout) dv[s][j] = 0.0f;
-        dt = max(dt, abs_bits(dv[s][j]));
-      }
+      for (int j = 0; j < 8; ++j)
+        if (s / 2 == OT - 1 && step_column(s, h) + j >= nout) v[j] = 0.0f;  // the next row's
+      ds[s] = split3(v);
     }
-    dt = max(dt, (uint32_t)__shfl_xor((int)dt, 32));
-    const Pow2 pd = pow2_for(dt);
-    Halves ds[OS];
-#pragma unroll
-    for (int s = 0; s < OS; ++s) ds[s] = split(dv[s] * pd.p);
     f32x16 out[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) out[ct] = f32x16{};
 #pragma unroll
     for (int t = 0; t < kHT; ++t) {
-      f32x16 a = f32x16{}, dh = f32x16{};
+      f32x16 a = f32x16{}, dh = f32x16{}, low = f32x16{};
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const int l = k % 2 == 0 ? lane0 : lane1;
-        a = mma(w1hi[k][t][l], cz[k], mma(w1lo[k][t][l], cz[k], a));
+      for (int q = 2; q >= 0; --q) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) a = mma(w1img[q][k][t][k % 2 == 0 ? lane0 : lane1], cz[k], a);
       }
 #pragma unroll
-      for (int k = 0; k < OS; ++k) dh = mma(Halves{w2hi[k][t][lane], w2lo[k][t][lane]}, ds[k], dh);
+      for (int k = 0; k < OS; ++k) {
+        Thirds w;
+        w.v[0] = w2img[0][k][t][lane];
+        if constexpr (P == 3) {
+          w.v[1] = w2img[1][k][t][lane];
+          w.v[2] = w2img[2][k][t][lane];
+        } else {
+          w.v[1] = w2r[k][t][0];
+          w.v[2] = w2r[k][t][1];
+        }
+        mma(w, ds[k], dh, low);
+      }
       if (t == kHT - 1) {  // into the registers that this tile's codes and dy leave
         __builtin_amdgcn_sched_barrier(0);
         load(tile + step);
         __builtin_amdgcn_sched_barrier(0);
       }
+      Thirds hs[2];
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         f32x8 v;
 #pragma unroll
         for (int g = 2 * p; g < 2 * p + 2; ++g) {
-          const f32x4 nb = *reinterpret_cast<const f32x4*>(nbs + kT * t + 8 * g + 4 * h);
+          const f32x4 bv = *reinterpret_cast<const f32x4*>(b1s + kT * t + 8 * g + 4 * h);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             // as torch: 0 where relu(a) <= 0, so a NaN lets the upstream pass
-            const float d = dh[4 * g + j] * shrink;
-            v[4 * (g - 2 * p) + j] = a[4 * g + j] * sc <= nb[j] ? 0.0f : d;
+            const float d = dh[4 * g + j] + low[4 * g + j];
+            v[4 * (g - 2 * p) + j] = a[4 * g + j] * sc + bv[j] <= 0.0f ? 0.0f : d;
           }
         }
-        const Halves hs = split(v);
+        hs[p] = split3(v);
+      }
+      // the tile's part is summed by itself, small products first, and added
+      // with a rounding to nearest
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) out[ct] = mma(hs, column(t, p, ct), out[ct]);
+      for (int ct = 0; ct < CT; ++ct) {
+        f32x16 part = f32x16{};
+#pragma unroll
+        for (int n = 0; n < 12; ++n) {
+          // pieces (dh, W1) in the order of their products' sizes
+          constexpr int kD[6] = {1, 2, 0, 1, 0, 0}, kW[6] = {1, 0, 2, 0, 1, 0};
+          part = mma(hs[n % 2].v[kD[n / 2]], column(t, n % 2, ct, kW[n / 2]), part);
+        }
+        out[ct] += part;
+        __builtin_amdgcn_sched_barrier(0);  // one tile's columns at a time: read ahead of their turn they spill
       }
     }
-    // rows are the registers now: their exponents come from the lanes that hold them
-    int* __restrict__ es = exps[threadIdx.x / 64];
-    if (h == 0) es[c] = (int)(__builtin_bit_cast(uint32_t, pd.ip) >> 23) - 127 + e2;
-    __builtin_amdgcn_wave_barrier();
     const __amdgpu_buffer_rsrc_t rz = rows_rsrc(dz + r0 * nin, nr * nin * 4);
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const i32x4 ev = *reinterpret_cast<const i32x4*>(es + 8 * g + 4 * h);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) out[ct][4 * g + j] = __builtin_ldexpf(out[ct][4 * g + j], ev[j]);
-      }
-      store_columns(rz, nin, kT * ct + c, h, out[ct]);
-    }
-    __builtin_amdgcn_wave_barrier();
+    for (int ct = 0; ct < CT; ++ct) store_columns(rz, nin, kT * ct + c, h, out[ct]);
   }
 }
 
@@ -748,7 +742,7 @@ __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_ml
     }
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const Thirds hs = split3(hv[p]), gs = split3(gv[p]);
+      const Thirds hs = split3<false>(hv[p]), gs = split3<false>(gv[p]);
 #pragma unroll
       for (int o = 0; o < OT; ++o) {
         Thirds d;
@@ -817,9 +811,10 @@ constexpr int kMaxKS = (kMaxMlpIn + 15) / 16, kMaxOS = kMaxMlpOut / 16, kMaxCT =
 // Workgroups of the row tile kernels: one a CU, a row tile for each where there
 // are fewer than the waves.
 // Their threads: two waves a SIMD where 256 registers hold a row tile, else one.
-// At 2^18 rows, us with two and one (the bounds' last and first past): forward
-// 112 -> 35 59 and 70, 150 -> 19 66 and 75, 163 -> 19 97 and 81, 130 -> 35 91 and 78;
-// input gradient with autograd's part 112 -> 35 163 and 171, 150 -> 19 205 and 177.
+// At 2^18 rows, us with two and one (the last below the bounds and the first
+// past them): forward 83 -> 35 65 and 71, 128 -> 30 69 and 76, 112 -> 35 88 and 82,
+// 150 -> 19 99 and 87; input gradient 83 -> 35 68 and 83, 128 -> 30 97 and 93, 112
+// -> 35 127 and 103.
 constexpr int tile_threads(bool two) { return two ? 512 : 256; }
 inline dim3 spread_grid(int64_t tiles) { return dim3((uint32_t)std::min<int64_t>(256, tiles)); }
 
@@ -832,7 +827,7 @@ void run_mlp_rows8_forward(const float* z, const float* w1, const float* b1, con
   const int64_t tiles = (rows + kT - 1) / kT;
   with_groups<kMaxCT>((nin + kT - 1) / kT, [&](auto ct) {
     with_groups<2>(nout <= kT ? 1 : 2, [&](auto ot) {
-      constexpr int CT = decltype(ct)::value, OT = decltype(ot)::value, T = tile_threads(CT + OT <= 6);
+      constexpr int CT = decltype(ct)::value, OT = decltype(ot)::value, T = tile_threads(CT + OT <= 5);
       hipLaunchKernelGGL((k_mlp_forward8<CT, OT, T>), spread_grid(tiles), dim3(T), 0, st, z, w1, b1, w2, b2, codes,
                          ld, scale, y, rows, nin, nout, tiles);
     });
@@ -849,13 +844,11 @@ void run_mlp_rows8_backward(const int8_t* codes, int64_t ld, const float* scale,
                             float* db2, int64_t rows, int nin, int nout, float* work, hipStream_t st) {
   const int64_t tiles = (rows + kT - 1) / kT;
   if (dz != nullptr && rows > 0) {
-    int drop = 15;
-    for (int n = 1; n < nout; n *= 2) ++drop;
     with_groups<kMaxCT>((nin + kT - 1) / kT, [&](auto ct) {
       with_groups<2>(nout <= kT ? 1 : 2, [&](auto ot) {
-        constexpr int CT = decltype(ct)::value, OT = decltype(ot)::value, T = tile_threads(CT <= 4);
+        constexpr int CT = decltype(ct)::value, OT = decltype(ot)::value, T = tile_threads(CT <= 3);
         hipLaunchKernelGGL((k_mlp_input_grad8<CT, OT, T>), spread_grid(tiles), dim3(T), 0, st,
-                           codes, ld, scale, dy, w1, b1, w2, dz, rows, nin, nout, drop, tiles);
+                           codes, ld, scale, dy, w1, b1, w2, dz, rows, nin, nout, tiles);
       });
     });
     SPHOPS_LAUNCHED();
