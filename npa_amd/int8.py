@@ -228,29 +228,51 @@ def mlp(z, w1, b1, w2, b2):
     return y
 
 
+def _leaves(t):
+    """The leaf tensors that t's graph leads to."""
+    todo, seen = [t.grad_fn], set()
+    while todo:
+        node = todo.pop()
+        if node is None or node in seen:
+            continue
+        seen.add(node)
+        if isinstance(getattr(node, "variable", None), torch.Tensor):
+            yield node.variable
+        todo.extend(n for n, _ in node.next_functions)
+
+
 class _Checkpoint(torch.autograd.Function):
+    """tensors: ``count`` params, then the parameters of ``function``'s own."""
+
     @staticmethod
-    def forward(ctx, function, x, *params):
+    def forward(ctx, function, count, x, *tensors):
         r = quantize_rows(x)
         ctx.function, ctx.shape, ctx.dtype = function, r.shape, x.dtype
+        ctx.count, ctx.own = count, tensors[count:]
         # without its cache, which would keep casts of params made here without a graph
         ctx.autocast = functools.partial(torch.autocast, "cuda", torch.get_autocast_dtype("cuda"),
                                          torch.is_autocast_enabled("cuda"), cache_enabled=False)
-        ctx.save_for_backward(r.codes, r.scale, *params)
+        ctx.save_for_backward(r.codes, r.scale, *tensors)
         with torch.no_grad(), ctx.autocast():
-            return function(x, *params)
+            return function(x, *tensors[:count])
 
     @staticmethod
     def backward(ctx, dy):
-        codes, scale, *params = ctx.saved_tensors
-        needs = ctx.needs_input_grad[1:]
+        codes, scale, *tensors = ctx.saved_tensors
+        needs = ctx.needs_input_grad[2:]
         with torch.enable_grad(), ctx.autocast():
             x = restore_rows(Rows8(codes, scale, ctx.shape), ctx.dtype).requires_grad_(needs[0])
-            params = [p.detach().requires_grad_(n) for p, n in zip(params, needs[1:])]
+            params = [p.detach().requires_grad_(n) for p, n in zip(tensors[:ctx.count], needs[1:])]
             y = ctx.function(x, *params)
-        wanted = [t for t, n in zip([x, *params], needs) if n]
+        inputs = [x, *params, *ctx.own]
+        needs = [n and t.requires_grad for t, n in zip(inputs, needs)]  # own ones may have been frozen since
+        wanted = [t for t, n in zip(inputs, needs) if n]
+        known = {id(t) for t in wanted}
+        if any(id(t) not in known for t in _leaves(y)):
+            raise RuntimeError("int8.checkpoint: the function reads a tensor that requires a gradient and is neither an "
+                               "argument nor a parameter of a module that it is: pass it as one of params")
         grads = iter(torch.autograd.grad(y, wanted, dy, allow_unused=True))
-        return (None, *(next(grads) if n else None for n in needs))
+        return (None, None, *(next(grads) if n else None for n in needs))
 
 
 def checkpoint(function, x, *params):
@@ -258,11 +280,16 @@ def checkpoint(function, x, *params):
     backward: there x is restored and the function runs again with gradients,
     under the forward's autocast; it must not draw random numbers.
     The rounding of x is passed straight through.  ``params``: the tensors
-    besides x that gradients are wanted of."""
+    besides x that gradients are wanted of.  Where ``function`` is a module, or
+    a method of one, the module's parameters get theirs without being named; any
+    other tensor that it reads and that requires a gradient makes the backward
+    raise."""
     _check_rows(x, "x")
-    if not torch.is_grad_enabled() or not any(t.requires_grad for t in (x, *params)):
+    module = function if isinstance(function, torch.nn.Module) else getattr(function, "__self__", None)
+    own = [p for p in module.parameters() if p.requires_grad] if isinstance(module, torch.nn.Module) else []
+    if not torch.is_grad_enabled() or not any(t.requires_grad for t in (x, *params, *own)):
         return function(x, *params)
-    return _Checkpoint.apply(function, x, *params)
+    return _Checkpoint.apply(function, len(params), x, *params, *own)
 
 
 def _kept_weight(layer):
