@@ -228,6 +228,31 @@ def mlp(z, w1, b1, w2, b2):
     return y
 
 
+class _Once(torch.autograd.Function):
+    """Gradients as they are; differentiated again they raise."""
+
+    @staticmethod
+    def forward(ctx, what, anchor, *grads):
+        ctx.what = what
+        return grads
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.what} has no second derivative")
+
+
+def first_order(what, *grads):
+    """What a backward without a graph returns.  Under create_graph these
+    gradients would count as constants and a second derivative would lose their
+    part silently; they raise there instead (whether or not the upstream requires
+    a gradient, which ``once_differentiable`` goes by)."""
+    some = [g for g in grads if g is not None]
+    if not torch.is_grad_enabled() or not some:
+        return grads
+    held = iter(_Once.apply(what, torch.zeros((), requires_grad=True), *some))
+    return tuple(None if g is None else next(held) for g in grads)
+
+
 def _leaves(t):
     """The leaf tensors that t's graph leads to."""
     todo, seen = [t.grad_fn], set()
@@ -272,7 +297,7 @@ class _Checkpoint(torch.autograd.Function):
             raise RuntimeError("int8.checkpoint: the function reads a tensor that requires a gradient and is neither an "
                                "argument nor a parameter of a module that it is: pass it as one of params")
         grads = iter(torch.autograd.grad(y, wanted, dy, allow_unused=True))
-        return (None, None, *(next(grads) if n else None for n in needs))
+        return (None, None, *first_order("int8.checkpoint", *(next(grads) if n else None for n in needs)))
 
 
 def checkpoint(function, x, *params):

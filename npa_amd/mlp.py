@@ -231,6 +231,7 @@ class LinearRows8(torch.autograd.Function):
             dx = (dy.reshape(-1, weight.shape[0]) @ weight).reshape(ctx.shape)
         if need_w:
             dw, db = int8.weight_grad(int8.Rows8(*kept, ctx.shape), dy, need_b and ctx.has_bias)
+            dw, db = int8.first_order("a weight gradient from rows in 8 bits", dw, db)
         elif need_b and ctx.has_bias:
             db = dy.reshape(-1, weight.shape[0]).sum(0)
         return dx, dw, db
@@ -258,7 +259,8 @@ class ReluLinear8(torch.autograd.Function):
             g = (dy.reshape(-1, weight.shape[0]) @ weight).reshape(ctx.shape)
             da = torch.where(int8.restore_rows(kept) <= 0, torch.zeros_like(g), g)
         if need_w or (need_b and ctx.has_bias):
-            dw, db = int8.weight_grad(kept, dy, ctx.has_bias)
+            dw, db = int8.first_order("a weight gradient from rows in 8 bits",
+                                      *int8.weight_grad(kept, dy, ctx.has_bias))
         return da, (dw if need_w else None), (db if need_b else None)
 
 
@@ -315,7 +317,8 @@ class MlpRows8(torch.autograd.Function):
             codes.data_ptr(), codes.shape[1], scale.data_ptr(), dy.data_ptr(), *map(_address, dense),
             *map(_address, (dz, dw1, db1, dw2, db2)), rows, in_f, hidden, out_f, work.data_ptr(),
             torch._C._cuda_getCurrentRawStream(dev.index)))
-        return (dz if dz is None or len(lead) == 1 else dz.reshape(*lead, in_f)), dw1, db1, dw2, db2
+        dz = dz if dz is None or len(lead) == 1 else dz.reshape(*lead, in_f)
+        return int8.first_order("the MLP with its input in 8 bits", dz, dw1, db1, dw2, db2)
 
 
 def _rows8_ok(x, layer):

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_int8 import _gen
+from test_gpu_int8 import _gen, _net
 
 pytestmark = pytest.mark.gpu
 
@@ -20,3 +20,32 @@ def test_checkpoint_of_a_module(needs_x):
     for p, ref in zip(net.parameters(), want):
         assert torch.equal(p.grad, ref)
     assert torch.equal(x.grad, want[-1]) if needs_x else x.grad is None
+
+
+@pytest.mark.parametrize("hidden,nout", [(128, 19), (64, 19), (256, 130)])
+def test_second_derivatives_are_right_or_refused(hidden, nout):
+    """Of layers with codes only dx is differentiated again, which is linear in the
+    upstream and the weights; the fused MLP's gradients and weight gradients raise."""
+    from npa_amd import mlp as M
+    net, g = _net(83, nout, True, hidden, hidden)
+    x = torch.randn(300, 83, device="cuda", generator=g).requires_grad_(True)
+
+    def penalty(y):
+        (dx,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        return dx.square().sum()
+
+    y = M.mlp(net, x, checkpoint="int8")
+    if hidden == 128:
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            (penalty(y) + net(x).sum()).backward()
+    else:  # each value of the saved rows is within 1/254 of its row's largest
+        got = torch.autograd.grad(penalty(y), list(net.parameters()))
+        for a, b in zip(got, torch.autograd.grad(penalty(net(x)), list(net.parameters()))):
+            assert ((a - b).norm() <= 0.02 * b.norm()).item()
+    y = M.mlp(net, x, checkpoint="int8")
+    dw = torch.autograd.grad(y.sum(), net[0].weight, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        dw.square().sum().backward()
+    first, again = (torch.autograd.grad(M.mlp(net, x, checkpoint="int8").sum(), list(net.parameters()), create_graph=c)
+                    for c in (True, False))
+    assert all(torch.equal(a, b) for a, b in zip(first, again))

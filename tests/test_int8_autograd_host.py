@@ -87,3 +87,16 @@ def test_gradients_of_captured_tensors_are_not_lost_silently(needs_x):
     x = torch.randn(5, 6).requires_grad_(True)
     int8.checkpoint(lambda v: v @ fixed, x).sum().backward()
     assert torch.allclose(x.grad, torch.ones(5, 6) @ fixed.T)
+
+
+def test_second_derivatives_are_refused():
+    """A gradient penalty beside another loss raises instead of losing its terms, also where the upstream is a constant."""
+    net, x = _block(), torch.randn(5, 6).requires_grad_(True)
+    for upstream in (lambda y: y.sum(), lambda y: y.square().sum()):
+        (dx,) = torch.autograd.grad(upstream(int8.checkpoint(net, x)), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            (dx.square().sum() + net(x).sum()).backward()
+    # the first derivative alone is as ever
+    got = torch.autograd.grad(int8.checkpoint(net, x).sum(), list(net.parameters()), create_graph=True)
+    for a, b in zip(got, torch.autograd.grad(net(x).sum(), list(net.parameters()))):
+        assert torch.allclose(a, b)
