@@ -54,7 +54,8 @@ class LinearRows(torch.autograd.Function):
         if need_x:
             dx = (dy2 @ weight).reshape(x.shape)
         if need_w or (need_b and ctx.has_bias):
-            dw, db = _weight_grad(x.reshape(-1, in_f), dy2, ctx.has_bias)
+            dw, db = int8.first_order("a linear layer's weight gradient",
+                                      *_weight_grad(x.reshape(-1, in_f), dy2, ctx.has_bias))
         return dx, (dw if need_w else None), (db if need_b else None)
 
 
@@ -130,7 +131,7 @@ class ReluLinear(torch.autograd.Function):
             da = da2.reshape(dy.shape[:-1] + (in_f,))
         if need_w or (need_b and ctx.has_bias):
             dw, db = _weight_grad(s2, dy2, ctx.has_bias, relu_x=ctx.pre)
-        return da, (dw if need_w else None), (db if need_b else None)
+        return int8.first_order("ReLU and Linear in one", da, dw if need_w else None, db if need_b else None)
 
 
 class MlpRows(torch.autograd.Function):
@@ -185,7 +186,7 @@ class MlpRows(torch.autograd.Function):
             _native.check(_lib.sphops_mlp_weight_grad(_ptr(z2), _ptr(a), _ptr(dy2), _ptr(w2c), _ptr(dw1), _ptr(db1),
                                                       _ptr(dw2), _ptr(db2), rows, in_f, hidden, out_f, _ptr(work),
                                                       st))
-        return dz, dw1, db1, dw2, db2, None
+        return (*int8.first_order("the MLP in one kernel", dz, dw1, db1, dw2, db2), None)
 
 
 def _mlp_rows_ok(z, first, second):

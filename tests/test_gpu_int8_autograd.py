@@ -49,3 +49,29 @@ def test_second_derivatives_are_right_or_refused(hidden, nout):
     first, again = (torch.autograd.grad(M.mlp(net, x, checkpoint="int8").sum(), list(net.parameters()), create_graph=c)
                     for c in (True, False))
     assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("hidden,nout", [(128, 19), (64, 19), (256, 130)])
+def test_second_derivatives_without_a_checkpoint(hidden, nout):
+    """The same of the float32 layers: a Linear's dx is differentiated again, what a kernel computes raises."""
+    from npa_amd import mlp as M
+    net, g = _net(83, nout, True, hidden, hidden)
+    x = torch.randn(300, 83, device="cuda", generator=g).requires_grad_(True)
+
+    def penalty(y):
+        (dx,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        return dx.square().sum()
+
+    if nout <= 64:
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            (penalty(M.mlp(net, x)) + net(x).sum()).backward()
+    else:
+        got = torch.autograd.grad(penalty(M.mlp(net, x)), list(net.parameters()))
+        for a, b in zip(got, torch.autograd.grad(penalty(net(x)), list(net.parameters()))):
+            assert ((a - b).norm() <= 1e-5 * b.norm()).item()
+    dw = torch.autograd.grad(M.mlp(net, x).sum(), net[0].weight, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        dw.square().sum().backward()
+    first, again = (torch.autograd.grad(M.mlp(net, x).sum(), list(net.parameters()), create_graph=c)
+                    for c in (True, False))
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
