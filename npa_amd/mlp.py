@@ -324,11 +324,15 @@ class MlpRows8(torch.autograd.Function):
 
 def _rows8_ok(x, layer):
     """What ``LinearRows8`` and ``ReluLinear8`` keep in 8 bits; any other input
-    keeps the layer's own function."""
+    keeps the layer's own function, rows that the weight gradient from codes
+    does not take among them."""
     tensors = [t for t in (x, layer.weight, layer.bias) if t is not None]
-    return (torch.is_grad_enabled() and any(t.requires_grad for t in tensors) and x.dim() >= 1
+    if not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors) and x.dim() >= 1
             and all(t.is_cuda and t.dtype == torch.float32 and t.device == x.device for t in tensors)
-            and not torch.is_autocast_enabled())
+            and not torch.is_autocast_enabled()):
+        return False
+    out_f, in_f = layer.weight.shape
+    return _lib.sphops_rows8_weight_grad_workspace_bytes(x.numel() // max(in_f, 1), in_f, out_f) >= 0
 
 
 def _check_checkpoint(checkpoint):

@@ -75,3 +75,20 @@ def test_second_derivatives_without_a_checkpoint(hidden, nout):
     first, again = (torch.autograd.grad(M.mlp(net, x).sum(), list(net.parameters()), create_graph=c)
                     for c in (True, False))
     assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_widths_that_no_codes_are_kept_of():
+    """Rows past the widest that is kept run as they do without a checkpoint."""
+    from npa_amd import mlp as M
+    layer = torch.nn.Linear(70000, 65).cuda().requires_grad_(False)
+    a = torch.randn(3, 70000, device="cuda", generator=_gen(2)).requires_grad_(True)
+    grads = []
+    for mode in (None, "int8"):
+        for net in (layer, torch.nn.Sequential(torch.nn.ReLU(), layer)):
+            y = M.mlp(net, a, checkpoint=mode)
+            grads.append((y.detach(), *torch.autograd.grad(y, a, torch.ones_like(y))))
+    assert all(torch.equal(p, q) for i in (0, 1) for p, q in zip(grads[i], grads[i + 2]))
+    with pytest.raises(RuntimeError):  # the layer's own weight gradient ends at 32768 features, with and without
+        M.mlp(layer.requires_grad_(True), a).sum().backward()
+    with pytest.raises(RuntimeError):
+        M.mlp(layer, a, checkpoint="int8").sum().backward()
