@@ -560,7 +560,8 @@ int sphops_mlp_weight_grad(const float* z, const float* a, const float* dy, cons
  * code is positive exactly where x is (in rows that are finite). */
 int sphops_quantize_rows(const void* x, int type, int64_t row_stride, int8_t* codes, int64_t ld, float* scale,
                          int64_t rows, int64_t cols, int relu, void* stream);
-/* out (rows x cols, dense, of `type`) = code * scale, rounded once. */
+/* out (rows x cols, dense, of `type`) = code * scale, rounded once.  Where m is
+ * float32's largest number 127 * scale rounds past it: that value is m. */
 int sphops_restore_rows(const int8_t* codes, int64_t ld, const float* scale, void* out, int type, int64_t rows,
                         int64_t cols, void* stream);
 

@@ -140,7 +140,7 @@ __global__ __launch_bounds__(kRowThreads) void k_restore_rows(const int8_t* __re
       for (int i = 0; i < V / 4; ++i) {
         const uint32_t w = k + 4 * i < (int)ld ? *reinterpret_cast<const uint32_t*>(row + k + 4 * i) : 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p.set(4 * i + j, from_f32<T>((float)(int8_t)(w >> (8 * j)) * s));
+        for (int j = 0; j < 4; ++j) p.set(4 * i + j, from_f32<T>(row_value((int)(int8_t)(w >> (8 * j)), s)));
       }
       p.store(out + r * cols, k, cols);
     }

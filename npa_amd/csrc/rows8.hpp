@@ -56,6 +56,13 @@ __device__ __forceinline__ uint32_t row_codes4(float a, float b, float c, float 
   return q.finite ? w : 0u;
 }
 
+// code * scale.  127 times m / 127 rounds past float32's largest number for that
+// one m alone, which stands in masks: it stays that number.
+__device__ __forceinline__ float row_value(int code, float scale) {
+  const float v = (float)code * scale;
+  return fabsf(v) > 0x1.fffffep127f ? copysignf(0x1.fffffep127f, v) : v;  // NaN stays
+}
+
 // Element types of the rows (SPHOPS_F32, SPHOPS_BF16, SPHOPS_F16).
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__hip_bfloat16 v) { return __bfloat162float(v); }

@@ -137,7 +137,8 @@ def quantize_rows(x, relu=False, align=4):
 
 
 def restore_rows(r, dtype=torch.float32):
-    """The tensor that ``r`` stands for, code * scale rounded once to dtype."""
+    """The tensor that ``r`` stands for, code * scale rounded once to dtype (a
+    row's float32 largest or lowest value, as masks hold, comes back as it was)."""
     _check_saved(r, "r")
     if dtype not in TYPES:
         raise TypeError("dtype must be float32, bfloat16 or float16")

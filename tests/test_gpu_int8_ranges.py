@@ -174,3 +174,18 @@ def test_rows_that_are_not_finite():
     keep = torch.ones(99, dtype=torch.bool, device="cuda")
     keep[[40, 41, 98]] = False
     assert torch.equal(got[keep], y[keep]) and torch.isnan(got[~keep]).all()
+
+def test_lowest_value_comes_back_finite():
+    """127 * (m / 127) rounds past float32's largest value for that value alone."""
+    from npa_amd import int8
+    big = -LOWEST
+    for cols in (1, 5, 83, 1030, 9000):
+        x = torch.zeros(3, cols, device="cuda")
+        x[0, cols // 2], x[1, 0], x[2, -1] = big, LOWEST, 3.0e38
+        r = int8.quantize_rows(x)
+        back = int8.restore_rows(r)
+        assert torch.equal(back[:2], x[:2]) and torch.isfinite(back).all()
+        assert torch.all((back.double() - x.double()).abs() <= 0.5 * r.scale.double()[:, None] * (1 + 2.0 ** -20))
+        x[0, 0] = float("nan")
+        back = int8.restore_rows(int8.quantize_rows(x))
+        assert torch.isnan(back[0]).all() and torch.isfinite(back[1:]).all()
