@@ -1297,6 +1297,7 @@ int sphops_rows8_weight_grad(const int8_t* codes, int64_t ld, const float* scale
     require_rows8(rows, in_features, ld);
     require(dw != nullptr && (rows == 0 || (codes && scale && dy && workspace)), "null buffer");
     require(reinterpret_cast<uintptr_t>(codes) % 4 == 0, "codes must be 4-byte aligned");
+    require(sphops::pk::aligned16(workspace), "workspace must be 16-byte aligned");
     sphops::run_rows8_weight_grad(codes, ld, scale, dy, dw, db, rows, in_features, out_features,
                                   static_cast<float*>(workspace), sphops::as_stream(stream));
   });
@@ -1316,6 +1317,7 @@ int sphops_linear8(const void* x, int type, int64_t row_stride, const int8_t* w_
     require_weight8(w_codes, w_ld, in_features);
     require(rows <= 1 || row_stride >= 0, "row_stride must be >= 0");
     require(rows == 0 || (x && w_codes && w_scale && y && workspace), "null buffer");
+    require(sphops::pk::aligned16(workspace), "workspace must be 16-byte aligned");
     sphops::run_linear8(x, type, row_stride, w_codes, w_ld, w_scale, b, y, rows, in_features, out_features, workspace,
                         sphops::as_stream(stream));
   });
@@ -1362,6 +1364,7 @@ int sphops_mlp_rows8_backward(const int8_t* codes, int64_t ld, const float* scal
     require_rows8(rows, in_features, ld);
     require(rows == 0 || (codes && scale && dy && w1 && w2 && workspace), "null buffer");
     require(reinterpret_cast<uintptr_t>(codes) % 4 == 0, "codes must be 4-byte aligned");
+    require(sphops::pk::aligned16(workspace), "workspace must be 16-byte aligned");
     sphops::run_mlp_rows8_backward(codes, ld, scale, dy, w1, b1, w2, dz, dw1, db1, dw2, db2, rows, in_features,
                                    out_features, static_cast<float*>(workspace), sphops::as_stream(stream));
   });
