@@ -557,7 +557,8 @@ int sphops_mlp_weight_grad(const float* z, const float* a, const float* dy, cons
 
 /* x: rows of `type`, row_stride elements apart (each row contiguous).  relu:
  * the rows kept are relu(x), and no positive value has the code 0, so that a
- * code is positive exactly where x is (in rows that are finite). */
+ * code is positive exactly where x is (in rows that are finite); values below
+ * half a scale stand for a whole one. */
 int sphops_quantize_rows(const void* x, int type, int64_t row_stride, int8_t* codes, int64_t ld, float* scale,
                          int64_t rows, int64_t cols, int relu, void* stream);
 /* out (rows x cols, dense, of `type`) = code * scale, rounded once.  Where m is

@@ -45,10 +45,11 @@ __device__ __forceinline__ void tile_of(uint32_t id, int mt, int nt, int& m, int
 // k = 16 (l / 32).
 //
 // Bound: the matrix cores and the loads' latency under them: 8192 x 4096 -> 8192
-// in 266 us with the 19 of putting x into 8 bits (2.2 POP/s; the library's int8
-// product alone 255), 4096^3 80.  The 256 and 128 tiles take 2 stages (4 for the
-// 128: 1024 x 4096 -> 4096 34 us for 35, but 2048 rows 60 for 53), the 64 tile, whose
-// workgroups are few and wait on memory, 4 (128 x 4096 -> 4096 15 us, 2 stages 21).
+// in 270 us for a call among others, 20 of them to put x into 8 bits (2.2 POP/s; the
+// library's int8 product alone 255; kernels profiled by themselves 292 + 20), 4096^3
+// 80.  The 256 and 128 tiles take 2 stages (4 for the 128: 1024 x 4096 -> 4096 34 us
+// for 35, but 2048 rows 60 for 53), the 64 tile, whose workgroups are few and wait on
+// memory, 4 (128 x 4096 -> 4096 15 us, 2 stages 21).
 //
 // xq's rows end in zeros up to a multiple of the step, so what a channel's last
 // step holds past its codes counts nothing; its address is kept inside the row.

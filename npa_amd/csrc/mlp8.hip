@@ -254,10 +254,11 @@ constexpr int lds_pieces(int ct, int ot) { return 12288 * image_steps(ct) + 2457
 // The largest of a product's six parts have sums of their own: they are rounded
 // as often as there are steps, not six times as often.
 //
-// Bound: matrix and vector work of the same SIMD; 2^20 rows, 83 -> 19 in 208 us
-// (192 matrix instructions of 32 cycles a row tile: 82 us of them at 2.4 GHz;
-// about 1300 vector ones, mostly splits; 0.52 GB, 101 us at the rate of a copy).
-// With shared powers of two and halves, half the matrix work: 146 us.
+// Bound: matrix and vector work, which add up; 2^20 rows, 83 -> 19 in 208 us (a
+// SIMD's 192 matrix instructions of 32 cycles and 1340 vector ones of 4 a row
+// tile make 197 + 171 thousand cycles, counted 360 to 400 in all; 0.52 GB, 101 us
+// at the rate of a copy).  With shared powers of two and halves, half the matrix
+// work: 146 us.
 template <int CT, int OT, int kThreads>
 __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
     const float* __restrict__ z, const float* __restrict__ w1, const float* __restrict__ b1,
@@ -417,8 +418,8 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_forward8(
 // in three bfloat16 pieces, as in the forward.  dz's stores are whole lines
 // because rows are registers in its product.
 //
-// Bound: as the forward's; 2^20 rows, 83 -> 19 in 240 us (264 matrix
-// instructions a row tile: 113 us at 2.4 GHz; 168 us with halves).
+// Bound: as the forward's; 2^20 rows, 83 -> 19 in 240 us (270 + 154 thousand
+// cycles of 410 to 456; 168 us with halves).
 template <int CT, int OT, int kThreads>
 __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
     const int8_t* __restrict__ codes, int64_t ld, const float* __restrict__ scale, const float* __restrict__ dy,
@@ -588,7 +589,7 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_mlp_input_grad8(
 
 constexpr int kGradThreads = 256;
 // Waves a SIMD: two where they do not spill.  us with one and two: 2^20 rows, 83 ->
-// 19 408 and 361 with the forward; 2^18, 112 -> 19 145 and 158, 83 -> 35 142 and 150.
+// 19 247 and 210; 2^18, 96 -> 30 73 and 68, 112 -> 19 83 and 87, 83 -> 35 83 and 91.
 constexpr int weight_grad8_waves(int ks, int os) { return ks > 6 || os > 2 ? 1 : 2; }
 
 // Workgroup = one chunk of rows, wave t the hidden units 32 t .. 32 t + 31 with
@@ -599,10 +600,10 @@ constexpr int weight_grad8_waves(int ks, int os) { return ks > 6 || os > 2 ? 1 :
 // The next tile is loaded under this one's products.  The chunk's partial sums:
 // dW1 (128 x nin), db1 (128), dW2 (nout x 128), db2 (nout).
 //
-// Six products of bfloat16 pieces, three against codes: halves with a running
-// power of two were faster at 2^20 rows (205 us for 245) and slower at 65 K (62 for
-// 48).  Bound: matrix and vector work in one wave in turn, two waves a SIMD; 2^20
-// rows, 83 -> 19 in 190..260 us as the clock allows.
+// Six products of bfloat16 pieces, three against codes.  Hidden values and
+// upstreams above the largest bfloat16, 3.39e38, count as infinite here.
+// Bound: matrix and vector work, which add up (246 + 196 thousand cycles of a SIMD,
+// counted 412 to 445 in all); 2^20 rows, 83 -> 19 in 208 us, in a profile 256.
 template <int KS, int OS>
 __global__ __launch_bounds__(kGradThreads, weight_grad8_waves(KS, OS)) void k_mlp_weight_grad8(
     const int8_t* __restrict__ codes, int64_t ld, const float* __restrict__ scale, const float* __restrict__ dy,

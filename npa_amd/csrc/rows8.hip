@@ -42,7 +42,9 @@ __device__ __forceinline__ void write_codes(int8_t* __restrict__ row, const Piec
 
 // L lanes a row, which they hold in N pieces each: the row is read once.  With
 // RELU the row kept is relu(x), and no positive value has the code 0: a code is
-// positive exactly where x is.  L = 256: the workgroup's four waves share a
+// positive exactly where x is (in finite rows).  Values below half a scale are
+// raised to a whole one for that, so what is computed from such codes leans
+// upward where most of a row is small beside its largest.  L = 256: the workgroup's four waves share a
 // row.
 //
 // Bound: HBM, x read once and a quarter of it written: 2^20 x 83 float32 in 91
@@ -402,10 +404,13 @@ void with_block(const Grad8Plan& p, F&& f) {
 
 // Waves: as many along the outputs as there are tiles, the rest along the inputs;
 // eight where both are many, which halves what a block reads (262144 rows, 256 ->
-// 256 123 us, four 182; 65536 rows, 163 -> 128 22 and 26).  Chunks: one for every
-// workgroup the card holds at once, two a CU or one of eight waves (2^20 rows, 83
+// 256 123 us, four 182; 65536 rows, 163 -> 128 22 and 26).  Chunks: two for every
+// CU, or one of eight waves, which is what the card holds at once (2^20 rows, 83
 // -> 128 136 us, half as many chunks 179, twice 147; 8192 rows, 2048 -> 2048 191,
-// 332 and 198), of at least two steps.
+// 332 and 198), of at least two steps.  Four input tiles a wave in one row or
+// column of waves (97 to 128 inputs and more than 64 outputs, 385 to 512 and up to
+// 32) take 84 KB of LDS, one workgroup a CU, and run these chunks in two turns: 2^20
+// rows, 128 -> 128 215 us beside 131 of 96 -> 128, 512 -> 32 204 beside 123 of 384.
 Grad8Plan grad8_plan(int64_t rows, int nin, int nout) {
   Grad8Plan p;
   const int ot = (nout + 31) / 32, it = (nin + 31) / 32;
@@ -448,8 +453,9 @@ void run_rows8_weight_grad(const int8_t* codes, int64_t ld, const float* scale, 
   }
   // few chunks, or enough elements to fill the card: a thread an element; else the
   // workgroups of linear_grad.hip share an element's chunks out.  Whole gradient:
-  // 512 rows, 2048 -> 2048 (8 chunks) 34 and 142 us; 8192, 512 -> 512 (32) 27 and 34;
-  // 65536, 256 -> 256 (128 chunks, 65792 elements) 45 and 38.
+  // 512 rows, 2048 -> 2048 (2 chunks) 35 and 144 us; 4096, 1024 -> 1024 (8) 41 and
+  // 67; 8192, 512 -> 512 (32) 28 and 35; 65536, 256 -> 256 (128 chunks, 65792
+  // elements) 45 and 39; 2048, 64 -> 64 (32 chunks, 4160 elements) 8.4 and 7.0.
   if (p.chunks <= 16 || (p.chunks <= 64 && n >= 131072))
     hipLaunchKernelGGL(k_rows8_sum, dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, st, work, dw, db, nw, nout,
                        p.chunks);

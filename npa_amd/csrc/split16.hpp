@@ -4,8 +4,8 @@
 // Products of float32 factors on the 16-bit matrix cores (a 32 x 32 x 16
 // instruction takes 32 cycles, eight float32 ones of 32 x 32 x 2 take 512): a
 // factor is split into three bfloat16 pieces, which hold its 24 bits at
-// float32's range, and the six products of pieces that are not below 2^-25 of
-// |a b| are summed in float32.  A value's pieces depend on nothing else, so
+// float32's range, and the six largest products of pieces are summed in float32
+// (the other three are at most 2^-26 of |a b| together).  A value's pieces depend on nothing else, so
 // each product is as exact whatever stands beside it in its row or matrix.
 // (Two float16 halves and three products are faster, but halves need a power of
 // two shared by a row or matrix: what is 2^-18 of the largest value there loses

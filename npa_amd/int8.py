@@ -8,7 +8,7 @@ code a value: with m = max(max |x|, 2^-100),
     scale = m / 127        code = round(x * (127 / m))        value = code * scale
 
 in float32 steps, ties to the even code, so a value is off by at most half a
-scale.  A row that holds a NaN or an infinity gets a NaN scale: whatever is
+scale (with ``relu`` by less than one: see ``quantize_rows``).  A row that holds a NaN or an infinity gets a NaN scale: whatever is
 computed from it is NaN.
 
 * ``quantize_rows`` / ``restore_rows``: a tensor to a ``Rows8`` and back;
@@ -16,7 +16,7 @@ computed from it is NaN.
   runs again in the backward.
 * ``weight_grad``: a linear layer's dW and db from its saved input;
   ``npa_amd.mlp.mlp(module, z, checkpoint="int8")`` trains a module's layers
-  that way, and NPA's Linear, ReLU, Linear keeps nothing but z in 8 bits (87
+  that way, and NPA's Linear, ReLU, Linear keeps nothing but z in 8 bits (88
   bytes a particle instead of 844 at 83 inputs).
 * ``linear`` / ``mlp`` and their modules ``Int8Linear`` / ``Int8Mlp``: inference
   with integer products, a scale for each row and each output channel.
@@ -120,8 +120,11 @@ def _rows_view(x):
 
 def quantize_rows(x, relu=False, align=4):
     """x's rows (last dimension) in 8 bits.  With ``relu`` the rows kept are
-    relu(x), and a code is positive exactly where x is.  ``align``: bytes a row
-    of codes is padded to (a multiple of 4)."""
+    relu(x), and in finite rows a code is positive exactly where x is: positive
+    values below half a scale have the code 1, not 0, and stand for up to a
+    scale more than they are.  That is little where rows have no outliers; in a
+    row whose largest value is hundreds of times the others' it is most of them.
+    ``align``: bytes a row of codes is padded to (a multiple of 4)."""
     _check_rows(x, "x")
     if align < 4 or align % 4:
         raise ValueError("align must be a multiple of 4")
