@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define SPHOPS_ABI_VERSION 25
+#define SPHOPS_ABI_VERSION 26
 
 #define SPHOPS_CLAMPED 0
 #define SPHOPS_PERIODIC 1
@@ -608,6 +608,80 @@ int sphops_mlp_rows8_backward(const int8_t* codes, int64_t ld, const float* scal
                               float* db2, int64_t rows, int in_features, int hidden, int out_features,
                               void* workspace, void* stream);
 int64_t sphops_mlp_rows8_workspace_bytes(int64_t rows, int in_features, int hidden, int out_features);
+
+/*
+ * Layer norm over rows of cols values of `type` (no reference counterpart):
+ * with m = mean x, v = mean (x - m)^2, y = (x - m) / sqrt(v + eps) * w + b, in
+ * float32 and rounded once.  w and b (cols) are float32 (wide) or of `type`;
+ * either may be NULL.  x's rows are row_stride elements apart, y's cols.  stats
+ * (two floats a row, 8-byte aligned, or NULL) is kept for the backward, which
+ * writes dx (rows x cols, dense), dw and db (of the weights' type); each may be
+ * NULL.  dw and db are summed in a fixed order.  workspace:
+ * sphops_layer_norm_workspace_bytes bytes (-1: not supported), 4-byte aligned.
+ */
+int sphops_layer_norm(const void* x, int type, int64_t row_stride, const void* w, const void* b, int wide, void* y,
+                      float* stats, int64_t rows, int64_t cols, float eps, void* stream);
+int64_t sphops_layer_norm_workspace_bytes(int type, int64_t rows, int64_t cols);
+int sphops_layer_norm_backward(const void* x, int64_t row_stride, const void* dy, int64_t dy_stride, int type,
+                               const void* w, int wide, const float* stats, void* dx, void* dw, void* db, int64_t rows,
+                               int64_t cols, void* workspace, void* stream);
+
+/*
+ * Rows sorted by expert (no reference counterpart).  Each of rows x choices
+ * entries of index (int32, or int64 with wide) names an expert, or none: any
+ * number outside 0 .. experts - 1.  A stable sort gives the entries places,
+ * expert after expert, those without one behind the last: offsets (experts + 1)
+ * receives each expert's first place (the last word: the first one behind them),
+ * slot (rows x choices) each entry's place, ~place for an entry without an
+ * expert, and source (rows x choices) the entry of each place.  experts is at
+ * most 1024, choices at most 64, rows x choices at most 2^30.  workspace:
+ * sphops_sort_rows_workspace_bytes bytes (-1: not supported), 4-byte aligned.
+ */
+int sphops_sort_rows(const void* index, int wide, int64_t rows, int choices, int experts, int32_t* offsets,
+                     int32_t* slot, int32_t* source, void* workspace, void* stream);
+int64_t sphops_sort_rows_workspace_bytes(int64_t rows, int choices, int experts);
+/* out (rows x choices places, dense): each row of x (rows, row_stride elements
+ * apart) at its entries' places, zeros at the places of entries without an
+ * expert. */
+int sphops_dispatch_rows(const void* x, int type, int64_t row_stride, const int32_t* slot, void* out, int64_t rows,
+                         int choices, int64_t cols, void* stream);
+/* y (rows, dense): the sum over a row's entries, in their order and in float32,
+ * of w (rows x choices; NULL: 1) times the place's row of results (dense);
+ * entries without an expert are left out.  With w NULL it is the gradient of
+ * sphops_dispatch_rows. */
+int sphops_combine_rows(const void* results, int type, const float* w, const int32_t* slot, void* y, int64_t rows,
+                        int choices, int64_t cols, void* stream);
+/* Its gradients: d_results (places; zeros for entries without an expert) and dw
+ * (rows x choices; 0 for them); each may be NULL, and results and w with dw and
+ * d_results. */
+int sphops_combine_rows_backward(const void* dy, int type, int64_t row_stride, const void* results, const float* w,
+                                 const int32_t* slot, void* d_results, float* dw, int64_t rows, int choices,
+                                 int64_t cols, void* stream);
+
+/*
+ * A linear layer for each of `experts` experts over slots rows sorted by expert
+ * (no reference counterpart): y = x w[e]^T + b[e] for the rows offsets[e] to
+ * offsets[e + 1] - 1 (device memory, from 0 on and not decreasing), zeros for the
+ * rows behind the last expert's.  All of `type`; w (experts, out_features,
+ * in_features) and b (experts, out_features, or NULL) dense, x's rows
+ * row_stride elements apart, y dense.  relu: y = max(y, 0).  Sums are float32;
+ * float32 factors are taken whole (three bfloat16 pieces each).
+ */
+int sphops_expert_linear(const void* x, int type, int64_t row_stride, const void* w, const void* b,
+                         const int32_t* offsets, void* y, int64_t slots, int experts, int in_features,
+                         int out_features, int relu, void* stream);
+/* dx (slots, in_features) = dy w[e]; with h (slots, in_features, dense) zero
+ * where h is not above 0.  Zeros behind the last expert's rows. */
+int sphops_expert_linear_input_grad(const void* dy, int type, int64_t dy_stride, const void* w, const void* h,
+                                    const int32_t* offsets, void* dx, int64_t slots, int experts, int in_features,
+                                    int out_features, void* stream);
+/* dw[e] = dy^T x and db[e] = the sums of dy over the expert's rows, in a fixed
+ * order; each may be NULL.  workspace: sphops_expert_linear_workspace_bytes bytes
+ * (-1: not supported), 16-byte aligned. */
+int sphops_expert_linear_weight_grad(const void* dy, int64_t dy_stride, const void* x, int type, int64_t row_stride,
+                                     const int32_t* offsets, void* dw, void* db, int64_t slots, int experts,
+                                     int in_features, int out_features, void* workspace, void* stream);
+int64_t sphops_expert_linear_workspace_bytes(int64_t slots, int experts, int in_features, int out_features);
 
 /* sphops_neighbor_candidates, _fill and _schedule in one call and two
  * launches fewer (no reference counterpart): counts (8-byte aligned) receives

@@ -1480,3 +1480,168 @@ int sphops_initialize_noalloc(int dim, int boundary, int mode, const int32_t* gr
 
 }  // extern "C"
 
+// ------------------------------------------------- layer norm and experts
+
+namespace {
+
+bool norm_fits(int type, int64_t rows, int64_t cols) {
+  return type >= SPHOPS_F32 && type <= SPHOPS_F16 && rows >= 0 && rows <= sphops::kMaxRows8Rows && cols >= 1 &&
+         cols <= sphops::kMaxRows8Cols;
+}
+bool sort_fits(int64_t rows, int choices, int experts) {
+  return rows >= 0 && choices >= 1 && choices <= sphops::kMaxChoices && experts >= 1 &&
+         experts <= sphops::kMaxExperts && rows <= sphops::kMaxSlots / choices;
+}
+void require_sorted(int type, int64_t rows, int choices, int64_t cols) {
+  require_type(type);
+  require(sort_fits(rows, choices, 1), "rows x choices must be in [0, 2^30], choices in [1, 64]");
+  require(cols >= 1 && cols <= sphops::kMaxGroupCols, "a row must have 1 to 65536 values");
+}
+bool expert_linear_fits(int64_t slots, int experts, int in_features, int out_features) {
+  return slots >= 0 && slots <= sphops::kMaxSlots && experts >= 1 && experts <= sphops::kMaxExperts &&
+         in_features >= 1 && in_features <= sphops::kMaxGroupCols && out_features >= 1 &&
+         out_features <= sphops::kMaxGroupCols &&
+         sphops::group_linear_fits(slots, experts, in_features, out_features);
+}
+void require_weight_type(const void* w, const void* b, bool wide, int type) {
+  const uintptr_t align = wide || type == SPHOPS_F32 ? 4 : 2;
+  require(reinterpret_cast<uintptr_t>(w) % align == 0 && reinterpret_cast<uintptr_t>(b) % align == 0,
+          "the weights must be aligned to their type");
+}
+
+}  // namespace
+
+extern "C" {
+
+int sphops_layer_norm(const void* x, int type, int64_t row_stride, const void* w, const void* b, int wide, void* y,
+                      float* stats, int64_t rows, int64_t cols, float eps, void* stream) {
+  return guarded([&] {
+    require_type(type);
+    require(norm_fits(type, rows, cols), "rows must be in [0, 2^30] and have 1 to 65536 values");
+    require(rows <= 1 || row_stride >= 0, "row_stride must be >= 0");
+    require(rows == 0 || (x && y), "null buffer");
+    require_weight_type(w, b, wide != 0, type);
+    require(reinterpret_cast<uintptr_t>(stats) % 8 == 0, "stats must be 8-byte aligned");
+    sphops::run_layer_norm(x, type, row_stride, w, b, wide != 0, y, stats, rows, cols, eps,
+                           sphops::as_stream(stream));
+  });
+}
+
+int64_t sphops_layer_norm_workspace_bytes(int type, int64_t rows, int64_t cols) {
+  if (!norm_fits(type, rows, cols)) return -1;
+  return sphops::layer_norm_backward_floats(type, rows, cols) * (int64_t)sizeof(float);
+}
+
+int sphops_layer_norm_backward(const void* x, int64_t row_stride, const void* dy, int64_t dy_stride, int type,
+                               const void* w, int wide, const float* stats, void* dx, void* dw, void* db, int64_t rows,
+                               int64_t cols, void* workspace, void* stream) {
+  return guarded([&] {
+    require_type(type);
+    require(norm_fits(type, rows, cols), "rows must be in [0, 2^30] and have 1 to 65536 values");
+    require(rows <= 1 || (row_stride >= 0 && dy_stride >= 0), "strides must be >= 0");
+    require(rows == 0 || (x && dy && stats && workspace), "null buffer");
+    require_weight_type(w, nullptr, wide != 0, type);
+    require(reinterpret_cast<uintptr_t>(stats) % 8 == 0, "stats must be 8-byte aligned");
+    require(reinterpret_cast<uintptr_t>(workspace) % 4 == 0, "workspace must be 4-byte aligned");
+    sphops::run_layer_norm_backward(x, row_stride, dy, dy_stride, type, w, wide != 0, stats, dx, dw, db, rows, cols,
+                                    static_cast<float*>(workspace), sphops::as_stream(stream));
+  });
+}
+
+int64_t sphops_sort_rows_workspace_bytes(int64_t rows, int choices, int experts) {
+  if (!sort_fits(rows, choices, experts)) return -1;
+  return sphops::sort_rows_workspace_words(rows * choices, experts) * (int64_t)sizeof(uint32_t);
+}
+
+int sphops_sort_rows(const void* index, int wide, int64_t rows, int choices, int experts, int32_t* offsets,
+                     int32_t* slot, int32_t* source, void* workspace, void* stream) {
+  return guarded([&] {
+    require(sort_fits(rows, choices, experts), "rows x choices must be in [0, 2^30], choices in [1, 64], experts in "
+                                               "[1, 1024]");
+    require(offsets && (rows == 0 || (index && slot && source)), "null buffer");
+    require(sphops::sort_rows_workspace_words(rows * choices, experts) == 0 || workspace, "null buffer");
+    require(reinterpret_cast<uintptr_t>(workspace) % 4 == 0, "workspace must be 4-byte aligned");
+    sphops::run_sort_rows(index, wide != 0, rows * choices, experts, offsets, slot, source,
+                          static_cast<uint32_t*>(workspace), sphops::as_stream(stream));
+  });
+}
+
+int sphops_dispatch_rows(const void* x, int type, int64_t row_stride, const int32_t* slot, void* out, int64_t rows,
+                         int choices, int64_t cols, void* stream) {
+  return guarded([&] {
+    require_sorted(type, rows, choices, cols);
+    require(rows <= 1 || row_stride >= 0, "row_stride must be >= 0");
+    require(rows == 0 || (x && slot && out), "null buffer");
+    sphops::run_dispatch_rows(x, type, row_stride, slot, out, rows, choices, cols, sphops::as_stream(stream));
+  });
+}
+
+int sphops_combine_rows(const void* results, int type, const float* w, const int32_t* slot, void* y, int64_t rows,
+                        int choices, int64_t cols, void* stream) {
+  return guarded([&] {
+    require_sorted(type, rows, choices, cols);
+    require(rows == 0 || (results && slot && y), "null buffer");
+    sphops::run_combine_rows(results, type, cols, w, slot, y, rows, choices, cols, sphops::as_stream(stream));
+  });
+}
+
+int sphops_combine_rows_backward(const void* dy, int type, int64_t row_stride, const void* results, const float* w,
+                                 const int32_t* slot, void* d_results, float* dw, int64_t rows, int choices,
+                                 int64_t cols, void* stream) {
+  return guarded([&] {
+    require_sorted(type, rows, choices, cols);
+    require(rows <= 1 || row_stride >= 0, "row_stride must be >= 0");
+    require(rows == 0 || (dy && slot && (dw == nullptr || results)), "null buffer");
+    sphops::run_combine_rows_backward(dy, type, row_stride, results, w, slot, d_results, dw, rows, choices, cols,
+                                      sphops::as_stream(stream));
+  });
+}
+
+int sphops_expert_linear(const void* x, int type, int64_t row_stride, const void* w, const void* b,
+                         const int32_t* offsets, void* y, int64_t slots, int experts, int in_features,
+                         int out_features, int relu, void* stream) {
+  return guarded([&] {
+    require_type(type);
+    require(expert_linear_fits(slots, experts, in_features, out_features), "layer not supported");
+    require(slots <= 1 || row_stride >= 0, "row_stride must be >= 0");
+    require(slots == 0 || (x && w && offsets && y), "null buffer");
+    sphops::run_group_linear(x, type, row_stride, w, b, nullptr, offsets, y, slots, experts, in_features,
+                             out_features, relu != 0, false, sphops::as_stream(stream));
+  });
+}
+
+int sphops_expert_linear_input_grad(const void* dy, int type, int64_t dy_stride, const void* w, const void* h,
+                                    const int32_t* offsets, void* dx, int64_t slots, int experts, int in_features,
+                                    int out_features, void* stream) {
+  return guarded([&] {
+    require_type(type);
+    require(expert_linear_fits(slots, experts, in_features, out_features), "layer not supported");
+    require(slots <= 1 || dy_stride >= 0, "dy_stride must be >= 0");
+    require(slots == 0 || (dy && w && offsets && dx), "null buffer");
+    sphops::run_group_linear(dy, type, dy_stride, w, nullptr, h, offsets, dx, slots, experts, out_features,
+                             in_features, false, true, sphops::as_stream(stream));
+  });
+}
+
+int64_t sphops_expert_linear_workspace_bytes(int64_t slots, int experts, int in_features, int out_features) {
+  if (!expert_linear_fits(slots, experts, in_features, out_features)) return -1;
+  return sphops::group_weight_grad_floats(slots, experts, in_features, out_features) * (int64_t)sizeof(float);
+}
+
+int sphops_expert_linear_weight_grad(const void* dy, int64_t dy_stride, const void* x, int type, int64_t row_stride,
+                                     const int32_t* offsets, void* dw, void* db, int64_t slots, int experts,
+                                     int in_features, int out_features, void* workspace, void* stream) {
+  return guarded([&] {
+    require_type(type);
+    require(expert_linear_fits(slots, experts, in_features, out_features), "layer not supported");
+    require(slots <= 1 || (row_stride >= 0 && dy_stride >= 0), "strides must be >= 0");
+    require(offsets && (slots == 0 || (dy && x)), "null buffer");
+    require(sphops::group_weight_grad_floats(slots, experts, in_features, out_features) == 0 || workspace,
+            "null buffer");
+    require(sphops::pk::aligned16(workspace), "workspace must be 16-byte aligned");
+    sphops::run_group_weight_grad(dy, dy_stride, x, type, row_stride, offsets, dw, db, slots, experts, in_features,
+                                  out_features, static_cast<float*>(workspace), sphops::as_stream(stream));
+  });
+}
+
+}  // extern "C"

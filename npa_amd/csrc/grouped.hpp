@@ -1,0 +1,281 @@
+// Products over rows sorted by expert (grouped.hip): which rows a workgroup's
+// tile holds, panels through LDS as 16-bit pieces, and the matrix products of a
+// tile.
+#pragma once
+
+#include "rows8.hpp"
+#include "split16.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace sphops {
+
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// Tile `id` of the groups' rows in tiles of `size`: group e's rows are
+// offsets[e] to offsets[e + 1], the group after the last expert's the rows
+// behind them all.  Offsets are clamped to the rows there are, so that no tile
+// leaves them whatever they hold.  Every wave finds it for itself.
+struct GroupTile {
+  int group;        // -1: no such tile
+  int64_t tile;     // within the group
+  int64_t lo, hi;   // the group's rows
+};
+__device__ __forceinline__ GroupTile group_tile(const int32_t* __restrict__ offsets, int experts, int64_t slots,
+                                                int64_t id, int64_t size, bool behind) {
+  const int lane = threadIdx.x & 63, groups = experts + (behind ? 1 : 0);
+  GroupTile g{-1, 0, 0, 0};
+  for (int base = 0; base < groups; base += 64) {
+    const int e = base + lane;
+    int64_t lo = 0, hi = 0;
+    if (e < groups) {
+      lo = e == 0 ? 0 : min<int64_t>(max(offsets[e], 0), slots);
+      hi = e == experts ? slots : max<int64_t>(lo, min<int64_t>(offsets[e + 1], slots));
+    }
+    const int64_t mine = (hi - lo + size - 1) / size;
+    int64_t upto = mine;
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) {
+      const int64_t other = __shfl_up(upto, s);
+      if (lane >= s) upto += other;
+    }
+    const uint64_t past = __ballot(upto > id);
+    if (past != 0) {
+      const int at = __ffsll((unsigned long long)past) - 1;
+      g.group = base + at;
+      g.tile = id - __shfl(upto - mine, at);
+      g.lo = __shfl(lo, at);
+      g.hi = __shfl(hi, at);
+      break;
+    }
+    id -= __shfl(upto, 63);
+  }
+  g.group = __builtin_amdgcn_readfirstlane(g.group);
+  return g;
+}
+
+// The products' 16-bit type and the pieces a value of T is split into.
+template <class T>
+struct Pieces {
+  static constexpr int P = 1;
+};
+template <>
+struct Pieces<float> {
+  static constexpr int P = 3;
+};
+
+template <class T>
+__device__ __forceinline__ f32x16 mma16(s16x8 a, s16x8 b, f32x16 c) {
+  if constexpr (std::is_same_v<T, __half>)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+}
+template <class T>
+__device__ __forceinline__ f32x4 mma16(s16x8 a, s16x8 b, f32x4 c) {
+  if constexpr (std::is_same_v<T, __half>)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+}
+
+// Four float32 values as the three bfloat16 pieces of each (see split3).
+__device__ __forceinline__ void split4(const Piece<float>& v, u32x2 (&out)[3]) {
+  constexpr float kTop = 0x1.fep127f;
+  float x[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = v.get(j);
+#pragma unroll
+  for (int p = 0; p < 3; ++p) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float a = x[2 * j], b = x[2 * j + 1];
+      if (p == 0) {
+        float q = __builtin_amdgcn_fmed3f(a, -kTop, kTop), r = __builtin_amdgcn_fmed3f(b, -kTop, kTop);
+        out[p][j] = bf16_pair(q, r);
+        x[2 * j] = a - __builtin_bit_cast(float, out[p][j] << 16);
+        x[2 * j + 1] = b - __builtin_bit_cast(float, out[p][j] & 0xffff0000u);
+      } else {
+        out[p][j] = bf16_pair(a, b);
+        x[2 * j] = a;
+        x[2 * j + 1] = b;
+      }
+    }
+  }
+}
+
+// A panel of a product's operand: `rows` rows of `cols` values in memory.  KMAJOR: a
+// row holds the values along the summed dimension of one output row (or
+// column); else a row is one step of the sum and its values are the outputs'.
+// What lies past the rows and columns counts as zeros.
+template <class T>
+struct Panel {
+  const T* base;
+  int64_t stride;
+  int rows, cols;
+};
+
+constexpr int kStepK = 32;  // of the sum a step
+constexpr int kSide = 128;  // a tile's rows and columns
+constexpr int kGroupThreads = 512;
+constexpr int kOutbox = kGroupThreads / 64 * 2048;  // 16-bit words of LDS: 4 KB a wave for results on their way out
+
+template <class T, bool KMAJOR>
+struct PanelImage {
+  static constexpr int P = Pieces<T>::P, V = Piece<T>::V;
+  static constexpr int kRowPieces = (KMAJOR ? kStepK : kSide) / V;
+  static constexpr int kLoads = kSide * kStepK / V / kGroupThreads;
+  // 16-bit values of a plane: rows of 64 bytes whose 16-byte pieces are exchanged
+  // by the row's bits, or 32 rows of an odd number of 64 bytes (read down columns)
+  static constexpr int kPitch = KMAJOR ? kStepK : (kSide / 32 | 1) * 32;
+  static constexpr int kPlane = (KMAJOR ? kSide : kStepK) * kPitch;
+  static_assert(kGroupThreads % kRowPieces == 0 && kLoads >= 1, "whole rows a turn");
+
+  // The step from `k` on of the summed dimension.
+  __device__ __forceinline__ static void load(const Panel<T>& p, int64_t k, Piece<T> (&out)[kLoads]) {
+    const int col = (int)threadIdx.x % kRowPieces * V, row = (int)threadIdx.x / kRowPieces;
+    const int at = KMAJOR ? (int)k + col : col;
+    const int64_t down = KMAJOR ? 0 : k;
+    const bool whole = (KMAJOR ? k + kStepK : kSide) <= p.cols;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int64_t r = down + row + i * (kGroupThreads / kRowPieces), kept = min(r, (int64_t)p.rows - 1);
+      if (whole) {
+        out[i].raw = *reinterpret_cast<const typename Piece<T>::Raw*>(p.base + kept * p.stride + at);
+        // a K-major panel's rows past the end give outputs that nobody stores
+        if (!KMAJOR && r >= p.rows) out[i].raw = typename Piece<T>::Raw{};
+      } else if (r < p.rows) {
+        out[i].load(p.base + r * p.stride, at, p.cols);
+      } else {
+        out[i].raw = typename Piece<T>::Raw{};
+      }
+    }
+  }
+  __device__ __forceinline__ static void store(const Piece<T> (&in)[kLoads], uint16_t* __restrict__ lds) {
+    const int col = (int)threadIdx.x % kRowPieces * V, row0 = (int)threadIdx.x / kRowPieces;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int row = row0 + i * (kGroupThreads / kRowPieces);
+      uint16_t* const to =
+          lds + row * kPitch + (KMAJOR ? 8 * ((col / 8) ^ (row >> 1 & 3)) + col % 8 : col);
+      if constexpr (P == 1) {
+        *reinterpret_cast<u32x4*>(to) = __builtin_bit_cast(u32x4, in[i].raw);
+      } else {
+        u32x2 s[3];
+        split4(in[i], s);
+#pragma unroll
+        for (int p = 0; p < P; ++p) *reinterpret_cast<u32x2*>(to + p * kPlane) = s[p];
+      }
+    }
+  }
+  // Operand of 32 rows from `first` on, steps 16 s .. + 15 of the sum: lane l's
+  // eight values are row l % 32, k = 16 s + 8 (l / 32) + 0 .. 7.
+  __device__ __forceinline__ static s16x8 read(const uint16_t* __restrict__ lds, int first, int s) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    if constexpr (KMAJOR) {
+      const int row = first + (lane & 31);
+      return *reinterpret_cast<const s16x8*>(lds + row * kPitch + 8 * ((2 * s + h) ^ (row >> 1 & 3)));
+    } else {
+      const int i = lane & 15, row = 16 * s + 8 * h + (i >> 2), col = first + 16 * (lane >> 4 & 1) + 4 * (i & 3);
+      return join(read_column(lds + row * kPitch + col), read_column(lds + (row + 4) * kPitch + col));
+    }
+  }
+};
+
+// Sums of a tile of 128 x 128 in eight waves of 64 rows by 32 columns.  Float32
+// factors are three bfloat16 pieces each: the product of the first ones has a
+// sum of its own, rounded once a step of 16, and every 128 of the summed
+// dimension both go into float32 sums that round to nearest (the matrix cores'
+// own round down).
+template <class T>
+struct TileSums {
+  static constexpr int P = Pieces<T>::P;
+  f32x16 acc[2], low[P == 3 ? 2 : 1], total[P == 3 ? 2 : 1];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) acc[i] = f32x16{};
+    if constexpr (P == 3) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) low[i] = total[i] = f32x16{};
+    }
+  }
+  __device__ __forceinline__ void flush() {
+    if constexpr (P == 3) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        total[i] += acc[i] + low[i];
+        acc[i] = low[i] = f32x16{};
+      }
+    }
+  }
+  // A's operand rows are the output's rows, B's its columns; result register r of
+  // lane l is column 8 (r / 4) + 4 (l / 32) + r % 4 of row l % 32.
+  template <class IA, class IB>
+  __device__ __forceinline__ void step(const uint16_t* __restrict__ a, const uint16_t* __restrict__ b, int row0,
+                                       int col0) {
+#pragma unroll
+    for (int s = 0; s < kStepK / 16; ++s) {
+      s16x8 bv[P], av[2][P];
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        bv[p] = IB::read(b + p * IB::kPlane, col0, s);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) av[i][p] = IA::read(a + p * IA::kPlane, row0 + 32 * i, s);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (P == 1) {
+          acc[i] = mma16<T>(bv[0], av[i][0], acc[i]);
+        } else {
+          low[i] = mma16<T>(bv[2], av[i][0], low[i]);
+          low[i] = mma16<T>(bv[0], av[i][2], low[i]);
+          low[i] = mma16<T>(bv[1], av[i][1], low[i]);
+          low[i] = mma16<T>(bv[1], av[i][0], low[i]);
+          low[i] = mma16<T>(bv[0], av[i][1], low[i]);
+          acc[i] = mma16<T>(bv[0], av[i][0], acc[i]);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ const f32x16& value(int i) const {
+    if constexpr (P == 3) return total[i];
+    else return acc[i];
+  }
+};
+
+// A wave's 32 x 32 results through 4 KB of LDS of its own and out as rows:
+// f(row, column, values) for pieces of V neighbouring columns.
+template <class T, class F>
+__device__ __forceinline__ void rows_of_tile(const f32x16& v, float* __restrict__ own, F&& f) {
+  constexpr int V = Piece<T>::V, kPieces = 32 / V;
+  const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    *reinterpret_cast<f32x4*>(own + 32 * c + 4 * ((2 * q + h) ^ (c & 7))) =
+        f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int n = 0; n < kPieces / 2; ++n) {
+    const int row = (64 * n + lane) / kPieces, at = (64 * n + lane) % kPieces;
+    float o[V];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      const f32x4 t = *reinterpret_cast<const f32x4*>(own + 32 * row + 4 * ((at * (V / 4) + i) ^ (row & 7)));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[4 * i + j] = t[j];
+    }
+    f(row, V * at, o);
+  }
+}
+
+}  // namespace
+
+}  // namespace sphops

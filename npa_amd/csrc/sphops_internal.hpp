@@ -401,6 +401,39 @@ void run_mlp_rows8_backward(const int8_t* codes, int64_t ld, const float* scale,
                             const float* b1, const float* w2, float* dz, float* dw1, float* db1, float* dw2,
                             float* db2, int64_t rows, int nin, int nout, float* work, hipStream_t st);
 
+// norm.hip: layer norm over rows; w and b float32 (wide) or of the rows' type
+void run_layer_norm(const void* x, int type, int64_t stride, const void* w, const void* b, bool wide, void* y,
+                    float* stats, int64_t rows, int64_t cols, float eps, hipStream_t st);
+int64_t layer_norm_backward_floats(int type, int64_t rows, int64_t cols);
+void run_layer_norm_backward(const void* x, int64_t stride, const void* dy, int64_t dy_stride, int type,
+                             const void* w, bool wide, const float* stats, void* dx, void* dw, void* db, int64_t rows,
+                             int64_t cols, float* work, hipStream_t st);
+
+// experts.hip: rows sorted by expert and back
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxChoices = 64;
+constexpr int64_t kMaxSlots = int64_t(1) << 30;
+int64_t sort_rows_workspace_words(int64_t n, int experts);
+void run_sort_rows(const void* index, bool wide, int64_t n, int experts, int32_t* offsets, int32_t* slot,
+                   int32_t* source, uint32_t* work, hipStream_t st);
+void run_dispatch_rows(const void* x, int type, int64_t stride, const int32_t* slot, void* out, int64_t rows,
+                       int choices, int64_t cols, hipStream_t st);
+void run_combine_rows(const void* results, int type, int64_t stride, const float* w, const int32_t* slot, void* y,
+                      int64_t rows, int choices, int64_t cols, hipStream_t st);
+void run_combine_rows_backward(const void* dy, int type, int64_t stride, const void* results, const float* w,
+                               const int32_t* slot, void* d_results, float* dw, int64_t rows, int choices,
+                               int64_t cols, hipStream_t st);
+// grouped.hip: linear layers of experts over sorted rows
+constexpr int64_t kMaxGroupCols = 65536;
+bool group_linear_fits(int64_t slots, int experts, int64_t cols, int64_t outs);
+void run_group_linear(const void* x, int type, int64_t xs, const void* w, const void* b, const void* mask,
+                      const int32_t* offsets, void* y, int64_t slots, int experts, int64_t cols, int64_t outs,
+                      bool relu, bool back, hipStream_t st);
+int64_t group_weight_grad_floats(int64_t slots, int experts, int64_t cols, int64_t outs);
+void run_group_weight_grad(const void* dy, int64_t dys, const void* x, int type, int64_t xs, const int32_t* offsets,
+                           void* dw, void* db, int64_t slots, int experts, int64_t cols, int64_t outs, float* work,
+                           hipStream_t st);
+
 constexpr uint32_t kMaxChannels = 64;
 constexpr int kRadixBins = 1024;  // digit values per radix-sort pass (10 bits)
 // Words of the radix histograms: kRadixBins tile counts per tile of 4096

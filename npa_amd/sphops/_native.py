@@ -10,7 +10,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get(
     "SPHOPS_HIP_LIB", os.path.join(os.path.dirname(_HERE), "_lib", "libsphops_hip.so"))
-ABI_VERSION = 25
+ABI_VERSION = 26
 
 if not os.path.exists(LIB_PATH):
     raise ImportError(
@@ -91,6 +91,18 @@ _SIGNATURES = {
     "sphops_mlp_rows8_backward": ([_p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _p, _p],
                                   _i32),
     "sphops_mlp_rows8_workspace_bytes": ([_i64, _i32, _i32, _i32], _i64),
+    "sphops_layer_norm": ([_p, _i32, _i64, _p, _p, _i32, _p, _p, _i64, _i64, _f32, _p], _i32),
+    "sphops_layer_norm_workspace_bytes": ([_i32, _i64, _i64], _i64),
+    "sphops_layer_norm_backward": ([_p, _i64, _p, _i64, _i32, _p, _i32, _p, _p, _p, _p, _i64, _i64, _p, _p], _i32),
+    "sphops_sort_rows": ([_p, _i32, _i64, _i32, _i32, _p, _p, _p, _p, _p], _i32),
+    "sphops_sort_rows_workspace_bytes": ([_i64, _i32, _i32], _i64),
+    "sphops_dispatch_rows": ([_p, _i32, _i64, _p, _p, _i64, _i32, _i64, _p], _i32),
+    "sphops_combine_rows": ([_p, _i32, _p, _p, _p, _i64, _i32, _i64, _p], _i32),
+    "sphops_combine_rows_backward": ([_p, _i32, _i64, _p, _p, _p, _p, _p, _i64, _i32, _i64, _p], _i32),
+    "sphops_expert_linear": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p], _i32),
+    "sphops_expert_linear_input_grad": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _p], _i32),
+    "sphops_expert_linear_weight_grad": ([_p, _i64, _p, _i32, _i64, _p, _p, _p, _i64, _i32, _i32, _i32, _p, _p], _i32),
+    "sphops_expert_linear_workspace_bytes": ([_i64, _i32, _i32, _i32], _i64),
     "sphops_forward": ([_p, _i32, _p, _p], _i32),
     "sphops_backward": ([_p, _i32, _i32, _i32, _i32, _p, _p], _i32),
     "sphops_neighbor_candidates": ([_p, _p, _p, _i32, _p], _i32),
