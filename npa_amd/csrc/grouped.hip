@@ -22,6 +22,52 @@ __device__ __forceinline__ void tile_of(uint32_t id, int64_t mt, int nt, int64_t
   n = (int)(at / size);
 }
 
+// The workgroup's row tile and column tile among those that there are (the
+// launch covers the most that there can be); false: neither.
+__device__ __forceinline__ bool rows_tile(const int32_t* __restrict__ offsets, int experts, int64_t slots, int size,
+                                          int nt, GroupTile& g, int& n) {
+  const int64_t mt = group_tiles(offsets, experts, slots, size, true);
+  const uint32_t id = xcd_block_id((uint32_t)(mt * nt));
+  if (id == 0xFFFFFFFFu) return false;
+  int64_t m;
+  tile_of(id, mt, nt, m, n);
+  g = group_tile(offsets, experts, slots, m, size, true);
+  return g.group >= 0;
+}
+
+// Rows behind the last expert's: zeros.
+template <class T>
+__device__ __forceinline__ void zero_rows(T* __restrict__ y, int64_t m0, int rows, int n0, int side, int outs) {
+  constexpr int V = Piece<T>::V;
+  for (int i = threadIdx.x; i < rows * (side / V); i += blockDim.x) {
+    Piece<T> o;
+    o.raw = typename Piece<T>::Raw{};
+    o.store(y + (m0 + i / (side / V)) * outs, n0 + i % (side / V) * V, outs);
+  }
+}
+
+// A piece of results on its way out: bias, then ReLU, then the mask.
+template <class T>
+__device__ __forceinline__ void finish(float (&v)[Piece<T>::V], const T* __restrict__ bias,
+                                       const T* __restrict__ mask, bool relu, T* __restrict__ y, int at, int outs) {
+  constexpr int V = Piece<T>::V;
+  Piece<T> o, t;
+  if (bias != nullptr) {
+    t.load(bias, at, outs);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] += t.get(j);
+  }
+  if (mask != nullptr) t.load(mask, at, outs);
+  o.raw = typename Piece<T>::Raw{};
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (relu) v[j] = v[j] <= 0.0f ? 0.0f : v[j];  // NaN stays
+    if (mask != nullptr && t.get(j) <= 0.0f) v[j] = 0.0f;
+    o.set(j, from_f32<T>(v[j]));
+  }
+  o.store(y, at, outs);
+}
+
 // y (slots x outs) = x (slots x cols) W_e^T + b_e, W_e (outs x cols); BACK: y = x
 // W_e with W_e (cols x outs), which is the input gradient.  relu: y = max(y, 0).
 // mask (slots x outs): y = 0 where it is not above 0.
@@ -31,27 +77,21 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_rows(const T* __restric
                                                               const T* __restrict__ mask,
                                                               const int32_t* __restrict__ offsets, T* __restrict__ y,
                                                               int64_t slots, int experts, int cols, int outs,
-                                                              bool relu, int64_t mt, int nt) {
+                                                              bool relu, int nt) {
   using IA = PanelImage<T, true>;
   using IB = PanelImage<T, !BACK>;
   constexpr int P = Pieces<T>::P, V = Piece<T>::V;
   __shared__ __attribute__((aligned(16))) uint16_t room[std::max(P * (IA::kPlane + IB::kPlane), kOutbox)];
   uint16_t *const as = room, *const bs = room + P * IA::kPlane;
-  int64_t m;
+  GroupTile g;
   int n;
-  tile_of(xcd_block_id(), mt, nt, m, n);
-  const GroupTile g = group_tile(offsets, experts, slots, m, kSide, true);
-  if (g.group < 0) return;
+  if (!rows_tile(offsets, experts, slots, kSide, nt, g, n)) return;
   const int64_t m0 = g.lo + g.tile * kSide;
   const int n0 = n * kSide, here = (int)min<int64_t>(kSide, g.hi - m0), outs_here = min(kSide, outs - n0);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
   const int row0 = wave / 4 * 64, col0 = wave % 4 * 32;
-  if (g.group == experts) {  // rows behind the last expert's
-    for (int i = threadIdx.x; i < here * (kSide / V); i += kGroupThreads) {
-      Piece<T> o;
-      o.raw = typename Piece<T>::Raw{};
-      o.store(y + (m0 + i / (kSide / V)) * outs, n0 + i % (kSide / V) * V, outs);
-    }
+  if (g.group == experts) {
+    zero_rows(y, m0, here, n0, kSide, outs);
     return;
   }
   const T* const we = w + (int64_t)g.group * cols * outs;
@@ -82,23 +122,78 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_rows(const T* __restric
     rows_of_tile<T>(sums.value(i), own, [&](int r, int c, float (&v)[V]) {
       const int row = row0 + 32 * i + r, at = n0 + col0 + c;
       if (row >= here || at >= outs) return;
-      Piece<T> o, t;
-      if (be != nullptr) {
-        t.load(be, at, outs);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] += t.get(j);
-      }
-      if (mask != nullptr) t.load(mask + (m0 + row) * outs, at, outs);
-      o.raw = typename Piece<T>::Raw{};
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (relu) v[j] = v[j] <= 0.0f ? 0.0f : v[j];  // NaN stays
-        if (mask != nullptr && t.get(j) <= 0.0f) v[j] = 0.0f;
-        o.set(j, from_f32<T>(v[j]));
-      }
-      o.store(y + (m0 + row) * outs, at, outs);
+      finish<T>(v, be, mask != nullptr ? mask + (m0 + row) * outs : nullptr, relu, y + (m0 + row) * outs, at, outs);
     });
   }
+}
+
+// The same for 16-bit rows in whole 16-byte pieces: panels straight from memory
+// to LDS.
+template <class T, bool BACK, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void k_group_rows_fast(const T* __restrict__ x, int64_t xs,
+                                                                  const T* __restrict__ w, const T* __restrict__ b,
+                                                                  const T* __restrict__ mask,
+                                                                  const int32_t* __restrict__ offsets,
+                                                                  T* __restrict__ y, int64_t slots, int experts,
+                                                                  int cols, int outs, bool relu, int nt) {
+  using Tile = FastTile<T, true, !BACK, BM, BN, WM, WN, false>;
+  constexpr int V = Piece<T>::V;
+  __shared__ __attribute__((aligned(16))) uint16_t s0[Tile::kStage], s1[Tile::kStage];
+  GroupTile g;
+  int n;
+  if (!rows_tile(offsets, experts, slots, BM, nt, g, n)) return;
+  const int64_t m0 = g.lo + g.tile * BM;
+  const int n0 = n * BN, here = (int)min<int64_t>(BM, g.hi - m0), outs_here = min(BN, outs - n0);
+  if (g.group == experts) {
+    zero_rows(y, m0, here, n0, BN, outs);
+    return;
+  }
+  const T* const we = w + (int64_t)g.group * cols * outs;
+  const typename Tile::A pa(Panel<T>{x + m0 * xs, xs, here, cols});
+  const typename Tile::B pb(BACK ? Panel<T>{we + n0, outs, cols, outs_here}
+                                 : Panel<T>{we + (int64_t)n0 * cols, cols, outs_here, cols});
+  Tile t;
+  t.run(pa, pb, cols, false, s0, s1);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+  const int row0 = wave / WN * (BM / WM), col0 = wave % WN * (BN / WN);
+  float* const own = reinterpret_cast<float*>(s0) + 1024 * wave;
+  static_assert(Tile::kWaves * 2048 <= Tile::kStage, "room");
+  const T* const be = b != nullptr ? b + (int64_t)g.group * outs : nullptr;
+#pragma unroll
+  for (int i = 0; i < Tile::TM; ++i) {
+#pragma unroll
+    for (int j = 0; j < Tile::TN; ++j) {
+      rows_of_tile<T>(t.acc[i][j], own, [&](int r, int c, float (&v)[V]) {
+        const int row = row0 + 32 * i + r, at = n0 + col0 + 32 * j + c;
+        if (row >= here || at >= outs) return;
+        finish<T>(v, be, mask != nullptr ? mask + (m0 + row) * outs : nullptr, relu, y + (m0 + row) * outs, at, outs);
+      });
+    }
+  }
+}
+
+// A weight gradient's workgroup: which piece (chunk of rows, or expert) and which
+// tile of dW.  A piece's tiles are dealt to the XCDs in contiguous shares, so that
+// each XCD works on every piece (experts differ in rows) and tiles that share
+// panels meet in its L2.
+struct GradTile {
+  int64_t piece;
+  int m, n;
+};
+__device__ __forceinline__ GradTile grad_tile(int mt, int nt) {
+  const uint32_t tiles = (uint32_t)(mt * nt), x = blockIdx.x % tiles;
+  const uint32_t xcd = x & 7u, q = tiles >> 3, rem = tiles & 7u, at = xcd * q + min(xcd, rem) + (x >> 3);
+  return GradTile{blockIdx.x / tiles, (int)(at / (uint32_t)nt), (int)(at % (uint32_t)nt)};
+}
+__device__ __forceinline__ GroupTile grad_rows(const int32_t* __restrict__ offsets, int experts, int64_t slots,
+                                               int64_t piece, int64_t chunk, bool chunks) {
+  if (chunks) return group_tile(offsets, experts, slots, piece, chunk, false);
+  GroupTile g;
+  g.group = (int)piece;
+  g.tile = 0;
+  g.lo = piece == 0 ? 0 : min<int64_t>(max(offsets[piece], 0), slots);
+  g.hi = max<int64_t>(g.lo, min<int64_t>(offsets[piece + 1], slots));
+  return g;
 }
 
 // dW_e (outs x cols) and db_e of a chunk of the expert's rows.  part null: the
@@ -116,21 +211,11 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_weight_grad(const T* __
   constexpr int P = Pieces<T>::P, V = Piece<T>::V;
   __shared__ __attribute__((aligned(16))) uint16_t room[std::max(P * 2 * I::kPlane, kOutbox)];
   uint16_t *const as = room, *const bs = room + P * I::kPlane;
-  const uint32_t id = xcd_block_id();
-  const int tiles = mt * nt, at = (int)(id % tiles);
-  const int64_t piece = id / tiles;
-  const int n = at % nt, m0 = at / nt * kSide, n0 = n * kSide;
-  GroupTile g;
-  if (part == nullptr) {
-    const int e = (int)piece;
-    g.group = e;
-    g.lo = e == 0 ? 0 : min<int64_t>(max(offsets[e], 0), slots);
-    g.hi = max<int64_t>(g.lo, min<int64_t>(offsets[e + 1], slots));
-    g.tile = 0;
-  } else {
-    g = group_tile(offsets, experts, slots, piece, chunk, false);
-    if (g.group < 0) return;
-  }
+  const GradTile at = grad_tile(mt, nt);
+  const int64_t piece = at.piece;
+  const int m0 = at.m * kSide, n0 = at.n * kSide;
+  const GroupTile g = grad_rows(offsets, experts, slots, piece, chunk, part != nullptr);
+  if (g.group < 0) return;
   const int64_t lo = g.lo + g.tile * chunk;
   const int rows = (int)min<int64_t>(chunk, g.hi - lo);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
@@ -205,6 +290,59 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_weight_grad(const T* __
   }
 }
 
+// The same for 16-bit rows in whole 16-byte pieces, straight from memory to LDS;
+// db from products with ones.
+template <class T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void k_group_weight_grad_fast(
+    const T* __restrict__ dy, int64_t dys, const T* __restrict__ x, int64_t xs, const int32_t* __restrict__ offsets,
+    T* __restrict__ dw, T* __restrict__ db, float* __restrict__ part, int64_t slots, int experts, int cols, int outs,
+    int64_t chunk, int mt, int nt) {
+  using Tile = FastTile<T, false, false, BM, BN, WM, WN, true>;
+  static_assert(Tile::TM <= WN, "a wave of the row for each tile of rows");
+  __shared__ __attribute__((aligned(16))) uint16_t s0[Tile::kStage], s1[Tile::kStage];
+  const GradTile at = grad_tile(mt, nt);
+  const int64_t piece = at.piece;
+  const int m0 = at.m * BM, n0 = at.n * BN;
+  const GroupTile g = grad_rows(offsets, experts, slots, piece, chunk, part != nullptr);
+  if (g.group < 0) return;
+  const int64_t lo = g.lo + g.tile * chunk;
+  const int rows = (int)min<int64_t>(chunk, g.hi - lo);
+  const typename Tile::A pa(Panel<T>{dy + lo * dys + m0, dys, rows, min(BM, outs - m0)});
+  const typename Tile::B pb(Panel<T>{x + lo * xs + n0, xs, rows, min(BN, cols - n0)});
+  Tile t;
+  t.run(pa, pb, rows, n0 == 0, s0, s1);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64), wn = wave % WN;
+  const int row0 = wave / WN * (BM / WM), col0 = wn * (BN / WN);
+  const int64_t nw = (int64_t)outs * cols;
+  float* const own = reinterpret_cast<float*>(s0) + 1024 * wave;
+  float* const mine = part != nullptr ? part + piece * (nw + outs) : nullptr;
+#pragma unroll
+  for (int i = 0; i < Tile::TM; ++i) {
+#pragma unroll
+    for (int j = 0; j < Tile::TN; ++j) {
+      auto put = [&](auto type, auto* to) {
+        using O = decltype(type);
+        rows_of_tile<O>(t.acc[i][j], own, [&](int r, int c, float (&v)[Piece<O>::V]) {
+          const int row = m0 + row0 + 32 * i + r, col = n0 + col0 + 32 * j + c;
+          if (row >= outs || col >= cols) return;
+          Piece<O> o;
+          o.raw = typename Piece<O>::Raw{};
+#pragma unroll
+          for (int e = 0; e < Piece<O>::V; ++e) o.set(e, from_f32<O>(v[e]));
+          o.store(to + (int64_t)row * cols, col, cols);
+        });
+      };
+      if (mine != nullptr) put(float{}, mine);
+      else if (dw != nullptr) put(T{}, dw + g.group * nw);
+    }
+  }
+  // every column of `ones` holds the same sums: lane l has row l % 32
+  const int row = m0 + row0 + 32 * wn + (int)(threadIdx.x & 31);
+  if (n0 != 0 || wn >= Tile::TM || (threadIdx.x & 63) >= 32 || row >= outs) return;
+  if (mine != nullptr) mine[nw + row] = t.ones[0];
+  else if (db != nullptr) db[(int64_t)g.group * outs + row] = from_f32<T>(t.ones[0]);
+}
+
 // dW and db of expert blockIdx.y: its chunks' sums in the chunks' order.
 template <class T>
 __global__ __launch_bounds__(256) void k_group_chunk_sum(const float* __restrict__ part,
@@ -250,16 +388,17 @@ int64_t most_tiles(int64_t slots, int64_t groups, int64_t size) {
 // rows at least and of kMaxGroupChunk at most.
 constexpr int64_t kMaxGroupChunk = 8192;
 struct GradPlan {
-  int mt, nt;
+  int side, mt, nt;
   int64_t chunk, chunks;  // chunks 0: a workgroup takes all of an expert's rows
 };
-GradPlan grad_plan(int64_t slots, int experts, int64_t cols, int64_t outs) {
+GradPlan grad_plan(int64_t slots, int experts, int64_t cols, int64_t outs, int side) {
   GradPlan p;
-  p.mt = (int)tiles_of(outs, kSide);
-  p.nt = (int)tiles_of(cols, kSide);
+  p.side = side;
+  p.mt = (int)tiles_of(outs, side);
+  p.nt = (int)tiles_of(cols, side);
   const int64_t tiles = (int64_t)p.mt * p.nt;
   const int64_t want = std::max<int64_t>(1, 512 / tiles);  // chunks in all
-  p.chunk = std::min(kMaxGroupChunk, std::max<int64_t>(256, tiles_of(tiles_of(slots, want), kStepK) * kStepK));
+  p.chunk = std::min(kMaxGroupChunk, std::max<int64_t>(256, tiles_of(tiles_of(slots, want), 64) * 64));
   p.chunks = most_tiles(slots, experts, p.chunk);
   if (slots <= p.chunk || (tiles * experts >= 512 && slots <= 2 * kMaxGroupChunk)) {
     p.chunk = std::max<int64_t>(slots, 1);
@@ -268,12 +407,25 @@ GradPlan grad_plan(int64_t slots, int experts, int64_t cols, int64_t outs) {
   return p;
 }
 
+// 16-bit rows of whole 16-byte pieces at multiples of 16 bytes, a panel's within 32 bits of its first.
+bool whole_pieces(const void* p, int64_t stride) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0 && stride <= (1 << 22);
+}
+
+// The tile of a product over rows: 256 where there are enough of them, else 128.
+int rows_side(int64_t slots, int experts, int64_t outs) {
+  return outs > 128 && slots / 256 * tiles_of(outs, 256) >= 192 ? 256 : 128;
+}
+int grad_side(int64_t slots, int experts, int64_t cols, int64_t outs) {
+  return outs > 128 && cols > 128 && tiles_of(outs, 256) * tiles_of(cols, 256) * experts >= 192 ? 256 : 128;
+}
+
 }  // namespace
 
 bool group_linear_fits(int64_t slots, int experts, int64_t cols, int64_t outs) {
   const int64_t mt = most_tiles(slots, experts + 1, kSide);
-  const GradPlan p = grad_plan(slots, experts, cols, outs);
-  const int64_t limit = (int64_t(1) << 32) / kGroupThreads;  // threads a launch
+  const GradPlan p = grad_plan(slots, experts, cols, outs, kSide);
+  const int64_t limit = (int64_t(1) << 32) / kGroupThreads - 8;  // threads a launch
   return mt * tiles_of(outs, kSide) < limit && mt * tiles_of(cols, kSide) < limit &&
          (int64_t)p.mt * p.nt * std::max<int64_t>(p.chunks, experts) < limit &&
          tiles_of(cols * outs + outs, 256) * experts < limit;
@@ -285,12 +437,25 @@ void run_group_linear(const void* x, int type, int64_t xs, const void* w, const 
   if (slots == 0) return;
   with_type(type, [&](auto t) {
     using T = decltype(t);
-    const int64_t mt = most_tiles(slots, experts + 1, kSide), nt = tiles_of(outs, kSide);
+    auto grid = [&](int side) {  // whole turns of the eight XCDs
+      return dim3((uint32_t)(tiles_of(most_tiles(slots, experts + 1, side) * tiles_of(outs, side), 8) * 8));
+    };
     auto launch = [&](auto bk) {
-      hipLaunchKernelGGL((k_group_rows<T, decltype(bk)::value>), dim3((uint32_t)(mt * nt)), dim3(kGroupThreads), 0, st,
-                         static_cast<const T*>(x), xs, static_cast<const T*>(w), static_cast<const T*>(b),
-                         static_cast<const T*>(mask), offsets, static_cast<T*>(y), slots, experts, (int)cols,
-                         (int)outs, relu, mt, (int)nt);
+      constexpr bool BACK = decltype(bk)::value;
+      const auto args = [&](auto kernel, int side, int threads) {
+        hipLaunchKernelGGL(kernel, grid(side), dim3(threads), 0, st, static_cast<const T*>(x), xs,
+                           static_cast<const T*>(w), static_cast<const T*>(b), static_cast<const T*>(mask), offsets,
+                           static_cast<T*>(y), slots, experts, (int)cols, (int)outs, relu, (int)tiles_of(outs, side));
+      };
+      if constexpr (!std::is_same_v<T, float>) {
+        if (whole_pieces(x, xs) && whole_pieces(w, BACK ? outs : cols) && cols % 8 == 0 &&
+            (!BACK || outs % 8 == 0)) {
+          if (rows_side(slots, experts, outs) == 256) args(k_group_rows_fast<T, BACK, 256, 256, 2, 4>, 256, 512);
+          else args(k_group_rows_fast<T, BACK, 128, 128, 2, 2>, 128, 256);
+          return;
+        }
+      }
+      args(k_group_rows<T, BACK>, kSide, kGroupThreads);
     };
     if (back) launch(std::true_type{});
     else launch(std::false_type{});
@@ -298,22 +463,34 @@ void run_group_linear(const void* x, int type, int64_t xs, const void* w, const 
   SPHOPS_LAUNCHED();
 }
 
+// The workspace holds the chunks of either kernel.
 int64_t group_weight_grad_floats(int64_t slots, int experts, int64_t cols, int64_t outs) {
-  return grad_plan(slots, experts, cols, outs).chunks * (cols * outs + outs);
+  return std::max(grad_plan(slots, experts, cols, outs, 128).chunks, grad_plan(slots, experts, cols, outs, 256).chunks) *
+         (cols * outs + outs);
 }
 
 void run_group_weight_grad(const void* dy, int64_t dys, const void* x, int type, int64_t xs, const int32_t* offsets,
                            void* dw, void* db, int64_t slots, int experts, int64_t cols, int64_t outs, float* work,
                            hipStream_t st) {
-  const GradPlan p = grad_plan(slots, experts, cols, outs);
   const int64_t nw = cols * outs;
   with_type(type, [&](auto t) {
     using T = decltype(t);
+    const bool fast = !std::is_same_v<T, float> && whole_pieces(dy, dys) && whole_pieces(x, xs) && cols % 8 == 0 &&
+                      outs % 8 == 0;
+    const GradPlan p = grad_plan(slots, experts, cols, outs, fast ? grad_side(slots, experts, cols, outs) : kSide);
     const int64_t blocks = (p.chunks > 0 ? p.chunks : experts) * p.mt * p.nt;
-    hipLaunchKernelGGL((k_group_weight_grad<T>), dim3((uint32_t)blocks), dim3(kGroupThreads), 0, st,
-                       static_cast<const T*>(dy), dys, static_cast<const T*>(x), xs, offsets, static_cast<T*>(dw),
-                       static_cast<T*>(db), p.chunks > 0 ? work : nullptr, slots, experts, (int)cols, (int)outs,
-                       p.chunk, p.mt, p.nt);
+    const auto launch = [&](auto kernel, int threads) {
+      hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(threads), 0, st, static_cast<const T*>(dy), dys,
+                         static_cast<const T*>(x), xs, offsets, static_cast<T*>(dw), static_cast<T*>(db),
+                         p.chunks > 0 ? work : nullptr, slots, experts, (int)cols, (int)outs, p.chunk, p.mt, p.nt);
+    };
+    if constexpr (!std::is_same_v<T, float>) {
+      if (!fast) launch(k_group_weight_grad<T>, kGroupThreads);
+      else if (p.side == 256) launch(k_group_weight_grad_fast<T, 256, 256, 2, 4>, 512);
+      else launch(k_group_weight_grad_fast<T, 128, 128, 2, 2>, 256);
+    } else {
+      launch(k_group_weight_grad<T>, kGroupThreads);
+    }
     SPHOPS_LAUNCHED();
     if (p.chunks > 0)
       hipLaunchKernelGGL((k_group_chunk_sum<T>), dim3((uint32_t)tiles_of(nw + outs, 256), (uint32_t)experts), dim3(256),

@@ -57,6 +57,24 @@ __device__ __forceinline__ GroupTile group_tile(const int32_t* __restrict__ offs
   return g;
 }
 
+// The tiles of all groups.
+__device__ __forceinline__ int64_t group_tiles(const int32_t* __restrict__ offsets, int experts, int64_t slots,
+                                               int64_t size, bool behind) {
+  const int lane = threadIdx.x & 63, groups = experts + (behind ? 1 : 0);
+  int64_t all = 0;
+  for (int base = 0; base < groups; base += 64) {
+    const int e = base + lane;
+    if (e < groups) {
+      const int64_t lo = e == 0 ? 0 : min<int64_t>(max(offsets[e], 0), slots);
+      const int64_t hi = e == experts ? slots : max<int64_t>(lo, min<int64_t>(offsets[e + 1], slots));
+      all += (hi - lo + size - 1) / size;
+    }
+  }
+#pragma unroll
+  for (int s = 1; s < 64; s *= 2) all += __shfl_xor(all, s);
+  return all;
+}
+
 // The products' 16-bit type and the pieces a value of T is split into.
 template <class T>
 struct Pieces {
@@ -275,6 +293,168 @@ __device__ __forceinline__ void rows_of_tile(const f32x16& v, float* __restrict_
     f(row, V * at, o);
   }
 }
+
+// ---- 16-bit operands straight from memory to LDS
+
+constexpr int kFastK = 64;  // of the sum a step
+
+// 64 lanes' 16 bytes from memory to LDS, lane l's to lds + 16 l, past the
+// registers; done once the wave's vector memory count says so.
+__device__ __forceinline__ void load_to_lds(const void* src, void* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+__device__ const uint4 kZeros16 = {0, 0, 0, 0};
+
+// A panel of SIDE outputs by kFastK of the sum, 128 SIDE bytes of LDS, loaded by
+// WAVES waves.  KMAJOR: rows of 128 bytes whose eight 16-byte pieces are
+// exchanged by the row's low bits (piece p stands at p ^ (row % 8)), read as
+// they are.  Else 64 rows of 2 SIDE bytes, read down their columns; the 64-byte
+// quarters are exchanged by the row's low two bits, so that the four rows of a
+// column read lie in different banks.
+// Rows are whole 16-byte pieces at multiples of 16 bytes.
+template <class T, bool KMAJOR, int SIDE, int WAVES>
+struct FastPanel {
+  static constexpr int kLoads = SIDE / 8 / WAVES;
+  static_assert(kLoads * 8 * WAVES == SIDE && SIDE >= 128, "whole loads, four quarters a row");
+  const T* base;
+  int64_t step;              // elements from one step to the next
+  uint32_t at[kLoads];       // of the lane's pieces, from base
+  int k[kLoads];             // where they stand in the sum's step
+
+  // rows x cols values (as in Panel) from p on
+  __device__ __forceinline__ FastPanel(const Panel<T>& p) : base(p.base) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+    step = KMAJOR ? kFastK : kFastK * p.stride;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      if constexpr (KMAJOR) {
+        const int row = min((i * WAVES + wave) * 8 + (lane >> 3), p.rows - 1);  // rows past the end: nobody stores them
+        k[i] = 8 * ((lane & 7) ^ (lane >> 3));
+        at[i] = (uint32_t)row * (uint32_t)p.stride + (uint32_t)k[i];
+      } else {
+        const int byte = (i * WAVES + wave) * 1024 + 16 * lane, row = byte / (2 * SIDE);
+        const int piece = byte % (2 * SIDE) / 16 ^ (row & 3) << 2;
+        k[i] = row;
+        at[i] = (uint32_t)row * (uint32_t)p.stride + (uint32_t)min(8 * piece, p.cols - 8);
+      }
+    }
+  }
+  // The step from k0 on into `lds`; `left`: what is left of the sum (zeros past it).
+  __device__ __forceinline__ void load(int64_t n, int left, uint16_t* lds) const {
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+    const T* __restrict__ from = base + n * step;
+    if (left >= kFastK) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) load_to_lds(from + at[i], lds + (i * WAVES + wave) * 512);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        load_to_lds(k[i] < left ? (const void*)(from + at[i]) : (const void*)&kZeros16, lds + (i * WAVES + wave) * 512);
+    }
+  }
+  // What a lane adds for the operand of 32 outputs from `first` on.
+  __device__ __forceinline__ static int place(int first) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    if constexpr (KMAJOR) {
+      return (first + (lane & 31)) * kFastK;
+    } else {
+      const int i = lane & 15, row = 8 * h + (i >> 2), col = first + 16 * (lane >> 4 & 1) + 4 * (i & 3);
+      return row * SIDE + 8 * (col / 8 ^ (row & 3) << 2) + col % 8;
+    }
+  }
+  // Steps 16 s .. + 15 of the sum: lane l's k = 16 s + 8 (l / 32) + 0 .. 7.
+  __device__ __forceinline__ static s16x8 read(const uint16_t* lds, int place, int s) {
+    if constexpr (KMAJOR) {
+      const int lane = threadIdx.x & 63;
+      return *reinterpret_cast<const s16x8*>(lds + place + 8 * ((2 * s + (lane >> 5)) ^ (lane & 7)));
+    } else {
+      return join(read_column(lds + place + 16 * s * SIDE), read_column(lds + place + (16 * s + 4) * SIDE));
+    }
+  }
+};
+
+// Sums of a tile of BM x BN outputs over `len` of the sum, in WM x WN waves of
+// BM / WM by BN / WN each.  Two stages of LDS: a step's panels are
+// loaded under the products of the one before.
+template <class T, bool KA, bool KB, int BM, int BN, int WM, int WN, bool ONES>
+struct FastTile {
+  static constexpr int kWaves = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+  static constexpr int kStage = (BM + BN) * kFastK;  // 16-bit words
+  using A = FastPanel<T, KA, BM, kWaves>;
+  using B = FastPanel<T, KB, BN, kWaves>;
+  f32x16 acc[TM][TN];
+  f32x16 ones;  // ONES: of A's rows alone, in wave wn of a row of waves those of its tile wn
+
+  __device__ __forceinline__ void run(const A& a, const B& b, int len, bool count, uint16_t* s0, uint16_t* s1) {
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64), wn = wave % WN;
+    int pa[TM], pb[TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      pa[i] = A::place(wave / WN * (BM / WM) + 32 * i);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = f32x16{};
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) pb[j] = B::place(wn * (BN / WN) + 32 * j);
+    ones = f32x16{};
+    s16x8 one;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) one[j] = std::is_same_v<T, __half> ? 0x3c00 : 0x3f80;
+    auto load = [&](int n, uint16_t* lds) {
+      // past the last step: the last one again, which nothing reads
+      const int at = min(n, (len - 1) / kFastK);
+      a.load(at, len - at * kFastK, lds);
+      b.load(at, len - at * kFastK, lds + BM * kFastK);
+      __builtin_amdgcn_sched_barrier(0);  // the loads go out before the products, not after them
+    };
+    auto compute = [&](const uint16_t* lds) {
+#pragma unroll
+      for (int s = 0; s < kFastK / 16; ++s) {
+        s16x8 x[TM], y[TN];
+#pragma unroll
+        for (int i = 0; i < TM; ++i) x[i] = A::read(lds, pa[i], s);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) y[j] = B::read(lds + BM * kFastK, pb[j], s);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] = mma16<T>(y[j], x[i], acc[i][j]);
+        }
+        if constexpr (ONES) {
+          if (count) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+              if (wn == i) ones = mma16<T>(one, x[i], ones);
+          }
+        }
+      }
+    };
+    if (len <= 0) return;
+    const int steps = (len + kFastK - 1) / kFastK;
+    load(0, s0);
+    // every wave's loads of a step have landed, and every wave has read the step
+    // before, whose place the next load takes
+#define SPHOPS_TURN()                    \
+  asm volatile("" ::: "memory");         \
+  __builtin_amdgcn_s_waitcnt(0x0070);    \
+  __builtin_amdgcn_s_barrier();          \
+  asm volatile("" ::: "memory")
+    int n = 0;
+    for (; n + 1 < steps; n += 2) {
+      SPHOPS_TURN();
+      load(n + 1, s1);
+      compute(s0);
+      SPHOPS_TURN();
+      load(n + 2, s0);
+      compute(s1);
+    }
+    SPHOPS_TURN();  // no load in flight where LDS is used again
+#undef SPHOPS_TURN
+    if (n < steps) compute(s0);
+    __syncthreads();
+  }
+};
 
 }  // namespace
 

@@ -294,6 +294,14 @@ def test_linear_of_wide_layers(dtype):
     _check_linear([500, 600], 100, 256, 1536, dtype, bias=False)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_linear_of_large_tiles(dtype):
+    """Enough tiles of 256 over the rows, and over the weights."""
+    _check_linear([20000, 0, 29000, 257, 1], 300, 72, 264, dtype)
+    _check_linear([20001, 255, 256, 30000], 0, 264, 392, dtype, bias=False)
+    _check_linear([300, 0, 64, 65, 1, 63, 500, 31, 32, 33, 7, 128], 3, 1032, 1000, dtype)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_linear_of_many_rows(dtype):
     _check_linear([20000, 3, 0, 9000, 40001], 77, 83, 35, dtype)
