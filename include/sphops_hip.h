@@ -683,6 +683,31 @@ int sphops_expert_linear_weight_grad(const void* dy, int64_t dy_stride, const vo
                                      int in_features, int out_features, void* workspace, void* stream);
 int64_t sphops_expert_linear_workspace_bytes(int64_t slots, int experts, int in_features, int out_features);
 
+/*
+ * sphops_mlp_forward's MLP (hidden = 128, in_features in [4, 168], out_features
+ * in [4, 64]) of each expert over sorted float32 rows, in one kernel each way (no
+ * reference counterpart): z (slots x in_features, dense), w1 (experts, hidden,
+ * in_features), b1 (experts, hidden; or NULL), w2 (experts, out_features,
+ * hidden), b2 (experts, out_features; or NULL), offsets as in
+ * sphops_expert_linear.  y is zero behind the last expert's rows.  mask (4 words a
+ * row, 8-byte aligned, or NULL) keeps where the hidden values are above 0 for the
+ * input gradient, which writes dz (zero behind the last expert's rows).  The
+ * weight gradients (each may be NULL) compute the hidden values again and are
+ * summed in a fixed order.  workspace: sphops_expert_mlp_workspace_bytes bytes
+ * (-1: not supported), 4-byte aligned.
+ */
+int sphops_expert_mlp_forward(const float* z, const float* w1, const float* b1, const float* w2, const float* b2,
+                              const int32_t* offsets, float* y, uint32_t* mask, int64_t slots, int experts,
+                              int in_features, int hidden, int out_features, void* stream);
+int sphops_expert_mlp_input_grad(const float* dy, const float* w1, const float* w2, const uint32_t* mask,
+                                 const int32_t* offsets, float* dz, int64_t slots, int experts, int in_features,
+                                 int hidden, int out_features, void* stream);
+int sphops_expert_mlp_weight_grad(const float* z, const float* dy, const float* w1, const float* b1, const float* w2,
+                                  const int32_t* offsets, float* dw1, float* db1, float* dw2, float* db2,
+                                  int64_t slots, int experts, int in_features, int hidden, int out_features,
+                                  void* workspace, void* stream);
+int64_t sphops_expert_mlp_workspace_bytes(int64_t slots, int experts, int in_features, int hidden, int out_features);
+
 /* sphops_neighbor_candidates, _fill and _schedule in one call and two
  * launches fewer (no reference counterpart): counts (8-byte aligned) receives
  * the pair total and the pairs not stored (two 64-bit words) and the wave

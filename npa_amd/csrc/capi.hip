@@ -1644,4 +1644,46 @@ int sphops_expert_linear_weight_grad(const void* dy, int64_t dy_stride, const vo
   });
 }
 
+int sphops_expert_mlp_forward(const float* z, const float* w1, const float* b1, const float* w2, const float* b2,
+                              const int32_t* offsets, float* y, uint32_t* mask, int64_t slots, int experts,
+                              int in_features, int hidden, int out_features, void* stream) {
+  return guarded([&] {
+    require(sphops::expert_mlp_fits(slots, experts, in_features, hidden, out_features), "MLP shape not supported");
+    require(slots == 0 || (z && w1 && w2 && offsets && y), "null buffer");
+    require(reinterpret_cast<uintptr_t>(mask) % 8 == 0, "mask must be 8-byte aligned");
+    sphops::run_expert_mlp_forward(z, w1, b1, w2, b2, offsets, y, mask, slots, experts, in_features, out_features,
+                                   sphops::as_stream(stream));
+  });
+}
+
+int sphops_expert_mlp_input_grad(const float* dy, const float* w1, const float* w2, const uint32_t* mask,
+                                 const int32_t* offsets, float* dz, int64_t slots, int experts, int in_features,
+                                 int hidden, int out_features, void* stream) {
+  return guarded([&] {
+    require(sphops::expert_mlp_fits(slots, experts, in_features, hidden, out_features), "MLP shape not supported");
+    require(slots == 0 || (dy && w1 && w2 && mask && offsets && dz), "null buffer");
+    require(reinterpret_cast<uintptr_t>(mask) % 8 == 0, "mask must be 8-byte aligned");
+    sphops::run_expert_mlp_input_grad(dy, w1, w2, mask, offsets, dz, slots, experts, in_features, out_features,
+                                      sphops::as_stream(stream));
+  });
+}
+
+int64_t sphops_expert_mlp_workspace_bytes(int64_t slots, int experts, int in_features, int hidden, int out_features) {
+  if (!sphops::expert_mlp_fits(slots, experts, in_features, hidden, out_features)) return -1;
+  return sphops::expert_mlp_floats(slots, experts, in_features, out_features) * (int64_t)sizeof(float);
+}
+
+int sphops_expert_mlp_weight_grad(const float* z, const float* dy, const float* w1, const float* b1, const float* w2,
+                                  const int32_t* offsets, float* dw1, float* db1, float* dw2, float* db2,
+                                  int64_t slots, int experts, int in_features, int hidden, int out_features,
+                                  void* workspace, void* stream) {
+  return guarded([&] {
+    require(sphops::expert_mlp_fits(slots, experts, in_features, hidden, out_features), "MLP shape not supported");
+    require(offsets && (slots == 0 || (z && dy && w1 && w2 && workspace)), "null buffer");
+    require(reinterpret_cast<uintptr_t>(workspace) % 4 == 0, "workspace must be 4-byte aligned");
+    sphops::run_expert_mlp_weight_grad(z, dy, w1, b1, w2, offsets, dw1, db1, dw2, db2, slots, experts, in_features,
+                                       out_features, static_cast<float*>(workspace), sphops::as_stream(stream));
+  });
+}
+
 }  // extern "C"

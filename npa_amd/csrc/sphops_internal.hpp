@@ -433,6 +433,18 @@ int64_t group_weight_grad_floats(int64_t slots, int experts, int64_t cols, int64
 void run_group_weight_grad(const void* dy, int64_t dys, const void* x, int type, int64_t xs, const int32_t* offsets,
                            void* dw, void* db, int64_t slots, int experts, int64_t cols, int64_t outs, float* work,
                            hipStream_t st);
+// expert_mlp.hip: Linear, ReLU, Linear of experts over sorted float32 rows, 128 hidden units
+bool expert_mlp_fits(int64_t slots, int experts, int nin, int hidden, int nout);
+void run_expert_mlp_forward(const float* z, const float* w1, const float* b1, const float* w2, const float* b2,
+                            const int32_t* offsets, float* y, uint32_t* mask, int64_t slots, int experts, int nin,
+                            int nout, hipStream_t st);
+void run_expert_mlp_input_grad(const float* dy, const float* w1, const float* w2, const uint32_t* mask,
+                               const int32_t* offsets, float* dz, int64_t slots, int experts, int nin, int nout,
+                               hipStream_t st);
+int64_t expert_mlp_floats(int64_t slots, int experts, int nin, int nout);
+void run_expert_mlp_weight_grad(const float* z, const float* dy, const float* w1, const float* b1, const float* w2,
+                                const int32_t* offsets, float* dw1, float* db1, float* dw2, float* db2, int64_t slots,
+                                int experts, int nin, int nout, float* work, hipStream_t st);
 
 constexpr uint32_t kMaxChannels = 64;
 constexpr int kRadixBins = 1024;  // digit values per radix-sort pass (10 bits)

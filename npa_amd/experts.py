@@ -229,6 +229,50 @@ class _Mlp(torch.autograd.Function):
         return (*_rows.first_order("the experts' MLP", dx, dw1, db1, dw2, db2), None)
 
 
+def _fused_forward(x, w1, b1, w2, b2, offsets, keep):
+    """y, and what the input gradient reads of the hidden values (a bit of each)."""
+    (experts, hidden, cols), outs, slots = w1.shape, w2.shape[1], x.shape[0]
+    y = torch.empty(slots, outs, device=x.device)
+    mask = torch.empty(slots, 4, dtype=torch.int32, device=x.device) if keep else None
+    _rows.call(_lib.sphops_expert_mlp_forward, x.device, x.data_ptr(), w1.data_ptr(), address(b1), w2.data_ptr(),
+               address(b2), offsets.data_ptr(), y.data_ptr(), address(mask), slots, experts, cols, hidden, outs)
+    return y, mask
+
+
+class _FusedMlp(torch.autograd.Function):
+    """``_Mlp`` of 128 hidden units in float32: x and a bit of each hidden value are kept."""
+
+    @staticmethod
+    def forward(ctx, x, w1, b1, w2, b2, offsets):
+        x = x if x.is_contiguous() else x.contiguous()
+        y, mask = _fused_forward(x, w1, b1, w2, b2, offsets, ctx.needs_input_grad[0])
+        ctx.save_for_backward(x, mask, w1, b1, w2, offsets)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, mask, w1, b1, w2, offsets = ctx.saved_tensors
+        need_x, need_w1, need_b1, need_w2, need_b2, _ = ctx.needs_input_grad
+        (experts, hidden, cols), outs, slots, dev = w1.shape, w2.shape[1], x.shape[0], x.device
+        dy = dy if dy.is_contiguous() else dy.contiguous()
+        dx = dw1 = db1 = dw2 = db2 = None
+        if need_x:
+            dx = torch.empty_like(x)
+            _rows.call(_lib.sphops_expert_mlp_input_grad, dev, dy.data_ptr(), w1.data_ptr(), w2.data_ptr(),
+                       mask.data_ptr(), offsets.data_ptr(), dx.data_ptr(), slots, experts, cols, hidden, outs)
+        if need_w1 or need_b1 or need_w2 or need_b2:
+            dw1 = torch.empty_like(w1) if need_w1 else None
+            db1 = torch.empty(experts, hidden, device=dev) if need_b1 else None
+            dw2 = torch.empty_like(w2) if need_w2 else None
+            db2 = torch.empty(experts, outs, device=dev) if need_b2 else None
+            work = torch.empty(max(_lib.sphops_expert_mlp_workspace_bytes(slots, experts, cols, hidden, outs), 1),
+                               dtype=torch.uint8, device=dev)
+            _rows.call(_lib.sphops_expert_mlp_weight_grad, dev, x.data_ptr(), dy.data_ptr(), w1.data_ptr(), address(b1),
+                       w2.data_ptr(), offsets.data_ptr(), address(dw1), address(db1), address(dw2), address(db2), slots,
+                       experts, cols, hidden, outs, work.data_ptr())
+        return (*_rows.first_order("the experts' MLP", dx, dw1, db1, dw2, db2), None)
+
+
 def _check_layer(x, weight, bias, slots, experts, cols, what):
     if weight.dim() != 3 or not 1 <= weight.shape[1] <= MAX_FEATURES:
         raise RuntimeError(f"{what} must have shape (experts, out, in), got {tuple(weight.shape)}")
@@ -267,14 +311,22 @@ def linear(x, weight, bias, offsets):
 
 
 def mlp(x, w1, b1, w2, b2, offsets):
-    """``linear(relu(linear(x, w1, b1, offsets)), w2, b2, offsets)`` with the ReLU
-    in the first layer's kernel and its mask in the second one's input gradient.
-    The hidden values, and their gradient, are kept in x's type."""
+    """``linear(relu(linear(x, w1, b1, offsets)), w2, b2, offsets)``.  float32 rows
+    of 4 to 168 values with 128 hidden units and 4 to 64 outputs, the shapes of an
+    automaton's update rule, take one kernel each way, which keeps the hidden
+    values in registers.  Elsewhere the ReLU is in the first layer's kernel and its
+    mask in the second one's input gradient, and the hidden values, and their
+    gradient, are kept in x's type."""
     slots, experts, cols = _check_sorted(x, offsets)
     w1, b1 = _check_layer(x, w1, b1, slots, experts, cols, "w1")
-    w2, b2 = _check_layer(x, w2, b2, slots, experts, w1.shape[1], "w2")
+    hidden = w1.shape[1]
+    w2, b2 = _check_layer(x, w2, b2, slots, experts, hidden, "w2")
+    fused = (x.dtype == torch.float32
+             and _lib.sphops_expert_mlp_workspace_bytes(slots, experts, cols, hidden, w2.shape[1]) >= 0)
     if _rows.wants_grad(x, w1, b1, w2, b2):
-        return _Mlp.apply(x, w1, b1, w2, b2, offsets)
+        return (_FusedMlp if fused else _Mlp).apply(x, w1, b1, w2, b2, offsets)
+    if fused:
+        return _fused_forward(x if x.is_contiguous() else x.contiguous(), w1, b1, w2, b2, offsets, False)[0]
     return _linear(_linear(x, w1, b1, offsets, relu=True), w2, b2, offsets)
 
 

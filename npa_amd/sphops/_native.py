@@ -103,6 +103,11 @@ _SIGNATURES = {
     "sphops_expert_linear_input_grad": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _p], _i32),
     "sphops_expert_linear_weight_grad": ([_p, _i64, _p, _i32, _i64, _p, _p, _p, _i64, _i32, _i32, _i32, _p, _p], _i32),
     "sphops_expert_linear_workspace_bytes": ([_i64, _i32, _i32, _i32], _i64),
+    "sphops_expert_mlp_forward": ([_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p], _i32),
+    "sphops_expert_mlp_input_grad": ([_p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p], _i32),
+    "sphops_expert_mlp_weight_grad": ([_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p],
+                                      _i32),
+    "sphops_expert_mlp_workspace_bytes": ([_i64, _i32, _i32, _i32, _i32], _i64),
     "sphops_forward": ([_p, _i32, _p, _p], _i32),
     "sphops_backward": ([_p, _i32, _i32, _i32, _i32, _p, _p], _i32),
     "sphops_neighbor_candidates": ([_p, _p, _p, _i32, _p], _i32),

@@ -75,3 +75,14 @@ def test_entry_points_check_their_arguments():
     _fails(lib.sphops_expert_linear_weight_grad(p, 8, p, 0, 8, p, p, p, 4, 2, 8, 8, ctypes.c_void_p(4100), None),
            "16-byte")
     assert lib.sphops_expert_linear_workspace_bytes(4, 1025, 8, 8) == -1
+    _fails(lib.sphops_expert_mlp_forward(p, p, p, p, p, p, p, p, 4, 2, 8, 64, 8, None), "not supported")
+    _fails(lib.sphops_expert_mlp_forward(p, p, p, p, p, None, p, p, 4, 2, 8, 128, 8, None), "null")
+    _fails(lib.sphops_expert_mlp_forward(p, p, p, p, p, p, p, ctypes.c_void_p(4100), 4, 2, 8, 128, 8, None), "8-byte")
+    _fails(lib.sphops_expert_mlp_input_grad(p, p, p, None, p, p, 4, 2, 8, 128, 8, None), "null")
+    _fails(lib.sphops_expert_mlp_weight_grad(p, p, p, p, p, p, p, p, p, p, 4, 2, 8, 128, 8, None, None), "null")
+    assert lib.sphops_expert_mlp_workspace_bytes(4, 2, 8, 128, 65) == -1
+    # no part of the rows' sums is longer than 8192 rows
+    for rows in (1, 1 << 20, 1 << 27):
+        partial = 4 * (128 * 83 + 128 + 19 * 128 + 19)
+        size = lib.sphops_expert_mlp_workspace_bytes(rows, 3, 83, 128, 19)
+        assert size % partial == 0 and size // partial - 3 >= rows // 8192
