@@ -29,8 +29,7 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 // of their own where they count), are cut into `shares` equal ones, and those
 // again where one expert's end and the next one's begin.  Workgroup i < shares has
 // the first part of share i, workgroup shares + e the part that begins with group
-// e's first tile inside a share: the two together are no more than a share, so the
-// short ones that start last fill what the short ones that start first leave.
+// e's first tile inside a share.
 struct Part {
   int group;       // -1: none
   int64_t lo, hi;  // rows
@@ -568,39 +567,52 @@ __global__ __launch_bounds__(kGradThreads, grad_waves(KS, OS)) void k_expert_mlp
 }
 
 // The gradients of expert blockIdx.y: its parts' sums, in a fixed order: wave q
-// of the workgroup adds every 16th of them.  `shares`: as the parts
-// were cut.
+// of the workgroup adds every 16th of them, four neighbouring values a lane.
+// `shares`: as the parts were cut.
 constexpr int kSumWaves = 16;
 __global__ __launch_bounds__(64 * kSumWaves) void k_expert_mlp_sum(const float* __restrict__ part,
                                                                    const int32_t* __restrict__ offsets,
                                                                    float* __restrict__ dw1, float* __restrict__ db1,
                                                                    float* __restrict__ dw2, float* __restrict__ db2,
                                                                    int64_t slots, int experts, int n1, int n2, int nout,
-                                                                   int64_t shares) {
-  __shared__ float red[kSumWaves][64];
+                                                                   int shares) {
+  __shared__ f32x4 red[kSumWaves][64];
   const int lane = threadIdx.x & 63, q = threadIdx.x >> 6, e = (int)blockIdx.y, n = n1 + kHid + n2 + nout;
-  const int64_t tiles = group_tiles(offsets, experts, slots, kT, false);
-  const int64_t before = e > 0 ? group_tiles(offsets, e, slots, kT, false) : 0;
-  const int64_t mine = group_tiles(offsets, e + 1, slots, kT, false) - before;
-  float t = 0.0f;
-  const int at = (int)blockIdx.x * 64 + lane;
-  if (mine > 0 && at < n) {
+  const GroupSpan g = group_span(offsets, experts, slots, kT, e);
+  f32x4 t = f32x4{};
+  const int at = (int)blockIdx.x * 256 + 4 * lane;
+  if (g.tiles > 0 && at < n) {
     // the first share's part is the expert's own where it begins inside the share
-    const int64_t cut = min<int64_t>(shares, tiles);
-    const int64_t first = ((before + 1) * cut - 1) / tiles, last = ((before + mine) * cut - 1) / tiles;
-    const bool inside = before != tiles * first / cut;
+    const int64_t cut = min<int64_t>(shares, g.all);
+    const int first = (int)(((g.before + 1) * cut - 1) / g.all), last = (int)(((g.before + g.tiles) * cut - 1) / g.all);
+    const bool inside = g.before != g.all * first / cut;
+    auto add = [&](int i) {
+      const float* __restrict__ p = part + (int64_t)(i == first && inside ? shares + e : i) * n + at;
+      if (at + 4 <= n) {
+        Piece<float> v;
+        v.load(p, 0, 4);
+        t += f32x4{v.get(0), v.get(1), v.get(2), v.get(3)};
+      } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+          if (at + j < n) t[j] += p[j];
+      }
+    };
+    int i = first + q;
+    if (i <= last) add(i);
 #pragma unroll 4
-    for (int64_t i = first + q; i <= last; i += kSumWaves)
-      t += part[(i == first && inside ? shares + e : i) * n + at];
+    for (i += kSumWaves; i <= last; i += kSumWaves) add(i);
   }
   red[q][lane] = t;
   __syncthreads();
-  if (q != 0 || at >= n) return;
-  t = 0.0f;
+  // thread i: value i of the workgroup's 256
+  const int to = (int)blockIdx.x * 256 + (int)threadIdx.x;
+  if (threadIdx.x >= 256 || to >= n) return;
+  float v = 0.0f;
 #pragma unroll
-  for (int k = 0; k < kSumWaves; ++k) t += red[k][lane];
-  auto put = [&](float* to, int first, int count) {
-    if (to != nullptr && at >= first && at < first + count) to[(int64_t)e * count + at - first] = t;
+  for (int k = 0; k < kSumWaves; ++k) v += red[k][threadIdx.x / 4][threadIdx.x % 4];
+  auto put = [&](float* out, int first, int count) {
+    if (out != nullptr && to >= first && to < first + count) out[(int64_t)e * count + to - first] = v;
   };
   put(dw1, 0, n1);
   put(db1, n1, kHid);
@@ -610,16 +622,19 @@ __global__ __launch_bounds__(64 * kSumWaves) void k_expert_mlp_sum(const float* 
 
 int64_t most_row_tiles(int64_t slots, int64_t groups) { return slots / kT + std::min(groups, slots); }
 
-// Shares of the weight gradients' rows: what the card holds at once, no more than
-// row tiles, and enough that none sums more than kMaxChunkRows rows.
+// Shares of the rows where the card holds `room` workgroups at once: their parts
+// should all fit, or those that come last wait for one of the others on their own
+// XCD (2^20 rows of 83 -> 19, 8 experts: forward 347 us with 256 shares, 1 with
+// 248).  Many experts give up no more than half of the room for that.
+int64_t shares_of(int64_t room, int64_t parts) { return room - std::min(parts, room / 2); }
+int64_t row_shares(int64_t slots, int experts) {
+  return std::min(shares_of(256, experts + 1), most_row_tiles(slots, experts + 1));
+}
+// For the weight gradients also enough that none sums more than kMaxChunkRows rows.
 int64_t grad_shares(int64_t slots, int experts, int nin, int nout) {
   const int64_t most = most_row_tiles(slots, experts);
-  const int64_t want = 256 * grad_waves((nin + 15) / 16, (nout + 15) / 16);
+  const int64_t want = shares_of(256 * grad_waves((nin + 15) / 16, (nout + 15) / 16), experts);
   return std::min(most, std::max(want, (most * kT + kMaxChunkRows - 1) / kMaxChunkRows));
-}
-
-int64_t row_shares(int64_t slots, int experts) {
-  return std::min<int64_t>(256, most_row_tiles(slots, experts + 1));
 }
 constexpr int share_threads(bool two) { return two ? 512 : 256; }
 
@@ -679,8 +694,8 @@ void run_expert_mlp_weight_grad(const float* z, const float* dy, const float* w1
     SPHOPS_LAUNCHED();
   }
   const int n1 = kHid * nin, n2 = nout * kHid, n = n1 + kHid + n2 + nout;
-  hipLaunchKernelGGL(k_expert_mlp_sum, dim3((uint32_t)((n + 63) / 64), (uint32_t)experts), dim3(64 * kSumWaves), 0, st,
-                     work, offsets, dw1, db1, dw2, db2, slots, experts, n1, n2, nout, shares);
+  hipLaunchKernelGGL(k_expert_mlp_sum, dim3((uint32_t)((n + 255) / 256), (uint32_t)experts), dim3(64 * kSumWaves), 0, st,
+                     work, offsets, dw1, db1, dw2, db2, slots, experts, n1, n2, nout, (int)shares);
   SPHOPS_LAUNCHED();
 }
 

@@ -350,21 +350,8 @@ __global__ __launch_bounds__(256) void k_group_chunk_sum(const float* __restrict
                                                          T* __restrict__ db, int64_t slots, int experts, int64_t nw,
                                                          int outs, int64_t chunk, int64_t chunks) {
   const int e = (int)blockIdx.y;
-  // the expert's first chunk: every wave counts the chunks of those before it
-  int64_t before = 0, mine = 0;
-  for (int base = 0; base <= e; base += 64) {
-    const int i = base + (int)(threadIdx.x & 63);
-    int64_t c = 0;
-    if (i <= e) {
-      const int64_t lo = i == 0 ? 0 : min<int64_t>(max(offsets[i], 0), slots);
-      c = (max<int64_t>(lo, min<int64_t>(offsets[i + 1], slots)) - lo + chunk - 1) / chunk;
-    }
-    if (e >= base && e < base + 64) mine = __shfl(c, e - base);
-    if (i == e) c = 0;
-#pragma unroll
-    for (int s = 1; s < 64; s *= 2) c += __shfl_xor(c, s);
-    before += c;
-  }
+  const GroupSpan g = group_span(offsets, experts, slots, chunk, e);
+  const int64_t before = g.before, mine = g.tiles;
   const int64_t n = nw + outs, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= n) return;
   float t = 0.0f;

@@ -75,6 +75,34 @@ __device__ __forceinline__ int64_t group_tiles(const int32_t* __restrict__ offse
   return all;
 }
 
+// Group e's tiles, those of the groups before it and those of all experts.
+struct GroupSpan {
+  int64_t before, tiles, all;
+};
+__device__ __forceinline__ GroupSpan group_span(const int32_t* __restrict__ offsets, int experts, int64_t slots,
+                                                int64_t size, int e) {
+  const int lane = threadIdx.x & 63;
+  GroupSpan g{0, 0, 0};
+  for (int base = 0; base < experts; base += 64) {
+    const int i = base + lane;
+    int64_t mine = 0;
+    if (i < experts) {
+      const int64_t lo = i == 0 ? 0 : min<int64_t>(max(offsets[i], 0), slots);
+      mine = (max<int64_t>(lo, min<int64_t>(offsets[i + 1], slots)) - lo + size - 1) / size;
+    }
+    int64_t before = i < e ? mine : 0;
+    if (e >= base && e < base + 64) g.tiles = __shfl(mine, e - base);
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) {
+      mine += __shfl_xor(mine, s);
+      before += __shfl_xor(before, s);
+    }
+    g.before += before;
+    g.all += mine;
+  }
+  return g;
+}
+
 // The products' 16-bit type and the pieces a value of T is split into.
 template <class T>
 struct Pieces {
