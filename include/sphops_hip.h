@@ -664,8 +664,7 @@ int sphops_combine_rows_backward(const void* dy, int type, int64_t row_stride, c
  * offsets[e + 1] - 1 (device memory, from 0 on and not decreasing), zeros for the
  * rows behind the last expert's.  All of `type`; w (experts, out_features,
  * in_features) and b (experts, out_features, or NULL) dense, x's rows
- * row_stride elements apart, y dense.  relu: y = max(y, 0).  Sums are float32;
- * float32 factors are taken whole (three bfloat16 pieces each).
+ * row_stride elements apart, y dense.  relu: y = max(y, 0).  Sums are float32.
  */
 int sphops_expert_linear(const void* x, int type, int64_t row_stride, const void* w, const void* b,
                          const int32_t* offsets, void* y, int64_t slots, int experts, int in_features,

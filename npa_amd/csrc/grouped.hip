@@ -3,9 +3,7 @@
 //   y[s] = x[s] W_e^T + b_e   dx[s] = dy[s] W_e   dW_e = sum of dy[s]^T x[s]   db_e = sum of dy[s]
 //
 // over the rows s of expert e, offsets[e] <= s < offsets[e + 1]; rows behind the
-// last expert's are zeros.  16-bit rows go to the matrix cores as they are,
-// float32 ones as three bfloat16 pieces of each factor and six products
-// (split16.hpp).  Sums are float32.
+// last expert's are zeros.  Sums are float32, and so are products of float32 rows.
 #include "grouped.hpp"
 
 namespace sphops {
@@ -80,9 +78,9 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_rows(const T* __restric
                                                               bool relu, int nt) {
   using IA = PanelImage<T, true>;
   using IB = PanelImage<T, !BACK>;
-  constexpr int P = Pieces<T>::P, V = Piece<T>::V;
-  __shared__ __attribute__((aligned(16))) uint16_t room[std::max(P * (IA::kPlane + IB::kPlane), kOutbox)];
-  uint16_t *const as = room, *const bs = room + P * IA::kPlane;
+  constexpr int V = Piece<T>::V;
+  __shared__ __attribute__((aligned(16))) uint16_t room[std::max(IA::kPlane + IB::kPlane, kOutbox)];
+  uint16_t *const as = room, *const bs = room + IA::kPlane;
   GroupTile g;
   int n;
   if (!rows_tile(offsets, experts, slots, kSide, nt, g, n)) return;
@@ -111,15 +109,13 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_rows(const T* __restric
       IB::load(pb, k + kStepK, rb);
     }
     sums.template step<IA, IB>(as, bs, row0, col0);
-    if ((k & (128 - kStepK)) == 128 - kStepK) sums.flush();
     __syncthreads();
   }
-  sums.flush();
   float* const own = reinterpret_cast<float*>(room) + 1024 * wave;  // every wave is done with the panels
   const T* const be = b != nullptr ? b + (int64_t)g.group * outs : nullptr;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    rows_of_tile<T>(sums.value(i), own, [&](int r, int c, float (&v)[V]) {
+    rows_of_tile<T>(sums.acc[i], own, [&](int r, int c, float (&v)[V]) {
       const int row = row0 + 32 * i + r, at = n0 + col0 + c;
       if (row >= here || at >= outs) return;
       finish<T>(v, be, mask != nullptr ? mask + (m0 + row) * outs : nullptr, relu, y + (m0 + row) * outs, at, outs);
@@ -172,6 +168,50 @@ __global__ __launch_bounds__(64 * WM * WN) void k_group_rows_fast(const T* __res
   }
 }
 
+// The same for float32 rows.  Three bfloat16 pieces of each factor and six products
+// take three eighths of the matrix cores' time, but putting them into pieces takes
+// vector work that does not overlap, and their sums registers: 8192 x 1024 -> 2048
+// in 337 us that way.
+template <bool BACK, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(kWideThreads) void k_group_rows_wide(const float* __restrict__ x, int64_t xs,
+                                                                  const float* __restrict__ w,
+                                                                  const float* __restrict__ b,
+                                                                  const float* __restrict__ mask,
+                                                                  const int32_t* __restrict__ offsets,
+                                                                  float* __restrict__ y, int64_t slots, int experts,
+                                                                  int cols, int outs, bool relu, int nt) {
+  using Tile = WideTile<true, !BACK, BM, BN, WM, WN>;
+  __shared__ __attribute__((aligned(16))) float room[Tile::kRoom];
+  GroupTile g;
+  int n;
+  if (!rows_tile(offsets, experts, slots, BM, nt, g, n)) return;
+  const int64_t m0 = g.lo + g.tile * BM;
+  const int n0 = n * BN, here = (int)min<int64_t>(BM, g.hi - m0), outs_here = min(BN, outs - n0);
+  if (g.group == experts) {
+    zero_rows(y, m0, here, n0, BN, outs);
+    return;
+  }
+  const float* const we = w + (int64_t)g.group * cols * outs;
+  Tile t;
+  t.run(Panel<float>{x + m0 * xs, xs, here, cols},
+        BACK ? Panel<float>{we + n0, outs, cols, outs_here} : Panel<float>{we + (int64_t)n0 * cols, cols, outs_here, cols},
+        cols, room, [](auto&) {});
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+  const int row0 = wave / WN * (BM / WM), col0 = wave % WN * (BN / WN);
+  const float* const be = b != nullptr ? b + (int64_t)g.group * outs : nullptr;
+#pragma unroll
+  for (int i = 0; i < Tile::TM; ++i) {
+#pragma unroll
+    for (int j = 0; j < Tile::TN; ++j) {
+      rows_of_tile<float>(t.acc[i][j], room + 1024 * wave, [&](int r, int c, float (&v)[4]) {
+        const int row = row0 + 32 * i + r, at = n0 + col0 + 32 * j + c;
+        if (row >= here || at >= outs) return;
+        finish<float>(v, be, mask != nullptr ? mask + (m0 + row) * outs : nullptr, relu, y + (m0 + row) * outs, at, outs);
+      });
+    }
+  }
+}
+
 // A weight gradient's workgroup: which piece (chunk of rows, or expert) and which
 // tile of dW.  A piece's tiles are dealt to the XCDs in contiguous shares, so that
 // each XCD works on every piece (experts differ in rows) and tiles that share
@@ -208,9 +248,9 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_weight_grad(const T* __
                                                                      int experts, int cols, int outs, int64_t chunk,
                                                                      int mt, int nt) {
   using I = PanelImage<T, false>;
-  constexpr int P = Pieces<T>::P, V = Piece<T>::V;
-  __shared__ __attribute__((aligned(16))) uint16_t room[std::max(P * 2 * I::kPlane, kOutbox)];
-  uint16_t *const as = room, *const bs = room + P * I::kPlane;
+  constexpr int V = Piece<T>::V;
+  __shared__ __attribute__((aligned(16))) uint16_t room[std::max(2 * I::kPlane, kOutbox)];
+  uint16_t *const as = room, *const bs = room + I::kPlane;
   const GradTile at = grad_tile(mt, nt);
   const int64_t piece = at.piece;
   const int m0 = at.m * kSide, n0 = at.n * kSide;
@@ -248,10 +288,8 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_weight_grad(const T* __
       I::load(pb, k + kStepK, rb);
     }
     sums.template step<I, I>(as, bs, row0, col0);
-    if ((k & (128 - kStepK)) == 128 - kStepK) sums.flush();
     __syncthreads();
   }
-  sums.flush();
   const int64_t nw = (int64_t)outs * cols;
   float* const own = reinterpret_cast<float*>(room) + 1024 * wave;  // every wave is done with the panels
   float* const mine = part != nullptr ? part + piece * (nw + outs) : nullptr;
@@ -259,7 +297,7 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_weight_grad(const T* __
   for (int i = 0; i < 2; ++i) {
     auto put = [&](auto type, auto* to) {
       using O = decltype(type);
-      rows_of_tile<O>(sums.value(i), own, [&](int r, int c, float (&v)[Piece<O>::V]) {
+      rows_of_tile<O>(sums.acc[i], own, [&](int r, int c, float (&v)[Piece<O>::V]) {
         const int row = m0 + row0 + 32 * i + r, col = n0 + col0 + c;
         if (row >= outs || col >= cols) return;
         Piece<O> o;
@@ -343,6 +381,60 @@ __global__ __launch_bounds__(64 * WM * WN) void k_group_weight_grad_fast(
   else if (db != nullptr) db[(int64_t)g.group * outs + row] = from_f32<T>(t.ones[0]);
 }
 
+// The same for float32 rows.
+template <int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(kWideThreads) void k_group_weight_grad_wide(
+    const float* __restrict__ dy, int64_t dys, const float* __restrict__ x, int64_t xs,
+    const int32_t* __restrict__ offsets, float* __restrict__ dw, float* __restrict__ db, float* __restrict__ part,
+    int64_t slots, int experts, int cols, int outs, int64_t chunk, int mt, int nt) {
+  using Tile = WideTile<false, false, BM, BN, WM, WN>;
+  __shared__ __attribute__((aligned(16))) float room[Tile::kRoom];
+  const GradTile at = grad_tile(mt, nt);
+  const int64_t piece = at.piece;
+  const int m0 = at.m * BM, n0 = at.n * BN;
+  const GroupTile g = grad_rows(offsets, experts, slots, piece, chunk, part != nullptr);
+  if (g.group < 0) return;
+  const int64_t lo = g.lo + g.tile * chunk;
+  const int rows = (int)min<int64_t>(chunk, g.hi - lo);
+  f32x4 bias = f32x4{};
+  Tile t;
+  t.run(Panel<float>{dy + lo * dys + m0, dys, rows, min(BM, outs - m0)},
+        Panel<float>{x + lo * xs + n0, xs, rows, min(BN, cols - n0)}, rows, room, [&](auto& pieces) {
+          if (n0 != 0) return;
+          for (auto& p : pieces) bias += f32x4{p.get(0), p.get(1), p.get(2), p.get(3)};
+        });
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+  const int row0 = wave / WN * (BM / WM), col0 = wave % WN * (BN / WN);
+  const int64_t nw = (int64_t)outs * cols;
+  float* const mine = part != nullptr ? part + piece * (nw + outs) : nullptr;
+  float* const to = mine != nullptr ? mine : dw != nullptr ? dw + g.group * nw : nullptr;
+#pragma unroll
+  for (int i = 0; i < Tile::TM; ++i) {
+#pragma unroll
+    for (int j = 0; j < Tile::TN; ++j) {
+      rows_of_tile<float>(t.acc[i][j], room + 1024 * wave, [&](int r, int c, float (&v)[4]) {
+        const int row = m0 + row0 + 32 * i + r, col = n0 + col0 + 32 * j + c;
+        if (to == nullptr || row >= outs || col >= cols) return;
+        Piece<float> o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o.set(e, v[e]);
+        o.store(to + (int64_t)row * cols, col, cols);
+      });
+    }
+  }
+  if (n0 != 0 || (mine == nullptr && db == nullptr)) return;
+  // a thread's columns again every kRowPieces threads
+  __syncthreads();
+  *reinterpret_cast<f32x4*>(room + 4 * threadIdx.x) = bias;
+  __syncthreads();
+  if ((int)threadIdx.x >= BM || m0 + (int)threadIdx.x >= outs) return;
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kWideThreads / Tile::A::kRowPieces; ++i) sum += room[i * BM + threadIdx.x];
+  if (mine != nullptr) mine[nw + m0 + threadIdx.x] = sum;
+  else db[(int64_t)g.group * outs + m0 + threadIdx.x] = sum;
+}
+
 // dW and db of expert blockIdx.y: its chunks' sums in the chunks' order.
 template <class T>
 __global__ __launch_bounds__(256) void k_group_chunk_sum(const float* __restrict__ part,
@@ -375,14 +467,15 @@ int64_t most_tiles(int64_t slots, int64_t groups, int64_t size) {
 // rows at least and of kMaxGroupChunk at most.
 constexpr int64_t kMaxGroupChunk = 8192;
 struct GradPlan {
-  int side, mt, nt;
+  int bm, bn, mt, nt;     // tiles of dW
   int64_t chunk, chunks;  // chunks 0: a workgroup takes all of an expert's rows
 };
-GradPlan grad_plan(int64_t slots, int experts, int64_t cols, int64_t outs, int side) {
+GradPlan grad_plan(int64_t slots, int experts, int64_t cols, int64_t outs, int bm, int bn) {
   GradPlan p;
-  p.side = side;
-  p.mt = (int)tiles_of(outs, side);
-  p.nt = (int)tiles_of(cols, side);
+  p.bm = bm;
+  p.bn = bn;
+  p.mt = (int)tiles_of(outs, bm);
+  p.nt = (int)tiles_of(cols, bn);
   const int64_t tiles = (int64_t)p.mt * p.nt;
   const int64_t want = std::max<int64_t>(1, 512 / tiles);  // chunks in all
   p.chunk = std::min(kMaxGroupChunk, std::max<int64_t>(256, tiles_of(tiles_of(slots, want), 64) * 64));
@@ -399,23 +492,41 @@ bool whole_pieces(const void* p, int64_t stride) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0 && stride <= (1 << 22);
 }
 
-// The tile of a product over rows: 256 where there are enough of them, else 128.
-int rows_side(int64_t slots, int experts, int64_t outs) {
+// 16-bit tiles: 256 where there are enough of them, else 128.
+int rows_side(int64_t slots, int64_t outs) {
   return outs > 128 && slots / 256 * tiles_of(outs, 256) >= 192 ? 256 : 128;
 }
-int grad_side(int64_t slots, int experts, int64_t cols, int64_t outs) {
+int grad_side(int experts, int64_t cols, int64_t outs) {
   return outs > 128 && cols > 128 && tiles_of(outs, 256) * tiles_of(cols, 256) * experts >= 192 ? 256 : 128;
+}
+// Float32 tiles: 32, 64 or 128 outputs, as few as hold them; 32 rows where an expert has no more on average.
+int wide_side(int64_t n) { return n <= 32 ? 32 : n <= 64 ? 64 : 128; }
+int wide_rows(int64_t slots, int experts) { return slots <= 32 * (int64_t)experts ? 32 : 128; }
+
+// The plan of a weight gradient for its type (wide: float32) and alignment (fast: whole pieces).
+GradPlan chosen_plan(int64_t slots, int experts, int64_t cols, int64_t outs, bool wide, bool fast) {
+  if (!wide) {
+    const int side = fast ? grad_side(experts, cols, outs) : kSide;
+    return grad_plan(slots, experts, cols, outs, side, side);
+  }
+  int bm = wide_side(outs), bn = wide_side(cols);
+  if (bm < 128 && bn < 128) bm = bn = 64;
+  return grad_plan(slots, experts, cols, outs, bm, bn);
 }
 
 }  // namespace
 
 bool group_linear_fits(int64_t slots, int experts, int64_t cols, int64_t outs) {
-  const int64_t mt = most_tiles(slots, experts + 1, kSide);
-  const GradPlan p = grad_plan(slots, experts, cols, outs, kSide);
   const int64_t limit = (int64_t(1) << 32) / kGroupThreads - 8;  // threads a launch
-  return mt * tiles_of(outs, kSide) < limit && mt * tiles_of(cols, kSide) < limit &&
-         (int64_t)p.mt * p.nt * std::max<int64_t>(p.chunks, experts) < limit &&
-         tiles_of(cols * outs + outs, 256) * experts < limit;
+  for (const int64_t n : {outs, cols}) {
+    if (most_tiles(slots, experts + 1, kSide) * tiles_of(n, 32) >= limit) return false;
+    if (slots <= 32 * (int64_t)experts && most_tiles(slots, experts + 1, 32) * tiles_of(n, kSide) >= limit) return false;
+  }
+  for (const bool wide : {false, true}) {
+    const GradPlan p = chosen_plan(slots, experts, cols, outs, wide, false);
+    if ((int64_t)p.mt * p.nt * std::max<int64_t>(p.chunks, experts) >= limit) return false;
+  }
+  return tiles_of(cols * outs + outs, 256) * experts < limit;
 }
 
 void run_group_linear(const void* x, int type, int64_t xs, const void* w, const void* b, const void* mask,
@@ -424,25 +535,27 @@ void run_group_linear(const void* x, int type, int64_t xs, const void* w, const 
   if (slots == 0) return;
   with_type(type, [&](auto t) {
     using T = decltype(t);
-    auto grid = [&](int side) {  // whole turns of the eight XCDs
-      return dim3((uint32_t)(tiles_of(most_tiles(slots, experts + 1, side) * tiles_of(outs, side), 8) * 8));
-    };
     auto launch = [&](auto bk) {
       constexpr bool BACK = decltype(bk)::value;
-      const auto args = [&](auto kernel, int side, int threads) {
-        hipLaunchKernelGGL(kernel, grid(side), dim3(threads), 0, st, static_cast<const T*>(x), xs,
-                           static_cast<const T*>(w), static_cast<const T*>(b), static_cast<const T*>(mask), offsets,
-                           static_cast<T*>(y), slots, experts, (int)cols, (int)outs, relu, (int)tiles_of(outs, side));
+      const auto with = [&](auto kernel, int bm, int bn, int threads) {
+        const int64_t tiles = most_tiles(slots, experts + 1, bm) * tiles_of(outs, bn);
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles_of(tiles, 8) * 8)) /* whole turns of the eight XCDs */,
+                           dim3(threads), 0, st, static_cast<const T*>(x), xs, static_cast<const T*>(w),
+                           static_cast<const T*>(b), static_cast<const T*>(mask), offsets, static_cast<T*>(y), slots,
+                           experts, (int)cols, (int)outs, relu, (int)tiles_of(outs, bn));
       };
-      if constexpr (!std::is_same_v<T, float>) {
-        if (whole_pieces(x, xs) && whole_pieces(w, BACK ? outs : cols) && cols % 8 == 0 &&
-            (!BACK || outs % 8 == 0)) {
-          if (rows_side(slots, experts, outs) == 256) args(k_group_rows_fast<T, BACK, 256, 256, 2, 4>, 256, 512);
-          else args(k_group_rows_fast<T, BACK, 128, 128, 2, 2>, 128, 256);
-          return;
-        }
+      if constexpr (std::is_same_v<T, float>) {
+        if (wide_rows(slots, experts) == 32) with(k_group_rows_wide<BACK, 32, 128, 1, 4>, 32, 128, kWideThreads);
+        else if (wide_side(outs) == 32) with(k_group_rows_wide<BACK, 128, 32, 4, 1>, 128, 32, kWideThreads);
+        else if (wide_side(outs) == 64) with(k_group_rows_wide<BACK, 128, 64, 4, 1>, 128, 64, kWideThreads);
+        else with(k_group_rows_wide<BACK, 128, 128, 2, 2>, 128, 128, kWideThreads);
+      } else if (whole_pieces(x, xs) && whole_pieces(w, BACK ? outs : cols) && cols % 8 == 0 &&
+                 (!BACK || outs % 8 == 0)) {
+        if (rows_side(slots, outs) == 256) with(k_group_rows_fast<T, BACK, 256, 256, 2, 4>, 256, 256, 512);
+        else with(k_group_rows_fast<T, BACK, 128, 128, 2, 2>, 128, 128, 256);
+      } else {
+        with(k_group_rows<T, BACK>, kSide, kSide, kGroupThreads);
       }
-      args(k_group_rows<T, BACK>, kSide, kGroupThreads);
     };
     if (back) launch(std::true_type{});
     else launch(std::false_type{});
@@ -450,10 +563,13 @@ void run_group_linear(const void* x, int type, int64_t xs, const void* w, const 
   SPHOPS_LAUNCHED();
 }
 
-// The workspace holds the chunks of either kernel.
+// The workspace holds the chunks of any of the kernels.
 int64_t group_weight_grad_floats(int64_t slots, int experts, int64_t cols, int64_t outs) {
-  return std::max(grad_plan(slots, experts, cols, outs, 128).chunks, grad_plan(slots, experts, cols, outs, 256).chunks) *
-         (cols * outs + outs);
+  int64_t chunks = 0;
+  for (const bool wide : {false, true}) {
+    for (const bool fast : {false, true}) chunks = std::max(chunks, chosen_plan(slots, experts, cols, outs, wide, fast).chunks);
+  }
+  return chunks * (cols * outs + outs);
 }
 
 void run_group_weight_grad(const void* dy, int64_t dys, const void* x, int type, int64_t xs, const int32_t* offsets,
@@ -462,21 +578,28 @@ void run_group_weight_grad(const void* dy, int64_t dys, const void* x, int type,
   const int64_t nw = cols * outs;
   with_type(type, [&](auto t) {
     using T = decltype(t);
-    const bool fast = !std::is_same_v<T, float> && whole_pieces(dy, dys) && whole_pieces(x, xs) && cols % 8 == 0 &&
-                      outs % 8 == 0;
-    const GradPlan p = grad_plan(slots, experts, cols, outs, fast ? grad_side(slots, experts, cols, outs) : kSide);
+    constexpr bool wide = std::is_same_v<T, float>;
+    const bool fast = !wide && whole_pieces(dy, dys) && whole_pieces(x, xs) && cols % 8 == 0 && outs % 8 == 0;
+    const GradPlan p = chosen_plan(slots, experts, cols, outs, wide, fast);
     const int64_t blocks = (p.chunks > 0 ? p.chunks : experts) * p.mt * p.nt;
-    const auto launch = [&](auto kernel, int threads) {
+    const auto with = [&](auto kernel, int threads) {
       hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(threads), 0, st, static_cast<const T*>(dy), dys,
                          static_cast<const T*>(x), xs, offsets, static_cast<T*>(dw), static_cast<T*>(db),
                          p.chunks > 0 ? work : nullptr, slots, experts, (int)cols, (int)outs, p.chunk, p.mt, p.nt);
     };
-    if constexpr (!std::is_same_v<T, float>) {
-      if (!fast) launch(k_group_weight_grad<T>, kGroupThreads);
-      else if (p.side == 256) launch(k_group_weight_grad_fast<T, 256, 256, 2, 4>, 512);
-      else launch(k_group_weight_grad_fast<T, 128, 128, 2, 2>, 256);
+    if constexpr (wide) {
+      if (p.bm == 128 && p.bn == 128) with(k_group_weight_grad_wide<128, 128, 2, 2>, kWideThreads);
+      else if (p.bm == 128 && p.bn == 64) with(k_group_weight_grad_wide<128, 64, 4, 1>, kWideThreads);
+      else if (p.bm == 64 && p.bn == 128) with(k_group_weight_grad_wide<64, 128, 1, 4>, kWideThreads);
+      else if (p.bm == 128) with(k_group_weight_grad_wide<128, 32, 4, 1>, kWideThreads);
+      else if (p.bn == 128) with(k_group_weight_grad_wide<32, 128, 1, 4>, kWideThreads);
+      else with(k_group_weight_grad_wide<64, 64, 2, 2>, kWideThreads);
+    } else if (!fast) {
+      with(k_group_weight_grad<T>, kGroupThreads);
+    } else if (p.bm == 256) {
+      with(k_group_weight_grad_fast<T, 256, 256, 2, 4>, 512);
     } else {
-      launch(k_group_weight_grad<T>, kGroupThreads);
+      with(k_group_weight_grad_fast<T, 128, 128, 2, 2>, 256);
     }
     SPHOPS_LAUNCHED();
     if (p.chunks > 0)

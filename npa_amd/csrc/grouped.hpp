@@ -103,16 +103,6 @@ __device__ __forceinline__ GroupSpan group_span(const int32_t* __restrict__ offs
   return g;
 }
 
-// The products' 16-bit type and the pieces a value of T is split into.
-template <class T>
-struct Pieces {
-  static constexpr int P = 1;
-};
-template <>
-struct Pieces<float> {
-  static constexpr int P = 3;
-};
-
 template <class T>
 __device__ __forceinline__ f32x16 mma16(s16x8 a, s16x8 b, f32x16 c) {
   if constexpr (std::is_same_v<T, __half>)
@@ -132,31 +122,6 @@ __device__ __forceinline__ f32x4 mma16(s16x8 a, s16x8 b, f32x4 c) {
                                                    0, 0);
 }
 
-// Four float32 values as the three bfloat16 pieces of each (see split3).
-__device__ __forceinline__ void split4(const Piece<float>& v, u32x2 (&out)[3]) {
-  constexpr float kTop = 0x1.fep127f;
-  float x[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) x[j] = v.get(j);
-#pragma unroll
-  for (int p = 0; p < 3; ++p) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float a = x[2 * j], b = x[2 * j + 1];
-      if (p == 0) {
-        float q = __builtin_amdgcn_fmed3f(a, -kTop, kTop), r = __builtin_amdgcn_fmed3f(b, -kTop, kTop);
-        out[p][j] = bf16_pair(q, r);
-        x[2 * j] = a - __builtin_bit_cast(float, out[p][j] << 16);
-        x[2 * j + 1] = b - __builtin_bit_cast(float, out[p][j] & 0xffff0000u);
-      } else {
-        out[p][j] = bf16_pair(a, b);
-        x[2 * j] = a;
-        x[2 * j + 1] = b;
-      }
-    }
-  }
-}
-
 // A panel of a product's operand: `rows` rows of `cols` values in memory.  KMAJOR: a
 // row holds the values along the summed dimension of one output row (or
 // column); else a row is one step of the sum and its values are the outputs'.
@@ -173,52 +138,52 @@ constexpr int kSide = 128;  // a tile's rows and columns
 constexpr int kGroupThreads = 512;
 constexpr int kOutbox = kGroupThreads / 64 * 2048;  // 16-bit words of LDS: 4 KB a wave for results on their way out
 
+// The pieces of a panel's step from `k` on that a thread of THREADS holds: piece
+// threadIdx.x % PIECES of rows threadIdx.x / PIECES and on.
+template <class T, bool KMAJOR, int PIECES, int LOADS, int THREADS, int STEP, int SIDE>
+__device__ __forceinline__ void load_panel(const Panel<T>& p, int64_t k, Piece<T> (&out)[LOADS]) {
+  const int col = (int)threadIdx.x % PIECES * Piece<T>::V, row = (int)threadIdx.x / PIECES;
+  const int at = KMAJOR ? (int)k + col : col;
+  const int64_t down = KMAJOR ? 0 : k;
+  const bool whole = (KMAJOR ? k + STEP : SIDE) <= p.cols;
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int64_t r = down + row + i * (THREADS / PIECES), kept = min(r, (int64_t)p.rows - 1);
+    if (whole) {
+      out[i].raw = *reinterpret_cast<const typename Piece<T>::Raw*>(p.base + kept * p.stride + at);
+      // a K-major panel's rows past the end give outputs that nobody stores
+      if (!KMAJOR && r >= p.rows) out[i].raw = typename Piece<T>::Raw{};
+    } else if (r < p.rows) {
+      out[i].load(p.base + r * p.stride, at, p.cols);
+    } else {
+      out[i].raw = typename Piece<T>::Raw{};
+    }
+  }
+}
+
+// 16-bit rows of any length at any place.
 template <class T, bool KMAJOR>
 struct PanelImage {
-  static constexpr int P = Pieces<T>::P, V = Piece<T>::V;
+  static constexpr int V = Piece<T>::V;
   static constexpr int kRowPieces = (KMAJOR ? kStepK : kSide) / V;
   static constexpr int kLoads = kSide * kStepK / V / kGroupThreads;
-  // 16-bit values of a plane: rows of 64 bytes whose 16-byte pieces are exchanged
-  // by the row's bits, or 32 rows of an odd number of 64 bytes (read down columns)
+  // 16-bit values: rows of 64 bytes whose 16-byte pieces are exchanged by the
+  // row's bits, or 32 rows of an odd number of 64 bytes (read down columns)
   static constexpr int kPitch = KMAJOR ? kStepK : (kSide / 32 | 1) * 32;
   static constexpr int kPlane = (KMAJOR ? kSide : kStepK) * kPitch;
   static_assert(kGroupThreads % kRowPieces == 0 && kLoads >= 1, "whole rows a turn");
 
   // The step from `k` on of the summed dimension.
   __device__ __forceinline__ static void load(const Panel<T>& p, int64_t k, Piece<T> (&out)[kLoads]) {
-    const int col = (int)threadIdx.x % kRowPieces * V, row = (int)threadIdx.x / kRowPieces;
-    const int at = KMAJOR ? (int)k + col : col;
-    const int64_t down = KMAJOR ? 0 : k;
-    const bool whole = (KMAJOR ? k + kStepK : kSide) <= p.cols;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int64_t r = down + row + i * (kGroupThreads / kRowPieces), kept = min(r, (int64_t)p.rows - 1);
-      if (whole) {
-        out[i].raw = *reinterpret_cast<const typename Piece<T>::Raw*>(p.base + kept * p.stride + at);
-        // a K-major panel's rows past the end give outputs that nobody stores
-        if (!KMAJOR && r >= p.rows) out[i].raw = typename Piece<T>::Raw{};
-      } else if (r < p.rows) {
-        out[i].load(p.base + r * p.stride, at, p.cols);
-      } else {
-        out[i].raw = typename Piece<T>::Raw{};
-      }
-    }
+    load_panel<T, KMAJOR, kRowPieces, kLoads, kGroupThreads, kStepK, kSide>(p, k, out);
   }
   __device__ __forceinline__ static void store(const Piece<T> (&in)[kLoads], uint16_t* __restrict__ lds) {
     const int col = (int)threadIdx.x % kRowPieces * V, row0 = (int)threadIdx.x / kRowPieces;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int row = row0 + i * (kGroupThreads / kRowPieces);
-      uint16_t* const to =
-          lds + row * kPitch + (KMAJOR ? 8 * ((col / 8) ^ (row >> 1 & 3)) + col % 8 : col);
-      if constexpr (P == 1) {
-        *reinterpret_cast<u32x4*>(to) = __builtin_bit_cast(u32x4, in[i].raw);
-      } else {
-        u32x2 s[3];
-        split4(in[i], s);
-#pragma unroll
-        for (int p = 0; p < P; ++p) *reinterpret_cast<u32x2*>(to + p * kPlane) = s[p];
-      }
+      *reinterpret_cast<u32x4*>(lds + row * kPitch + (KMAJOR ? 8 * ((col / 8) ^ (row >> 1 & 3)) : col)) =
+          __builtin_bit_cast(u32x4, in[i].raw);
     }
   }
   // Operand of 32 rows from `first` on, steps 16 s .. + 15 of the sum: lane l's
@@ -235,32 +200,11 @@ struct PanelImage {
   }
 };
 
-// Sums of a tile of 128 x 128 in eight waves of 64 rows by 32 columns.  Float32
-// factors are three bfloat16 pieces each: the product of the first ones has a
-// sum of its own, rounded once a step of 16, and every 128 of the summed
-// dimension both go into float32 sums that round to nearest (the matrix cores'
-// own round down).
+// Sums of a tile of 128 x 128 in eight waves of 64 rows by 32 columns.
 template <class T>
 struct TileSums {
-  static constexpr int P = Pieces<T>::P;
-  f32x16 acc[2], low[P == 3 ? 2 : 1], total[P == 3 ? 2 : 1];
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) acc[i] = f32x16{};
-    if constexpr (P == 3) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) low[i] = total[i] = f32x16{};
-    }
-  }
-  __device__ __forceinline__ void flush() {
-    if constexpr (P == 3) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        total[i] += acc[i] + low[i];
-        acc[i] = low[i] = f32x16{};
-      }
-    }
-  }
+  f32x16 acc[2];
+  __device__ __forceinline__ void clear() { acc[0] = acc[1] = f32x16{}; }
   // A's operand rows are the output's rows, B's its columns; result register r of
   // lane l is column 8 (r / 4) + 4 (l / 32) + r % 4 of row l % 32.
   template <class IA, class IB>
@@ -268,31 +212,106 @@ struct TileSums {
                                        int col0) {
 #pragma unroll
     for (int s = 0; s < kStepK / 16; ++s) {
-      s16x8 bv[P], av[2][P];
+      const s16x8 y = IB::read(b, col0, s);
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
-        bv[p] = IB::read(b + p * IB::kPlane, col0, s);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) av[i][p] = IA::read(a + p * IA::kPlane, row0 + 32 * i, s);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if constexpr (P == 1) {
-          acc[i] = mma16<T>(bv[0], av[i][0], acc[i]);
-        } else {
-          low[i] = mma16<T>(bv[2], av[i][0], low[i]);
-          low[i] = mma16<T>(bv[0], av[i][2], low[i]);
-          low[i] = mma16<T>(bv[1], av[i][1], low[i]);
-          low[i] = mma16<T>(bv[1], av[i][0], low[i]);
-          low[i] = mma16<T>(bv[0], av[i][1], low[i]);
-          acc[i] = mma16<T>(bv[0], av[i][0], acc[i]);
-        }
-      }
+      for (int i = 0; i < 2; ++i) acc[i] = mma16<T>(y, IA::read(a, row0 + 32 * i, s), acc[i]);
     }
   }
-  __device__ __forceinline__ const f32x16& value(int i) const {
-    if constexpr (P == 3) return total[i];
-    else return acc[i];
+};
+
+// ---- float32 rows, on the float32 matrix cores
+
+constexpr int kWideThreads = 256;
+
+// SIDE outputs by kStepK of the sum.  KMAJOR: rows of 128 bytes whose eight
+// 16-byte pieces are exchanged by the row's low bits; else 32 rows, four of which
+// are 32 banks apart.
+template <bool KMAJOR, int SIDE>
+struct WidePanel {
+  static constexpr int kRowPieces = (KMAJOR ? kStepK : SIDE) / 4;
+  static constexpr int kLoads = SIDE * kStepK / 4 / kWideThreads;
+  static constexpr int kPitch = KMAJOR ? kStepK : SIDE + 8;
+  static constexpr int kFloats = (KMAJOR ? SIDE : kStepK) * kPitch;
+  static_assert(kWideThreads % kRowPieces == 0 && kLoads >= 1, "whole rows a turn");
+
+  __device__ __forceinline__ static void load(const Panel<float>& p, int64_t k, Piece<float> (&out)[kLoads]) {
+    load_panel<float, KMAJOR, kRowPieces, kLoads, kWideThreads, kStepK, SIDE>(p, k, out);
+  }
+  __device__ __forceinline__ static void store(const Piece<float> (&in)[kLoads], float* __restrict__ lds) {
+    const int piece = (int)threadIdx.x % kRowPieces, row0 = (int)threadIdx.x / kRowPieces;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int row = row0 + i * (kWideThreads / kRowPieces);
+      *reinterpret_cast<u32x4*>(lds + row * kPitch + 4 * (KMAJOR ? piece ^ (row & 7) : piece)) =
+          __builtin_bit_cast(u32x4, in[i].raw);
+    }
+  }
+  // Operand of 32 outputs from `first` on, steps 8 s .. + 7 of the sum: lane l's four
+  // values are output l % 32, k = 8 s + 4 (l / 32) + 0 .. 3.
+  __device__ __forceinline__ static f32x4 read(const float* __restrict__ lds, int first, int s) {
+    const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31;
+    if constexpr (KMAJOR) {
+      return *reinterpret_cast<const f32x4*>(lds + (first + c) * kPitch + 4 * ((2 * s + h) ^ (c & 7)));
+    } else {
+      const float* const at = lds + (8 * s + 4 * h) * kPitch + first + c;
+      return f32x4{at[0], at[kPitch], at[2 * kPitch], at[3 * kPitch]};
+    }
+  }
+};
+
+// Sums of a tile of BM x BN in WM x WN waves over `len` of the sum; seen(pieces) is
+// given A's pieces of each step (which of them a thread holds, does not change).
+template <bool KA, bool KB, int BM, int BN, int WM, int WN>
+struct WideTile {
+  static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
+  static_assert(WM * WN * 64 == kWideThreads && TM >= 1 && TN >= 1, "four waves");
+  using A = WidePanel<KA, BM>;
+  using B = WidePanel<KB, BN>;
+  static constexpr int kRoom = std::max(A::kFloats + B::kFloats, kWideThreads / 64 * 1024);  // floats of LDS
+  f32x16 acc[TM][TN];
+
+  template <class F>
+  __device__ __forceinline__ void run(const Panel<float>& pa, const Panel<float>& pb, int len, float* room, F&& seen) {
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+    const int row0 = wave / WN * (BM / WM), col0 = wave % WN * (BN / WN);
+    float *const as = room, *const bs = room + A::kFloats;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = f32x16{};
+    }
+    if (len <= 0) return;
+    Piece<float> ra[A::kLoads], rb[B::kLoads];
+    A::load(pa, 0, ra);
+    B::load(pb, 0, rb);
+    for (int k = 0; k < len; k += kStepK) {
+      A::store(ra, as);
+      B::store(rb, bs);
+      seen(ra);
+      __syncthreads();
+      if (k + kStepK < len) {
+        A::load(pa, k + kStepK, ra);
+        B::load(pb, k + kStepK, rb);
+      }
+#pragma unroll
+      for (int s = 0; s < kStepK / 8; ++s) {
+        f32x4 x[TM], y[TN];
+#pragma unroll
+        for (int i = 0; i < TM; ++i) x[i] = A::read(as, row0 + 32 * i, s);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) y[j] = B::read(bs, col0 + 32 * j, s);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+          for (int i = 0; i < TM; ++i) {
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(y[j][e], x[i][e], acc[i][j], 0, 0, 0);
+          }
+        }
+      }
+      __syncthreads();
+    }
   }
 };
 
