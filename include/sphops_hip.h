@@ -664,23 +664,27 @@ int sphops_combine_rows_backward(const void* dy, int type, int64_t row_stride, c
  * offsets[e + 1] - 1 (device memory, from 0 on and not decreasing), zeros for the
  * rows behind the last expert's.  All of `type`; w (experts, out_features,
  * in_features) and b (experts, out_features, or NULL) dense, x's rows
- * row_stride elements apart, y dense.  relu: y = max(y, 0).  Sums are float32.
+ * row_stride elements apart, y dense.  relu: y = max(y, 0).  Sums are float32, and
+ * float32 factors keep their 24 bits.  workspace:
+ * sphops_expert_linear_workspace_bytes bytes (-1: not supported), 16-byte aligned.
  */
 int sphops_expert_linear(const void* x, int type, int64_t row_stride, const void* w, const void* b,
                          const int32_t* offsets, void* y, int64_t slots, int experts, int in_features,
-                         int out_features, int relu, void* stream);
-/* dx (slots, in_features) = dy w[e]; with h (slots, in_features, dense) zero
- * where h is not above 0.  Zeros behind the last expert's rows. */
-int sphops_expert_linear_input_grad(const void* dy, int type, int64_t dy_stride, const void* w, const void* h,
-                                    const int32_t* offsets, void* dx, int64_t slots, int experts, int in_features,
-                                    int out_features, void* stream);
-/* dw[e] = dy^T x and db[e] = the sums of dy over the expert's rows, in a fixed
- * order; each may be NULL.  workspace: sphops_expert_linear_workspace_bytes bytes
- * (-1: not supported), 16-byte aligned. */
-int sphops_expert_linear_weight_grad(const void* dy, int64_t dy_stride, const void* x, int type, int64_t row_stride,
-                                     const int32_t* offsets, void* dw, void* db, int64_t slots, int experts,
-                                     int in_features, int out_features, void* workspace, void* stream);
-int64_t sphops_expert_linear_workspace_bytes(int64_t slots, int experts, int in_features, int out_features);
+                         int out_features, int relu, void* workspace, void* stream);
+int64_t sphops_expert_linear_workspace_bytes(int type, int64_t slots, int experts, int in_features,
+                                             int out_features);
+/* Its gradients: dx (slots, in_features; zeros behind the last expert's rows)
+ * = dy w[e], with h (slots, in_features, dense) zero where h is not above 0; dw[e] =
+ * dy^T x and db[e] = the sums of dy over the expert's rows, in a fixed order.  dx, dw
+ * and db may each be NULL.  workspace:
+ * sphops_expert_linear_backward_workspace_bytes bytes (-1: not supported), 16-byte
+ * aligned. */
+int sphops_expert_linear_backward(const void* dy, int64_t dy_stride, const void* x, int type, int64_t row_stride,
+                                  const void* w, const void* h, const int32_t* offsets, void* dx, void* dw, void* db,
+                                  int64_t slots, int experts, int in_features, int out_features, void* workspace,
+                                  void* stream);
+int64_t sphops_expert_linear_backward_workspace_bytes(int type, int64_t slots, int experts, int in_features,
+                                                      int out_features);
 
 /*
  * sphops_mlp_forward's MLP (hidden = 128, in_features in [4, 168], out_features

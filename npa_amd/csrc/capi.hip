@@ -1497,8 +1497,8 @@ void require_sorted(int type, int64_t rows, int choices, int64_t cols) {
   require(sort_fits(rows, choices, 1), "rows x choices must be in [0, 2^30], choices in [1, 64]");
   require(cols >= 1 && cols <= sphops::kMaxGroupCols, "a row must have 1 to 65536 values");
 }
-bool expert_linear_fits(int64_t slots, int experts, int in_features, int out_features) {
-  return slots >= 0 && slots <= sphops::kMaxSlots && experts >= 1 && experts <= sphops::kMaxExperts &&
+bool expert_linear_fits(int type, int64_t slots, int experts, int in_features, int out_features) {
+  return type >= SPHOPS_F32 && type <= SPHOPS_F16 && slots >= 0 && slots <= sphops::kMaxSlots && experts >= 1 && experts <= sphops::kMaxExperts &&
          in_features >= 1 && in_features <= sphops::kMaxGroupCols && out_features >= 1 &&
          out_features <= sphops::kMaxGroupCols &&
          sphops::group_linear_fits(slots, experts, in_features, out_features);
@@ -1597,50 +1597,48 @@ int sphops_combine_rows_backward(const void* dy, int type, int64_t row_stride, c
   });
 }
 
+int64_t sphops_expert_linear_workspace_bytes(int type, int64_t slots, int experts, int in_features,
+                                             int out_features) {
+  if (!expert_linear_fits(type, slots, experts, in_features, out_features)) return -1;
+  return sphops::group_linear_workspace_bytes(type, slots, experts, in_features, out_features);
+}
+
 int sphops_expert_linear(const void* x, int type, int64_t row_stride, const void* w, const void* b,
                          const int32_t* offsets, void* y, int64_t slots, int experts, int in_features,
-                         int out_features, int relu, void* stream) {
+                         int out_features, int relu, void* workspace, void* stream) {
   return guarded([&] {
     require_type(type);
-    require(expert_linear_fits(slots, experts, in_features, out_features), "layer not supported");
+    require(expert_linear_fits(type, slots, experts, in_features, out_features), "layer not supported");
     require(slots <= 1 || row_stride >= 0, "row_stride must be >= 0");
     require(slots == 0 || (x && w && offsets && y), "null buffer");
-    sphops::run_group_linear(x, type, row_stride, w, b, nullptr, offsets, y, slots, experts, in_features,
-                             out_features, relu != 0, false, sphops::as_stream(stream));
-  });
-}
-
-int sphops_expert_linear_input_grad(const void* dy, int type, int64_t dy_stride, const void* w, const void* h,
-                                    const int32_t* offsets, void* dx, int64_t slots, int experts, int in_features,
-                                    int out_features, void* stream) {
-  return guarded([&] {
-    require_type(type);
-    require(expert_linear_fits(slots, experts, in_features, out_features), "layer not supported");
-    require(slots <= 1 || dy_stride >= 0, "dy_stride must be >= 0");
-    require(slots == 0 || (dy && w && offsets && dx), "null buffer");
-    sphops::run_group_linear(dy, type, dy_stride, w, nullptr, h, offsets, dx, slots, experts, out_features,
-                             in_features, false, true, sphops::as_stream(stream));
-  });
-}
-
-int64_t sphops_expert_linear_workspace_bytes(int64_t slots, int experts, int in_features, int out_features) {
-  if (!expert_linear_fits(slots, experts, in_features, out_features)) return -1;
-  return sphops::group_weight_grad_floats(slots, experts, in_features, out_features) * (int64_t)sizeof(float);
-}
-
-int sphops_expert_linear_weight_grad(const void* dy, int64_t dy_stride, const void* x, int type, int64_t row_stride,
-                                     const int32_t* offsets, void* dw, void* db, int64_t slots, int experts,
-                                     int in_features, int out_features, void* workspace, void* stream) {
-  return guarded([&] {
-    require_type(type);
-    require(expert_linear_fits(slots, experts, in_features, out_features), "layer not supported");
-    require(slots <= 1 || (row_stride >= 0 && dy_stride >= 0), "strides must be >= 0");
-    require(offsets && (slots == 0 || (dy && x)), "null buffer");
-    require(sphops::group_weight_grad_floats(slots, experts, in_features, out_features) == 0 || workspace,
+    require(workspace || sphops::group_linear_workspace_bytes(type, slots, experts, in_features, out_features) == 0,
             "null buffer");
     require(sphops::pk::aligned16(workspace), "workspace must be 16-byte aligned");
-    sphops::run_group_weight_grad(dy, dy_stride, x, type, row_stride, offsets, dw, db, slots, experts, in_features,
-                                  out_features, static_cast<float*>(workspace), sphops::as_stream(stream));
+    sphops::run_group_linear(x, type, row_stride, w, b, offsets, y, slots, experts, in_features, out_features,
+                             relu != 0, workspace, sphops::as_stream(stream));
+  });
+}
+
+int64_t sphops_expert_linear_backward_workspace_bytes(int type, int64_t slots, int experts, int in_features,
+                                                      int out_features) {
+  if (!expert_linear_fits(type, slots, experts, in_features, out_features)) return -1;
+  return sphops::group_backward_workspace_bytes(type, slots, experts, in_features, out_features);
+}
+
+int sphops_expert_linear_backward(const void* dy, int64_t dy_stride, const void* x, int type, int64_t row_stride,
+                                  const void* w, const void* h, const int32_t* offsets, void* dx, void* dw, void* db,
+                                  int64_t slots, int experts, int in_features, int out_features, void* workspace,
+                                  void* stream) {
+  return guarded([&] {
+    require_type(type);
+    require(expert_linear_fits(type, slots, experts, in_features, out_features), "layer not supported");
+    require(slots <= 1 || (row_stride >= 0 && dy_stride >= 0), "strides must be >= 0");
+    require(offsets && (slots == 0 || (dy && x && w)), "null buffer");
+    require(workspace || sphops::group_backward_workspace_bytes(type, slots, experts, in_features, out_features) == 0,
+            "null buffer");
+    require(sphops::pk::aligned16(workspace), "workspace must be 16-byte aligned");
+    sphops::run_group_backward(dy, dy_stride, x, type, row_stride, w, h, offsets, dx, dw, db, slots, experts,
+                               in_features, out_features, workspace, sphops::as_stream(stream));
   });
 }
 

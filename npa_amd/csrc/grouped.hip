@@ -20,6 +20,45 @@ __device__ __forceinline__ void tile_of(uint32_t id, int64_t mt, int nt, int64_t
   n = (int)(at / size);
 }
 
+// What the matrix cores are given of a type: itself, or three bfloat16 pieces.
+template <class T>
+using Piece16 = std::conditional_t<std::is_same_v<T, float>, __hip_bfloat16, T>;
+template <class T>
+constexpr int kPieces = std::is_same_v<T, float> ? 3 : 1;
+
+__host__ __device__ __forceinline__ constexpr int64_t whole8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// Rows laid out for the kernels that load whole 16-byte pieces: out (rows x ld, ld
+// a multiple of 8, zeros past cols) as they are, or as three planes of bfloat16
+// pieces.
+constexpr int kLayThreads = 256;
+template <class T>
+__global__ __launch_bounds__(kLayThreads) void k_lay_out(const T* __restrict__ x, int64_t stride,
+                                                         uint16_t* __restrict__ out, int64_t rows, int cols, int ld) {
+  const int pieces = ld / 8;
+  const int64_t n = rows * pieces;
+  for (int64_t i = (int64_t)blockIdx.x * kLayThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kLayThreads) {
+    const int64_t row = i / pieces;
+    const int k = (int)(i - row * pieces) * 8;
+    uint16_t* const to = out + row * ld + k;
+    if constexpr (std::is_same_v<T, float>) {
+      Piece<float> p[2];
+      p[0].load(x + row * stride, k, cols);
+      p[1].load(x + row * stride, k + 4, cols);
+      f32x8 v;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = p[j / 4].get(j % 4);
+      const Thirds t = split3(v);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) *reinterpret_cast<bf16x8*>(to + q * rows * ld) = t.v[q];
+    } else {
+      Piece<T> p;
+      p.load(x + row * stride, k, cols);
+      *reinterpret_cast<u32x4*>(to) = __builtin_bit_cast(u32x4, p.raw);
+    }
+  }
+}
+
 // The workgroup's row tile and column tile among those that there are (the
 // launch covers the most that there can be); false: neither.
 __device__ __forceinline__ bool rows_tile(const int32_t* __restrict__ offsets, int experts, int64_t slots, int size,
@@ -123,16 +162,19 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_rows(const T* __restric
   }
 }
 
-// The same for 16-bit rows in whole 16-byte pieces: panels straight from memory
-// to LDS.
+// The same for 16-bit rows in whole 16-byte pieces, or for float32 rows laid out
+// as three bfloat16 pieces a value (xp and wp elements apart): panels straight
+// from memory to LDS.
 template <class T, bool BACK, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void k_group_rows_fast(const T* __restrict__ x, int64_t xs,
-                                                                  const T* __restrict__ w, const T* __restrict__ b,
+__global__ __launch_bounds__(64 * WM * WN) void k_group_rows_fast(const Piece16<T>* __restrict__ x, int64_t xs, int64_t xp,
+                                                                  const Piece16<T>* __restrict__ w, int64_t ws,
+                                                                  int64_t wp, const T* __restrict__ b,
                                                                   const T* __restrict__ mask,
                                                                   const int32_t* __restrict__ offsets,
                                                                   T* __restrict__ y, int64_t slots, int experts,
                                                                   int cols, int outs, bool relu, int nt) {
-  using Tile = FastTile<T, true, !BACK, BM, BN, WM, WN, false>;
+  using E = Piece16<T>;
+  using Tile = FastTile<E, kPieces<T>, true, !BACK, BM, BN, WM, WN, false>;
   constexpr int V = Piece<T>::V;
   __shared__ __attribute__((aligned(16))) uint16_t s0[Tile::kStage], s1[Tile::kStage];
   GroupTile g;
@@ -144,10 +186,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_group_rows_fast(const T* __res
     zero_rows(y, m0, here, n0, BN, outs);
     return;
   }
-  const T* const we = w + (int64_t)g.group * cols * outs;
-  const typename Tile::A pa(Panel<T>{x + m0 * xs, xs, here, cols});
-  const typename Tile::B pb(BACK ? Panel<T>{we + n0, outs, cols, outs_here}
-                                 : Panel<T>{we + (int64_t)n0 * cols, cols, outs_here, cols});
+  // W_e has a row for each output, or (BACK) for each input
+  const E* const we = w + (int64_t)g.group * (BACK ? cols : outs) * ws;
+  const typename Tile::A pa(Panel<E>{x + m0 * xs, xs, here, cols}, xp);
+  const typename Tile::B pb(BACK ? Panel<E>{we + n0, ws, cols, min(BN, (int)ws - n0)}
+                                 : Panel<E>{we + (int64_t)n0 * ws, ws, outs_here, cols}, wp);
   Tile t;
   t.run(pa, pb, cols, false, s0, s1);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
@@ -168,10 +211,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_group_rows_fast(const T* __res
   }
 }
 
-// The same for float32 rows.  Three bfloat16 pieces of each factor and six products
-// take three eighths of the matrix cores' time, but putting them into pieces takes
-// vector work that does not overlap, and their sums registers: 8192 x 1024 -> 2048
-// in 337 us that way.
+// The same for float32 rows as they are, on the float32 matrix cores.
 template <bool BACK, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(kWideThreads) void k_group_rows_wide(const float* __restrict__ x, int64_t xs,
                                                                   const float* __restrict__ w,
@@ -328,16 +368,18 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_weight_grad(const T* __
   }
 }
 
-// The same for 16-bit rows in whole 16-byte pieces, straight from memory to LDS;
-// db from products with ones.
+// The same for 16-bit rows in whole 16-byte pieces, or float32 rows laid out in
+// bfloat16 pieces, straight from memory to LDS; db from products with ones.
 template <class T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void k_group_weight_grad_fast(
-    const T* __restrict__ dy, int64_t dys, const T* __restrict__ x, int64_t xs, const int32_t* __restrict__ offsets,
-    T* __restrict__ dw, T* __restrict__ db, float* __restrict__ part, int64_t slots, int experts, int cols, int outs,
-    int64_t chunk, int mt, int nt) {
-  using Tile = FastTile<T, false, false, BM, BN, WM, WN, true>;
+    const Piece16<T>* __restrict__ dy, int64_t dys, int64_t dyp, const Piece16<T>* __restrict__ x, int64_t xs, int64_t xp,
+    const int32_t* __restrict__ offsets, T* __restrict__ dw, T* __restrict__ db, float* __restrict__ part,
+    int64_t slots, int experts, int cols, int outs, int64_t chunk, int mt, int nt) {
+  using E = Piece16<T>;
+  using Tile = FastTile<E, kPieces<T>, false, false, BM, BN, WM, WN, true>;
   static_assert(Tile::TM <= WN, "a wave of the row for each tile of rows");
   __shared__ __attribute__((aligned(16))) uint16_t s0[Tile::kStage], s1[Tile::kStage];
+  static_assert(Tile::kWaves * 2048 <= Tile::kStage, "room");
   const GradTile at = grad_tile(mt, nt);
   const int64_t piece = at.piece;
   const int m0 = at.m * BM, n0 = at.n * BN;
@@ -345,8 +387,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_group_weight_grad_fast(
   if (g.group < 0) return;
   const int64_t lo = g.lo + g.tile * chunk;
   const int rows = (int)min<int64_t>(chunk, g.hi - lo);
-  const typename Tile::A pa(Panel<T>{dy + lo * dys + m0, dys, rows, min(BM, outs - m0)});
-  const typename Tile::B pb(Panel<T>{x + lo * xs + n0, xs, rows, min(BN, cols - n0)});
+  const typename Tile::A pa(Panel<E>{dy + lo * dys + m0, dys, rows, (int)min<int64_t>(BM, whole8(outs) - m0)}, dyp);
+  const typename Tile::B pb(Panel<E>{x + lo * xs + n0, xs, rows, (int)min<int64_t>(BN, whole8(cols) - n0)}, xp);
   Tile t;
   t.run(pa, pb, rows, n0 == 0, s0, s1);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64), wn = wave % WN;
@@ -374,11 +416,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_group_weight_grad_fast(
       else if (dw != nullptr) put(T{}, dw + g.group * nw);
     }
   }
-  // every column of `ones` holds the same sums: lane l has row l % 32
   const int row = m0 + row0 + 32 * wn + (int)(threadIdx.x & 31);
   if (n0 != 0 || wn >= Tile::TM || (threadIdx.x & 63) >= 32 || row >= outs) return;
-  if (mine != nullptr) mine[nw + row] = t.ones[0];
-  else if (db != nullptr) db[(int64_t)g.group * outs + row] = from_f32<T>(t.ones[0]);
+  if (mine != nullptr) mine[nw + row] = t.ones;
+  else if (db != nullptr) db[(int64_t)g.group * outs + row] = from_f32<T>(t.ones);
 }
 
 // The same for float32 rows.
@@ -529,85 +570,212 @@ bool group_linear_fits(int64_t slots, int experts, int64_t cols, int64_t outs) {
   return tiles_of(cols * outs + outs, 256) * experts < limit;
 }
 
-void run_group_linear(const void* x, int type, int64_t xs, const void* w, const void* b, const void* mask,
-                      const int32_t* offsets, void* y, int64_t slots, int experts, int64_t cols, int64_t outs,
-                      bool relu, bool back, hipStream_t st) {
+namespace {
+
+// A matrix as the fast kernels read it.
+struct Laid {
+  const void* base;
+  int64_t stride, plane;
+};
+
+// Takes places for laid out rows off a workspace; without one it counts bytes.
+struct Layouts {
+  char* work;
+  int64_t used = 0;
+  int64_t take(int64_t bytes) {
+    const int64_t at = used;
+    used += (bytes + 15) / 16 * 16;
+    return at;
+  }
+  static int64_t bytes_of(int type, int64_t rows, int64_t cols) {
+    return (type == SPHOPS_F32 ? 3 : 1) * rows * whole8(cols) * 2;
+  }
+};
+
+template <class T>
+Laid lay_out(Layouts& l, const T* x, int64_t stride, int64_t rows, int64_t cols, hipStream_t st) {
+  const int64_t ld = whole8(cols);
+  uint16_t* const to = reinterpret_cast<uint16_t*>(
+      l.work + l.take(Layouts::bytes_of(std::is_same_v<T, float> ? SPHOPS_F32 : SPHOPS_BF16, rows, cols)));
+  const int64_t groups = std::min<int64_t>(tiles_of(rows * ld / 8, kLayThreads), 16384);
+  if (groups > 0) {
+    hipLaunchKernelGGL((k_lay_out<T>), dim3((uint32_t)groups), dim3(kLayThreads), 0, st, x, stride, to, rows, (int)cols,
+                       (int)ld);
+    SPHOPS_LAUNCHED();
+  }
+  return Laid{to, ld, rows * ld};
+}
+
+// Whether a product's operands are laid out first: float32 and 16-bit rows of
+// any kind where the product is large beside them.
+bool lays_out(int type, int64_t slots, int experts, int64_t cols, int64_t outs) {
+  if (cols < 64 || outs < 64 || slots < 64 * (int64_t)experts) return false;
+  return slots * cols * outs >= (int64_t(1) << (type == SPHOPS_F32 ? 32 : 31));
+}
+
+// Tiles of a product over rows on the fast kernels.
+template <class T, bool BACK>
+void rows_fast(const Laid& x, const Laid& w, const T* b, const T* mask, const int32_t* offsets, T* y, int64_t slots,
+               int experts, int64_t cols, int64_t outs, bool relu, hipStream_t st) {
+  using E = Piece16<T>;
+  const auto with = [&](auto kernel, int bm, int bn, int threads) {
+    const int64_t tiles = most_tiles(slots, experts + 1, bm) * tiles_of(outs, bn);
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles_of(tiles, 8) * 8)) /* whole turns of the eight XCDs */,
+                       dim3(threads), 0, st, static_cast<const E*>(x.base), x.stride, x.plane,
+                       static_cast<const E*>(w.base), w.stride, w.plane, b, mask, offsets, y, slots, experts, (int)cols,
+                       (int)outs, relu, (int)tiles_of(outs, bn));
+  };
+  if constexpr (std::is_same_v<T, float>) {
+    if (slots / 256 * tiles_of(outs, 128) >= 192) with(k_group_rows_fast<T, BACK, 256, 128, 4, 2>, 256, 128, 512);
+    else with(k_group_rows_fast<T, BACK, 128, 128, 2, 2>, 128, 128, 256);
+  } else {
+    if (rows_side(slots, outs) == 256) with(k_group_rows_fast<T, BACK, 256, 256, 2, 4>, 256, 256, 512);
+    else with(k_group_rows_fast<T, BACK, 128, 128, 2, 2>, 128, 128, 256);
+  }
+}
+
+// As they are.
+template <class T, bool BACK>
+void rows_plain(const T* x, int64_t xs, const T* w, const T* b, const T* mask, const int32_t* offsets, T* y,
+                int64_t slots, int experts, int64_t cols, int64_t outs, bool relu, hipStream_t st) {
+  const auto with = [&](auto kernel, int bm, int bn, int threads) {
+    const int64_t tiles = most_tiles(slots, experts + 1, bm) * tiles_of(outs, bn);
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles_of(tiles, 8) * 8)), dim3(threads), 0, st, x, xs, w, b, mask,
+                       offsets, y, slots, experts, (int)cols, (int)outs, relu, (int)tiles_of(outs, bn));
+  };
+  if constexpr (std::is_same_v<T, float>) {
+    if (wide_rows(slots, experts) == 32) with(k_group_rows_wide<BACK, 32, 128, 1, 4>, 32, 128, kWideThreads);
+    else if (wide_side(outs) == 32) with(k_group_rows_wide<BACK, 128, 32, 4, 1>, 128, 32, kWideThreads);
+    else if (wide_side(outs) == 64) with(k_group_rows_wide<BACK, 128, 64, 4, 1>, 128, 64, kWideThreads);
+    else with(k_group_rows_wide<BACK, 128, 128, 2, 2>, 128, 128, kWideThreads);
+  } else {
+    with(k_group_rows<T, BACK>, kSide, kSide, kGroupThreads);
+  }
+}
+
+template <class T>
+bool fast_as_is(const void* x, int64_t xs, int64_t cols, const void* w, int64_t ws) {
+  return !std::is_same_v<T, float> && whole_pieces(x, xs) && cols % 8 == 0 && whole_pieces(w, ws);
+}
+
+}  // namespace
+
+int64_t group_linear_workspace_bytes(int type, int64_t slots, int experts, int64_t cols, int64_t outs) {
+  if (!lays_out(type, slots, experts, cols, outs)) return 0;
+  Layouts l{nullptr};
+  l.take(Layouts::bytes_of(type, slots, cols));
+  l.take(Layouts::bytes_of(type, experts * outs, cols));
+  return l.used;
+}
+
+void run_group_linear(const void* x, int type, int64_t xs, const void* w, const void* b, const int32_t* offsets,
+                      void* y, int64_t slots, int experts, int64_t cols, int64_t outs, bool relu, void* work,
+                      hipStream_t st) {
   if (slots == 0) return;
   with_type(type, [&](auto t) {
     using T = decltype(t);
-    auto launch = [&](auto bk) {
-      constexpr bool BACK = decltype(bk)::value;
-      const auto with = [&](auto kernel, int bm, int bn, int threads) {
-        const int64_t tiles = most_tiles(slots, experts + 1, bm) * tiles_of(outs, bn);
-        hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles_of(tiles, 8) * 8)) /* whole turns of the eight XCDs */,
-                           dim3(threads), 0, st, static_cast<const T*>(x), xs, static_cast<const T*>(w),
-                           static_cast<const T*>(b), static_cast<const T*>(mask), offsets, static_cast<T*>(y), slots,
-                           experts, (int)cols, (int)outs, relu, (int)tiles_of(outs, bn));
-      };
-      if constexpr (std::is_same_v<T, float>) {
-        if (wide_rows(slots, experts) == 32) with(k_group_rows_wide<BACK, 32, 128, 1, 4>, 32, 128, kWideThreads);
-        else if (wide_side(outs) == 32) with(k_group_rows_wide<BACK, 128, 32, 4, 1>, 128, 32, kWideThreads);
-        else if (wide_side(outs) == 64) with(k_group_rows_wide<BACK, 128, 64, 4, 1>, 128, 64, kWideThreads);
-        else with(k_group_rows_wide<BACK, 128, 128, 2, 2>, 128, 128, kWideThreads);
-      } else if (whole_pieces(x, xs) && whole_pieces(w, BACK ? outs : cols) && cols % 8 == 0 &&
-                 (!BACK || outs % 8 == 0)) {
-        if (rows_side(slots, outs) == 256) with(k_group_rows_fast<T, BACK, 256, 256, 2, 4>, 256, 256, 512);
-        else with(k_group_rows_fast<T, BACK, 128, 128, 2, 2>, 128, 128, 256);
-      } else {
-        with(k_group_rows<T, BACK>, kSide, kSide, kGroupThreads);
-      }
-    };
-    if (back) launch(std::true_type{});
-    else launch(std::false_type{});
+    const T *px = static_cast<const T*>(x), *pw = static_cast<const T*>(w), *pb = static_cast<const T*>(b);
+    T* const py = static_cast<T*>(y);
+    const bool as_is = fast_as_is<T>(x, xs, cols, w, cols);
+    if (as_is || lays_out(type, slots, experts, cols, outs)) {
+      Layouts l{static_cast<char*>(work)};
+      const Laid lx = as_is ? Laid{x, xs, 0} : lay_out(l, px, xs, slots, cols, st);
+      const Laid lw = as_is ? Laid{w, cols, 0} : lay_out(l, pw, cols, experts * outs, cols, st);
+      rows_fast<T, false>(lx, lw, pb, nullptr, offsets, py, slots, experts, cols, outs, relu, st);
+    } else {
+      rows_plain<T, false>(px, xs, pw, pb, nullptr, offsets, py, slots, experts, cols, outs, relu, st);
+    }
   });
   SPHOPS_LAUNCHED();
 }
 
-// The workspace holds the chunks of any of the kernels.
-int64_t group_weight_grad_floats(int64_t slots, int experts, int64_t cols, int64_t outs) {
+// The chunks of any of the kernels, and the laid out operands of both products.
+int64_t group_backward_workspace_bytes(int type, int64_t slots, int experts, int64_t cols, int64_t outs) {
   int64_t chunks = 0;
-  for (const bool wide : {false, true}) {
-    for (const bool fast : {false, true}) chunks = std::max(chunks, chosen_plan(slots, experts, cols, outs, wide, fast).chunks);
+  for (const bool fast : {false, true})
+    chunks = std::max(chunks, chosen_plan(slots, experts, cols, outs, type == SPHOPS_F32, fast).chunks);
+  if (type == SPHOPS_F32)
+    chunks = std::max(chunks, grad_plan(slots, experts, cols, outs, 256, 128).chunks);
+  Layouts l{nullptr};
+  l.take(chunks * (cols * outs + outs) * (int64_t)sizeof(float));
+  if (lays_out(type, slots, experts, cols, outs)) {
+    l.take(Layouts::bytes_of(type, slots, outs));
+    l.take(Layouts::bytes_of(type, experts * outs, cols));
+    l.take(Layouts::bytes_of(type, slots, cols));
   }
-  return chunks * (cols * outs + outs);
+  return l.used;
 }
 
-void run_group_weight_grad(const void* dy, int64_t dys, const void* x, int type, int64_t xs, const int32_t* offsets,
-                           void* dw, void* db, int64_t slots, int experts, int64_t cols, int64_t outs, float* work,
-                           hipStream_t st) {
+void run_group_backward(const void* dy, int64_t dys, const void* x, int type, int64_t xs, const void* w,
+                        const void* mask, const int32_t* offsets, void* dx, void* dw, void* db, int64_t slots,
+                        int experts, int64_t cols, int64_t outs, void* work, hipStream_t st) {
   const int64_t nw = cols * outs;
+  const bool sums = dw != nullptr || db != nullptr;
   with_type(type, [&](auto t) {
     using T = decltype(t);
     constexpr bool wide = std::is_same_v<T, float>;
-    const bool fast = !wide && whole_pieces(dy, dys) && whole_pieces(x, xs) && cols % 8 == 0 && outs % 8 == 0;
-    const GradPlan p = chosen_plan(slots, experts, cols, outs, wide, fast);
-    const int64_t blocks = (p.chunks > 0 ? p.chunks : experts) * p.mt * p.nt;
-    const auto with = [&](auto kernel, int threads) {
-      hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(threads), 0, st, static_cast<const T*>(dy), dys,
-                         static_cast<const T*>(x), xs, offsets, static_cast<T*>(dw), static_cast<T*>(db),
-                         p.chunks > 0 ? work : nullptr, slots, experts, (int)cols, (int)outs, p.chunk, p.mt, p.nt);
-    };
-    if constexpr (wide) {
-      if (p.bm == 128 && p.bn == 128) with(k_group_weight_grad_wide<128, 128, 2, 2>, kWideThreads);
-      else if (p.bm == 128 && p.bn == 64) with(k_group_weight_grad_wide<128, 64, 4, 1>, kWideThreads);
-      else if (p.bm == 64 && p.bn == 128) with(k_group_weight_grad_wide<64, 128, 1, 4>, kWideThreads);
-      else if (p.bm == 128) with(k_group_weight_grad_wide<128, 32, 4, 1>, kWideThreads);
-      else if (p.bn == 128) with(k_group_weight_grad_wide<32, 128, 1, 4>, kWideThreads);
-      else with(k_group_weight_grad_wide<64, 64, 2, 2>, kWideThreads);
-    } else if (!fast) {
-      with(k_group_weight_grad<T>, kGroupThreads);
-    } else if (p.bm == 256) {
-      with(k_group_weight_grad_fast<T, 256, 256, 2, 4>, 512);
+    const T *pdy = static_cast<const T*>(dy), *px = static_cast<const T*>(x), *pw = static_cast<const T*>(w);
+    const T* const pm = static_cast<const T*>(mask);
+    const bool laid = lays_out(type, slots, experts, cols, outs);
+    const bool rows_as_is = fast_as_is<T>(dy, dys, outs, w, cols) && cols % 8 == 0;
+    const bool grad_as_is = fast_as_is<T>(dy, dys, outs, x, xs) && cols % 8 == 0;
+    Layouts l{static_cast<char*>(work)};
+    int64_t chunks = 0;
+    for (const bool fast : {false, true}) chunks = std::max(chunks, chosen_plan(slots, experts, cols, outs, wide, fast).chunks);
+    if (wide) chunks = std::max(chunks, grad_plan(slots, experts, cols, outs, 256, 128).chunks);
+    float* const part = reinterpret_cast<float*>(l.work + l.take(chunks * (nw + outs) * (int64_t)sizeof(float)));
+    Laid ldy{dy, dys, 0};
+    const bool lay_dy = slots > 0 && laid && ((dx != nullptr && !rows_as_is) || (sums && !grad_as_is));
+    if (lay_dy) ldy = lay_out(l, pdy, dys, slots, outs, st);
+    if (dx != nullptr && slots > 0) {
+      if (rows_as_is || laid) {
+        const Laid lw = rows_as_is ? Laid{w, cols, 0} : lay_out(l, pw, cols, experts * outs, cols, st);
+        rows_fast<T, true>(ldy, lw, nullptr, pm, offsets, static_cast<T*>(dx), slots, experts, outs, cols, false, st);
+      } else {
+        rows_plain<T, true>(pdy, dys, pw, nullptr, pm, offsets, static_cast<T*>(dx), slots, experts, outs, cols, false, st);
+      }
+      SPHOPS_LAUNCHED();
+    }
+    if (!sums) return;
+    const bool fast = grad_as_is || (laid && slots > 0);
+    const GradPlan p = wide && fast ? grad_plan(slots, experts, cols, outs, 256, 128)
+                                    : chosen_plan(slots, experts, cols, outs, wide, fast);
+    float* const to = p.chunks > 0 ? part : nullptr;
+    const dim3 grid((uint32_t)((p.chunks > 0 ? p.chunks : experts) * p.mt * p.nt));
+    T *const pdw = static_cast<T*>(dw), *const pdb = static_cast<T*>(db);
+    if (fast) {
+      using E = Piece16<T>;
+      const Laid lx = grad_as_is ? Laid{x, xs, 0} : lay_out(l, px, xs, slots, cols, st);
+      const auto with = [&](auto kernel, int threads) {
+        hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, st, static_cast<const E*>(ldy.base), ldy.stride, ldy.plane,
+                           static_cast<const E*>(lx.base), lx.stride, lx.plane, offsets, pdw, pdb, to, slots, experts,
+                           (int)cols, (int)outs, p.chunk, p.mt, p.nt);
+      };
+      if constexpr (wide) with(k_group_weight_grad_fast<T, 256, 128, 4, 2>, 512);
+      else if (p.bm == 256) with(k_group_weight_grad_fast<T, 256, 256, 2, 4>, 512);
+      else with(k_group_weight_grad_fast<T, 128, 128, 2, 2>, 256);
     } else {
-      with(k_group_weight_grad_fast<T, 128, 128, 2, 2>, 256);
+      const auto with = [&](auto kernel, int threads) {
+        hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, st, pdy, dys, px, xs, offsets, pdw, pdb, to, slots, experts,
+                           (int)cols, (int)outs, p.chunk, p.mt, p.nt);
+      };
+      if constexpr (wide) {
+        if (p.bm == 128 && p.bn == 128) with(k_group_weight_grad_wide<128, 128, 2, 2>, kWideThreads);
+        else if (p.bm == 128 && p.bn == 64) with(k_group_weight_grad_wide<128, 64, 4, 1>, kWideThreads);
+        else if (p.bm == 64 && p.bn == 128) with(k_group_weight_grad_wide<64, 128, 1, 4>, kWideThreads);
+        else if (p.bm == 128) with(k_group_weight_grad_wide<128, 32, 4, 1>, kWideThreads);
+        else if (p.bn == 128) with(k_group_weight_grad_wide<32, 128, 1, 4>, kWideThreads);
+        else with(k_group_weight_grad_wide<64, 64, 2, 2>, kWideThreads);
+      } else {
+        with(k_group_weight_grad<T>, kGroupThreads);
+      }
     }
     SPHOPS_LAUNCHED();
     if (p.chunks > 0)
       hipLaunchKernelGGL((k_group_chunk_sum<T>), dim3((uint32_t)tiles_of(nw + outs, 256), (uint32_t)experts), dim3(256),
-                         0, st, work, offsets, static_cast<T*>(dw), static_cast<T*>(db), slots, experts, nw, (int)outs,
-                         p.chunk, p.chunks);
+                         0, st, part, offsets, pdw, pdb, slots, experts, nw, (int)outs, p.chunk, p.chunks);
+    SPHOPS_LAUNCHED();
   });
-  SPHOPS_LAUNCHED();
 }
 
 }  // namespace sphops

@@ -343,8 +343,6 @@ __device__ __forceinline__ void rows_of_tile(const f32x16& v, float* __restrict_
 
 // ---- 16-bit operands straight from memory to LDS
 
-constexpr int kFastK = 64;  // of the sum a step
-
 // 64 lanes' 16 bytes from memory to LDS, lane l's to lds + 16 l, past the
 // registers; done once the wave's vector memory count says so.
 __device__ __forceinline__ void load_to_lds(const void* src, void* lds) {
@@ -353,58 +351,66 @@ __device__ __forceinline__ void load_to_lds(const void* src, void* lds) {
 }
 __device__ const uint4 kZeros16 = {0, 0, 0, 0};
 
-// A panel of SIDE outputs by kFastK of the sum, 128 SIDE bytes of LDS, loaded by
-// WAVES waves.  KMAJOR: rows of 128 bytes whose eight 16-byte pieces are
-// exchanged by the row's low bits (piece p stands at p ^ (row % 8)), read as
-// they are.  Else 64 rows of 2 SIDE bytes, read down their columns; the 64-byte
-// quarters are exchanged by the row's low two bits, so that the four rows of a
-// column read lie in different banks.
-// Rows are whole 16-byte pieces at multiples of 16 bytes.
-template <class T, bool KMAJOR, int SIDE, int WAVES>
+// A panel of SIDE outputs by KS of the sum, 2 KS SIDE bytes of LDS for each of P
+// pieces of its values, loaded by WAVES waves.  KMAJOR: rows of 2 KS bytes whose
+// 16-byte pieces are exchanged by the row's low bits, read as they are.  Else KS
+// rows of 2 SIDE bytes, read down their columns; the 64-byte quarters are
+// exchanged by the row's low two bits, so that the four rows of a column read
+// lie in different banks.
+// Rows are whole 16-byte pieces at multiples of 16 bytes; the values' pieces are
+// `plane` elements apart.
+template <class T, int P, int KS, bool KMAJOR, int SIDE, int WAVES>
 struct FastPanel {
-  static constexpr int kLoads = SIDE / 8 / WAVES;
-  static_assert(kLoads * 8 * WAVES == SIDE && SIDE >= 128, "whole loads, four quarters a row");
+  static constexpr int kLoads = SIDE * KS / 512 / WAVES, kPiece = SIDE * KS;  // 16-bit words
+  static constexpr int kRowPieces = KS / 8;
+  static_assert(kLoads * 512 * WAVES == SIDE * KS && SIDE >= 128, "whole loads, four quarters a row");
   const T* base;
-  int64_t step;              // elements from one step to the next
-  uint32_t at[kLoads];       // of the lane's pieces, from base
-  int k[kLoads];             // where they stand in the sum's step
+  int64_t plane;
+  int64_t step;         // elements from one step to the next
+  uint32_t at[kLoads];  // of the lane's 16 bytes, from base
+  int k[kLoads];        // where they stand in the sum's step
 
-  // rows x cols values (as in Panel) from p on
-  __device__ __forceinline__ FastPanel(const Panel<T>& p) : base(p.base) {
+  __device__ __forceinline__ static int exchange(int row) { return KS == 64 ? row & 7 : row >> 1 & 3; }
+
+  __device__ __forceinline__ FastPanel(const Panel<T>& p, int64_t plane) : base(p.base), plane(plane) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
-    step = KMAJOR ? kFastK : kFastK * p.stride;
+    step = KMAJOR ? KS : KS * p.stride;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
+      const int word = (i * WAVES + wave) * 512 + 8 * lane;
       if constexpr (KMAJOR) {
-        const int row = min((i * WAVES + wave) * 8 + (lane >> 3), p.rows - 1);  // rows past the end: nobody stores them
-        k[i] = 8 * ((lane & 7) ^ (lane >> 3));
-        at[i] = (uint32_t)row * (uint32_t)p.stride + (uint32_t)k[i];
+        const int row = word / KS;
+        k[i] = 8 * (word % KS / 8 ^ exchange(row));
+        at[i] = (uint32_t)min(row, p.rows - 1) * (uint32_t)p.stride + (uint32_t)k[i];  // rows past the end: nobody stores them
       } else {
-        const int byte = (i * WAVES + wave) * 1024 + 16 * lane, row = byte / (2 * SIDE);
-        const int piece = byte % (2 * SIDE) / 16 ^ (row & 3) << 2;
+        const int row = word / SIDE, col = 8 * (word % SIDE / 8 ^ (row & 3) << 2);
         k[i] = row;
-        at[i] = (uint32_t)row * (uint32_t)p.stride + (uint32_t)min(8 * piece, p.cols - 8);
+        at[i] = (uint32_t)row * (uint32_t)p.stride + (uint32_t)min(col, p.cols - 8);
       }
     }
   }
-  // The step from k0 on into `lds`; `left`: what is left of the sum (zeros past it).
+  // Step n into `lds`; `left`: what is left of the sum (zeros past it).
   __device__ __forceinline__ void load(int64_t n, int left, uint16_t* lds) const {
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
-    const T* __restrict__ from = base + n * step;
-    if (left >= kFastK) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) load_to_lds(from + at[i], lds + (i * WAVES + wave) * 512);
-    } else {
+    for (int p = 0; p < P; ++p) {
+      const T* __restrict__ from = base + n * step + p * plane;
+      uint16_t* const to = lds + p * kPiece;
+      if (left >= KS) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        load_to_lds(k[i] < left ? (const void*)(from + at[i]) : (const void*)&kZeros16, lds + (i * WAVES + wave) * 512);
+        for (int i = 0; i < kLoads; ++i) load_to_lds(from + at[i], to + (i * WAVES + wave) * 512);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+          load_to_lds(k[i] < left ? (const void*)(from + at[i]) : (const void*)&kZeros16, to + (i * WAVES + wave) * 512);
+      }
     }
   }
   // What a lane adds for the operand of 32 outputs from `first` on.
   __device__ __forceinline__ static int place(int first) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
     if constexpr (KMAJOR) {
-      return (first + (lane & 31)) * kFastK;
+      return (first + (lane & 31)) * KS;
     } else {
       const int i = lane & 15, row = 8 * h + (i >> 2), col = first + 16 * (lane >> 4 & 1) + 4 * (i & 3);
       return row * SIDE + 8 * (col / 8 ^ (row & 3) << 2) + col % 8;
@@ -414,7 +420,7 @@ struct FastPanel {
   __device__ __forceinline__ static s16x8 read(const uint16_t* lds, int place, int s) {
     if constexpr (KMAJOR) {
       const int lane = threadIdx.x & 63;
-      return *reinterpret_cast<const s16x8*>(lds + place + 8 * ((2 * s + (lane >> 5)) ^ (lane & 7)));
+      return *reinterpret_cast<const s16x8*>(lds + place + 8 * ((2 * s + (lane >> 5)) ^ exchange(lane & 31)));
     } else {
       return join(read_column(lds + place + 16 * s * SIDE), read_column(lds + place + (16 * s + 4) * SIDE));
     }
@@ -422,16 +428,22 @@ struct FastPanel {
 };
 
 // Sums of a tile of BM x BN outputs over `len` of the sum, in WM x WN waves of
-// BM / WM by BN / WN each.  Two stages of LDS: a step's panels are
-// loaded under the products of the one before.
-template <class T, bool KA, bool KB, int BM, int BN, int WM, int WN, bool ONES>
+// BM / WM by BN / WN each.  Two stages of LDS: a step's panels are loaded under
+// the products of the one before.
+//
+// P = 3: values as three bfloat16 pieces, largest first, and the six largest
+// products.  A step's products have sums of their own, which are added to the
+// total in float32 with a rounding to nearest: the matrix cores' own sums round
+// down.
+template <class T, int P, bool KA, bool KB, int BM, int BN, int WM, int WN, bool ONES>
 struct FastTile {
+  static constexpr int KS = P == 1 ? 64 : 32;
   static constexpr int kWaves = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
-  static constexpr int kStage = (BM + BN) * kFastK;  // 16-bit words
-  using A = FastPanel<T, KA, BM, kWaves>;
-  using B = FastPanel<T, KB, BN, kWaves>;
+  static constexpr int kPanelA = P * BM * KS, kStage = kPanelA + P * BN * KS;  // 16-bit words
+  using A = FastPanel<T, P, KS, KA, BM, kWaves>;
+  using B = FastPanel<T, P, KS, KB, BN, kWaves>;
   f32x16 acc[TM][TN];
-  f32x16 ones;  // ONES: of A's rows alone, in wave wn of a row of waves those of its tile wn
+  float ones;  // ONES: of A's rows alone: lane l's row l % 32 of the wave's tile wn
 
   __device__ __forceinline__ void run(const A& a, const B& b, int len, bool count, uint16_t* s0, uint16_t* s1) {
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64), wn = wave % WN;
@@ -444,41 +456,80 @@ struct FastTile {
     }
 #pragma unroll
     for (int j = 0; j < TN; ++j) pb[j] = B::place(wn * (BN / WN) + 32 * j);
-    ones = f32x16{};
+    ones = 0.0f;
     s16x8 one;
 #pragma unroll
     for (int j = 0; j < 8; ++j) one[j] = std::is_same_v<T, __half> ? 0x3c00 : 0x3f80;
     auto load = [&](int n, uint16_t* lds) {
       // past the last step: the last one again, which nothing reads
-      const int at = min(n, (len - 1) / kFastK);
-      a.load(at, len - at * kFastK, lds);
-      b.load(at, len - at * kFastK, lds + BM * kFastK);
+      const int at = min(n, (len - 1) / KS);
+      a.load(at, len - at * KS, lds);
+      b.load(at, len - at * KS, lds + kPanelA);
       __builtin_amdgcn_sched_barrier(0);  // the loads go out before the products, not after them
     };
     auto compute = [&](const uint16_t* lds) {
-#pragma unroll
-      for (int s = 0; s < kFastK / 16; ++s) {
-        s16x8 x[TM], y[TN];
-#pragma unroll
-        for (int i = 0; i < TM; ++i) x[i] = A::read(lds, pa[i], s);
-#pragma unroll
-        for (int j = 0; j < TN; ++j) y[j] = B::read(lds + BM * kFastK, pb[j], s);
+      f32x16 part[P == 3 ? TM : 1][P == 3 ? TN : 1];
+      if constexpr (P == 3) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
 #pragma unroll
-          for (int j = 0; j < TN; ++j) acc[i][j] = mma16<T>(y[j], x[i], acc[i][j]);
+          for (int j = 0; j < TN; ++j) part[i][j] = f32x16{};
         }
-        if constexpr (ONES) {
-          if (count) {
+      }
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
-              if (wn == i) ones = mma16<T>(one, x[i], ones);
+      for (int s = 0; s < KS / 16; ++s) {
+        s16x8 x[TM][P], y[TN][P];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+#pragma unroll
+          for (int i = 0; i < TM; ++i) x[i][p] = A::read(lds + p * A::kPiece, pa[i], s);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) y[j][p] = B::read(lds + kPanelA + p * B::kPiece, pb[j], s);
+        }
+        if constexpr (P == 1) {
+#pragma unroll
+          for (int i = 0; i < TM; ++i) {
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = mma16<T>(y[j][0], x[i][0], acc[i][j]);
           }
+        } else {
+          constexpr int kX[6] = {1, 2, 0, 1, 0, 0}, kY[6] = {1, 0, 2, 0, 1, 0};  // small products first
+#pragma unroll
+          for (int q = 0; q < 6; ++q) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+#pragma unroll
+              for (int j = 0; j < TN; ++j) part[i][j] = mma16<T>(y[j][kY[q]], x[i][kX[q]], part[i][j]);
+            }
+          }
+        }
+      }
+      if constexpr (P == 3) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] += part[i][j];
+        }
+      }
+      if constexpr (ONES) {
+        if (count) {  // after the products, whose registers it would add to
+          __builtin_amdgcn_sched_barrier(0);
+          f32x16 sum = f32x16{};
+#pragma unroll
+          for (int i = 0; i < TM; ++i) {
+            if (wn != i) continue;
+#pragma unroll
+            for (int s = 0; s < KS / 16; ++s) {
+#pragma unroll
+              for (int p = P - 1; p >= 0; --p) sum = mma16<T>(one, A::read(lds + p * A::kPiece, pa[i], s), sum);
+            }
+          }
+          ones += sum[0];
         }
       }
     };
     if (len <= 0) return;
-    const int steps = (len + kFastK - 1) / kFastK;
+    const int steps = (len + KS - 1) / KS;
     load(0, s0);
     // every wave's loads of a step have landed, and every wave has read the step
     // before, whose place the next load takes

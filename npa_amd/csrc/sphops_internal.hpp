@@ -426,13 +426,15 @@ void run_combine_rows_backward(const void* dy, int type, int64_t stride, const v
 // grouped.hip: linear layers of experts over sorted rows
 constexpr int64_t kMaxGroupCols = 65536;
 bool group_linear_fits(int64_t slots, int experts, int64_t cols, int64_t outs);
-void run_group_linear(const void* x, int type, int64_t xs, const void* w, const void* b, const void* mask,
-                      const int32_t* offsets, void* y, int64_t slots, int experts, int64_t cols, int64_t outs,
-                      bool relu, bool back, hipStream_t st);
-int64_t group_weight_grad_floats(int64_t slots, int experts, int64_t cols, int64_t outs);
-void run_group_weight_grad(const void* dy, int64_t dys, const void* x, int type, int64_t xs, const int32_t* offsets,
-                           void* dw, void* db, int64_t slots, int experts, int64_t cols, int64_t outs, float* work,
-                           hipStream_t st);
+int64_t group_linear_workspace_bytes(int type, int64_t slots, int experts, int64_t cols, int64_t outs);
+void run_group_linear(const void* x, int type, int64_t xs, const void* w, const void* b, const int32_t* offsets,
+                      void* y, int64_t slots, int experts, int64_t cols, int64_t outs, bool relu, void* work,
+                      hipStream_t st);
+int64_t group_backward_workspace_bytes(int type, int64_t slots, int experts, int64_t cols, int64_t outs);
+// dx (0 where mask, slots x cols, is given and not above 0), dw and db; any of them may be null
+void run_group_backward(const void* dy, int64_t dys, const void* x, int type, int64_t xs, const void* w,
+                        const void* mask, const int32_t* offsets, void* dx, void* dw, void* db, int64_t slots,
+                        int experts, int64_t cols, int64_t outs, void* work, hipStream_t st);
 // expert_mlp.hip: Linear, ReLU, Linear of experts over sorted float32 rows, 128 hidden units
 bool expert_mlp_fits(int64_t slots, int experts, int nin, int hidden, int nout);
 void run_expert_mlp_forward(const float* z, const float* w1, const float* b1, const float* w2, const float* b2,

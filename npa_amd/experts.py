@@ -159,36 +159,35 @@ def combine(results, weight, routing):
     return _gather(results, weight, slot)
 
 
+def _work(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
 def _linear(x, w, b, offsets, relu=False):
-    (experts, outs, cols), slots = w.shape, x.shape[0]
+    (experts, outs, cols), slots, kind = w.shape, x.shape[0], TYPES[x.dtype]
     v, _, stride = _rows.rows_view(x)
     y = torch.empty(slots, outs, dtype=x.dtype, device=x.device)
-    _rows.call(_lib.sphops_expert_linear, x.device, v.data_ptr(), TYPES[x.dtype], stride, w.data_ptr(), address(b),
-               offsets.data_ptr(), y.data_ptr(), slots, experts, cols, outs, int(relu))
+    work = _work(_lib.sphops_expert_linear_workspace_bytes(kind, slots, experts, cols, outs), x.device)
+    _rows.call(_lib.sphops_expert_linear, x.device, v.data_ptr(), kind, stride, w.data_ptr(), address(b),
+               offsets.data_ptr(), y.data_ptr(), slots, experts, cols, outs, int(relu), address(work))
     return y
 
 
-def _input_grad(dy, w, offsets, h=None):
-    (experts, outs, cols), slots = w.shape, dy.shape[0]
-    u, _, stride = _rows.rows_view(dy)
-    dx = torch.empty(slots, cols, dtype=dy.dtype, device=dy.device)
-    _rows.call(_lib.sphops_expert_linear_input_grad, dy.device, u.data_ptr(), TYPES[dy.dtype], stride, w.data_ptr(),
-               address(h), offsets.data_ptr(), dx.data_ptr(), slots, experts, cols, outs)
-    return dx
-
-
-def _weight_grad(dy, x, offsets, shape, need_w, need_b):
-    (experts, outs, cols), slots = shape, dy.shape[0]
+def _gradients(dy, x, w, offsets, need_x, need_w, need_b, h=None):
+    """dx (zero where h is not above 0), dW and db, those that are needed."""
+    (experts, outs, cols), slots, kind, dev = w.shape, x.shape[0], TYPES[x.dtype], x.device
+    if not (need_x or need_w or need_b):
+        return None, None, None
     u, _, dy_stride = _rows.rows_view(dy)
     v, _, stride = _rows.rows_view(x)
-    dw = torch.empty(shape, dtype=dy.dtype, device=dy.device) if need_w else None
-    db = torch.empty(experts, outs, dtype=dy.dtype, device=dy.device) if need_b else None
-    nbytes = _lib.sphops_expert_linear_workspace_bytes(slots, experts, cols, outs)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes else None
-    _rows.call(_lib.sphops_expert_linear_weight_grad, dy.device, u.data_ptr(), dy_stride, v.data_ptr(),
-               TYPES[dy.dtype], stride, offsets.data_ptr(), address(dw), address(db), slots, experts, cols, outs,
-               address(work))
-    return dw, db
+    dx = torch.empty(slots, cols, dtype=x.dtype, device=dev) if need_x else None
+    dw = torch.empty(w.shape, dtype=x.dtype, device=dev) if need_w else None
+    db = torch.empty(experts, outs, dtype=x.dtype, device=dev) if need_b else None
+    work = _work(_lib.sphops_expert_linear_backward_workspace_bytes(kind, slots, experts, cols, outs), dev)
+    _rows.call(_lib.sphops_expert_linear_backward, dev, u.data_ptr(), dy_stride, v.data_ptr(), kind, stride,
+               w.data_ptr(), address(h), offsets.data_ptr(), address(dx), address(dw), address(db), slots, experts, cols,
+               outs, address(work))
+    return dx, dw, db
 
 
 class _Linear(torch.autograd.Function):
@@ -200,10 +199,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         x, w, offsets = ctx.saved_tensors
-        need_x, need_w, need_b, _ = ctx.needs_input_grad
-        dx = _input_grad(dy, w, offsets) if need_x else None
-        dw, db = _weight_grad(dy, x, offsets, w.shape, need_w, need_b) if need_w or need_b else (None, None)
-        return (*_rows.first_order("the experts' layer", dx, dw, db), None)
+        return (*_rows.first_order("the experts' layer", *_gradients(dy, x, w, offsets, *ctx.needs_input_grad[:3])), None)
 
 
 class _Mlp(torch.autograd.Function):
@@ -217,15 +213,9 @@ class _Mlp(torch.autograd.Function):
     def backward(ctx, dy):
         x, h, w1, w2, offsets = ctx.saved_tensors
         need_x, need_w1, need_b1, need_w2, need_b2, _ = ctx.needs_input_grad
-        dx = dw1 = db1 = dw2 = db2 = None
-        if need_w2 or need_b2:
-            dw2, db2 = _weight_grad(dy, h, offsets, w2.shape, need_w2, need_b2)
-        if need_x or need_w1 or need_b1:
-            da = _input_grad(dy, w2, offsets, h)
-            if need_w1 or need_b1:
-                dw1, db1 = _weight_grad(da, x, offsets, w1.shape, need_w1, need_b1)
-            if need_x:
-                dx = _input_grad(da, w1, offsets)
+        first = need_x or need_w1 or need_b1
+        da, dw2, db2 = _gradients(dy, h, w2, offsets, first, need_w2, need_b2, h)
+        dx, dw1, db1 = _gradients(da, x, w1, offsets, need_x, need_w1, need_b1) if first else (None, None, None)
         return (*_rows.first_order("the experts' MLP", dx, dw1, db1, dw2, db2), None)
 
 
@@ -279,7 +269,7 @@ def _check_layer(x, weight, bias, slots, experts, cols, what):
     outs = weight.shape[1]
     weight = _rows.check_weight(weight, (experts, outs, cols), (x.dtype,), x.device, what)
     bias = _rows.check_weight(bias, (experts, outs), (x.dtype,), x.device, f"the bias beside {what}")
-    if _lib.sphops_expert_linear_workspace_bytes(slots, experts, cols, outs) < 0:
+    if _lib.sphops_expert_linear_workspace_bytes(TYPES[x.dtype], slots, experts, cols, outs) < 0:
         raise RuntimeError(f"no layer of {experts} experts for {slots} rows of {cols} inputs and {outs} outputs")
     return weight, bias
 

@@ -99,10 +99,11 @@ _SIGNATURES = {
     "sphops_dispatch_rows": ([_p, _i32, _i64, _p, _p, _i64, _i32, _i64, _p], _i32),
     "sphops_combine_rows": ([_p, _i32, _p, _p, _p, _i64, _i32, _i64, _p], _i32),
     "sphops_combine_rows_backward": ([_p, _i32, _i64, _p, _p, _p, _p, _p, _i64, _i32, _i64, _p], _i32),
-    "sphops_expert_linear": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p], _i32),
-    "sphops_expert_linear_input_grad": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _p], _i32),
-    "sphops_expert_linear_weight_grad": ([_p, _i64, _p, _i32, _i64, _p, _p, _p, _i64, _i32, _i32, _i32, _p, _p], _i32),
-    "sphops_expert_linear_workspace_bytes": ([_i64, _i32, _i32, _i32], _i64),
+    "sphops_expert_linear": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p], _i32),
+    "sphops_expert_linear_workspace_bytes": ([_i32, _i64, _i32, _i32, _i32], _i64),
+    "sphops_expert_linear_backward": ([_p, _i64, _p, _i32, _i64, _p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _p,
+                                       _p], _i32),
+    "sphops_expert_linear_backward_workspace_bytes": ([_i32, _i64, _i32, _i32, _i32], _i64),
     "sphops_expert_mlp_forward": ([_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p], _i32),
     "sphops_expert_mlp_input_grad": ([_p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p], _i32),
     "sphops_expert_mlp_weight_grad": ([_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p],

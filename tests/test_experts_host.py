@@ -67,14 +67,17 @@ def test_entry_points_check_their_arguments():
     _fails(lib.sphops_combine_rows(p, 5, p, p, p, 1, 1, 8, None), "element type")
     _fails(lib.sphops_combine_rows(p, 0, p, None, p, 1, 1, 8, None), "null")
     _fails(lib.sphops_combine_rows_backward(p, 0, 8, None, p, p, p, p, 1, 1, 8, None), "null")
-    _fails(lib.sphops_expert_linear(p, 0, 8, p, p, p, p, 4, 0, 8, 8, 0, None), "not supported")
-    _fails(lib.sphops_expert_linear(p, 0, 8, p, p, p, p, 4, 2, 0, 8, 0, None), "not supported")
-    _fails(lib.sphops_expert_linear(p, 0, 8, p, p, None, p, 4, 2, 8, 8, 0, None), "null")
-    _fails(lib.sphops_expert_linear_input_grad(p, 0, 8, p, None, p, p, -4, 2, 8, 8, None), "not supported")
-    _fails(lib.sphops_expert_linear_weight_grad(p, 8, p, 0, 8, None, p, p, 4, 2, 8, 8, p, None), "null")
-    _fails(lib.sphops_expert_linear_weight_grad(p, 8, p, 0, 8, p, p, p, 4, 2, 8, 8, ctypes.c_void_p(4100), None),
+    _fails(lib.sphops_expert_linear(p, 0, 8, p, p, p, p, 4, 0, 8, 8, 0, p, None), "not supported")
+    _fails(lib.sphops_expert_linear(p, 0, 8, p, p, p, p, 4, 2, 0, 8, 0, p, None), "not supported")
+    _fails(lib.sphops_expert_linear(p, 0, 8, p, p, None, p, 4, 2, 8, 8, 0, p, None), "null")
+    _fails(lib.sphops_expert_linear(p, 0, 8, p, p, p, p, 1 << 16, 2, 1024, 1024, 0, None, None), "null")
+    _fails(lib.sphops_expert_linear(p, 0, 8, p, p, p, p, 4, 2, 8, 8, 0, ctypes.c_void_p(4100), None), "16-byte")
+    _fails(lib.sphops_expert_linear_backward(p, 8, p, 0, 8, p, None, p, p, p, p, -4, 2, 8, 8, p, None), "not supported")
+    _fails(lib.sphops_expert_linear_backward(p, 8, p, 0, 8, p, None, None, p, p, p, 4, 2, 8, 8, p, None), "null")
+    _fails(lib.sphops_expert_linear_backward(p, 8, p, 0, 8, p, None, p, p, p, p, 4, 2, 8, 8, ctypes.c_void_p(4100), None),
            "16-byte")
-    assert lib.sphops_expert_linear_workspace_bytes(4, 1025, 8, 8) == -1
+    assert lib.sphops_expert_linear_workspace_bytes(0, 4, 1025, 8, 8) == -1
+    assert lib.sphops_expert_linear_backward_workspace_bytes(3, 4, 2, 8, 8) == -1
     _fails(lib.sphops_expert_mlp_forward(p, p, p, p, p, p, p, p, 4, 2, 8, 64, 8, None), "not supported")
     _fails(lib.sphops_expert_mlp_forward(p, p, p, p, p, None, p, p, 4, 2, 8, 128, 8, None), "null")
     _fails(lib.sphops_expert_mlp_forward(p, p, p, p, p, p, p, ctypes.c_void_p(4100), 4, 2, 8, 128, 8, None), "8-byte")
