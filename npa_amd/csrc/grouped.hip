@@ -162,53 +162,152 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_rows(const T* __restric
   }
 }
 
+// How the fast kernels' tiles fall on the card, which holds `room` of their
+// workgroups at once: whole turns of `room` tiles, and the tiles that are left, cut
+// along the sum into `slices` each where that fills a turn better.  Without cuts
+// 8192 x 2048 -> 1024 float32, 272 tiles of 256 x 128 on 256 CUs, took two turns.
+struct Turns {
+  uint32_t whole, left, slices;
+};
+constexpr int kMaxSlices = 16, kSliceSteps = 4;  // at most; steps of the sum a slice has at least
+__host__ __device__ __forceinline__ Turns turns_of(uint32_t tiles, uint32_t room, int steps, bool cut) {
+  Turns t;
+  t.whole = tiles / room * room;
+  t.left = tiles - t.whole;
+  t.slices = 1;
+  if (cut && t.left > 0) {
+    const uint32_t most = room / t.left, deep = (uint32_t)(steps / kSliceSteps);
+    t.slices = most < deep ? most : deep;
+    t.slices = t.slices < 1 ? 1 : t.slices > kMaxSlices ? kMaxSlices : t.slices;
+  }
+  return t;
+}
+
+// Tile `id` of the fast kernels.
+__device__ __forceinline__ bool fast_tile(const int32_t* __restrict__ offsets, int experts, int64_t slots, int size,
+                                          int nt, int64_t mt, uint32_t id, GroupTile& g, int& n) {
+  int64_t m;
+  tile_of(id, mt, nt, m, n);
+  g = group_tile(offsets, experts, slots, m, size, true);
+  return g.group >= 0;
+}
+
+// Results of a wave's 32 x 32 on their way out, bias, ReLU and mask applied.
+template <class T>
+__device__ __forceinline__ void put_rows(const f32x16& acc, float* __restrict__ own, int row0, int col0, int64_t m0,
+                                         int here, const T* __restrict__ bias, const T* __restrict__ mask, bool relu,
+                                         T* __restrict__ y, int outs) {
+  rows_of_tile<T>(acc, own, [&](int r, int c, float (&v)[Piece<T>::V]) {
+    const int row = row0 + r, at = col0 + c;
+    if (row >= here || at >= outs) return;
+    finish<T>(v, bias, mask != nullptr ? mask + (m0 + row) * outs : nullptr, relu, y + (m0 + row) * outs, at, outs);
+  });
+}
+
 // The same for 16-bit rows in whole 16-byte pieces, or for float32 rows laid out
 // as three bfloat16 pieces a value (xp and wp elements apart): panels straight
-// from memory to LDS.
+// from memory to LDS.  A slice's sums go to `slices` (null: no tile is cut) as
+// they stand in registers.
 template <class T, bool BACK, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void k_group_rows_fast(const Piece16<T>* __restrict__ x, int64_t xs, int64_t xp,
-                                                                  const Piece16<T>* __restrict__ w, int64_t ws,
-                                                                  int64_t wp, const T* __restrict__ b,
-                                                                  const T* __restrict__ mask,
-                                                                  const int32_t* __restrict__ offsets,
-                                                                  T* __restrict__ y, int64_t slots, int experts,
-                                                                  int cols, int outs, bool relu, int nt) {
+__global__ __launch_bounds__(64 * WM * WN) void k_group_rows_fast(
+    const Piece16<T>* __restrict__ x, int64_t xs, int64_t xp, const Piece16<T>* __restrict__ w, int64_t ws, int64_t wp,
+    const T* __restrict__ b, const T* __restrict__ mask, const int32_t* __restrict__ offsets, T* __restrict__ y,
+    int64_t slots, int experts, int cols, int outs, bool relu, int nt, int room, f32x4* __restrict__ slices) {
   using E = Piece16<T>;
   using Tile = FastTile<E, kPieces<T>, true, !BACK, BM, BN, WM, WN, false>;
-  constexpr int V = Piece<T>::V;
   __shared__ __attribute__((aligned(16))) uint16_t s0[Tile::kStage], s1[Tile::kStage];
+  const int64_t mt = group_tiles(offsets, experts, slots, BM, true);
+  const int steps = (cols + Tile::KS - 1) / Tile::KS;
+  const Turns turns = turns_of((uint32_t)(mt * nt), (uint32_t)room, steps, slices != nullptr);
+  uint32_t id = blockIdx.x;
+  int slice = 0, cuts = 1;
+  if (id < turns.whole) {
+    id = (id & 7u) * (turns.whole >> 3) + (id >> 3);  // contiguous eighths to the XCDs
+  } else {
+    const uint32_t at = id - turns.whole;
+    if (at >= turns.left * turns.slices) return;
+    cuts = (int)turns.slices;
+    id = turns.whole + at / turns.slices;
+    slice = (int)(at % turns.slices);
+  }
+  id = (uint32_t)__builtin_amdgcn_readfirstlane((int)id);
+  slice = __builtin_amdgcn_readfirstlane(slice);
   GroupTile g;
   int n;
-  if (!rows_tile(offsets, experts, slots, BM, nt, g, n)) return;
+  if (!fast_tile(offsets, experts, slots, BM, nt, mt, id, g, n)) return;
   const int64_t m0 = g.lo + g.tile * BM;
   const int n0 = n * BN, here = (int)min<int64_t>(BM, g.hi - m0), outs_here = min(BN, outs - n0);
   if (g.group == experts) {
-    zero_rows(y, m0, here, n0, BN, outs);
+    if (slice == 0) zero_rows(y, m0, here, n0, BN, outs);
     return;
   }
   // W_e has a row for each output, or (BACK) for each input
   const E* const we = w + (int64_t)g.group * (BACK ? cols : outs) * ws;
-  const typename Tile::A pa(Panel<E>{x + m0 * xs, xs, here, cols}, xp);
-  const typename Tile::B pb(BACK ? Panel<E>{we + n0, ws, cols, min(BN, (int)ws - n0)}
-                                 : Panel<E>{we + (int64_t)n0 * ws, ws, outs_here, cols}, wp);
+  typename Tile::A pa(Panel<E>{x + m0 * xs, xs, here, cols}, xp);
+  typename Tile::B pb(BACK ? Panel<E>{we + n0, ws, cols, min(BN, (int)ws - n0)}
+                           : Panel<E>{we + (int64_t)n0 * ws, ws, outs_here, cols}, wp);
+  const int first = steps * slice / cuts, last = steps * (slice + 1) / cuts;
+  pa.base += first * pa.step;
+  pb.base += first * pb.step;
   Tile t;
-  t.run(pa, pb, cols, false, s0, s1);
+  t.run(pa, pb, min(cols, last * Tile::KS) - first * Tile::KS, false, s0, s1);
+  if (cuts > 1) {
+    f32x4* const to = slices + (int64_t)(blockIdx.x - turns.whole) * (BM * BN / 4) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < Tile::TM; ++i) {
+#pragma unroll
+      for (int j = 0; j < Tile::TN; ++j) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          to[((i * Tile::TN + j) * 4 + q) * (64 * Tile::kWaves)] =
+              f32x4{t.acc[i][j][4 * q], t.acc[i][j][4 * q + 1], t.acc[i][j][4 * q + 2], t.acc[i][j][4 * q + 3]};
+      }
+    }
+    return;
+  }
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
-  const int row0 = wave / WN * (BM / WM), col0 = wave % WN * (BN / WN);
   float* const own = reinterpret_cast<float*>(s0) + 1024 * wave;
   static_assert(Tile::kWaves * 2048 <= Tile::kStage, "room");
-  const T* const be = b != nullptr ? b + (int64_t)g.group * outs : nullptr;
 #pragma unroll
   for (int i = 0; i < Tile::TM; ++i) {
 #pragma unroll
-    for (int j = 0; j < Tile::TN; ++j) {
-      rows_of_tile<T>(t.acc[i][j], own, [&](int r, int c, float (&v)[V]) {
-        const int row = row0 + 32 * i + r, at = n0 + col0 + 32 * j + c;
-        if (row >= here || at >= outs) return;
-        finish<T>(v, be, mask != nullptr ? mask + (m0 + row) * outs : nullptr, relu, y + (m0 + row) * outs, at, outs);
-      });
+    for (int j = 0; j < Tile::TN; ++j)
+      put_rows<T>(t.acc[i][j], own, wave / WN * (BM / WM) + 32 * i, n0 + wave % WN * (BN / WN) + 32 * j, m0, here,
+                  b != nullptr ? b + (int64_t)g.group * outs : nullptr, mask, relu, y, outs);
+  }
+}
+
+// The cut tiles: slices added in their order.  Workgroup (tile, one 32 x 32 of each of its waves').
+template <class T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void k_group_rows_join(const T* __restrict__ b, const T* __restrict__ mask,
+                                                                  const int32_t* __restrict__ offsets,
+                                                                  T* __restrict__ y, int64_t slots, int experts,
+                                                                  int steps, int outs, bool relu, int nt, int room,
+                                                                  const f32x4* __restrict__ slices) {
+  constexpr int kWaves = WM * WN, TN = BN / WN / 32;
+  __shared__ __attribute__((aligned(16))) float room_of[kWaves][1024];
+  const int64_t mt = group_tiles(offsets, experts, slots, BM, true);
+  const Turns turns = turns_of((uint32_t)(mt * nt), (uint32_t)room, steps, true);
+  if (turns.slices == 1 || blockIdx.x >= turns.left) return;
+  GroupTile g;
+  int n;
+  if (!fast_tile(offsets, experts, slots, BM, nt, mt, turns.whole + blockIdx.x, g, n) || g.group == experts) return;
+  const int64_t m0 = g.lo + g.tile * BM;
+  const int n0 = n * BN, here = (int)min<int64_t>(BM, g.hi - m0), ij = (int)blockIdx.y;
+  const f32x4* from = slices + (int64_t)blockIdx.x * turns.slices * (BM * BN / 4) + (int64_t)ij * 4 * (64 * kWaves) + threadIdx.x;
+  f32x16 acc = f32x16{};
+#pragma unroll 4
+  for (uint32_t s = 0; s < turns.slices; ++s, from += BM * BN / 4) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 v = from[q * (64 * kWaves)];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[4 * q + e] += v[e];
     }
   }
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+  put_rows<T>(acc, room_of[wave], wave / WN * (BM / WM) + 32 * (ij / TN), n0 + wave % WN * (BN / WN) + 32 * (ij % TN), m0,
+              here, b != nullptr ? b + (int64_t)g.group * outs : nullptr, mask, relu, y, outs);
 }
 
 // The same for float32 rows as they are, on the float32 matrix cores.
@@ -558,7 +657,7 @@ GradPlan chosen_plan(int64_t slots, int experts, int64_t cols, int64_t outs, boo
 }  // namespace
 
 bool group_linear_fits(int64_t slots, int experts, int64_t cols, int64_t outs) {
-  const int64_t limit = (int64_t(1) << 32) / kGroupThreads - 8;  // threads a launch
+  const int64_t limit = (int64_t(1) << 32) / kGroupThreads - 512;  // threads a launch
   for (const int64_t n : {outs, cols}) {
     if (most_tiles(slots, experts + 1, kSide) * tiles_of(n, 32) >= limit) return false;
     if (slots <= 32 * (int64_t)experts && most_tiles(slots, experts + 1, 32) * tiles_of(n, kSide) >= limit) return false;
@@ -613,25 +712,60 @@ bool lays_out(int type, int64_t slots, int experts, int64_t cols, int64_t outs) 
   return slots * cols * outs >= (int64_t(1) << (type == SPHOPS_F32 ? 32 : 31));
 }
 
-// Tiles of a product over rows on the fast kernels.
-template <class T, bool BACK>
-void rows_fast(const Laid& x, const Laid& w, const T* b, const T* mask, const int32_t* offsets, T* y, int64_t slots,
-               int experts, int64_t cols, int64_t outs, bool relu, hipStream_t st) {
-  using E = Piece16<T>;
-  const auto with = [&](auto kernel, int bm, int bn, int threads) {
-    const int64_t tiles = most_tiles(slots, experts + 1, bm) * tiles_of(outs, bn);
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles_of(tiles, 8) * 8)) /* whole turns of the eight XCDs */,
-                       dim3(threads), 0, st, static_cast<const E*>(x.base), x.stride, x.plane,
-                       static_cast<const E*>(w.base), w.stride, w.plane, b, mask, offsets, y, slots, experts, (int)cols,
-                       (int)outs, relu, (int)tiles_of(outs, bn));
-  };
-  if constexpr (std::is_same_v<T, float>) {
-    if (slots / 256 * tiles_of(outs, 128) >= 192) with(k_group_rows_fast<T, BACK, 256, 128, 4, 2>, 256, 128, 512);
-    else with(k_group_rows_fast<T, BACK, 128, 128, 2, 2>, 128, 128, 256);
+// Tiles of a product over rows on the fast kernels: rows, columns, and how many
+// of their workgroups the card holds.
+struct FastPlan {
+  int bm, bn, room;
+  bool cut;
+  int64_t slices_bytes() const { return cut ? (int64_t)room * bm * bn * 4 : 0; }
+};
+FastPlan fast_plan(int type, int64_t slots, int experts, int64_t cols, int64_t outs) {
+  FastPlan p;
+  if (type == SPHOPS_F32) {
+    const bool tall = slots / 256 * tiles_of(outs, 128) >= 192;
+    p = FastPlan{tall ? 256 : 128, 128, 256, false};
   } else {
-    if (rows_side(slots, outs) == 256) with(k_group_rows_fast<T, BACK, 256, 256, 2, 4>, 256, 256, 512);
-    else with(k_group_rows_fast<T, BACK, 128, 128, 2, 2>, 128, 128, 256);
+    const bool large = rows_side(slots, outs) == 256;
+    p = FastPlan{large ? 256 : 128, large ? 256 : 128, large ? 256 : 512, false};
   }
+  // two slices at least, and more than a few rows an expert: then few tiles have a reader each
+  p.cut = cols >= 2 * kSliceSteps * (type == SPHOPS_F32 ? 32 : 64) && slots > 16 * (int64_t)experts;
+  return p;
+}
+int64_t fast_bytes(int type, int64_t slots, int experts, int64_t cols, int64_t outs) {
+  return fast_plan(type, slots, experts, cols, outs).slices_bytes();
+}
+
+template <class T, bool BACK>
+void rows_fast(Layouts& l, const Laid& x, const Laid& w, const T* b, const T* mask, const int32_t* offsets, T* y,
+               int64_t slots, int experts, int64_t cols, int64_t outs, bool relu, hipStream_t st) {
+  using E = Piece16<T>;
+  constexpr int type = std::is_same_v<T, float> ? SPHOPS_F32 : SPHOPS_BF16, KS = kPieces<T> == 3 ? 32 : 64;
+  const FastPlan p = fast_plan(type, slots, experts, cols, outs);
+  f32x4* const slices = p.cut ? reinterpret_cast<f32x4*>(l.work + l.take(p.slices_bytes())) : nullptr;
+  const int64_t tiles = most_tiles(slots, experts + 1, p.bm) * tiles_of(outs, p.bn);
+  const auto with = [&](auto bm, auto bn, auto wm, auto wn) {
+    constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
+    const int nt = (int)tiles_of(outs, BN);
+    hipLaunchKernelGGL((k_group_rows_fast<T, BACK, BM, BN, WM, WN>), dim3((uint32_t)(tiles + (p.cut ? p.room : 0))),
+                       dim3(64 * WM * WN), 0, st, static_cast<const E*>(x.base), x.stride, x.plane,
+                       static_cast<const E*>(w.base), w.stride, w.plane, b, mask, offsets, y, slots, experts, (int)cols,
+                       (int)outs, relu, nt, p.room, slices);
+    SPHOPS_LAUNCHED();
+    if (p.cut)
+      hipLaunchKernelGGL((k_group_rows_join<T, BM, BN, WM, WN>), dim3((uint32_t)(p.room / 2), BM / WM / 32 * (BN / WN / 32)),
+                         dim3(64 * WM * WN), 0, st, b, mask, offsets, y, slots, experts, (int)tiles_of(cols, KS),
+                         (int)outs, relu, nt, p.room, slices);
+  };
+#define SPHOPS_N(n) std::integral_constant<int, n>{}
+  if constexpr (std::is_same_v<T, float>) {
+    if (p.bm == 256) with(SPHOPS_N(256), SPHOPS_N(128), SPHOPS_N(4), SPHOPS_N(2));
+    else with(SPHOPS_N(128), SPHOPS_N(128), SPHOPS_N(2), SPHOPS_N(2));
+  } else {
+    if (p.bm == 256) with(SPHOPS_N(256), SPHOPS_N(256), SPHOPS_N(2), SPHOPS_N(4));
+    else with(SPHOPS_N(128), SPHOPS_N(128), SPHOPS_N(2), SPHOPS_N(2));
+  }
+#undef SPHOPS_N
 }
 
 // As they are.
@@ -661,10 +795,13 @@ bool fast_as_is(const void* x, int64_t xs, int64_t cols, const void* w, int64_t 
 }  // namespace
 
 int64_t group_linear_workspace_bytes(int type, int64_t slots, int experts, int64_t cols, int64_t outs) {
-  if (!lays_out(type, slots, experts, cols, outs)) return 0;
   Layouts l{nullptr};
-  l.take(Layouts::bytes_of(type, slots, cols));
-  l.take(Layouts::bytes_of(type, experts * outs, cols));
+  const bool laid = lays_out(type, slots, experts, cols, outs);
+  if (laid) {
+    l.take(Layouts::bytes_of(type, slots, cols));
+    l.take(Layouts::bytes_of(type, experts * outs, cols));
+  }
+  if (laid || type != SPHOPS_F32) l.take(fast_bytes(type, slots, experts, cols, outs));
   return l.used;
 }
 
@@ -681,7 +818,7 @@ void run_group_linear(const void* x, int type, int64_t xs, const void* w, const 
       Layouts l{static_cast<char*>(work)};
       const Laid lx = as_is ? Laid{x, xs, 0} : lay_out(l, px, xs, slots, cols, st);
       const Laid lw = as_is ? Laid{w, cols, 0} : lay_out(l, pw, cols, experts * outs, cols, st);
-      rows_fast<T, false>(lx, lw, pb, nullptr, offsets, py, slots, experts, cols, outs, relu, st);
+      rows_fast<T, false>(l, lx, lw, pb, nullptr, offsets, py, slots, experts, cols, outs, relu, st);
     } else {
       rows_plain<T, false>(px, xs, pw, pb, nullptr, offsets, py, slots, experts, cols, outs, relu, st);
     }
@@ -698,11 +835,13 @@ int64_t group_backward_workspace_bytes(int type, int64_t slots, int experts, int
     chunks = std::max(chunks, grad_plan(slots, experts, cols, outs, 256, 128).chunks);
   Layouts l{nullptr};
   l.take(chunks * (cols * outs + outs) * (int64_t)sizeof(float));
-  if (lays_out(type, slots, experts, cols, outs)) {
+  const bool laid = lays_out(type, slots, experts, cols, outs);
+  if (laid) {
     l.take(Layouts::bytes_of(type, slots, outs));
     l.take(Layouts::bytes_of(type, experts * outs, cols));
     l.take(Layouts::bytes_of(type, slots, cols));
   }
+  if (laid || type != SPHOPS_F32) l.take(fast_bytes(type, slots, experts, outs, cols));
   return l.used;
 }
 
@@ -730,7 +869,7 @@ void run_group_backward(const void* dy, int64_t dys, const void* x, int type, in
     if (dx != nullptr && slots > 0) {
       if (rows_as_is || laid) {
         const Laid lw = rows_as_is ? Laid{w, cols, 0} : lay_out(l, pw, cols, experts * outs, cols, st);
-        rows_fast<T, true>(ldy, lw, nullptr, pm, offsets, static_cast<T*>(dx), slots, experts, outs, cols, false, st);
+        rows_fast<T, true>(l, ldy, lw, nullptr, pm, offsets, static_cast<T*>(dx), slots, experts, outs, cols, false, st);
       } else {
         rows_plain<T, true>(pdy, dys, pw, nullptr, pm, offsets, static_cast<T*>(dx), slots, experts, outs, cols, false, st);
       }
