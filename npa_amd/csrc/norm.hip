@@ -22,6 +22,34 @@ __device__ __forceinline__ float weight_at(const void* __restrict__ w, bool wide
   return wide ? static_cast<const float*>(w)[k] : to_f32(static_cast<const T*>(w)[k]);
 }
 
+// V of them from k on, `fill` past the row's end and everywhere without weights.
+template <class T>
+__device__ __forceinline__ void weights_at(const void* __restrict__ w, bool wide, int k, int cols, float fill,
+                                           float (&out)[Piece<T>::V]) {
+  constexpr int V = Piece<T>::V;
+#pragma unroll
+  for (int j = 0; j < V; ++j) out[j] = fill;
+  if (w == nullptr || k >= cols) return;
+  if (k + V > cols) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (k + j < cols) out[j] = weight_at<T>(w, wide, k + j);
+  } else if (wide) {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      Piece<float> p;
+      p.load(static_cast<const float*>(w), k + 4 * i, cols);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) out[4 * i + j] = p.get(j);
+    }
+  } else {
+    Piece<T> p;
+    p.load(static_cast<const T*>(w), k, cols);
+#pragma unroll
+    for (int j = 0; j < V; ++j) out[j] = p.get(j);
+  }
+}
+
 // Sums of a row's L lanes, K of them at a time, in every lane.  L > 64: a row's
 // waves meet in LDS, two sets in turn (a wave writes a set again only after the
 // other turn's barrier).
@@ -52,6 +80,59 @@ struct RowSums {
   }
 };
 
+template <class T>
+__device__ __forceinline__ void load_piece(Piece<T>& p, bool whole, const T* __restrict__ row, int k, int cols) {
+  if (whole) p.raw = *reinterpret_cast<const typename Piece<T>::Raw*>(row + k);
+  else p.load(row, k, cols);
+}
+
+// A wave's rows on their way out, which stand one after another in memory: short
+// ones (up to 16 lanes each) go through LDS of the wave's own and leave in whole
+// runs of 1024 bytes, whatever the row's length.
+template <class T, int L, int N>
+struct RowsOut {
+  static constexpr bool kStaged = L <= 16;
+  static constexpr int V = Piece<T>::V;
+  uint32_t words[kStaged ? N * 256 : 1];
+  // o: the lane's pieces of row `first` + lane / L of y; rows from `rows` on are not written
+  __device__ __forceinline__ void operator()(const Piece<T> (&o)[N], T* __restrict__ y, int64_t first, int64_t rows,
+                                             int cols) {
+    const int lane = threadIdx.x & 63, l = threadIdx.x % L;
+    if (kStaged && (sizeof(T) == 4 || cols % 2 == 0)) {  // words of LDS stay whole
+      T* const own = reinterpret_cast<T*>(words);
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int k = (n * L + l) * V, at = ((lane / L) * cols + k) * (int)sizeof(T) / 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n < N - 1 || k + j * V / 4 < cols) words[at + j] = o[n].raw.w[j];
+      }
+      __builtin_amdgcn_wave_barrier();
+      const int64_t left = rows - first;
+      const int all = (int)(left < 0 ? 0 : left < 64 / L ? left : 64 / L) * cols;
+      T* const to = y + first * cols;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int k = (n * 64 + lane) * V;
+        if (k >= all) continue;
+        Piece<T> p;
+        __builtin_memcpy(&p.raw, own + k, 16);
+        p.store(to, k, all);
+      }
+    } else {
+      const int64_t r = first + lane / L;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int k = (n * L + l) * V;
+        if (r >= rows) continue;
+        if (n < N - 1) *reinterpret_cast<typename Piece<T>::Raw*>(y + r * cols + k) = o[n].raw;
+        else o[n].store(y + r * cols, k, cols);
+      }
+    }
+  }
+};
+
 // L lanes a row, which they hold in N pieces of 16 bytes each: the row is read
 // once.  A lane keeps its columns' weights over all of its rows.
 template <class T, int L, int N, int TH>
@@ -62,25 +143,29 @@ __global__ __launch_bounds__(TH) void k_norm_forward(const T* __restrict__ x, in
   constexpr int V = Piece<T>::V, kRows = TH / L;
   __shared__ RowSums<L, 1, TH> sum1;
   __shared__ RowSums<L, 2, TH> sum2;
+  __shared__ __attribute__((aligned(16))) RowsOut<T, L, N> outs[TH / 64];
   const int l = threadIdx.x % L;
   const float inv = 1.0f / (float)cols;
-  int turn1 = 0, turn2 = 0;
+  int turn1 = 0, turn2 = 0;  // of the sums
   float ww[N][V], bb[N][V];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int k = (n * L + l) * V + j;
-      ww[n][j] = w != nullptr && k < cols ? weight_at<T>(w, wide, k) : 1.0f;
-      bb[n][j] = b != nullptr && k < cols ? weight_at<T>(b, wide, k) : 0.0f;
-    }
+    weights_at<T>(w, wide, (n * L + l) * V, cols, 1.0f, ww[n]);
+    weights_at<T>(b, wide, (n * L + l) * V, cols, 0.0f, bb[n]);
   }
-  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += (int64_t)gridDim.x * kRows) {
+  const int64_t turn = (int64_t)gridDim.x * kRows;
+  Piece<T> p[N], next[N];
+  auto load = [&](int64_t r0, Piece<T> (&to)[N]) {
     const int64_t r = min<int64_t>(r0 + threadIdx.x / L, rows - 1);  // lanes past the last row do it again
-    const T* __restrict__ row = x + r * stride;
-    Piece<T> p[N];
 #pragma unroll
-    for (int n = 0; n < N; ++n) p[n].load(row, (n * L + l) * V, cols);
+    for (int n = 0; n < N; ++n) load_piece(to[n], n < N - 1, x + r * stride, (n * L + l) * V, cols);
+  };
+  load((int64_t)blockIdx.x * kRows, next);
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += turn) {
+    const int64_t r = min<int64_t>(r0 + threadIdx.x / L, rows - 1);
+#pragma unroll
+    for (int n = 0; n < N; ++n) p[n] = next[n];
+    load(r0 + turn, next);  // in flight under this turn's sums
     float s[1] = {0.0f};
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -94,7 +179,8 @@ __global__ __launch_bounds__(TH) void k_norm_forward(const T* __restrict__ x, in
     for (int n = 0; n < N; ++n) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = (n * L + l) * V + j < cols ? p[n].get(j) - c : 0.0f;
+        // only the last pieces reach past the row's end (with_lanes)
+        const float d = n < N - 1 || (n * L + l) * V + j < cols ? p[n].get(j) - c : 0.0f;
         q[0] += d;
         q[1] += d * d;
       }
@@ -103,14 +189,16 @@ __global__ __launch_bounds__(TH) void k_norm_forward(const T* __restrict__ x, in
     const float e = q[0] * inv, var = fmaxf(q[1] * inv - e * e, 0.0f);
     const float rstd = 1.0f / sqrtf((q[1] != q[1] ? q[1] : var) + eps);  // fmaxf drops a NaN
     if (stats != nullptr && l == 0) stats[r] = float2{c, rstd};
+    Piece<T> o[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int k = (n * L + l) * V;
-      Piece<T> o = p[n];
+      float v[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) o.set(j, from_f32<T>((p[n].get(j) - c - e) * rstd * ww[n][j] + bb[n][j]));
-      o.store(y + r * cols, k, cols);
+      for (int j = 0; j < V; ++j) v[j] = (p[n].get(j) - c - e) * rstd * ww[n][j] + bb[n][j];
+      o[n] = piece_of<T>(v);
     }
+    const int wave = (int)threadIdx.x / 64;
+    outs[wave](o, y, r0 + wave * 64 / L, rows, cols);
   }
 }
 
@@ -173,44 +261,53 @@ __global__ __launch_bounds__(kLongThreads) void k_norm_forward_long(const T* __r
 // its rows, the workgroup's rows meet in LDS and leave as one row of `part`
 // (2 x cols: dw, then db), in a fixed order.
 template <class T, int L, int N, int TH>
-__global__ __launch_bounds__(TH) void k_norm_backward(const T* __restrict__ x, int64_t stride,
+__global__ __launch_bounds__(TH, N * Piece<T>::V <= 12 ? 4 : 2) void k_norm_backward(const T* __restrict__ x, int64_t stride,
                                                       const T* __restrict__ dy, int64_t dy_stride,
                                                       const void* __restrict__ w, bool wide,
                                                       const float2* __restrict__ stats, T* __restrict__ dx,
                                                       float* __restrict__ part, int64_t rows, int cols) {
   constexpr int V = Piece<T>::V, kRows = TH / L;
   __shared__ RowSums<L, 3, TH> sums;
+  __shared__ __attribute__((aligned(16))) RowsOut<T, L, N> outs[TH / 64];
   const int l = threadIdx.x % L;
   const float inv = 1.0f / (float)cols;
   int turn = 0;
   float ww[N][V], dw[N][V], db[N][V];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
+    weights_at<T>(w, wide, (n * L + l) * V, cols, 1.0f, ww[n]);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int k = (n * L + l) * V + j;
-      ww[n][j] = w != nullptr && k < cols ? weight_at<T>(w, wide, k) : 1.0f;
-      dw[n][j] = db[n][j] = 0.0f;
-    }
+    for (int j = 0; j < V; ++j) dw[n][j] = db[n][j] = 0.0f;
   }
-  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += (int64_t)gridDim.x * kRows) {
-    const bool live = r0 + threadIdx.x / L < rows;
-    const int64_t r = live ? r0 + threadIdx.x / L : rows - 1;
-    const T* __restrict__ row = x + r * stride;
-    const T* __restrict__ up = dy + r * dy_stride;
-    Piece<T> p[N], u[N];
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  Piece<T> p[N], u[N], pn[N], un[N];
+  float2 sn;
+  auto load = [&](int64_t r0) {
+    const int64_t r = min<int64_t>(r0 + threadIdx.x / L, rows - 1);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      p[n].load(row, (n * L + l) * V, cols);
-      u[n].load(up, (n * L + l) * V, cols);
+      load_piece(pn[n], n < N - 1, x + r * stride, (n * L + l) * V, cols);
+      load_piece(un[n], n < N - 1, dy + r * dy_stride, (n * L + l) * V, cols);
     }
-    const float2 st = stats[r];
+    sn = stats[r];
+  };
+  load((int64_t)blockIdx.x * kRows);
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += step) {
+    const bool live = r0 + threadIdx.x / L < rows;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      p[n] = pn[n];
+      u[n] = un[n];
+    }
+    const float2 st = sn;
+    load(r0 + step);  // in flight under this turn's sums
     float s[3] = {0.0f, 0.0f, 0.0f};  // of d, g and g d
 #pragma unroll
     for (int n = 0; n < N; ++n) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = (n * L + l) * V + j < cols ? p[n].get(j) - st.x : 0.0f, g = u[n].get(j) * ww[n][j];
+        const float d = n < N - 1 || (n * L + l) * V + j < cols ? p[n].get(j) - st.x : 0.0f;
+        const float g = u[n].get(j) * ww[n][j];
         s[0] += d;
         s[1] += g;
         s[2] += g * d;
@@ -218,20 +315,23 @@ __global__ __launch_bounds__(TH) void k_norm_backward(const T* __restrict__ x, i
     }
     sums(s, turn);
     const float e = s[0] * inv, mg = s[1] * inv, mgh = (s[2] - e * s[1]) * inv * st.y;
+    Piece<T> o[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      Piece<T> o = p[n];
+      float v[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float h = (p[n].get(j) - st.x - e) * st.y, up = u[n].get(j);
-        o.set(j, from_f32<T>(st.y * (up * ww[n][j] - mg - h * mgh)));
+        v[j] = st.y * (up * ww[n][j] - mg - h * mgh);
         if (live) {
           dw[n][j] += up * h;
           db[n][j] += up;
         }
       }
-      if (dx != nullptr) o.store(dx + r * cols, (n * L + l) * V, cols);
+      o[n] = piece_of<T>(v);
     }
+    const int wave = (int)threadIdx.x / 64;
+    if (dx != nullptr) outs[wave](o, dx, r0 + wave * 64 / L, rows, cols);
   }
   if (part == nullptr) return;
   float* __restrict__ to = part + (int64_t)blockIdx.x * 2 * cols;
@@ -367,7 +467,8 @@ __global__ __launch_bounds__(1024) void k_norm_column_sum(const float* __restric
 }
 
 // f(integral_constants L, N) for rows of `pieces` 16-byte pieces; false: longer
-// than all of them.
+// than all of them.  A row has more than L (N - 1) pieces, so only the last of a
+// lane's reach past its end.
 template <class F>
 bool with_lanes(int64_t pieces, F&& f) {
   auto at = [&](auto l, auto n) {

@@ -7,6 +7,8 @@
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
+#include <type_traits>
+
 namespace sphops {
 
 // Rows whose largest value is smaller are held against this one: 127 / m and
@@ -124,6 +126,24 @@ struct Piece {
     }
   }
 };
+
+// Floats as a piece, each rounded once to the nearest, two at a time.
+template <class T>
+__device__ __forceinline__ Piece<T> piece_of(const float (&v)[Piece<T>::V]) {
+  Piece<T> p;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p.raw.w[j] = __builtin_bit_cast(uint32_t, v[j]);
+  } else {
+    using E = std::conditional_t<std::is_same_v<T, __half>, _Float16, __bf16>;
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef E e16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      p.raw.w[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[2 * j], v[2 * j + 1]}), e16x2));
+  }
+  return p;
+}
 
 template <bool RELU>
 __device__ __forceinline__ uint32_t top_of(uint32_t top, float v) {
