@@ -83,7 +83,8 @@ struct RowSums {
 template <class T>
 __device__ __forceinline__ void load_piece(Piece<T>& p, bool whole, const T* __restrict__ row, int k, int cols) {
   if (whole) p.raw = *reinterpret_cast<const typename Piece<T>::Raw*>(row + k);
-  else p.load(row, k, cols);
+  else if (k < cols) p.load(row, k, cols);
+  else p.raw = typename Piece<T>::Raw{};
 }
 
 // A wave's rows on their way out, which stand one after another in memory: short
@@ -127,7 +128,7 @@ struct RowsOut {
         const int k = (n * L + l) * V;
         if (r >= rows) continue;
         if (n < N - 1) *reinterpret_cast<typename Piece<T>::Raw*>(y + r * cols + k) = o[n].raw;
-        else o[n].store(y + r * cols, k, cols);
+        else if (k < cols) o[n].store(y + r * cols, k, cols);
       }
     }
   }
@@ -189,12 +190,13 @@ __global__ __launch_bounds__(TH) void k_norm_forward(const T* __restrict__ x, in
     const float e = q[0] * inv, var = fmaxf(q[1] * inv - e * e, 0.0f);
     const float rstd = 1.0f / sqrtf((q[1] != q[1] ? q[1] : var) + eps);  // fmaxf drops a NaN
     if (stats != nullptr && l == 0) stats[r] = float2{c, rstd};
+    const float er = e * rstd;
     Piece<T> o[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       float v[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = (p[n].get(j) - c - e) * rstd * ww[n][j] + bb[n][j];
+      for (int j = 0; j < V; ++j) v[j] = ((p[n].get(j) - c) * rstd - er) * ww[n][j] + bb[n][j];
       o[n] = piece_of<T>(v);
     }
     const int wave = (int)threadIdx.x / 64;
@@ -315,14 +317,15 @@ __global__ __launch_bounds__(TH, N * Piece<T>::V <= 12 ? 4 : 2) void k_norm_back
     }
     sums(s, turn);
     const float e = s[0] * inv, mg = s[1] * inv, mgh = (s[2] - e * s[1]) * inv * st.y;
+    const float er = e * st.y, mgr = mg * st.y, mghr = mgh * st.y;
     Piece<T> o[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       float v[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float h = (p[n].get(j) - st.x - e) * st.y, up = u[n].get(j);
-        v[j] = st.y * (up * ww[n][j] - mg - h * mgh);
+        const float h = (p[n].get(j) - st.x) * st.y - er, up = u[n].get(j);
+        v[j] = (up * ww[n][j]) * st.y - mgr - h * mghr;
         if (live) {
           dw[n][j] += up * h;
           db[n][j] += up;
@@ -487,13 +490,15 @@ bool with_lanes(int64_t pieces, F&& f) {
 constexpr int kForwardGroups = 2048;  // workgroups that keep their weights over many rows
 constexpr int kBackwardGroups = 512;  // rows of `part`
 constexpr int64_t kLongChunk = 64;
+// Threads of a backward's workgroup: several rows, or one (whose barriers then hold up no other).
+constexpr int backward_threads(int l) { return l > 64 ? l : 512; }
 
 template <class T>
 int64_t norm_chunks(int64_t rows, int64_t cols) {
   const int64_t pieces = (cols + Piece<T>::V - 1) / Piece<T>::V;
   int64_t chunks = 0;
   const bool held = with_lanes(pieces, [&](auto l, auto) {
-    constexpr int kRows = 512 / decltype(l)::value;
+    constexpr int kRows = backward_threads(decltype(l)::value) / decltype(l)::value;
     chunks = std::min<int64_t>((rows + kRows - 1) / kRows, kBackwardGroups);
   });
   if (!held) chunks = std::min<int64_t>((rows + kLongChunk - 1) / kLongChunk, kBackwardGroups);
@@ -545,8 +550,8 @@ void run_layer_norm_backward(const void* x, int64_t stride, const void* dy, int6
     float2* const ps = reinterpret_cast<float2*>(const_cast<float*>(stats));
     if (rows > 0) {
       const bool held = with_lanes(pieces, [&](auto l, auto n) {
-        constexpr int L = decltype(l)::value;
-        hipLaunchKernelGGL((k_norm_backward<T, L, decltype(n)::value, 512>), dim3((uint32_t)chunks), dim3(512), 0, st,
+        constexpr int L = decltype(l)::value, TH = backward_threads(L);
+        hipLaunchKernelGGL((k_norm_backward<T, L, decltype(n)::value, TH>), dim3((uint32_t)chunks), dim3(TH), 0, st,
                            px, stride, pdy, dy_stride, w, wide, ps, static_cast<T*>(dx), sums ? work : nullptr, rows,
                            (int)cols);
       });
