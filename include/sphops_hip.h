@@ -642,9 +642,9 @@ int sphops_sort_rows(const void* index, int wide, int64_t rows, int choices, int
 int64_t sphops_sort_rows_workspace_bytes(int64_t rows, int choices, int experts);
 /* out (rows x choices places, dense): each row of x (rows, row_stride elements
  * apart) at its entries' places, zeros at the places of entries without an
- * expert. */
-int sphops_dispatch_rows(const void* x, int type, int64_t row_stride, const int32_t* slot, void* out, int64_t rows,
-                         int choices, int64_t cols, void* stream);
+ * expert.  source may be NULL. */
+int sphops_dispatch_rows(const void* x, int type, int64_t row_stride, const int32_t* slot, const int32_t* source,
+                         void* out, int64_t rows, int choices, int64_t cols, void* stream);
 /* y (rows, dense): the sum over a row's entries, in their order and in float32,
  * of w (rows x choices; NULL: 1) times the place's row of results (dense);
  * entries without an expert are left out.  With w NULL it is the gradient of
@@ -652,11 +652,11 @@ int sphops_dispatch_rows(const void* x, int type, int64_t row_stride, const int3
 int sphops_combine_rows(const void* results, int type, const float* w, const int32_t* slot, void* y, int64_t rows,
                         int choices, int64_t cols, void* stream);
 /* Its gradients: d_results (places; zeros for entries without an expert) and dw
- * (rows x choices; 0 for them); each may be NULL, and results and w with dw and
- * d_results. */
+ * (rows x choices; 0 for them); each may be NULL, and so may w (1), source, and
+ * results without dw. */
 int sphops_combine_rows_backward(const void* dy, int type, int64_t row_stride, const void* results, const float* w,
-                                 const int32_t* slot, void* d_results, float* dw, int64_t rows, int choices,
-                                 int64_t cols, void* stream);
+                                 const int32_t* slot, const int32_t* source, void* d_results, float* dw, int64_t rows,
+                                 int choices, int64_t cols, void* stream);
 
 /*
  * A linear layer for each of `experts` experts over slots rows sorted by expert

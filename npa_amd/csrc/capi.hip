@@ -1566,13 +1566,13 @@ int sphops_sort_rows(const void* index, int wide, int64_t rows, int choices, int
   });
 }
 
-int sphops_dispatch_rows(const void* x, int type, int64_t row_stride, const int32_t* slot, void* out, int64_t rows,
-                         int choices, int64_t cols, void* stream) {
+int sphops_dispatch_rows(const void* x, int type, int64_t row_stride, const int32_t* slot, const int32_t* source,
+                         void* out, int64_t rows, int choices, int64_t cols, void* stream) {
   return guarded([&] {
     require_sorted(type, rows, choices, cols);
     require(rows <= 1 || row_stride >= 0, "row_stride must be >= 0");
     require(rows == 0 || (x && slot && out), "null buffer");
-    sphops::run_dispatch_rows(x, type, row_stride, slot, out, rows, choices, cols, sphops::as_stream(stream));
+    sphops::run_dispatch_rows(x, type, row_stride, slot, source, out, rows, choices, cols, sphops::as_stream(stream));
   });
 }
 
@@ -1586,14 +1586,14 @@ int sphops_combine_rows(const void* results, int type, const float* w, const int
 }
 
 int sphops_combine_rows_backward(const void* dy, int type, int64_t row_stride, const void* results, const float* w,
-                                 const int32_t* slot, void* d_results, float* dw, int64_t rows, int choices,
-                                 int64_t cols, void* stream) {
+                                 const int32_t* slot, const int32_t* source, void* d_results, float* dw, int64_t rows,
+                                 int choices, int64_t cols, void* stream) {
   return guarded([&] {
     require_sorted(type, rows, choices, cols);
     require(rows <= 1 || row_stride >= 0, "row_stride must be >= 0");
     require(rows == 0 || (dy && slot && (dw == nullptr || results)), "null buffer");
-    sphops::run_combine_rows_backward(dy, type, row_stride, results, w, slot, d_results, dw, rows, choices, cols,
-                                      sphops::as_stream(stream));
+    sphops::run_combine_rows_backward(dy, type, row_stride, results, w, slot, source, d_results, dw, rows,
+                                      choices, cols, sphops::as_stream(stream));
   });
 }
 

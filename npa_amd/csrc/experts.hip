@@ -6,7 +6,7 @@
 // into their entries' places, and the experts' results come back as the sum
 // over a row's entries of weight times result.  Nothing is added by atomics on
 // floats: a row's entries are summed in their order.
-#include "rows8.hpp"
+#include "rows_out.hpp"
 
 #include <type_traits>
 
@@ -189,10 +189,10 @@ constexpr int kMoveThreads = 256;
 // Values of a row's piece times w, each rounded once.
 template <class T>
 __device__ __forceinline__ Piece<T> scaled(const Piece<T>& p, float w) {
-  Piece<T> o = p;
+  float v[Piece<T>::V];
 #pragma unroll
-  for (int j = 0; j < Piece<T>::V; ++j) o.set(j, from_f32<T>(p.get(j) * w));
-  return o;
+  for (int j = 0; j < Piece<T>::V; ++j) v[j] = p.get(j) * w;
+  return piece_of<T>(v);
 }
 
 // out[slot[r, j]] = x[r], zeros for an entry without an expert.  L lanes a row's
@@ -295,11 +295,12 @@ __global__ __launch_bounds__(kMoveThreads) void k_rows_in(const T* __restrict__ 
                                                           const float* __restrict__ w,
                                                           const int32_t* __restrict__ slot, T* __restrict__ y,
                                                           int64_t rows, int choices, int cols) {
-  constexpr int V = Piece<T>::V;
-  const int l = threadIdx.x % L, k0 = (int)blockIdx.y * L * N * V;
+  constexpr int V = Piece<T>::V, kRows = kMoveThreads / L;
+  __shared__ __attribute__((aligned(16))) RowsOut<T, L, N> outs[kMoveThreads / 64];
+  const int l = threadIdx.x % L, k0 = (int)blockIdx.y * L * N * V, wave = (int)threadIdx.x / 64;
   const int64_t slots = rows * choices;
-  for (int64_t r = (int64_t)blockIdx.x * (kMoveThreads / L) + threadIdx.x / L; r < rows;
-       r += (int64_t)gridDim.x * (kMoveThreads / L)) {
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += (int64_t)gridDim.x * kRows) {
+    const int64_t r = min<int64_t>(r0 + threadIdx.x / L, rows - 1);
     float sum[N][V];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -314,18 +315,71 @@ __global__ __launch_bounds__(kMoveThreads) void k_rows_in(const T* __restrict__ 
 #pragma unroll
       for (int n = 0; n < N; ++n) {
         Piece<T> p;
-        p.load(results + (int64_t)s * stride, k0 + (n * L + l) * V, cols);
+        load_piece(p, false, results + (int64_t)s * stride, k0 + (n * L + l) * V, cols);
 #pragma unroll
         for (int v = 0; v < V; ++v) sum[n][v] += weight * p.get(v);
       }
     }
+    Piece<T> o[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) o[n] = piece_of<T>(sum[n]);
+    if (RowsOut<T, L, N>::kStaged) {  // one block of columns
+      outs[wave](o, y, r0 + wave * 64 / L, rows, cols);
+    } else if (r0 + threadIdx.x / L < rows) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int k = k0 + (n * L + l) * V;
+        if (k < cols) o[n].store(y + r * cols, k, cols);
+      }
+    }
+  }
+}
+
+// k_rows_out and k_rows_in_backward over the places, for rows that have one entry
+// each and few values: out[p] = w[r] x[r] for the row r = source[p] (w null: 1; zeros
+// without an expert) and dw[r] = results[p] . x[r] (dw null: not wanted).  What is
+// written lies in order and leaves in whole runs: 2^20 x 83 float32 out 175 us row by
+// row, 1 so.
+template <class T, int L, int N>
+__global__ __launch_bounds__(kMoveThreads) void k_places_out(const T* __restrict__ x, int64_t stride,
+                                                             const T* __restrict__ results,
+                                                             const float* __restrict__ w,
+                                                             const int32_t* __restrict__ slot,
+                                                             const int32_t* __restrict__ source, T* __restrict__ out,
+                                                             float* __restrict__ dw, int64_t places, int cols) {
+  constexpr int V = Piece<T>::V, kRows = kMoveThreads / L;
+  __shared__ __attribute__((aligned(16))) RowsOut<T, L, N> outs[kMoveThreads / 64];
+  const int l = threadIdx.x % L, wave = (int)threadIdx.x / 64;
+  for (int64_t p0 = (int64_t)blockIdx.x * kRows; p0 < places; p0 += (int64_t)gridDim.x * kRows) {
+    const int64_t p = min<int64_t>(p0 + threadIdx.x / L, places - 1);
+    const int32_t from = source[p];
+    const bool known = from >= 0 && from < places, has = known && slot[known ? from : 0] == (int32_t)p;
+    const int64_t r = known ? from : 0;
+    const float weight = has && w != nullptr ? w[r] : 1.0f;
+    Piece<T> v[N], q[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      Piece<T> o;
-      o.raw = typename Piece<T>::Raw{};
+      load_piece(v[n], n < N - 1, x + r * stride, (n * L + l) * V, cols);
+      if (dw != nullptr) load_piece(q[n], n < N - 1, results + p * cols, (n * L + l) * V, cols);
+    }
+    if (dw != nullptr) {
+      float dot = 0.0f;
 #pragma unroll
-      for (int v = 0; v < V; ++v) o.set(v, from_f32<T>(sum[n][v]));
-      o.store(y + r * cols, k0 + (n * L + l) * V, cols);
+      for (int n = 0; n < N; ++n) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) dot += v[n].get(j) * q[n].get(j);
+      }
+#pragma unroll
+      for (int d = 1; d < L; d *= 2) dot += __shfl_xor(dot, d);
+      if (l == 0 && known) dw[r] = has ? dot : 0.0f;
+    }
+    if (out != nullptr) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        if (w != nullptr) v[n] = scaled(v[n], weight);
+        if (!has) v[n].raw = typename Piece<T>::Raw{};
+      }
+      outs[wave](v, out, p0 + wave * 64 / L, places, cols);
     }
   }
 }
@@ -360,13 +414,42 @@ int key_bits(int experts) {
   return bits;
 }
 
-int64_t sort_tiles(int64_t n) { return n <= 4 * kSortTile ? 1 : (n + kSortTile - 1) / kSortTile; }
+int64_t sort_tiles(int64_t n) { return (n + kSortTile - 1) / kSortTile; }
+
+// Rows of one entry each that k_places_out takes.
+template <class T>
+bool by_places(int choices, const int32_t* source, int64_t cols) {
+  return choices == 1 && source != nullptr && pieces_of<T>(cols) <= 48;
+}
+// f(integral_constants L, N) for them.
+template <class F>
+void with_place_lanes(int64_t pieces, F&& f) {
+#define SPHOPS_LANES(L, N) f(std::integral_constant<int, L>{}, std::integral_constant<int, N>{})
+  if (pieces <= 4) SPHOPS_LANES(4, 1);
+  else if (pieces <= 8) SPHOPS_LANES(8, 1);
+  else if (pieces <= 16) SPHOPS_LANES(8, 2);
+  else if (pieces <= 24) SPHOPS_LANES(8, 3);
+  else if (pieces <= 32) SPHOPS_LANES(16, 2);
+  else SPHOPS_LANES(16, 3);
+#undef SPHOPS_LANES
+}
+
+template <class T>
+void launch_places(const void* x, int64_t stride, const void* results, const float* w, const int32_t* slot,
+                   const int32_t* source, void* out, float* dw, int64_t places, int64_t cols, hipStream_t st) {
+  with_place_lanes(pieces_of<T>(cols), [&](auto l, auto n) {
+    constexpr int L = decltype(l)::value;
+    hipLaunchKernelGGL((k_places_out<T, L, decltype(n)::value>), move_grid(places, kMoveThreads / L, 1),
+                       dim3(kMoveThreads), 0, st, static_cast<const T*>(x), stride, static_cast<const T*>(results), w,
+                       slot, source, static_cast<T*>(out), dw, places, (int)cols);
+  });
+}
 
 }  // namespace
 
 int64_t sort_rows_workspace_words(int64_t n, int experts) {
   const int64_t tiles = sort_tiles(n);
-  return tiles == 1 ? 0 : (tiles + 1) * (experts + 1);
+  return tiles <= 1 ? 0 : (tiles + 1) * (experts + 1);
 }
 
 void run_sort_rows(const void* index, bool wide, int64_t n, int experts, int32_t* offsets, int32_t* slot,
@@ -375,13 +458,12 @@ void run_sort_rows(const void* index, bool wide, int64_t n, int experts, int32_t
   const uint32_t lds = (uint32_t)((kSortWaves + 1) * (experts + 1) * sizeof(uint32_t));
   const int64_t tiles = sort_tiles(n);
   auto place = [&](auto items, const uint32_t* hist, const uint32_t* totals) {
-    hipLaunchKernelGGL((k_sort_place<decltype(items)::value>), dim3((uint32_t)tiles), dim3(kSortThreads), lds, st,
+    hipLaunchKernelGGL((k_sort_place<decltype(items)::value>), dim3((uint32_t)std::max<int64_t>(tiles, 1)), dim3(kSortThreads), lds, st,
                        index, wide, n, experts, bits, hist, totals, offsets, slot, source);
   };
-  if (tiles == 1) {
+  if (tiles <= 1) {
     if (n <= kSortThreads) place(std::integral_constant<int, 1>{}, nullptr, nullptr);
-    else if (n <= kSortTile) place(std::integral_constant<int, kTileItems>{}, nullptr, nullptr);
-    else place(std::integral_constant<int, 4 * kTileItems>{}, nullptr, nullptr);
+    else place(std::integral_constant<int, kTileItems>{}, nullptr, nullptr);
     SPHOPS_LAUNCHED();
     return;
   }
@@ -395,11 +477,15 @@ void run_sort_rows(const void* index, bool wide, int64_t n, int experts, int32_t
   SPHOPS_LAUNCHED();
 }
 
-void run_dispatch_rows(const void* x, int type, int64_t stride, const int32_t* slot, void* out, int64_t rows,
-                       int choices, int64_t cols, hipStream_t st) {
+void run_dispatch_rows(const void* x, int type, int64_t stride, const int32_t* slot, const int32_t* source, void* out,
+                       int64_t rows, int choices, int64_t cols, hipStream_t st) {
   if (rows == 0) return;
   with_type(type, [&](auto t) {
     using T = decltype(t);
+    if (by_places<T>(choices, source, cols)) {
+      launch_places<T>(x, stride, nullptr, nullptr, slot, source, out, nullptr, rows, cols, st);
+      return;
+    }
     with_lanes(pieces_of<T>(cols), [&](auto l, auto n) {
       constexpr int L = decltype(l)::value, N = decltype(n)::value, V = Piece<T>::V;
       hipLaunchKernelGGL((k_rows_out<T, L, N>), move_grid(rows, kMoveThreads / L, (cols + L * N * V - 1) / (L * N * V)),
@@ -426,11 +512,15 @@ void run_combine_rows(const void* results, int type, int64_t stride, const float
 }
 
 void run_combine_rows_backward(const void* dy, int type, int64_t stride, const void* results, const float* w,
-                               const int32_t* slot, void* d_results, float* dw, int64_t rows, int choices,
-                               int64_t cols, hipStream_t st) {
+                               const int32_t* slot, const int32_t* source, void* d_results, float* dw, int64_t rows,
+                               int choices, int64_t cols, hipStream_t st) {
   if (rows == 0) return;
   with_type(type, [&](auto t) {
     using T = decltype(t);
+    if (by_places<T>(choices, source, cols)) {
+      launch_places<T>(dy, stride, results, w, slot, source, d_results, dw, rows, cols, st);
+      return;
+    }
     const int64_t pieces = pieces_of<T>(cols);
     auto launch = [&](auto l, auto n, auto held) {
       constexpr int L = decltype(l)::value;

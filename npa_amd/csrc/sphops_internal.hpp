@@ -416,13 +416,14 @@ constexpr int64_t kMaxSlots = int64_t(1) << 30;
 int64_t sort_rows_workspace_words(int64_t n, int experts);
 void run_sort_rows(const void* index, bool wide, int64_t n, int experts, int32_t* offsets, int32_t* slot,
                    int32_t* source, uint32_t* work, hipStream_t st);
-void run_dispatch_rows(const void* x, int type, int64_t stride, const int32_t* slot, void* out, int64_t rows,
-                       int choices, int64_t cols, hipStream_t st);
+// source (or null) lets rows of one entry each be written in order
+void run_dispatch_rows(const void* x, int type, int64_t stride, const int32_t* slot, const int32_t* source, void* out,
+                       int64_t rows, int choices, int64_t cols, hipStream_t st);
 void run_combine_rows(const void* results, int type, int64_t stride, const float* w, const int32_t* slot, void* y,
                       int64_t rows, int choices, int64_t cols, hipStream_t st);
 void run_combine_rows_backward(const void* dy, int type, int64_t stride, const void* results, const float* w,
-                               const int32_t* slot, void* d_results, float* dw, int64_t rows, int choices,
-                               int64_t cols, hipStream_t st);
+                               const int32_t* slot, const int32_t* source, void* d_results, float* dw, int64_t rows,
+                               int choices, int64_t cols, hipStream_t st);
 // grouped.hip: linear layers of experts over sorted rows
 constexpr int64_t kMaxGroupCols = 65536;
 bool group_linear_fits(int64_t slots, int experts, int64_t cols, int64_t outs);

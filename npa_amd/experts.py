@@ -69,13 +69,19 @@ def sort_rows(index, experts):
 
 
 def _check_slot(routing, device):
-    slot = routing.slot
+    """slot, source, rows and entries a row."""
+    slot, source = routing.slot, routing.source
     if slot.dtype != torch.int32 or slot.device != device:
         raise TypeError(f"routing must hold int32 tensors on {device}")
     if slot.dim() < 1 or not 1 <= slot.shape[-1] <= MAX_CHOICES or not slot.is_contiguous():
         raise RuntimeError(f"routing.slot must be contiguous with 1 to {MAX_CHOICES} entries a row, got shape "
                            f"{tuple(slot.shape)}")
-    return slot, slot.numel() // slot.shape[-1], slot.shape[-1]
+    if source.dtype != torch.int32 or source.device != device:
+        raise TypeError(f"routing must hold int32 tensors on {device}")
+    if source.shape != (slot.numel(),) or not source.is_contiguous():
+        raise RuntimeError(f"routing.source must be contiguous and have shape {(slot.numel(),)}, got "
+                           f"{tuple(source.shape)}")
+    return slot, source, slot.numel() // slot.shape[-1], slot.shape[-1]
 
 
 def _check_features(t, what):
@@ -84,12 +90,12 @@ def _check_features(t, what):
         raise RuntimeError(f"{what} must have rows of at most {MAX_FEATURES} values")
 
 
-def _spread(x, slot):
+def _spread(x, slot, source):
     rows, choices, cols = slot.numel() // slot.shape[-1], slot.shape[-1], x.shape[-1]
     v, _, stride = _rows.rows_view(x)
     out = torch.empty(rows * choices, cols, dtype=x.dtype, device=x.device)
     _rows.call(_lib.sphops_dispatch_rows, x.device, v.data_ptr(), TYPES[x.dtype], stride, slot.data_ptr(),
-               out.data_ptr(), rows, choices, cols)
+               source.data_ptr(), out.data_ptr(), rows, choices, cols)
     return out
 
 
@@ -104,44 +110,44 @@ def _gather(results, weight, slot):
 
 class _Dispatch(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, slot):
+    def forward(ctx, x, slot, source):
         ctx.save_for_backward(slot)
-        return _spread(x, slot)
+        return _spread(x, slot, source)
 
     @staticmethod
     def backward(ctx, d_out):
         slot, = ctx.saved_tensors
-        return (*_rows.first_order("dispatch", _gather(d_out, None, slot)), None)
+        return (*_rows.first_order("dispatch", _gather(d_out, None, slot)), None, None)
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, results, weight, slot):
-        ctx.save_for_backward(results, weight, slot)
+    def forward(ctx, results, weight, slot, source):
+        ctx.save_for_backward(results, weight, slot, source)
         return _gather(results, weight, slot)
 
     @staticmethod
     def backward(ctx, dy):
-        results, weight, slot = ctx.saved_tensors
-        need_r, need_w, _ = ctx.needs_input_grad
+        results, weight, slot, source = ctx.saved_tensors
+        need_r, need_w = ctx.needs_input_grad[:2]
         results = results if results.is_contiguous() else results.contiguous()
         u, rows, stride = _rows.rows_view(dy)
         d_results = torch.empty_like(results) if need_r else None
         dw = torch.empty(slot.shape, device=dy.device) if need_w else None
         _rows.call(_lib.sphops_combine_rows_backward, dy.device, u.data_ptr(), TYPES[dy.dtype], stride,
-                   results.data_ptr(), address(weight), slot.data_ptr(), address(d_results), address(dw), rows,
-                   slot.shape[-1], dy.shape[-1])
-        return (*_rows.first_order("combine", d_results, dw), None)
+                   results.data_ptr(), address(weight), slot.data_ptr(), source.data_ptr(), address(d_results),
+                   address(dw), rows, slot.shape[-1], dy.shape[-1])
+        return (*_rows.first_order("combine", d_results, dw), None, None)
 
 
 def dispatch(x, routing):
     """Rows at their entries' places: x (..., cols) to (places, cols), a row k
     times; places of entries without an expert hold zeros."""
     _check_features(x, "x")
-    slot, rows, _ = _check_slot(routing, x.device)
+    slot, source, _, _ = _check_slot(routing, x.device)
     if x.shape[:-1] != slot.shape[:-1]:
         raise RuntimeError(f"x must have shape {tuple(slot.shape[:-1])} + (cols,), got {tuple(x.shape)}")
-    return _Dispatch.apply(x, slot) if _rows.wants_grad(x) else _spread(x, slot)
+    return _Dispatch.apply(x, slot, source) if _rows.wants_grad(x) else _spread(x, slot, source)
 
 
 def combine(results, weight, routing):
@@ -150,12 +156,12 @@ def combine(results, weight, routing):
     place's row of ``results`` (places, cols).  Entries without an expert are left
     out, whatever their weight and place hold."""
     _check_features(results, "results")
-    slot, rows, choices = _check_slot(routing, results.device)
+    slot, source, rows, choices = _check_slot(routing, results.device)
     if results.dim() != 2 or results.shape[0] != rows * choices:
         raise RuntimeError(f"results must have {rows * choices} rows, got shape {tuple(results.shape)}")
     weight = _rows.check_weight(weight, slot.shape, (torch.float32,), results.device, "weight")
     if _rows.wants_grad(results, weight):
-        return _Combine.apply(results, weight, slot)
+        return _Combine.apply(results, weight, slot, source)
     return _gather(results, weight, slot)
 
 

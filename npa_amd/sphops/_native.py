@@ -96,9 +96,9 @@ _SIGNATURES = {
     "sphops_layer_norm_backward": ([_p, _i64, _p, _i64, _i32, _p, _i32, _p, _p, _p, _p, _i64, _i64, _p, _p], _i32),
     "sphops_sort_rows": ([_p, _i32, _i64, _i32, _i32, _p, _p, _p, _p, _p], _i32),
     "sphops_sort_rows_workspace_bytes": ([_i64, _i32, _i32], _i64),
-    "sphops_dispatch_rows": ([_p, _i32, _i64, _p, _p, _i64, _i32, _i64, _p], _i32),
+    "sphops_dispatch_rows": ([_p, _i32, _i64, _p, _p, _p, _i64, _i32, _i64, _p], _i32),
     "sphops_combine_rows": ([_p, _i32, _p, _p, _p, _i64, _i32, _i64, _p], _i32),
-    "sphops_combine_rows_backward": ([_p, _i32, _i64, _p, _p, _p, _p, _p, _i64, _i32, _i64, _p], _i32),
+    "sphops_combine_rows_backward": ([_p, _i32, _i64, _p, _p, _p, _p, _p, _p, _i64, _i32, _i64, _p], _i32),
     "sphops_expert_linear": ([_p, _i32, _i64, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p], _i32),
     "sphops_expert_linear_workspace_bytes": ([_i32, _i64, _i32, _i32, _i32], _i64),
     "sphops_expert_linear_backward": ([_p, _i64, _p, _i32, _i64, _p, _p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _p,

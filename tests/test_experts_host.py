@@ -62,11 +62,11 @@ def test_entry_points_check_their_arguments():
     _fails(lib.sphops_sort_rows(p, 0, 4, 1, 3, None, p, p, p, None), "null")
     _fails(lib.sphops_sort_rows(p, 0, 1 << 20, 1, 3, p, p, p, None, None), "null")
     assert lib.sphops_sort_rows_workspace_bytes(1, 0, 3) == -1
-    _fails(lib.sphops_dispatch_rows(p, 0, 8, p, None, 1, 1, 8, None), "null")
-    _fails(lib.sphops_dispatch_rows(p, 0, 8, p, p, 1, 1, 0, None), "values")
+    _fails(lib.sphops_dispatch_rows(p, 0, 8, p, None, None, 1, 1, 8, None), "null")
+    _fails(lib.sphops_dispatch_rows(p, 0, 8, p, p, p, 1, 1, 0, None), "values")
     _fails(lib.sphops_combine_rows(p, 5, p, p, p, 1, 1, 8, None), "element type")
     _fails(lib.sphops_combine_rows(p, 0, p, None, p, 1, 1, 8, None), "null")
-    _fails(lib.sphops_combine_rows_backward(p, 0, 8, None, p, p, p, p, 1, 1, 8, None), "null")
+    _fails(lib.sphops_combine_rows_backward(p, 0, 8, None, p, p, p, p, p, 1, 1, 8, None), "null")
     _fails(lib.sphops_expert_linear(p, 0, 8, p, p, p, p, 4, 0, 8, 8, 0, p, None), "not supported")
     _fails(lib.sphops_expert_linear(p, 0, 8, p, p, p, p, 4, 2, 0, 8, 0, p, None), "not supported")
     _fails(lib.sphops_expert_linear(p, 0, 8, p, p, None, p, 4, 2, 8, 8, 0, p, None), "null")
