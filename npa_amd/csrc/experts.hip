@@ -15,8 +15,10 @@ namespace sphops {
 namespace {
 
 constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;
-constexpr int kTileItems = 8;  // entries a thread takes where there are many tiles
-constexpr int kSortTile = kSortThreads * kTileItems;
+// Entries a thread takes of a tile: few while tiles are few, whose steps follow one
+// another (16384 entries, 64 experts: 9 us a launch with eight, 1 with two).
+constexpr int kFewItems = 2, kManyItems = 8;
+constexpr int64_t kManyEntries = 1 << 18;
 
 // An entry's key: its expert, `experts` for none.
 __device__ __forceinline__ uint32_t key_of(const void* __restrict__ index, bool wide, int64_t i, int experts) {
@@ -96,11 +98,12 @@ __device__ __forceinline__ void scan_experts(uint32_t* __restrict__ total, int e
 }
 
 // hist[key * tiles + tile]: the tile's entries of each key.
+template <int ITEMS>
 __global__ __launch_bounds__(kSortThreads) void k_sort_count(const void* __restrict__ index, bool wide, int64_t n,
                                                              int experts, int bits, uint32_t* __restrict__ hist) {
   extern __shared__ uint32_t counts[];
-  uint32_t key[kTileItems], rank[kTileItems];
-  rank_tile<kTileItems>(index, wide, (int64_t)blockIdx.x * kSortTile, n, experts, bits, counts, key, rank);
+  uint32_t key[ITEMS], rank[ITEMS];
+  rank_tile<ITEMS>(index, wide, (int64_t)blockIdx.x * kSortThreads * ITEMS, n, experts, bits, counts, key, rank);
   for (int e = threadIdx.x; e <= experts; e += kSortThreads) {
     uint32_t t = 0;
 #pragma unroll
@@ -414,7 +417,15 @@ int key_bits(int experts) {
   return bits;
 }
 
-int64_t sort_tiles(int64_t n) { return (n + kSortTile - 1) / kSortTile; }
+// One workgroup's work takes no other launch.
+int sort_items(int64_t n) {
+  if (n <= kSortThreads) return 1;
+  return n <= kSortThreads * kManyItems || n > kManyEntries ? kManyItems : kFewItems;
+}
+int64_t sort_tiles(int64_t n) {
+  const int64_t tile = (int64_t)kSortThreads * sort_items(n);
+  return (n + tile - 1) / tile;
+}
 
 // Rows of one entry each that k_places_out takes.
 template <class T>
@@ -461,19 +472,26 @@ void run_sort_rows(const void* index, bool wide, int64_t n, int experts, int32_t
     hipLaunchKernelGGL((k_sort_place<decltype(items)::value>), dim3((uint32_t)std::max<int64_t>(tiles, 1)), dim3(kSortThreads), lds, st,
                        index, wide, n, experts, bits, hist, totals, offsets, slot, source);
   };
+  const auto with_items = [&](auto&& f) {
+    const int items = sort_items(n);
+    if (items == 1) f(std::integral_constant<int, 1>{});
+    else if (items == kFewItems) f(std::integral_constant<int, kFewItems>{});
+    else f(std::integral_constant<int, kManyItems>{});
+  };
   if (tiles <= 1) {
-    if (n <= kSortThreads) place(std::integral_constant<int, 1>{}, nullptr, nullptr);
-    else place(std::integral_constant<int, kTileItems>{}, nullptr, nullptr);
+    with_items([&](auto items) { place(items, nullptr, nullptr); });
     SPHOPS_LAUNCHED();
     return;
   }
   uint32_t* const totals = work + tiles * (experts + 1);
-  hipLaunchKernelGGL(k_sort_count, dim3((uint32_t)tiles), dim3(kSortThreads), lds, st, index, wide, n, experts, bits,
-                     work);
+  with_items([&](auto items) {
+    hipLaunchKernelGGL((k_sort_count<decltype(items)::value>), dim3((uint32_t)tiles), dim3(kSortThreads), lds, st, index,
+                       wide, n, experts, bits, work);
+  });
   SPHOPS_LAUNCHED();
   hipLaunchKernelGGL(k_sort_scan, dim3((uint32_t)(experts + 1)), dim3(256), 0, st, work, (int)tiles, totals);
   SPHOPS_LAUNCHED();
-  place(std::integral_constant<int, kTileItems>{}, work, totals);
+  with_items([&](auto items) { place(items, work, totals); });
   SPHOPS_LAUNCHED();
 }
 

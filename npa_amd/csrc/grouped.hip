@@ -351,6 +351,108 @@ __global__ __launch_bounds__(kWideThreads) void k_group_rows_wide(const float* _
   }
 }
 
+// A few rows an expert (single tokens): workgroup = 16 outputs of an expert and 64
+// of its rows, the sum shared out over its waves, whose loads go to registers, eight
+// lines of 128 bytes a row of W in flight: nothing waits for anything but memory.
+// Bound: HBM, the weights of the experts that have rows.
+constexpr int kTokenThreads = 256, kTokenWaves = 4, kTokenRows = 64;
+template <class T>
+struct Tokens {
+  static constexpr int V = Piece<T>::V, kLine = 128 / (int)sizeof(T), kAhead = 8;  // values of a line; lines in flight
+  f32x4 sums[kTokenWaves][4][64];
+
+  // The lane's two pieces of a line from k on: 32 bytes at 32 (l / 16).
+  __device__ __forceinline__ static void load(Piece<T> (&p)[2], const T* __restrict__ row, int k, int cols, bool whole) {
+    const int at = k + 2 * V * ((int)(threadIdx.x & 63) >> 4);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (whole) p[i].raw = *reinterpret_cast<const typename Piece<T>::Raw*>(row + at + V * i);
+      else if (at + V * i < cols) p[i].load(row, at + V * i, cols);
+      else p[i].raw = typename Piece<T>::Raw{};
+    }
+  }
+  __device__ __forceinline__ static f32x4 product(const Piece<T>& x, const Piece<T>& w, f32x4 c) {
+    if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x.get(j), w.get(j), c, 0, 0, 0);
+      return c;
+    } else {
+      return mma16<T>(__builtin_bit_cast(s16x8, x.raw), __builtin_bit_cast(s16x8, w.raw), c);
+    }
+  }
+  // Rows 0 .. here - 1 of x, up to 16 MT of them, times outputs n0 .. of W.
+  template <int MT>
+  __device__ __forceinline__ void run(const T* __restrict__ x, int64_t xs, int here, const T* __restrict__ w,
+                                      const T* __restrict__ bias, T* __restrict__ y, int n0, int cols, int outs,
+                                      bool relu) {
+    const int lane = threadIdx.x & 63, c = lane & 15, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+    const T* __restrict__ wr = w + (int64_t)min(n0 + c, outs - 1) * cols;
+    const T* __restrict__ xr[MT];
+    f32x4 acc[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      xr[m] = x + (int64_t)min(16 * m + c, here - 1) * xs;
+      acc[m] = f32x4{};
+    }
+    const int lines = (cols + kLine - 1) / kLine, first = lines * wave / kTokenWaves, last = lines * (wave + 1) / kTokenWaves;
+    for (int n = first; n < last; n += kAhead) {
+      Piece<T> p[kAhead][2];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (n + u < last) load(p[u], wr, (n + u) * kLine, cols, (n + u + 1) * kLine <= cols);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (n + u >= last) break;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          Piece<T> q[2];
+          load(q, xr[m], (n + u) * kLine, cols, (n + u + 1) * kLine <= cols);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) acc[m] = product(q[i], p[u][i], acc[m]);
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) sums[wave][m][lane] = acc[m];
+    __syncthreads();
+    // result register r of lane l is row 4 (l / 16) + r, output l % 16
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int row = (int)threadIdx.x / 16, n = (int)threadIdx.x % 16, at = n0 + n;
+      if (16 * m + row >= here || at >= outs) continue;
+      float v = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kTokenWaves; ++i) v += sums[i][m][16 * (row / 4) + n][row % 4];
+      if (bias != nullptr) v += to_f32(bias[at]);
+      if (relu) v = v <= 0.0f ? 0.0f : v;  // NaN stays
+      y[(int64_t)(16 * m + row) * outs + at] = from_f32<T>(v);
+    }
+  }
+};
+template <class T>
+__global__ __launch_bounds__(kTokenThreads) void k_group_tokens(const T* __restrict__ x, int64_t xs,
+                                                                const T* __restrict__ w, const T* __restrict__ b,
+                                                                const int32_t* __restrict__ offsets,
+                                                                T* __restrict__ y, int64_t slots, int experts, int cols,
+                                                                int outs, bool relu) {
+  __shared__ Tokens<T> tokens;
+  const int e = (int)blockIdx.y, n0 = (int)blockIdx.x * 16;
+  const int64_t lo = e == 0 ? 0 : min<int64_t>(max(offsets[e], 0), slots);
+  const int64_t hi = e == experts ? slots : max<int64_t>(lo, min<int64_t>(offsets[e + 1], slots));
+  const int64_t m0 = lo + (int64_t)blockIdx.z * kTokenRows;
+  if (m0 >= hi) return;
+  const int here = (int)min<int64_t>(kTokenRows, hi - m0);
+  if (e == experts) {
+    zero_rows(y, m0, here, n0, 16, outs);
+    return;
+  }
+  const T* const we = w + (int64_t)e * cols * outs;
+  const T* const be = b != nullptr ? b + (int64_t)e * outs : nullptr;
+  if (here <= 16) tokens.template run<1>(x + m0 * xs, xs, here, we, be, y + m0 * outs, n0, cols, outs, relu);
+  else tokens.template run<4>(x + m0 * xs, xs, here, we, be, y + m0 * outs, n0, cols, outs, relu);
+}
+
 // A weight gradient's workgroup: which piece (chunk of rows, or expert) and which
 // tile of dW.  A piece's tiles are dealt to the XCDs in contiguous shares, so that
 // each XCD works on every piece (experts differ in rows) and tiles that share
@@ -787,6 +889,12 @@ void rows_plain(const T* x, int64_t xs, const T* w, const T* b, const T* mask, c
   }
 }
 
+// Few rows an expert: k_group_tokens.
+constexpr int64_t kTokenSlots = 1024;
+bool few_rows(int64_t slots, int experts, int64_t outs) {
+  return slots <= kTokenSlots && slots <= 16 * (int64_t)experts;
+}
+
 template <class T>
 bool fast_as_is(const void* x, int64_t xs, int64_t cols, const void* w, int64_t ws) {
   return !std::is_same_v<T, float> && whole_pieces(x, xs) && cols % 8 == 0 && whole_pieces(w, ws);
@@ -814,7 +922,11 @@ void run_group_linear(const void* x, int type, int64_t xs, const void* w, const 
     const T *px = static_cast<const T*>(x), *pw = static_cast<const T*>(w), *pb = static_cast<const T*>(b);
     T* const py = static_cast<T*>(y);
     const bool as_is = fast_as_is<T>(x, xs, cols, w, cols);
-    if (as_is || lays_out(type, slots, experts, cols, outs)) {
+    if (few_rows(slots, experts, outs)) {
+      const dim3 grid((uint32_t)tiles_of(outs, 16), (uint32_t)(experts + 1), (uint32_t)tiles_of(slots, kTokenRows));
+      hipLaunchKernelGGL((k_group_tokens<T>), grid, dim3(kTokenThreads), 0, st, px, xs, pw, pb, offsets, py, slots,
+                         experts, (int)cols, (int)outs, relu);
+    } else if (as_is || lays_out(type, slots, experts, cols, outs)) {
       Layouts l{static_cast<char*>(work)};
       const Laid lx = as_is ? Laid{x, xs, 0} : lay_out(l, px, xs, slots, cols, st);
       const Laid lw = as_is ? Laid{w, cols, 0} : lay_out(l, pw, cols, experts * outs, cols, st);
