@@ -624,8 +624,8 @@ int64_t most_row_tiles(int64_t slots, int64_t groups) { return slots / kT + std:
 
 // Shares of the rows where the card holds `room` workgroups at once: their parts
 // should all fit, or those that come last wait for one of the others on their own
-// XCD (2^20 rows of 83 -> 19, 8 experts: forward 347 us with 256 shares, 1 with
-// 248).  Many experts give up no more than half of the room for that.
+// XCD (2^20 rows of 83 -> 19, 8 experts: forward 347 us with 256 shares, 265 with
+// 247, in a profile).  Many experts give up no more than half of the room for that.
 int64_t shares_of(int64_t room, int64_t parts) { return room - std::min(parts, room / 2); }
 int64_t row_shares(int64_t slots, int experts) {
   return std::min(shares_of(256, experts + 1), most_row_tiles(slots, experts + 1));

@@ -59,17 +59,69 @@ __global__ __launch_bounds__(kLayThreads) void k_lay_out(const T* __restrict__ x
   }
 }
 
-// The workgroup's row tile and column tile among those that there are (the
-// launch covers the most that there can be); false: neither.
-__device__ __forceinline__ bool rows_tile(const int32_t* __restrict__ offsets, int experts, int64_t slots, int size,
-                                          int nt, GroupTile& g, int& n) {
+// How a product's tiles fall on the card, which holds `room` of their workgroups at
+// once: whole turns of `room` tiles, and the tiles that are left, cut along the sum
+// into `slices` each where that fills a turn better.  Without cuts 8192 x 2048 ->
+// 1024 float32, 272 tiles of 256 x 128 on 256 CUs, took two turns (366 us, 239 with
+// them), and 955 x 1545 -> 125, 20 tiles, one long one.
+struct Turns {
+  uint32_t whole, left, slices;
+};
+constexpr int kMaxSlices = 16, kSliceDepth = 256;  // at most; of the sum that a slice has at least
+__device__ __forceinline__ Turns turns_of(uint32_t tiles, uint32_t room, int depth, bool cut) {
+  Turns t;
+  t.whole = tiles / room * room;
+  t.left = tiles - t.whole;
+  t.slices = 1;
+  if (cut && t.left > 0) t.slices = max(1u, min(min(room / t.left, (uint32_t)(depth / kSliceDepth)), (uint32_t)kMaxSlices));
+  return t;
+}
+
+// A workgroup's part of a product over rows: a tile, or a slice of one.  The
+// launch covers the most that there can be.
+struct RowsJob {
+  GroupTile g;
+  int n;                // column tile
+  int slice, slices;    // of the sum
+  int64_t place;        // of a slice's sums
+  // steps first .. last - 1 of `steps`
+  __device__ __forceinline__ int first(int steps) const { return (int)((int64_t)steps * slice / slices); }
+  __device__ __forceinline__ int last(int steps) const { return (int)((int64_t)steps * (slice + 1) / slices); }
+};
+__device__ __forceinline__ bool rows_job(const int32_t* __restrict__ offsets, int experts, int64_t slots, int size,
+                                         int nt, int room, int depth, bool cut, RowsJob& j) {
   const int64_t mt = group_tiles(offsets, experts, slots, size, true);
-  const uint32_t id = xcd_block_id((uint32_t)(mt * nt));
-  if (id == 0xFFFFFFFFu) return false;
+  const Turns t = turns_of((uint32_t)(mt * nt), (uint32_t)room, depth, cut);
+  uint32_t id = blockIdx.x;
+  j.slice = 0;
+  j.slices = 1;
+  j.place = 0;
+  if (id < t.whole) {
+    id = (id & 7u) * (t.whole >> 3) + (id >> 3);  // contiguous eighths to the XCDs (room is a multiple of 8)
+  } else {
+    const uint32_t at = id - t.whole;
+    if (at >= t.left * t.slices) return false;
+    j.slices = (int)t.slices;
+    j.place = at;
+    id = t.whole + at / t.slices;
+    j.slice = __builtin_amdgcn_readfirstlane((int)(at % t.slices));
+  }
   int64_t m;
-  tile_of(id, mt, nt, m, n);
-  g = group_tile(offsets, experts, slots, m, size, true);
-  return g.group >= 0;
+  tile_of((uint32_t)__builtin_amdgcn_readfirstlane((int)id), mt, nt, m, j.n);
+  j.g = group_tile(offsets, experts, slots, m, size, true);
+  return j.g.group >= 0;
+}
+
+// A slice's sums as they stand in registers, `threads` lanes beside each other.
+template <int TILES>
+__device__ __forceinline__ void put_slice(f32x4* __restrict__ to, int threads, const f32x16 (&acc)[TILES]) {
+#pragma unroll
+  for (int i = 0; i < TILES; ++i) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      to[(i * 4 + q) * threads + threadIdx.x] =
+          f32x4{acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]};
+  }
 }
 
 // Rows behind the last expert's: zeros.
@@ -105,93 +157,6 @@ __device__ __forceinline__ void finish(float (&v)[Piece<T>::V], const T* __restr
   o.store(y, at, outs);
 }
 
-// y (slots x outs) = x (slots x cols) W_e^T + b_e, W_e (outs x cols); BACK: y = x
-// W_e with W_e (cols x outs), which is the input gradient.  relu: y = max(y, 0).
-// mask (slots x outs): y = 0 where it is not above 0.
-template <class T, bool BACK>
-__global__ __launch_bounds__(kGroupThreads) void k_group_rows(const T* __restrict__ x, int64_t xs,
-                                                              const T* __restrict__ w, const T* __restrict__ b,
-                                                              const T* __restrict__ mask,
-                                                              const int32_t* __restrict__ offsets, T* __restrict__ y,
-                                                              int64_t slots, int experts, int cols, int outs,
-                                                              bool relu, int nt) {
-  using IA = PanelImage<T, true>;
-  using IB = PanelImage<T, !BACK>;
-  constexpr int V = Piece<T>::V;
-  __shared__ __attribute__((aligned(16))) uint16_t room[std::max(IA::kPlane + IB::kPlane, kOutbox)];
-  uint16_t *const as = room, *const bs = room + IA::kPlane;
-  GroupTile g;
-  int n;
-  if (!rows_tile(offsets, experts, slots, kSide, nt, g, n)) return;
-  const int64_t m0 = g.lo + g.tile * kSide;
-  const int n0 = n * kSide, here = (int)min<int64_t>(kSide, g.hi - m0), outs_here = min(kSide, outs - n0);
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
-  const int row0 = wave / 4 * 64, col0 = wave % 4 * 32;
-  if (g.group == experts) {
-    zero_rows(y, m0, here, n0, kSide, outs);
-    return;
-  }
-  const T* const we = w + (int64_t)g.group * cols * outs;
-  const Panel<T> pa{x + m0 * xs, xs, here, cols};
-  const Panel<T> pb = BACK ? Panel<T>{we + n0, outs, cols, outs_here} : Panel<T>{we + (int64_t)n0 * cols, cols, outs_here, cols};
-  Piece<T> ra[IA::kLoads], rb[IB::kLoads];
-  TileSums<T> sums;
-  sums.clear();
-  IA::load(pa, 0, ra);
-  IB::load(pb, 0, rb);
-  for (int k = 0; k < cols; k += kStepK) {
-    IA::store(ra, as);
-    IB::store(rb, bs);
-    __syncthreads();
-    if (k + kStepK < cols) {
-      IA::load(pa, k + kStepK, ra);
-      IB::load(pb, k + kStepK, rb);
-    }
-    sums.template step<IA, IB>(as, bs, row0, col0);
-    __syncthreads();
-  }
-  float* const own = reinterpret_cast<float*>(room) + 1024 * wave;  // every wave is done with the panels
-  const T* const be = b != nullptr ? b + (int64_t)g.group * outs : nullptr;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    rows_of_tile<T>(sums.acc[i], own, [&](int r, int c, float (&v)[V]) {
-      const int row = row0 + 32 * i + r, at = n0 + col0 + c;
-      if (row >= here || at >= outs) return;
-      finish<T>(v, be, mask != nullptr ? mask + (m0 + row) * outs : nullptr, relu, y + (m0 + row) * outs, at, outs);
-    });
-  }
-}
-
-// How the fast kernels' tiles fall on the card, which holds `room` of their
-// workgroups at once: whole turns of `room` tiles, and the tiles that are left, cut
-// along the sum into `slices` each where that fills a turn better.  Without cuts
-// 8192 x 2048 -> 1024 float32, 272 tiles of 256 x 128 on 256 CUs, took two turns.
-struct Turns {
-  uint32_t whole, left, slices;
-};
-constexpr int kMaxSlices = 16, kSliceSteps = 4;  // at most; steps of the sum a slice has at least
-__host__ __device__ __forceinline__ Turns turns_of(uint32_t tiles, uint32_t room, int steps, bool cut) {
-  Turns t;
-  t.whole = tiles / room * room;
-  t.left = tiles - t.whole;
-  t.slices = 1;
-  if (cut && t.left > 0) {
-    const uint32_t most = room / t.left, deep = (uint32_t)(steps / kSliceSteps);
-    t.slices = most < deep ? most : deep;
-    t.slices = t.slices < 1 ? 1 : t.slices > kMaxSlices ? kMaxSlices : t.slices;
-  }
-  return t;
-}
-
-// Tile `id` of the fast kernels.
-__device__ __forceinline__ bool fast_tile(const int32_t* __restrict__ offsets, int experts, int64_t slots, int size,
-                                          int nt, int64_t mt, uint32_t id, GroupTile& g, int& n) {
-  int64_t m;
-  tile_of(id, mt, nt, m, n);
-  g = group_tile(offsets, experts, slots, m, size, true);
-  return g.group >= 0;
-}
-
 // Results of a wave's 32 x 32 on their way out, bias, ReLU and mask applied.
 template <class T>
 __device__ __forceinline__ void put_rows(const f32x16& acc, float* __restrict__ own, int row0, int col0, int64_t m0,
@@ -202,6 +167,63 @@ __device__ __forceinline__ void put_rows(const f32x16& acc, float* __restrict__ 
     if (row >= here || at >= outs) return;
     finish<T>(v, bias, mask != nullptr ? mask + (m0 + row) * outs : nullptr, relu, y + (m0 + row) * outs, at, outs);
   });
+}
+
+// y (slots x outs) = x (slots x cols) W_e^T + b_e, W_e (outs x cols); BACK: y = x
+// W_e with W_e (cols x outs), which is the input gradient.  relu: y = max(y, 0).
+// mask (slots x outs): y = 0 where it is not above 0.
+// A slice's sums go to `slices` (null: no tile is cut).
+template <class T, bool BACK>
+__global__ __launch_bounds__(kGroupThreads) void k_group_rows(const T* __restrict__ x, int64_t xs,
+                                                              const T* __restrict__ w, const T* __restrict__ b,
+                                                              const T* __restrict__ mask,
+                                                              const int32_t* __restrict__ offsets, T* __restrict__ y,
+                                                              int64_t slots, int experts, int cols, int outs,
+                                                              bool relu, int nt, int room,
+                                                              f32x4* __restrict__ slices) {
+  using IA = PanelImage<T, true>;
+  using IB = PanelImage<T, !BACK>;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[std::max(IA::kPlane + IB::kPlane, kOutbox)];
+  uint16_t *const as = lds, *const bs = lds + IA::kPlane;
+  RowsJob j;
+  if (!rows_job(offsets, experts, slots, kSide, nt, room, cols, slices != nullptr, j)) return;
+  const int64_t m0 = j.g.lo + j.g.tile * kSide;
+  const int n0 = j.n * kSide, here = (int)min<int64_t>(kSide, j.g.hi - m0), outs_here = min(kSide, outs - n0);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+  const int row0 = wave / 4 * 64, col0 = wave % 4 * 32;
+  if (j.g.group == experts) {
+    if (j.slice == 0) zero_rows(y, m0, here, n0, kSide, outs);
+    return;
+  }
+  const T* const we = w + (int64_t)j.g.group * cols * outs;
+  const Panel<T> pa{x + m0 * xs, xs, here, cols};
+  const Panel<T> pb = BACK ? Panel<T>{we + n0, outs, cols, outs_here} : Panel<T>{we + (int64_t)n0 * cols, cols, outs_here, cols};
+  const int steps = (cols + kStepK - 1) / kStepK, first = j.first(steps), last = j.last(steps);
+  Piece<T> ra[IA::kLoads], rb[IB::kLoads];
+  TileSums<T> sums;
+  sums.clear();
+  IA::load(pa, first * kStepK, ra);
+  IB::load(pb, first * kStepK, rb);
+  for (int n = first; n < last; ++n) {
+    IA::store(ra, as);
+    IB::store(rb, bs);
+    __syncthreads();
+    if (n + 1 < last) {
+      IA::load(pa, (n + 1) * kStepK, ra);
+      IB::load(pb, (n + 1) * kStepK, rb);
+    }
+    sums.template step<IA, IB>(as, bs, row0, col0);
+    __syncthreads();
+  }
+  if (j.slices > 1) {
+    put_slice<2>(slices + j.place * (kSide * kSide / 4), kGroupThreads, sums.acc);
+    return;
+  }
+  float* const own = reinterpret_cast<float*>(lds) + 1024 * wave;  // every wave is done with the panels
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    put_rows<T>(sums.acc[i], own, row0 + 32 * i, n0 + col0, m0, here,
+                b != nullptr ? b + (int64_t)j.g.group * outs : nullptr, mask, relu, y, outs);
 }
 
 // The same for 16-bit rows in whole 16-byte pieces, or for float32 rows laid out
@@ -216,29 +238,13 @@ __global__ __launch_bounds__(64 * WM * WN) void k_group_rows_fast(
   using E = Piece16<T>;
   using Tile = FastTile<E, kPieces<T>, true, !BACK, BM, BN, WM, WN, false>;
   __shared__ __attribute__((aligned(16))) uint16_t s0[Tile::kStage], s1[Tile::kStage];
-  const int64_t mt = group_tiles(offsets, experts, slots, BM, true);
-  const int steps = (cols + Tile::KS - 1) / Tile::KS;
-  const Turns turns = turns_of((uint32_t)(mt * nt), (uint32_t)room, steps, slices != nullptr);
-  uint32_t id = blockIdx.x;
-  int slice = 0, cuts = 1;
-  if (id < turns.whole) {
-    id = (id & 7u) * (turns.whole >> 3) + (id >> 3);  // contiguous eighths to the XCDs
-  } else {
-    const uint32_t at = id - turns.whole;
-    if (at >= turns.left * turns.slices) return;
-    cuts = (int)turns.slices;
-    id = turns.whole + at / turns.slices;
-    slice = (int)(at % turns.slices);
-  }
-  id = (uint32_t)__builtin_amdgcn_readfirstlane((int)id);
-  slice = __builtin_amdgcn_readfirstlane(slice);
-  GroupTile g;
-  int n;
-  if (!fast_tile(offsets, experts, slots, BM, nt, mt, id, g, n)) return;
+  RowsJob j;
+  if (!rows_job(offsets, experts, slots, BM, nt, room, cols, slices != nullptr, j)) return;
+  const GroupTile& g = j.g;
   const int64_t m0 = g.lo + g.tile * BM;
-  const int n0 = n * BN, here = (int)min<int64_t>(BM, g.hi - m0), outs_here = min(BN, outs - n0);
+  const int n0 = j.n * BN, here = (int)min<int64_t>(BM, g.hi - m0), outs_here = min(BN, outs - n0);
   if (g.group == experts) {
-    if (slice == 0) zero_rows(y, m0, here, n0, BN, outs);
+    if (j.slice == 0) zero_rows(y, m0, here, n0, BN, outs);
     return;
   }
   // W_e has a row for each output, or (BACK) for each input
@@ -246,23 +252,15 @@ __global__ __launch_bounds__(64 * WM * WN) void k_group_rows_fast(
   typename Tile::A pa(Panel<E>{x + m0 * xs, xs, here, cols}, xp);
   typename Tile::B pb(BACK ? Panel<E>{we + n0, ws, cols, min(BN, (int)ws - n0)}
                            : Panel<E>{we + (int64_t)n0 * ws, ws, outs_here, cols}, wp);
-  const int first = steps * slice / cuts, last = steps * (slice + 1) / cuts;
+  const int steps = (cols + Tile::KS - 1) / Tile::KS, first = j.first(steps), last = j.last(steps);
   pa.base += first * pa.step;
   pb.base += first * pb.step;
   Tile t;
   t.run(pa, pb, min(cols, last * Tile::KS) - first * Tile::KS, false, s0, s1);
-  if (cuts > 1) {
-    f32x4* const to = slices + (int64_t)(blockIdx.x - turns.whole) * (BM * BN / 4) + threadIdx.x;
+  if (j.slices > 1) {
 #pragma unroll
-    for (int i = 0; i < Tile::TM; ++i) {
-#pragma unroll
-      for (int j = 0; j < Tile::TN; ++j) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          to[((i * Tile::TN + j) * 4 + q) * (64 * Tile::kWaves)] =
-              f32x4{t.acc[i][j][4 * q], t.acc[i][j][4 * q + 1], t.acc[i][j][4 * q + 2], t.acc[i][j][4 * q + 3]};
-      }
-    }
+    for (int i = 0; i < Tile::TM; ++i)
+      put_slice<Tile::TN>(slices + j.place * (BM * BN / 4) + i * Tile::TN * 4 * (64 * Tile::kWaves), 64 * Tile::kWaves, t.acc[i]);
     return;
   }
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
@@ -271,8 +269,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_group_rows_fast(
 #pragma unroll
   for (int i = 0; i < Tile::TM; ++i) {
 #pragma unroll
-    for (int j = 0; j < Tile::TN; ++j)
-      put_rows<T>(t.acc[i][j], own, wave / WN * (BM / WM) + 32 * i, n0 + wave % WN * (BN / WN) + 32 * j, m0, here,
+    for (int k = 0; k < Tile::TN; ++k)
+      put_rows<T>(t.acc[i][k], own, wave / WN * (BM / WM) + 32 * i, n0 + wave % WN * (BN / WN) + 32 * k, m0, here,
                   b != nullptr ? b + (int64_t)g.group * outs : nullptr, mask, relu, y, outs);
   }
 }
@@ -282,16 +280,18 @@ template <class T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void k_group_rows_join(const T* __restrict__ b, const T* __restrict__ mask,
                                                                   const int32_t* __restrict__ offsets,
                                                                   T* __restrict__ y, int64_t slots, int experts,
-                                                                  int steps, int outs, bool relu, int nt, int room,
+                                                                  int depth, int outs, bool relu, int nt, int room,
                                                                   const f32x4* __restrict__ slices) {
   constexpr int kWaves = WM * WN, TN = BN / WN / 32;
   __shared__ __attribute__((aligned(16))) float room_of[kWaves][1024];
   const int64_t mt = group_tiles(offsets, experts, slots, BM, true);
-  const Turns turns = turns_of((uint32_t)(mt * nt), (uint32_t)room, steps, true);
+  const Turns turns = turns_of((uint32_t)(mt * nt), (uint32_t)room, depth, true);
   if (turns.slices == 1 || blockIdx.x >= turns.left) return;
-  GroupTile g;
+  int64_t m;
   int n;
-  if (!fast_tile(offsets, experts, slots, BM, nt, mt, turns.whole + blockIdx.x, g, n) || g.group == experts) return;
+  tile_of(turns.whole + blockIdx.x, mt, nt, m, n);
+  const GroupTile g = group_tile(offsets, experts, slots, m, BM, true);
+  if (g.group < 0 || g.group == experts) return;
   const int64_t m0 = g.lo + g.tile * BM;
   const int n0 = n * BN, here = (int)min<int64_t>(BM, g.hi - m0), ij = (int)blockIdx.y;
   const f32x4* from = slices + (int64_t)blockIdx.x * turns.slices * (BM * BN / 4) + (int64_t)ij * 4 * (64 * kWaves) + threadIdx.x;
@@ -318,36 +318,38 @@ __global__ __launch_bounds__(kWideThreads) void k_group_rows_wide(const float* _
                                                                   const float* __restrict__ mask,
                                                                   const int32_t* __restrict__ offsets,
                                                                   float* __restrict__ y, int64_t slots, int experts,
-                                                                  int cols, int outs, bool relu, int nt) {
+                                                                  int cols, int outs, bool relu, int nt, int room,
+                                                                  f32x4* __restrict__ slices) {
   using Tile = WideTile<true, !BACK, BM, BN, WM, WN>;
-  __shared__ __attribute__((aligned(16))) float room[Tile::kRoom];
-  GroupTile g;
-  int n;
-  if (!rows_tile(offsets, experts, slots, BM, nt, g, n)) return;
+  __shared__ __attribute__((aligned(16))) float lds[Tile::kRoom];
+  RowsJob j;
+  if (!rows_job(offsets, experts, slots, BM, nt, room, cols, slices != nullptr, j)) return;
+  const GroupTile& g = j.g;
   const int64_t m0 = g.lo + g.tile * BM;
-  const int n0 = n * BN, here = (int)min<int64_t>(BM, g.hi - m0), outs_here = min(BN, outs - n0);
+  const int n0 = j.n * BN, here = (int)min<int64_t>(BM, g.hi - m0), outs_here = min(BN, outs - n0);
   if (g.group == experts) {
-    zero_rows(y, m0, here, n0, BN, outs);
+    if (j.slice == 0) zero_rows(y, m0, here, n0, BN, outs);
     return;
   }
   const float* const we = w + (int64_t)g.group * cols * outs;
+  const int steps = (cols + kStepK - 1) / kStepK;
   Tile t;
   t.run(Panel<float>{x + m0 * xs, xs, here, cols},
         BACK ? Panel<float>{we + n0, outs, cols, outs_here} : Panel<float>{we + (int64_t)n0 * cols, cols, outs_here, cols},
-        cols, room, [](auto&) {});
+        j.first(steps) * kStepK, min(cols, j.last(steps) * kStepK), lds, [](auto&) {});
+  if (j.slices > 1) {
+#pragma unroll
+    for (int i = 0; i < Tile::TM; ++i)
+      put_slice<Tile::TN>(slices + j.place * (BM * BN / 4) + i * Tile::TN * 4 * kWideThreads, kWideThreads, t.acc[i]);
+    return;
+  }
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
-  const int row0 = wave / WN * (BM / WM), col0 = wave % WN * (BN / WN);
-  const float* const be = b != nullptr ? b + (int64_t)g.group * outs : nullptr;
 #pragma unroll
   for (int i = 0; i < Tile::TM; ++i) {
 #pragma unroll
-    for (int j = 0; j < Tile::TN; ++j) {
-      rows_of_tile<float>(t.acc[i][j], room + 1024 * wave, [&](int r, int c, float (&v)[4]) {
-        const int row = row0 + 32 * i + r, at = n0 + col0 + 32 * j + c;
-        if (row >= here || at >= outs) return;
-        finish<float>(v, be, mask != nullptr ? mask + (m0 + row) * outs : nullptr, relu, y + (m0 + row) * outs, at, outs);
-      });
-    }
+    for (int k = 0; k < Tile::TN; ++k)
+      put_rows<float>(t.acc[i][k], lds + 1024 * wave, wave / WN * (BM / WM) + 32 * i, n0 + wave % WN * (BN / WN) + 32 * k,
+                      m0, here, b != nullptr ? b + (int64_t)g.group * outs : nullptr, mask, relu, y, outs);
   }
 }
 
@@ -466,14 +468,32 @@ __device__ __forceinline__ GradTile grad_tile(int mt, int nt) {
   const uint32_t xcd = x & 7u, q = tiles >> 3, rem = tiles & 7u, at = xcd * q + min(xcd, rem) + (x >> 3);
   return GradTile{blockIdx.x / tiles, (int)(at / (uint32_t)nt), (int)(at % (uint32_t)nt)};
 }
+// Its rows.  Pieces that are whole experts come in the order of their rows, most
+// first (up to 64 experts): what starts last is short.
 __device__ __forceinline__ GroupTile grad_rows(const int32_t* __restrict__ offsets, int experts, int64_t slots,
                                                int64_t piece, int64_t chunk, bool chunks) {
   if (chunks) return group_tile(offsets, experts, slots, piece, chunk, false);
   GroupTile g;
   g.group = (int)piece;
   g.tile = 0;
-  g.lo = piece == 0 ? 0 : min<int64_t>(max(offsets[piece], 0), slots);
-  g.hi = max<int64_t>(g.lo, min<int64_t>(offsets[piece + 1], slots));
+  if (experts <= 64) {
+    const int e = (int)(threadIdx.x & 63);
+    int mine = -1;
+    if (e < experts) {
+      const int64_t lo = e == 0 ? 0 : min<int64_t>(max(offsets[e], 0), slots);
+      mine = (int)(max<int64_t>(lo, min<int64_t>(offsets[e + 1], slots)) - lo);
+    }
+    int before = 0;
+    for (int i = 0; i < experts; ++i) {
+      const int other = __builtin_amdgcn_readlane(mine, i);
+      before += other > mine || (other == mine && i < e) ? 1 : 0;
+    }
+    const uint64_t at = __ballot(e < experts && before == (int)piece);
+    g.group = __ffsll((unsigned long long)at) - 1;
+  }
+  const int e = g.group;
+  g.lo = e == 0 ? 0 : min<int64_t>(max(offsets[e], 0), slots);
+  g.hi = max<int64_t>(g.lo, min<int64_t>(offsets[e + 1], slots));
   return g;
 }
 
@@ -641,7 +661,7 @@ __global__ __launch_bounds__(kWideThreads) void k_group_weight_grad_wide(
   f32x4 bias = f32x4{};
   Tile t;
   t.run(Panel<float>{dy + lo * dys + m0, dys, rows, min(BM, outs - m0)},
-        Panel<float>{x + lo * xs + n0, xs, rows, min(BN, cols - n0)}, rows, room, [&](auto& pieces) {
+        Panel<float>{x + lo * xs + n0, xs, rows, min(BN, cols - n0)}, 0, rows, room, [&](auto& pieces) {
           if (n0 != 0) return;
           for (auto& p : pieces) bias += f32x4{p.get(0), p.get(1), p.get(2), p.get(3)};
         });
@@ -808,56 +828,67 @@ Laid lay_out(Layouts& l, const T* x, int64_t stride, int64_t rows, int64_t cols,
 }
 
 // Whether a product's operands are laid out first: float32 and 16-bit rows of
-// any kind where the product is large beside them.
+// any kind where the product is large beside them, and not where that takes more
+// than 16 GB.
 bool lays_out(int type, int64_t slots, int experts, int64_t cols, int64_t outs) {
   if (cols < 64 || outs < 64 || slots < 64 * (int64_t)experts) return false;
+  if (Layouts::bytes_of(type, slots, cols + outs) + Layouts::bytes_of(type, experts * outs, cols) > int64_t(1) << 34) return false;
   return slots * cols * outs >= (int64_t(1) << (type == SPHOPS_F32 ? 32 : 31));
 }
 
-// Tiles of a product over rows on the fast kernels: rows, columns, and how many
-// of their workgroups the card holds.
-struct FastPlan {
+// A product over rows: its tiles, how many of their workgroups the card holds, and
+// whether tiles may be cut: sums of two slices' depth.
+struct RowsPlan {
   int bm, bn, room;
   bool cut;
-  int64_t slices_bytes() const { return cut ? (int64_t)room * bm * bn * 4 : 0; }
+  int64_t tiles = 0;  // the most that there can be
+  int64_t slices_bytes() const { return cut ? std::min<int64_t>(room, tiles * kMaxSlices) * bm * bn * 4 : 0; }
 };
-FastPlan fast_plan(int type, int64_t slots, int experts, int64_t cols, int64_t outs) {
-  FastPlan p;
-  if (type == SPHOPS_F32) {
-    const bool tall = slots / 256 * tiles_of(outs, 128) >= 192;
-    p = FastPlan{tall ? 256 : 128, 128, 256, false};
+RowsPlan rows_plan(int type, bool fast, int64_t slots, int experts, int64_t cols, int64_t outs) {
+  RowsPlan p{128, 128, 512, cols >= 2 * kSliceDepth, 0};
+  if (type != SPHOPS_F32) {
+    if (fast && rows_side(slots, outs) == 256) p.bm = p.bn = p.room = 256;
+  } else if (fast) {
+    p.bm = slots / 256 * tiles_of(outs, 128) >= 192 ? 256 : 128;
+    p.room = 256;
+  } else if (wide_rows(slots, experts) == 32) {
+    p.bm = 32;
   } else {
-    const bool large = rows_side(slots, outs) == 256;
-    p = FastPlan{large ? 256 : 128, large ? 256 : 128, large ? 256 : 512, false};
+    p.bn = wide_side(outs);
   }
-  // two slices at least, and more than a few rows an expert: then few tiles have a reader each
-  p.cut = cols >= 2 * kSliceSteps * (type == SPHOPS_F32 ? 32 : 64) && slots > 16 * (int64_t)experts;
+  p.tiles = most_tiles(slots, experts + 1, p.bm) * tiles_of(outs, p.bn);
   return p;
 }
-int64_t fast_bytes(int type, int64_t slots, int experts, int64_t cols, int64_t outs) {
-  return fast_plan(type, slots, experts, cols, outs).slices_bytes();
+
+// Launches kernel(...) for the plan's tiles and the join of cut ones.
+template <class T, int BM, int BN, int WM, int WN, class Kernel>
+void launch_rows(const RowsPlan& p, Layouts& l, const T* b, const T* mask, const int32_t* offsets, T* y, int64_t slots,
+                 int experts, int64_t cols, int64_t outs, bool relu, hipStream_t st, Kernel&& kernel) {
+  f32x4* const slices = p.cut ? reinterpret_cast<f32x4*>(l.work + l.take(p.slices_bytes())) : nullptr;
+  const int nt = (int)tiles_of(outs, BN);
+  kernel(dim3((uint32_t)(p.tiles + (p.cut ? p.room : 0))), dim3(64 * WM * WN), nt, slices);
+  SPHOPS_LAUNCHED();
+  if (!p.cut) return;
+  hipLaunchKernelGGL((k_group_rows_join<T, BM, BN, WM, WN>),
+                     dim3((uint32_t)std::min<int64_t>(p.room / 2, p.tiles), BM / WM / 32 * (BN / WN / 32)),
+                     dim3(64 * WM * WN), 0, st, b, mask, offsets, y, slots, experts, (int)cols, (int)outs, relu, nt,
+                     p.room, slices);
+  SPHOPS_LAUNCHED();
 }
 
 template <class T, bool BACK>
 void rows_fast(Layouts& l, const Laid& x, const Laid& w, const T* b, const T* mask, const int32_t* offsets, T* y,
                int64_t slots, int experts, int64_t cols, int64_t outs, bool relu, hipStream_t st) {
   using E = Piece16<T>;
-  constexpr int type = std::is_same_v<T, float> ? SPHOPS_F32 : SPHOPS_BF16, KS = kPieces<T> == 3 ? 32 : 64;
-  const FastPlan p = fast_plan(type, slots, experts, cols, outs);
-  f32x4* const slices = p.cut ? reinterpret_cast<f32x4*>(l.work + l.take(p.slices_bytes())) : nullptr;
-  const int64_t tiles = most_tiles(slots, experts + 1, p.bm) * tiles_of(outs, p.bn);
+  const RowsPlan p = rows_plan(std::is_same_v<T, float> ? SPHOPS_F32 : SPHOPS_BF16, true, slots, experts, cols, outs);
   const auto with = [&](auto bm, auto bn, auto wm, auto wn) {
     constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
-    const int nt = (int)tiles_of(outs, BN);
-    hipLaunchKernelGGL((k_group_rows_fast<T, BACK, BM, BN, WM, WN>), dim3((uint32_t)(tiles + (p.cut ? p.room : 0))),
-                       dim3(64 * WM * WN), 0, st, static_cast<const E*>(x.base), x.stride, x.plane,
-                       static_cast<const E*>(w.base), w.stride, w.plane, b, mask, offsets, y, slots, experts, (int)cols,
-                       (int)outs, relu, nt, p.room, slices);
-    SPHOPS_LAUNCHED();
-    if (p.cut)
-      hipLaunchKernelGGL((k_group_rows_join<T, BM, BN, WM, WN>), dim3((uint32_t)(p.room / 2), BM / WM / 32 * (BN / WN / 32)),
-                         dim3(64 * WM * WN), 0, st, b, mask, offsets, y, slots, experts, (int)tiles_of(cols, KS),
-                         (int)outs, relu, nt, p.room, slices);
+    launch_rows<T, BM, BN, WM, WN>(p, l, b, mask, offsets, y, slots, experts, cols, outs, relu, st,
+                                   [&](dim3 grid, dim3 block, int nt, f32x4* slices) {
+      hipLaunchKernelGGL((k_group_rows_fast<T, BACK, BM, BN, WM, WN>), grid, block, 0, st, static_cast<const E*>(x.base),
+                         x.stride, x.plane, static_cast<const E*>(w.base), w.stride, w.plane, b, mask, offsets, y, slots,
+                         experts, (int)cols, (int)outs, relu, nt, p.room, slices);
+    });
   };
 #define SPHOPS_N(n) std::integral_constant<int, n>{}
   if constexpr (std::is_same_v<T, float>) {
@@ -867,31 +898,46 @@ void rows_fast(Layouts& l, const Laid& x, const Laid& w, const T* b, const T* ma
     if (p.bm == 256) with(SPHOPS_N(256), SPHOPS_N(256), SPHOPS_N(2), SPHOPS_N(4));
     else with(SPHOPS_N(128), SPHOPS_N(128), SPHOPS_N(2), SPHOPS_N(2));
   }
-#undef SPHOPS_N
 }
 
 // As they are.
 template <class T, bool BACK>
-void rows_plain(const T* x, int64_t xs, const T* w, const T* b, const T* mask, const int32_t* offsets, T* y,
+void rows_plain(Layouts& l, const T* x, int64_t xs, const T* w, const T* b, const T* mask, const int32_t* offsets, T* y,
                 int64_t slots, int experts, int64_t cols, int64_t outs, bool relu, hipStream_t st) {
-  const auto with = [&](auto kernel, int bm, int bn, int threads) {
-    const int64_t tiles = most_tiles(slots, experts + 1, bm) * tiles_of(outs, bn);
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles_of(tiles, 8) * 8)), dim3(threads), 0, st, x, xs, w, b, mask,
-                       offsets, y, slots, experts, (int)cols, (int)outs, relu, (int)tiles_of(outs, bn));
+  const RowsPlan p = rows_plan(std::is_same_v<T, float> ? SPHOPS_F32 : SPHOPS_BF16, false, slots, experts, cols, outs);
+  const auto with = [&](auto bm, auto bn, auto wm, auto wn) {
+    constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
+    launch_rows<T, BM, BN, WM, WN>(p, l, b, mask, offsets, y, slots, experts, cols, outs, relu, st,
+                                   [&](dim3 grid, dim3 block, int nt, f32x4* slices) {
+      if constexpr (std::is_same_v<T, float>)
+        hipLaunchKernelGGL((k_group_rows_wide<BACK, BM, BN, WM, WN>), grid, block, 0, st, x, xs, w, b, mask, offsets, y,
+                           slots, experts, (int)cols, (int)outs, relu, nt, p.room, slices);
+      else
+        hipLaunchKernelGGL((k_group_rows<T, BACK>), grid, block, 0, st, x, xs, w, b, mask, offsets, y, slots, experts,
+                           (int)cols, (int)outs, relu, nt, p.room, slices);
+    });
   };
   if constexpr (std::is_same_v<T, float>) {
-    if (wide_rows(slots, experts) == 32) with(k_group_rows_wide<BACK, 32, 128, 1, 4>, 32, 128, kWideThreads);
-    else if (wide_side(outs) == 32) with(k_group_rows_wide<BACK, 128, 32, 4, 1>, 128, 32, kWideThreads);
-    else if (wide_side(outs) == 64) with(k_group_rows_wide<BACK, 128, 64, 4, 1>, 128, 64, kWideThreads);
-    else with(k_group_rows_wide<BACK, 128, 128, 2, 2>, 128, 128, kWideThreads);
+    if (p.bm == 32) with(SPHOPS_N(32), SPHOPS_N(128), SPHOPS_N(1), SPHOPS_N(4));
+    else if (p.bn == 32) with(SPHOPS_N(128), SPHOPS_N(32), SPHOPS_N(4), SPHOPS_N(1));
+    else if (p.bn == 64) with(SPHOPS_N(128), SPHOPS_N(64), SPHOPS_N(4), SPHOPS_N(1));
+    else with(SPHOPS_N(128), SPHOPS_N(128), SPHOPS_N(2), SPHOPS_N(2));
   } else {
-    with(k_group_rows<T, BACK>, kSide, kSide, kGroupThreads);
+    with(SPHOPS_N(128), SPHOPS_N(128), SPHOPS_N(2), SPHOPS_N(4));
   }
+#undef SPHOPS_N
+}
+
+// Bytes of slices: as the product runs, or (16-bit rows) as either alignment does.
+int64_t rows_bytes(int type, int64_t slots, int experts, int64_t cols, int64_t outs, bool laid) {
+  if (type == SPHOPS_F32) return rows_plan(type, laid, slots, experts, cols, outs).slices_bytes();
+  return std::max(rows_plan(type, true, slots, experts, cols, outs).slices_bytes(),
+                  rows_plan(type, false, slots, experts, cols, outs).slices_bytes());
 }
 
 // Few rows an expert: k_group_tokens.
 constexpr int64_t kTokenSlots = 1024;
-bool few_rows(int64_t slots, int experts, int64_t outs) {
+bool few_rows(int64_t slots, int experts) {
   return slots <= kTokenSlots && slots <= 16 * (int64_t)experts;
 }
 
@@ -909,7 +955,7 @@ int64_t group_linear_workspace_bytes(int type, int64_t slots, int experts, int64
     l.take(Layouts::bytes_of(type, slots, cols));
     l.take(Layouts::bytes_of(type, experts * outs, cols));
   }
-  if (laid || type != SPHOPS_F32) l.take(fast_bytes(type, slots, experts, cols, outs));
+  if (!few_rows(slots, experts)) l.take(rows_bytes(type, slots, experts, cols, outs, laid));
   return l.used;
 }
 
@@ -922,17 +968,17 @@ void run_group_linear(const void* x, int type, int64_t xs, const void* w, const 
     const T *px = static_cast<const T*>(x), *pw = static_cast<const T*>(w), *pb = static_cast<const T*>(b);
     T* const py = static_cast<T*>(y);
     const bool as_is = fast_as_is<T>(x, xs, cols, w, cols);
-    if (few_rows(slots, experts, outs)) {
+    Layouts l{static_cast<char*>(work)};
+    if (few_rows(slots, experts)) {
       const dim3 grid((uint32_t)tiles_of(outs, 16), (uint32_t)(experts + 1), (uint32_t)tiles_of(slots, kTokenRows));
       hipLaunchKernelGGL((k_group_tokens<T>), grid, dim3(kTokenThreads), 0, st, px, xs, pw, pb, offsets, py, slots,
                          experts, (int)cols, (int)outs, relu);
     } else if (as_is || lays_out(type, slots, experts, cols, outs)) {
-      Layouts l{static_cast<char*>(work)};
       const Laid lx = as_is ? Laid{x, xs, 0} : lay_out(l, px, xs, slots, cols, st);
       const Laid lw = as_is ? Laid{w, cols, 0} : lay_out(l, pw, cols, experts * outs, cols, st);
       rows_fast<T, false>(l, lx, lw, pb, nullptr, offsets, py, slots, experts, cols, outs, relu, st);
     } else {
-      rows_plain<T, false>(px, xs, pw, pb, nullptr, offsets, py, slots, experts, cols, outs, relu, st);
+      rows_plain<T, false>(l, px, xs, pw, pb, nullptr, offsets, py, slots, experts, cols, outs, relu, st);
     }
   });
   SPHOPS_LAUNCHED();
@@ -953,7 +999,7 @@ int64_t group_backward_workspace_bytes(int type, int64_t slots, int experts, int
     l.take(Layouts::bytes_of(type, experts * outs, cols));
     l.take(Layouts::bytes_of(type, slots, cols));
   }
-  if (laid || type != SPHOPS_F32) l.take(fast_bytes(type, slots, experts, outs, cols));
+  l.take(rows_bytes(type, slots, experts, outs, cols, laid));
   return l.used;
 }
 
@@ -983,7 +1029,7 @@ void run_group_backward(const void* dy, int64_t dys, const void* x, int type, in
         const Laid lw = rows_as_is ? Laid{w, cols, 0} : lay_out(l, pw, cols, experts * outs, cols, st);
         rows_fast<T, true>(l, ldy, lw, nullptr, pm, offsets, static_cast<T*>(dx), slots, experts, outs, cols, false, st);
       } else {
-        rows_plain<T, true>(pdy, dys, pw, nullptr, pm, offsets, static_cast<T*>(dx), slots, experts, outs, cols, false, st);
+        rows_plain<T, true>(l, pdy, dys, pw, nullptr, pm, offsets, static_cast<T*>(dx), slots, experts, outs, cols, false, st);
       }
       SPHOPS_LAUNCHED();
     }

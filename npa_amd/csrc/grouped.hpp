@@ -259,7 +259,8 @@ struct WidePanel {
   }
 };
 
-// Sums of a tile of BM x BN in WM x WN waves over `len` of the sum; seen(pieces) is
+// Sums of a tile of BM x BN in WM x WN waves over from .. to - 1 of the sum (from a
+// multiple of a step); seen(pieces) is
 // given A's pieces of each step (which of them a thread holds, does not change).
 template <bool KA, bool KB, int BM, int BN, int WM, int WN>
 struct WideTile {
@@ -271,7 +272,8 @@ struct WideTile {
   f32x16 acc[TM][TN];
 
   template <class F>
-  __device__ __forceinline__ void run(const Panel<float>& pa, const Panel<float>& pb, int len, float* room, F&& seen) {
+  __device__ __forceinline__ void run(const Panel<float>& pa, const Panel<float>& pb, int from, int to, float* room,
+                                      F&& seen) {
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
     const int row0 = wave / WN * (BM / WM), col0 = wave % WN * (BN / WN);
     float *const as = room, *const bs = room + A::kFloats;
@@ -280,16 +282,16 @@ struct WideTile {
 #pragma unroll
       for (int j = 0; j < TN; ++j) acc[i][j] = f32x16{};
     }
-    if (len <= 0) return;
+    if (from >= to) return;
     Piece<float> ra[A::kLoads], rb[B::kLoads];
-    A::load(pa, 0, ra);
-    B::load(pb, 0, rb);
-    for (int k = 0; k < len; k += kStepK) {
+    A::load(pa, from, ra);
+    B::load(pb, from, rb);
+    for (int k = from; k < to; k += kStepK) {
       A::store(ra, as);
       B::store(rb, bs);
       seen(ra);
       __syncthreads();
-      if (k + kStepK < len) {
+      if (k + kStepK < to) {
         A::load(pa, k + kStepK, ra);
         B::load(pb, k + kStepK, rb);
       }

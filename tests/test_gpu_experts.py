@@ -302,6 +302,17 @@ def test_linear_of_large_tiles(dtype):
     _check_linear([300, 0, 64, 65, 1, 63, 500, 31, 32, 33, 7, 128], 3, 1032, 1000, dtype)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_linear_of_cut_tiles(dtype):
+    """Long sums over few tiles, which are cut along the sum: laid out first, as they are, short tiles, few outputs."""
+    _check_linear([2000, 2200, 1, 0], 100, 1030, 1060, dtype)
+    _check_linear([600, 90, 1], 40, 2048, 1536, dtype, bias=False)
+    _check_linear([300, 0, 77], 9, 1545, 125, dtype)
+    _check_linear([300, 0, 77], 9, 1000, 33, dtype)
+    _check_linear([30, 9, 18, 0], 200, 700, 520, dtype)
+    _check_linear([530, 3], 0, 20, 1030, dtype)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_linear_of_many_rows(dtype):
     _check_linear([20000, 3, 0, 9000, 40001], 77, 83, 35, dtype)
