@@ -182,7 +182,7 @@ struct PanelImage {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int row = row0 + i * (kGroupThreads / kRowPieces);
-      *reinterpret_cast<u32x4*>(lds + row * kPitch + (KMAJOR ? 8 * ((col / 8) ^ (row >> 1 & 3)) : col)) =
+      *reinterpret_cast<u32x4*>(lds + row * kPitch + (KMAJOR ? 8 * ((col / 8) ^ (row >> 2 & 3)) : col)) =
           __builtin_bit_cast(u32x4, in[i].raw);
     }
   }
@@ -192,7 +192,7 @@ struct PanelImage {
     const int lane = threadIdx.x & 63, h = lane >> 5;
     if constexpr (KMAJOR) {
       const int row = first + (lane & 31);
-      return *reinterpret_cast<const s16x8*>(lds + row * kPitch + 8 * ((2 * s + h) ^ (row >> 1 & 3)));
+      return *reinterpret_cast<const s16x8*>(lds + row * kPitch + 8 * ((2 * s + h) ^ (row >> 2 & 3)));
     } else {
       const int i = lane & 15, row = 16 * s + 8 * h + (i >> 2), col = first + 16 * (lane >> 4 & 1) + 4 * (i & 3);
       return join(read_column(lds + row * kPitch + col), read_column(lds + (row + 4) * kPitch + col));
@@ -242,7 +242,7 @@ struct WidePanel {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int row = row0 + i * (kWideThreads / kRowPieces);
-      *reinterpret_cast<u32x4*>(lds + row * kPitch + 4 * (KMAJOR ? piece ^ (row & 7) : piece)) =
+      *reinterpret_cast<u32x4*>(lds + row * kPitch + 4 * (KMAJOR ? piece ^ (row >> 1 & 7) : piece)) =
           __builtin_bit_cast(u32x4, in[i].raw);
     }
   }
@@ -251,7 +251,7 @@ struct WidePanel {
   __device__ __forceinline__ static f32x4 read(const float* __restrict__ lds, int first, int s) {
     const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31;
     if constexpr (KMAJOR) {
-      return *reinterpret_cast<const f32x4*>(lds + (first + c) * kPitch + 4 * ((2 * s + h) ^ (c & 7)));
+      return *reinterpret_cast<const f32x4*>(lds + (first + c) * kPitch + 4 * ((2 * s + h) ^ (c >> 1 & 7)));
     } else {
       const float* const at = lds + (8 * s + 4 * h) * kPitch + first + c;
       return f32x4{at[0], at[kPitch], at[2 * kPitch], at[3 * kPitch]};
@@ -326,7 +326,7 @@ __device__ __forceinline__ void rows_of_tile(const f32x16& v, float* __restrict_
   __builtin_amdgcn_wave_barrier();
 #pragma unroll
   for (int q = 0; q < 4; ++q)
-    *reinterpret_cast<f32x4*>(own + 32 * c + 4 * ((2 * q + h) ^ (c & 7))) =
+    *reinterpret_cast<f32x4*>(own + 32 * c + 4 * ((2 * q + h) ^ (c >> 1 & 7))) =
         f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
   __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -335,7 +335,7 @@ __device__ __forceinline__ void rows_of_tile(const f32x16& v, float* __restrict_
     float o[V];
 #pragma unroll
     for (int i = 0; i < V / 4; ++i) {
-      const f32x4 t = *reinterpret_cast<const f32x4*>(own + 32 * row + 4 * ((at * (V / 4) + i) ^ (row & 7)));
+      const f32x4 t = *reinterpret_cast<const f32x4*>(own + 32 * row + 4 * ((at * (V / 4) + i) ^ (row >> 1 & 7)));
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[4 * i + j] = t[j];
     }
@@ -372,7 +372,8 @@ struct FastPanel {
   uint32_t at[kLoads];  // of the lane's 16 bytes, from base
   int k[kLoads];        // where they stand in the sum's step
 
-  __device__ __forceinline__ static int exchange(int row) { return KS == 64 ? row & 7 : row >> 1 & 3; }
+  // so that the 16 rows of a quarter wave's read lie in different 16 bytes of the 64 banks
+  __device__ __forceinline__ static int exchange(int row) { return KS == 64 ? row >> 1 & 7 : row >> 2 & 3; }
 
   __device__ __forceinline__ FastPanel(const Panel<T>& p, int64_t plane) : base(p.base), plane(plane) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
