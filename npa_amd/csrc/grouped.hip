@@ -827,13 +827,16 @@ Laid lay_out(Layouts& l, const T* x, int64_t stride, int64_t rows, int64_t cols,
   return Laid{to, ld, rows * ld};
 }
 
-// Whether a product's operands are laid out first: float32 and 16-bit rows of
-// any kind where the product is large beside them, and not where that takes more
-// than 16 GB.
-bool lays_out(int type, int64_t slots, int experts, int64_t cols, int64_t outs) {
-  if (cols < 64 || outs < 64 || slots < 64 * (int64_t)experts) return false;
+// Whether a layer's products have their operands laid out first: float32, and
+// 16-bit rows that are not whole pieces.  The copies pay where experts have rows
+// enough for their weights' and each value meets enough others, and not where they
+// take more than 16 GB.  us so, and as they are: float16 8191 rows of 4 experts, 2049
+// -> 1030, 98 and 104, with gradients 302 and 494; 1023 rows of 7 60 and 51, 200 and
+// 149; float32 291 and 355, 951 and 1567; 4000 rows of 16 305 and 286.
+bool lays_out(int type, int64_t slots, int experts, int64_t cols, int64_t outs, bool back) {
+  if (cols < 256 || outs < 256 || slots < 512 * (int64_t)experts) return false;
   if (Layouts::bytes_of(type, slots, cols + outs) + Layouts::bytes_of(type, experts * outs, cols) > int64_t(1) << 34) return false;
-  return slots * cols * outs >= (int64_t(1) << (type == SPHOPS_F32 ? 32 : 31));
+  return slots * cols * outs >= (int64_t(1) << (type != SPHOPS_F32 && !back ? 35 : 32));
 }
 
 // A product over rows: its tiles, how many of their workgroups the card holds, and
@@ -950,7 +953,7 @@ bool fast_as_is(const void* x, int64_t xs, int64_t cols, const void* w, int64_t 
 
 int64_t group_linear_workspace_bytes(int type, int64_t slots, int experts, int64_t cols, int64_t outs) {
   Layouts l{nullptr};
-  const bool laid = lays_out(type, slots, experts, cols, outs);
+  const bool laid = lays_out(type, slots, experts, cols, outs, false);
   if (laid) {
     l.take(Layouts::bytes_of(type, slots, cols));
     l.take(Layouts::bytes_of(type, experts * outs, cols));
@@ -973,7 +976,7 @@ void run_group_linear(const void* x, int type, int64_t xs, const void* w, const 
       const dim3 grid((uint32_t)tiles_of(outs, 16), (uint32_t)(experts + 1), (uint32_t)tiles_of(slots, kTokenRows));
       hipLaunchKernelGGL((k_group_tokens<T>), grid, dim3(kTokenThreads), 0, st, px, xs, pw, pb, offsets, py, slots,
                          experts, (int)cols, (int)outs, relu);
-    } else if (as_is || lays_out(type, slots, experts, cols, outs)) {
+    } else if (as_is || lays_out(type, slots, experts, cols, outs, false)) {
       const Laid lx = as_is ? Laid{x, xs, 0} : lay_out(l, px, xs, slots, cols, st);
       const Laid lw = as_is ? Laid{w, cols, 0} : lay_out(l, pw, cols, experts * outs, cols, st);
       rows_fast<T, false>(l, lx, lw, pb, nullptr, offsets, py, slots, experts, cols, outs, relu, st);
@@ -993,7 +996,7 @@ int64_t group_backward_workspace_bytes(int type, int64_t slots, int experts, int
     chunks = std::max(chunks, grad_plan(slots, experts, cols, outs, 256, 128).chunks);
   Layouts l{nullptr};
   l.take(chunks * (cols * outs + outs) * (int64_t)sizeof(float));
-  const bool laid = lays_out(type, slots, experts, cols, outs);
+  const bool laid = lays_out(type, slots, experts, cols, outs, true);
   if (laid) {
     l.take(Layouts::bytes_of(type, slots, outs));
     l.take(Layouts::bytes_of(type, experts * outs, cols));
@@ -1013,7 +1016,7 @@ void run_group_backward(const void* dy, int64_t dys, const void* x, int type, in
     constexpr bool wide = std::is_same_v<T, float>;
     const T *pdy = static_cast<const T*>(dy), *px = static_cast<const T*>(x), *pw = static_cast<const T*>(w);
     const T* const pm = static_cast<const T*>(mask);
-    const bool laid = lays_out(type, slots, experts, cols, outs);
+    const bool laid = lays_out(type, slots, experts, cols, outs, true);
     const bool rows_as_is = fast_as_is<T>(dy, dys, outs, w, cols) && cols % 8 == 0;
     const bool grad_as_is = fast_as_is<T>(dy, dys, outs, x, xs) && cols % 8 == 0;
     Layouts l{static_cast<char*>(work)};

@@ -306,6 +306,8 @@ def test_linear_of_large_tiles(dtype):
 def test_linear_of_cut_tiles(dtype):
     """Long sums over few tiles, which are cut along the sum: laid out first, as they are, short tiles, few outputs."""
     _check_linear([2000, 2200, 1, 0], 100, 1030, 1060, dtype)
+    _check_linear([5500, 0, 4900], 100, 1999, 1801, dtype)
+    _check_linear([1100, 3], 100, 2001, 2009, dtype, bias=False)
     _check_linear([600, 90, 1], 40, 2048, 1536, dtype, bias=False)
     _check_linear([300, 0, 77], 9, 1545, 125, dtype)
     _check_linear([300, 0, 77], 9, 1000, 33, dtype)
