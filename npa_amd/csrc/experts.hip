@@ -99,6 +99,8 @@ __device__ __forceinline__ void scan_experts(uint32_t* __restrict__ total, int e
 }
 
 // hist[key * tiles + tile]: the tile's entries of each key.
+// Bound (this, the scan and the places): latency; 2^20 entries of 4 experts in 9 + 5
+// + 9 us, 16384 of 64 in 4 + 3 + 5, one launch of 3 for a few.
 template <int ITEMS>
 __global__ __launch_bounds__(kSortThreads) void k_sort_count(const void* __restrict__ index, bool wide, int64_t n,
                                                              int experts, int bits, uint32_t* __restrict__ hist) {
@@ -200,7 +202,8 @@ __device__ __forceinline__ Piece<T> scaled(const Piece<T>& p, float w) {
 }
 
 // out[slot[r, j]] = x[r], zeros for an entry without an expert.  L lanes a row's
-// block of L x N pieces.
+// block of L x N pieces.  Bound: HBM; 8192 x 4096 bfloat16, two entries each, in 34 us
+// (201 MB, part of them in cache).
 template <class T, int L, int N>
 __global__ __launch_bounds__(kMoveThreads) void k_rows_out(const T* __restrict__ x, int64_t stride,
                                                            const int32_t* __restrict__ slot, T* __restrict__ out,
@@ -228,7 +231,8 @@ __global__ __launch_bounds__(kMoveThreads) void k_rows_out(const T* __restrict__
 
 // The backward of k_rows_in: out[slot[r, j]] = w[r, j] dy[r] (zeros without an
 // expert) and dw[r, j] = result[slot[r, j]] . dy[r] (0 without one).  HELD: the
-// row's pieces stay in registers over its entries.
+// row's pieces stay in registers over its entries.  Bound: HBM; 8192 x 4096
+// bfloat16, two entries each, in 61 us (5.5 TB/s).
 template <class T, int L, int N, bool HELD>
 __global__ __launch_bounds__(kMoveThreads) void k_rows_in_backward(
     const T* __restrict__ dy, int64_t stride, const T* __restrict__ results, const float* __restrict__ w,
@@ -293,7 +297,9 @@ __global__ __launch_bounds__(kMoveThreads) void k_rows_in_backward(
 }
 
 // y[r] = the sum over its entries, in their order, of w[r, j] result[slot[r,
-// j]] (w null: 1), in float32; entries without an expert are left out.
+// j]] (w null: 1), in float32; entries without an expert are left out.  Bound: HBM;
+// 2^20 x 83 float32, one entry each, in 150 us (4.6 TB/s), 8192 x 4096 bfloat16, two, in
+// 43.
 template <class T, int L, int N>
 __global__ __launch_bounds__(kMoveThreads) void k_rows_in(const T* __restrict__ results, int64_t stride,
                                                           const float* __restrict__ w,
