@@ -796,6 +796,16 @@ GradPlan chosen_plan(int64_t slots, int experts, int64_t cols, int64_t outs, boo
   return grad_plan(slots, experts, cols, outs, bm, bn);
 }
 
+// That of float32 rows laid out in pieces: tiles of 256 x 128 where they fill the
+// chip, else 128 x 128, of which more need no chunks (with gradients, 256 x 128
+// against 128 x 128: 16384 rows of 8 experts, 1024 -> 1024, 861 us and 797; 4096 of 4
+// 319 and 300; 8192 of 4, 1024 -> 2048, 805 and 779; but 16384 of 2, 1024 -> 1024,
+// 732 and 747).
+GradPlan laid_plan(int64_t slots, int experts, int64_t cols, int64_t outs) {
+  const bool tall = tiles_of(outs, 256) * tiles_of(cols, 128) * experts >= 512;
+  return grad_plan(slots, experts, cols, outs, tall ? 256 : 128, 128);
+}
+
 }  // namespace
 
 bool group_linear_fits(int64_t slots, int experts, int64_t cols, int64_t outs) {
@@ -1013,7 +1023,7 @@ int64_t group_backward_workspace_bytes(int type, int64_t slots, int experts, int
   for (const bool fast : {false, true})
     chunks = std::max(chunks, chosen_plan(slots, experts, cols, outs, type == SPHOPS_F32, fast).chunks);
   if (type == SPHOPS_F32)
-    chunks = std::max(chunks, grad_plan(slots, experts, cols, outs, 256, 128).chunks);
+    chunks = std::max(chunks, laid_plan(slots, experts, cols, outs).chunks);
   Layouts l{nullptr};
   l.take(chunks * (cols * outs + outs) * (int64_t)sizeof(float));
   const bool laid = lays_out(type, slots, experts, cols, outs, true);
@@ -1042,7 +1052,7 @@ void run_group_backward(const void* dy, int64_t dys, const void* x, int type, in
     Layouts l{static_cast<char*>(work)};
     int64_t chunks = 0;
     for (const bool fast : {false, true}) chunks = std::max(chunks, chosen_plan(slots, experts, cols, outs, wide, fast).chunks);
-    if (wide) chunks = std::max(chunks, grad_plan(slots, experts, cols, outs, 256, 128).chunks);
+    if (wide) chunks = std::max(chunks, laid_plan(slots, experts, cols, outs).chunks);
     float* const part = reinterpret_cast<float*>(l.work + l.take(chunks * (nw + outs) * (int64_t)sizeof(float)));
     Laid ldy{dy, dys, 0};
     const bool lay_dy = slots > 0 && laid && ((dx != nullptr && !rows_as_is) || (sums && !grad_as_is));
@@ -1058,7 +1068,7 @@ void run_group_backward(const void* dy, int64_t dys, const void* x, int type, in
     }
     if (!sums) return;
     const bool fast = grad_as_is || (laid && slots > 0);
-    const GradPlan p = wide && fast ? grad_plan(slots, experts, cols, outs, 256, 128)
+    const GradPlan p = wide && fast ? laid_plan(slots, experts, cols, outs)
                                     : chosen_plan(slots, experts, cols, outs, wide, fast);
     float* const to = p.chunks > 0 ? part : nullptr;
     const dim3 grid((uint32_t)((p.chunks > 0 ? p.chunks : experts) * p.mt * p.nt));
@@ -1071,7 +1081,10 @@ void run_group_backward(const void* dy, int64_t dys, const void* x, int type, in
                            static_cast<const E*>(lx.base), lx.stride, lx.plane, offsets, pdw, pdb, to, slots, experts,
                            (int)cols, (int)outs, p.chunk, p.mt, p.nt);
       };
-      if constexpr (wide) with(k_group_weight_grad_fast<T, 256, 128, 4, 2>, 512);
+      if constexpr (wide) {
+        if (p.bm == 256) with(k_group_weight_grad_fast<T, 256, 128, 4, 2>, 512);
+        else with(k_group_weight_grad_fast<T, 128, 128, 2, 2>, 256);
+      }
       else if (p.bm == 256) with(k_group_weight_grad_fast<T, 256, 256, 2, 4>, 512);
       else with(k_group_weight_grad_fast<T, 128, 128, 2, 2>, 256);
     } else {
