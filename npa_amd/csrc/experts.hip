@@ -100,7 +100,7 @@ __device__ __forceinline__ void scan_experts(uint32_t* __restrict__ total, int e
 
 // hist[key * tiles + tile]: the tile's entries of each key.
 // Bound (this, the scan and the places): latency; 2^20 entries of 4 experts in 9 + 5
-// + 9 us, 16384 of 64 in 4 + 3 + 5, one launch of 3 for a few.
+// + 9 us, 16384 of 64 in 5 + 5 + 5, one launch of 3 for a few.
 template <int ITEMS>
 __global__ __launch_bounds__(kSortThreads) void k_sort_count(const void* __restrict__ index, bool wide, int64_t n,
                                                              int experts, int bits, uint32_t* __restrict__ hist) {
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(kMoveThreads) void k_rows_out(const T* __restrict__
 // The backward of k_rows_in: out[slot[r, j]] = w[r, j] dy[r] (zeros without an
 // expert) and dw[r, j] = result[slot[r, j]] . dy[r] (0 without one).  HELD: the
 // row's pieces stay in registers over its entries.  Bound: HBM; 8192 x 4096
-// bfloat16, two entries each, in 61 us (5.5 TB/s).
+// bfloat16, two entries each, in 62 us (5.4 TB/s).
 template <class T, int L, int N, bool HELD>
 __global__ __launch_bounds__(kMoveThreads) void k_rows_in_backward(
     const T* __restrict__ dy, int64_t stride, const T* __restrict__ results, const float* __restrict__ w,
@@ -298,8 +298,8 @@ __global__ __launch_bounds__(kMoveThreads) void k_rows_in_backward(
 
 // y[r] = the sum over its entries, in their order, of w[r, j] result[slot[r,
 // j]] (w null: 1), in float32; entries without an expert are left out.  Bound: HBM;
-// 2^20 x 83 float32, one entry each, in 150 us (4.6 TB/s), 8192 x 4096 bfloat16, two, in
-// 43.
+// 2^20 x 83 float32, one entry each, in 155 us (4.5 TB/s), 8192 x 4096 bfloat16, two, in
+// 46.
 template <class T, int L, int N>
 __global__ __launch_bounds__(kMoveThreads) void k_rows_in(const T* __restrict__ results, int64_t stride,
                                                           const float* __restrict__ w,
