@@ -795,13 +795,15 @@ GradPlan chosen_plan(int64_t slots, int experts, int64_t cols, int64_t outs, boo
   return grad_plan(slots, experts, cols, outs, bm, bn);
 }
 
-// That of float32 rows laid out in pieces: tiles of 256 x 128 where they fill the
-// chip, else 128 x 128, of which more need no chunks (with gradients, 256 x 128
-// against 128 x 128: 16384 rows of 8 experts, 1024 -> 1024, 861 us and 797; 4096 of 4
-// 319 and 300; 8192 of 4, 1024 -> 2048, 805 and 779; but 16384 of 2, 1024 -> 1024,
-// 732 and 747).
+// That of float32 rows laid out in pieces: 256 x 128 where such tiles fill the chip
+// without chunks and an expert has rows for a long sum, else 128 x 128.  us with
+// gradients, 256 x 128 and 128 x 128: 16384 rows of 8 experts, 2048 -> 2048, 2689 and
+// 2790; 16384 of 4, 2048 -> 4096, 4922 and 5150; short sums: 16384 of 16, 1024 ->
+// 1024, 1009 and 859; 8192 of 8, 1024 -> 2048, 871 and 806; few tiles: 16384 of 8, 1024
+// -> 1024, 861 and 797; 8192 of 4, 1024 -> 2048, 805 and 779; but 16384 of 2, 1024 ->
+// 1024, 732 and 747.
 GradPlan laid_plan(int64_t slots, int experts, int64_t cols, int64_t outs) {
-  const bool tall = tiles_of(outs, 256) * tiles_of(cols, 128) * experts >= 512;
+  const bool tall = tiles_of(outs, 256) * tiles_of(cols, 128) * experts >= 512 && slots >= 2048 * (int64_t)experts;
   return grad_plan(slots, experts, cols, outs, tall ? 256 : 128, 128);
 }
 

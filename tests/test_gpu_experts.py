@@ -315,6 +315,12 @@ def test_linear_of_cut_tiles(dtype):
     _check_linear([530, 3], 0, 20, 1030, dtype)
 
 
+@pytest.mark.parametrize("counts", [[4095, 9], [17000, 9]])
+def test_linear_of_tall_weight_tiles(counts):
+    """float32 weight gradients of many tiles, long sums: whole, and in chunks."""
+    _check_linear(counts, 5, 4000, 4080, F32)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_linear_of_many_rows(dtype):
     _check_linear([20000, 3, 0, 9000, 40001], 77, 83, 35, dtype)
