@@ -298,7 +298,11 @@ def linear(x, weight, bias, offsets):
     last expert's zeros.  ``weight`` (experts, out, in) and ``bias`` (experts,
     out; may be None) are of x's type; ``offsets`` (int32, as in a ``Routing``)
     starts at 0 and does not decrease.  The gradients of an expert without rows
-    are zeros."""
+    are zeros.
+
+    Large float32 products run on bfloat16 pieces of their factors: there a value
+    that is not finite may give NaN where float32 gives an infinity, and factors below
+    2^-110 lose their last bits."""
     slots, experts, cols = _check_sorted(x, offsets)
     weight, bias = _check_layer(x, weight, bias, slots, experts, cols, "weight")
     if _rows.wants_grad(x, weight, bias):
@@ -312,7 +316,7 @@ def mlp(x, w1, b1, w2, b2, offsets):
     automaton's update rule, take one kernel each way, which keeps the hidden
     values in registers.  Elsewhere the ReLU is in the first layer's kernel and its
     mask in the second one's input gradient, and the hidden values, and their
-    gradient, are kept in x's type."""
+    gradient, are kept in x's type.  float32 as in ``linear``."""
     slots, experts, cols = _check_sorted(x, offsets)
     w1, b1 = _check_layer(x, w1, b1, slots, experts, cols, "w1")
     hidden = w1.shape[1]
