@@ -176,7 +176,7 @@ __device__ __forceinline__ void put_rows(const f32x16& acc, float* __restrict__ 
 // A slice's sums go to `slices` (null: no tile is cut).
 // 16-bit rows of any length at any place, through registers into LDS, the next
 // step's loads under this one's products.  Bound: their latency, two barriers a
-// step: 1023 rows of 7 experts, 2049 -> 1030 float16, in 26 us and 9 for the join.
+// step: 1023 rows of 7 experts, 2049 -> 1030 float16, in 25 us and 9 for the join.
 template <class T, bool BACK>
 __global__ __launch_bounds__(kGroupThreads) void k_group_rows(const T* __restrict__ x, int64_t xs,
                                                               const T* __restrict__ w, const T* __restrict__ b,
@@ -235,10 +235,10 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_rows(const T* __restric
 // from memory to LDS.  A slice's sums go to `slices` (null: no tile is cut) as
 // they stand in registers.
 // Bound: the matrix cores and what stands between two steps (one barrier, then the
-// operands' first reads): 16384 rows of 8 experts, 2048 -> 4096 bfloat16 in 403 us
+// operands' first reads): 16384 rows of 8 experts, 2048 -> 4096 bfloat16 in 404 us
 // (0.68 PFLOP/s, its fastest run 326; the library's one product of that size without experts 242), 41% of
-// the cycles matrix-busy; 8192 rows of 4, 1024 -> 2048 float32 in 258 us (133
-// TFLOP/s, the library's float32 135), 43%.  Reading the operands of the next 16 of
+// the cycles matrix-busy; 8192 rows of 4, 1024 -> 2048 float32 in 249 us (138
+// TFLOP/s, the library's float32 135), 46%.  Reading the operands of the next 16 of
 // the sum under the products of these changed nothing.
 template <class T, bool BACK, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void k_group_rows_fast(
@@ -604,7 +604,7 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_weight_grad(const T* __
 // The same for 16-bit rows in whole 16-byte pieces, or float32 rows laid out in
 // bfloat16 pieces, straight from memory to LDS; db from products with ones.
 // Bound: as k_group_rows_fast; 16384 rows of 8 experts, 2048 and 4096 wide, bfloat16
-// in 356 us (0.77 PFLOP/s), 8192 rows of 4, 1024 and 2048, float32 in 301.
+// in 356 us (0.77 PFLOP/s), 8192 rows of 4, 1024 and 2048, float32 in 293.
 template <class T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void k_group_weight_grad_fast(
     const Piece16<T>* __restrict__ dy, int64_t dys, int64_t dyp, const Piece16<T>* __restrict__ x, int64_t xs, int64_t xp,
