@@ -133,7 +133,7 @@ class _Combine(torch.autograd.Function):
         results = results if results.is_contiguous() else results.contiguous()
         u, rows, stride = _rows.rows_view(dy)
         d_results = torch.empty_like(results) if need_r else None
-        dw = torch.empty(slot.shape, device=dy.device) if need_w else None
+        dw = torch.empty(slot.shape, dtype=torch.float32, device=dy.device) if need_w else None
         _rows.call(_lib.sphops_combine_rows_backward, dy.device, u.data_ptr(), TYPES[dy.dtype], stride,
                    results.data_ptr(), address(weight), slot.data_ptr(), source.data_ptr(), address(d_results),
                    address(dw), rows, slot.shape[-1], dy.shape[-1])
@@ -228,7 +228,7 @@ class _Mlp(torch.autograd.Function):
 def _fused_forward(x, w1, b1, w2, b2, offsets, keep):
     """y, and what the input gradient reads of the hidden values (a bit of each)."""
     (experts, hidden, cols), outs, slots = w1.shape, w2.shape[1], x.shape[0]
-    y = torch.empty(slots, outs, device=x.device)
+    y = torch.empty(slots, outs, dtype=torch.float32, device=x.device)
     mask = torch.empty(slots, 4, dtype=torch.int32, device=x.device) if keep else None
     _rows.call(_lib.sphops_expert_mlp_forward, x.device, x.data_ptr(), w1.data_ptr(), address(b1), w2.data_ptr(),
                address(b2), offsets.data_ptr(), y.data_ptr(), address(mask), slots, experts, cols, hidden, outs)
@@ -258,9 +258,9 @@ class _FusedMlp(torch.autograd.Function):
                        mask.data_ptr(), offsets.data_ptr(), dx.data_ptr(), slots, experts, cols, hidden, outs)
         if need_w1 or need_b1 or need_w2 or need_b2:
             dw1 = torch.empty_like(w1) if need_w1 else None
-            db1 = torch.empty(experts, hidden, device=dev) if need_b1 else None
+            db1 = torch.empty(experts, hidden, dtype=torch.float32, device=dev) if need_b1 else None
             dw2 = torch.empty_like(w2) if need_w2 else None
-            db2 = torch.empty(experts, outs, device=dev) if need_b2 else None
+            db2 = torch.empty(experts, outs, dtype=torch.float32, device=dev) if need_b2 else None
             work = torch.empty(max(_lib.sphops_expert_mlp_workspace_bytes(slots, experts, cols, hidden, outs), 1),
                                dtype=torch.uint8, device=dev)
             _rows.call(_lib.sphops_expert_mlp_weight_grad, dev, x.data_ptr(), dy.data_ptr(), w1.data_ptr(), address(b1),

@@ -68,10 +68,10 @@ def _weight_grad(x2, dy2, has_bias, relu_x=False):
     x2, dy2 = x2.contiguous(), dy2.contiguous()
     rows, in_f = x2.shape
     out_f = dy2.shape[1]
-    dw = torch.empty(out_f, in_f, device=x2.device)
-    db = torch.empty(out_f, device=x2.device) if has_bias else None
+    dw = torch.empty(out_f, in_f, dtype=torch.float32, device=x2.device)
+    db = torch.empty(out_f, dtype=torch.float32, device=x2.device) if has_bias else None
     nbytes = _lib.sphops_linear_weight_grad_workspace_bytes(rows, in_f, out_f)
-    work = torch.empty(max(nbytes // 4, 1), device=x2.device)
+    work = torch.empty(max(nbytes // 4, 1), dtype=torch.float32, device=x2.device)
     st = ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(x2.device.index))
     fn = _lib.sphops_relu_linear_weight_grad if relu_x else _lib.sphops_linear_weight_grad
     _native.check(fn(_ptr(x2), _ptr(dy2), _ptr(dw), _ptr(db), rows, in_f, out_f, _ptr(work), st))
@@ -104,7 +104,7 @@ class ReluLinear(torch.autograd.Function):
             a2 = a2.clone()
         w = weight.detach().contiguous()
         b = None if bias is None else bias.detach().contiguous()
-        y = torch.empty(a2.shape[0], out_f, device=a.device)
+        y = torch.empty(a2.shape[0], out_f, dtype=torch.float32, device=a.device)
         st = ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(a.device.index))
         _native.check(_lib.sphops_relu_linear_forward(_ptr(a2), _ptr(w), _ptr(b), _ptr(y), a2.shape[0], in_f,
                                                       out_f, st))
@@ -152,8 +152,8 @@ class MlpRows(torch.autograd.Function):
         dense = [None if t is None else t.detach().contiguous() for t in (w1, b1, w2, b2)]
         ctx.shape = (rows, in_f, hidden, out_f)
         ctx.biases = (b1 is not None, b2 is not None)
-        a = torch.empty(rows, hidden, device=z.device) if keep else None
-        y = torch.empty(rows, out_f, device=z.device)
+        a = torch.empty(rows, hidden, dtype=torch.float32, device=z.device) if keep else None
+        y = torch.empty(rows, out_f, dtype=torch.float32, device=z.device)
         _native.check(_lib.sphops_mlp_forward(_ptr(z2), *(_ptr(t) for t in dense), _ptr(a), _ptr(y), rows, in_f,
                                               hidden, out_f, _stream(z)))
         if keep:
@@ -177,12 +177,12 @@ class MlpRows(torch.autograd.Function):
             dz = dz.reshape(dy.shape[:-1] + (in_f,))
         if need_w1 or need_b1 or need_w2 or need_b2:
             dev = z2.device
-            dw1 = torch.empty(hidden, in_f, device=dev) if need_w1 else None
-            db1 = torch.empty(hidden, device=dev) if need_b1 else None
-            dw2 = torch.empty(out_f, hidden, device=dev) if need_w2 else None
-            db2 = torch.empty(out_f, device=dev) if need_b2 else None
+            dw1 = torch.empty(hidden, in_f, dtype=torch.float32, device=dev) if need_w1 else None
+            db1 = torch.empty(hidden, dtype=torch.float32, device=dev) if need_b1 else None
+            dw2 = torch.empty(out_f, hidden, dtype=torch.float32, device=dev) if need_w2 else None
+            db2 = torch.empty(out_f, dtype=torch.float32, device=dev) if need_b2 else None
             nbytes = _lib.sphops_mlp_weight_grad_workspace_bytes(rows, in_f, hidden, out_f)
-            work = torch.empty(max(nbytes // 4, 1), device=dev)
+            work = torch.empty(max(nbytes // 4, 1), dtype=torch.float32, device=dev)
             _native.check(_lib.sphops_mlp_weight_grad(_ptr(z2), _ptr(a), _ptr(dy2), _ptr(w2c), _ptr(dw1), _ptr(db1),
                                                       _ptr(dw2), _ptr(db2), rows, in_f, hidden, out_f, _ptr(work),
                                                       st))
@@ -294,8 +294,8 @@ class MlpRows8(torch.autograd.Function):
         dense = [_dense(t) for t in (w1, b1, w2, b2)]
         ctx.shape, ctx.has_b2 = (rows, in_f, hidden, out_f), b2 is not None
         codes = torch.empty(rows, -(-in_f // 4) * 4, dtype=torch.int8, device=dev)
-        scale = torch.empty(rows, device=dev)
-        y = torch.empty(rows, out_f, device=dev)
+        scale = torch.empty(rows, dtype=torch.float32, device=dev)
+        y = torch.empty(rows, out_f, dtype=torch.float32, device=dev)
         _native.check(_lib.sphops_mlp_rows8_forward(
             z2.data_ptr(), *map(_address, dense), codes.data_ptr(), codes.shape[1], scale.data_ptr(), y.data_ptr(),
             rows, in_f, hidden, out_f, torch._C._cuda_getCurrentRawStream(dev.index)))
@@ -311,11 +311,11 @@ class MlpRows8(torch.autograd.Function):
             raise TypeError("the MLP kernels take float32 GPU tensors")
         lead, dev = dy.shape[:-1], dy.device
         dy = _dense(dy if dy.dim() == 2 else dy.reshape(-1, out_f))
-        dz = torch.empty(rows, in_f, device=dev) if need_z else None
-        dw1 = torch.empty(hidden, in_f, device=dev) if need_w1 else None
-        db1 = torch.empty(hidden, device=dev) if need_b1 and b1 is not None else None
-        dw2 = torch.empty(out_f, hidden, device=dev) if need_w2 else None
-        db2 = torch.empty(out_f, device=dev) if need_b2 and ctx.has_b2 else None
+        dz = torch.empty(rows, in_f, dtype=torch.float32, device=dev) if need_z else None
+        dw1 = torch.empty(hidden, in_f, dtype=torch.float32, device=dev) if need_w1 else None
+        db1 = torch.empty(hidden, dtype=torch.float32, device=dev) if need_b1 and b1 is not None else None
+        dw2 = torch.empty(out_f, hidden, dtype=torch.float32, device=dev) if need_w2 else None
+        db2 = torch.empty(out_f, dtype=torch.float32, device=dev) if need_b2 and ctx.has_b2 else None
         dense = [_dense(t) for t in (w1, b1, w2)]
         work = torch.empty(max(_lib.sphops_mlp_rows8_workspace_bytes(rows, in_f, hidden, out_f), 1),
                            dtype=torch.uint8, device=dev)

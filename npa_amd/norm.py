@@ -26,7 +26,7 @@ def _forward(x, weight, bias, eps, keep):
     cols = x.shape[-1]
     v, rows, stride = _rows.rows_view(x)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty(rows, 2, device=x.device) if keep else None
+    stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device) if keep else None
     wide = any(t is not None and t.dtype == torch.float32 for t in (weight, bias))
     _rows.call(_lib.sphops_layer_norm, x.device, v.data_ptr(), TYPES[x.dtype], stride, address(weight), address(bias),
                int(wide), y.data_ptr(), address(stats), rows, cols, eps)
