@@ -133,7 +133,7 @@ def quantize_rows(x, relu=False, align=4):
     v, rows, stride = _rows_view(x)
     ld = -(-cols // align) * align
     codes = torch.empty(rows, ld, dtype=torch.int8, device=x.device)
-    scale = torch.empty(rows, device=x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
     _native.check(_lib.sphops_quantize_rows(_ptr(v), TYPES[x.dtype], stride, _ptr(codes), ld, _ptr(scale), rows, cols,
                                             int(relu), _stream(x)))
     return Rows8(codes, scale, tuple(x.shape))
@@ -165,8 +165,8 @@ def weight_grad(r, dy, bias=True):
     nbytes = _lib.sphops_rows8_weight_grad_workspace_bytes(rows, nin, nout)
     if nbytes < 0:
         raise RuntimeError(f"no weight gradient for {rows} rows of {nin} inputs and {nout} outputs")
-    dw = torch.empty(nout, nin, device=dy.device)
-    db = torch.empty(nout, device=dy.device) if bias else None
+    dw = torch.empty(nout, nin, dtype=torch.float32, device=dy.device)
+    db = torch.empty(nout, dtype=torch.float32, device=dy.device) if bias else None
     work = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dy.device)
     _native.check(_lib.sphops_rows8_weight_grad(_ptr(r.codes), r.codes.shape[1], _ptr(r.scale), _ptr(dy), _ptr(dw),
                                                 _ptr(db), rows, nin, nout, _ptr(work), _stream(dy)))
@@ -223,7 +223,7 @@ def mlp(z, w1, b1, w2, b2):
     rows = zc.numel() // nin
     if rows > MAX_ROWS:
         raise RuntimeError(f"z must have at most {MAX_ROWS} rows")
-    y = torch.empty(*z.shape[:-1], nout, device=z.device)
+    y = torch.empty(*z.shape[:-1], nout, dtype=torch.float32, device=z.device)
     _native.check(_lib.sphops_mlp8_forward(
         zc.data_ptr(), w1.codes.data_ptr(), w1.codes.shape[1], w1.scale.data_ptr(),
         None if b1 is None else b1.data_ptr(), w2.codes.data_ptr(), w2.codes.shape[1], w2.scale.data_ptr(),
@@ -253,7 +253,7 @@ def first_order(what, *grads):
     some = [g for g in grads if g is not None]
     if not torch.is_grad_enabled() or not some:
         return grads
-    held = iter(_Once.apply(what, torch.zeros((), requires_grad=True), *some))
+    held = iter(_Once.apply(what, torch.zeros((), dtype=torch.float32, requires_grad=True), *some))
     return tuple(None if g is None else next(held) for g in grads)
 
 

@@ -85,10 +85,10 @@ class PerceptionFeatures(torch.autograd.Function):
         dz = dz.contiguous()
         B, N = dz.shape[:2]
         need = ctx.needs_input_grad
-        d_s = torch.empty(B, N, C, device=dz.device) if need[0] else None
-        d_blur = torch.empty(B, N, C, device=dz.device) if need[1] else None
-        d_gs = torch.empty(B, N, C, dim, device=dz.device) if need[2] and grad_s is not None else None
-        d_gr = torch.empty(B, N, dim, device=dz.device) if need[3] and grad_rho is not None else None
+        d_s = torch.empty(B, N, C, dtype=torch.float32, device=dz.device) if need[0] else None
+        d_blur = torch.empty(B, N, C, dtype=torch.float32, device=dz.device) if need[1] else None
+        d_gs = torch.empty(B, N, C, dim, dtype=torch.float32, device=dz.device) if need[2] and grad_s is not None else None
+        d_gr = torch.empty(B, N, dim, dtype=torch.float32, device=dz.device) if need[3] and grad_rho is not None else None
         _native.check(_lib.sphops_perception_features_backward(
             dim, _ptr(dz), _ptr(grad_s), _ptr(grad_rho), _ptr(d_s), _ptr(d_blur), _ptr(d_gs), _ptr(d_gr), B * N, C,
             coef_s, coef_rho, total_mass, flags, _stream(dz)))
@@ -164,7 +164,8 @@ class Perceive(torch.autograd.Function):
             if t is not None and (t.dtype != torch.float32 or t.device != dev):
                 raise TypeError("perceive's gradients must be float32 on the inputs' device")
         if not through:  # only the binning was differentiated
-            dx, ds = (torch.zeros(shape, device=dev) if t is None else t for t, shape in zip(ups[1:], ctx.shapes))
+            dx, ds = (torch.zeros(shape, dtype=torch.float32, device=dev) if t is None else t
+                      for t, shape in zip(ups[1:], ctx.shapes))
             grad_x, grad_s = torch.empty_like(dx), torch.empty_like(ds)
             sph._unbin(snap, dx, ds, None, grad_x, grad_s, None)
             return (grad_x if need_x else None, grad_s if need_s else None) + (None,) * 6

@@ -151,7 +151,7 @@ class HashGrid:
         if self.boundary == "periodic":
             out = []
             for d in range(self.dim):
-                L = torch.tensor(self.grid_size[d] * self.eps, device=x.device)
+                L = torch.tensor(self.grid_size[d] * self.eps, dtype=torch.float32, device=x.device)
                 half_L = 0.5 * L
                 out.append(torch.remainder(x[..., d] + half_L, L) - half_L)
             return torch.stack(out, dim=-1)

@@ -35,7 +35,7 @@ class Splat(torch.autograd.Function):
             raise RuntimeError(f"x must be (N, 2) and color (N, >= 3); got {tuple(x.shape)}, {tuple(color.shape)}")
         x, color = x.contiguous(), color.contiguous()
         images = starts.numel() - 1
-        out = torch.empty(images, img_size, img_size, 4, device=x.device)
+        out = torch.empty(images, img_size, img_size, 4, dtype=torch.float32, device=x.device)
         args = (x.shape[0], color.shape[1], img_size, float(sigma), float(lo), float(hi), int(bool(normalize_color)),
                 int(bool(y_up)), float(pixel_size))
         work = torch.empty(max(1, _lib.sphops_splat_workspace_bytes(x.shape[0])), dtype=torch.uint8, device=x.device)

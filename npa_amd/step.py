@@ -58,7 +58,7 @@ class EulerUpdate(torch.autograd.Function):
                     raise RuntimeError(f"{what} must have shape {shape}, got {tuple(t.shape)}")
         x_out = torch.empty_like(x_bin)
         s_out = torch.empty_like(s_bin)
-        dx_norm = torch.empty(B, N, device=y.device)
+        dx_norm = torch.empty(B, N, dtype=torch.float32, device=y.device)
         st = ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(y.device.index))
         _native.check(_lib.sphops_euler_update_forward(
             dim, P, _ptr(y), _ptr(x_bin), _ptr(s_bin), _ptr(mask), _ptr(noise), _ptr(x_out), _ptr(s_out),

@@ -21,7 +21,8 @@ def other_default(request):
     torch.set_default_dtype(before)
 
 
-@pytest.mark.parametrize("module", ["norm.py", "experts.py", "mlp.py"])
+@pytest.mark.parametrize("module", ["norm.py", "experts.py", "mlp.py", "int8.py", "step.py", "perceive.py",
+                                    "splatting.py", "sphops/sph.py", "sphops/sph_hip.py"])
 def test_allocations_name_their_type(module):
     with open(os.path.join(ROOT, module)) as f:
         tree = ast.parse(f.read())

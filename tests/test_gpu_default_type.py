@@ -61,8 +61,59 @@ def _module(g):
     return [_randn(g, 90, 20), *mix.parameters()], lambda x, *_: mix(x)
 
 
+def _int8(g):
+    from npa_amd import int8
+    w = int8.quantize_rows(_randn(g, 30, 83), align=16)
+    dy = _randn(g, 70, 12)
+
+    def run(x):
+        r = int8.quantize_rows(x)
+        assert r.scale.dtype == torch.float32
+        with torch.no_grad():
+            out = [int8.linear(x, w), *int8.weight_grad(r, dy), r.codes.float(), r.scale]
+        return torch.cat([t.flatten() for t in out]) + int8.restore_rows(r).sum() + 0 * x.sum()
+
+    return [_randn(g, 70, 83)], run
+
+
+def _step(dim):
+    """A step of an automaton, perception and splatted image with it."""
+    def make(g):
+        import types
+
+        import npa_amd.sphops as sp
+        from npa_amd.splatting import splat_particles_batch
+        from npa_amd.step import step_euler
+        C, N = 8, 400
+        cols = 2 * C + dim * C + dim
+        rule = torch.nn.Sequential(torch.nn.Linear(cols, 128), torch.nn.ReLU(), torch.nn.Linear(128, dim + C))
+        rule = rule.to("cuda", torch.float32)
+        with torch.no_grad():
+            for p in rule.parameters():
+                p.copy_(0.1 * _randn(g, *p.shape))
+        model = types.SimpleNamespace(spatial_dims=dim, eps0=0.1, alpha=0.5, model=rule, state_grad=True,
+                                      density_grad=True, log_norm_grad=True, log_norm_density_grad=True,
+                                      stopgrad_pos=False, stopgrad_state=False)
+        x = 1.2 * torch.rand(1, N, dim, dtype=torch.float32, device="cuda", generator=g) - 0.6
+
+        def run(s, *_):
+            grid = sp.HashGrid(dim=dim, boundary="periodic", mode="grid", grid_size=[16] * dim, eps=0.1, num_particles=N,
+                               batch_size=1, max_particles_per_block=64)
+            at = grid.wrap_positions(x)
+            at = torch.cat([at, torch.zeros_like(at[..., :1])], -1) if dim == 3 else at  # rows of 4 in 3D
+            xs, ss, _ = step_euler(model, at, s, grid, update_prob=1.0)
+            out = [xs.flatten(), ss.flatten()]
+            if dim == 2:
+                out.append(splat_particles_batch(xs, ss.sigmoid(), img_size=32).flatten())
+            return torch.cat(out)
+
+        return [_randn(g, 1, N, C), *rule.parameters()], run
+    return make
+
+
 @pytest.mark.parametrize("default", [torch.bfloat16, torch.float64])
-@pytest.mark.parametrize("make", [_norm, _combine, _experts(128), _experts(36), _layers(None), _mlp_rows, _module])
+@pytest.mark.parametrize("make", [_norm, _combine, _experts(128), _experts(36), _layers(None), _mlp_rows, _module,
+                                  _layers("int8"), _int8, _step(2), _step(3)])
 def test_results_do_not_depend_on_the_default_type(make, default):
     def run():
         g = torch.Generator(device="cuda").manual_seed(7)
