@@ -60,24 +60,6 @@ __global__ __launch_bounds__(kLayThreads) void k_lay_out(const T* __restrict__ x
   }
 }
 
-// How a product's tiles fall on the card, which holds `room` of their workgroups at
-// once: whole turns of `room` tiles, and the tiles that are left, cut along the sum
-// into `slices` each where that fills a turn better.  Without cuts 8192 x 2048 ->
-// 1024 float32, 272 tiles of 256 x 128 on 256 CUs, took two turns (366 us, 239 with
-// them), and 955 x 1545 -> 125, 20 tiles, one long one.
-struct Turns {
-  uint32_t whole, left, slices;
-};
-constexpr int kMaxSlices = 16, kSliceDepth = 256;  // at most; of the sum that a slice has at least
-__device__ __forceinline__ Turns turns_of(uint32_t tiles, uint32_t room, int depth, bool cut) {
-  Turns t;
-  t.whole = tiles / room * room;
-  t.left = tiles - t.whole;
-  t.slices = 1;
-  if (cut && t.left > 0) t.slices = max(1u, min(min(room / t.left, (uint32_t)(depth / kSliceDepth)), (uint32_t)kMaxSlices));
-  return t;
-}
-
 // A workgroup's part of a product over rows: a tile, or a slice of one.  The
 // launch covers the most that there can be.
 struct RowsJob {
@@ -90,9 +72,9 @@ struct RowsJob {
   __device__ __forceinline__ int last(int steps) const { return (int)((int64_t)steps * (slice + 1) / slices); }
 };
 __device__ __forceinline__ bool rows_job(const int32_t* __restrict__ offsets, int experts, int64_t slots, int size,
-                                         int nt, int room, int depth, bool cut, RowsJob& j) {
+                                         int nt, int room, int places, int depth, RowsJob& j) {
   const int64_t mt = group_tiles(offsets, experts, slots, size, true);
-  const Turns t = turns_of((uint32_t)(mt * nt), (uint32_t)room, depth, cut);
+  const Turns t = turns_of((uint32_t)(mt * nt), (uint32_t)room, (uint32_t)places, depth);
   uint32_t id = blockIdx.x;
   j.slice = 0;
   j.slices = 1;
@@ -183,14 +165,14 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_rows(const T* __restric
                                                               const T* __restrict__ mask,
                                                               const int32_t* __restrict__ offsets, T* __restrict__ y,
                                                               int64_t slots, int experts, int cols, int outs,
-                                                              bool relu, int nt, int room,
+                                                              bool relu, int nt, int room, int places,
                                                               f32x4* __restrict__ slices) {
   using IA = PanelImage<T, true>;
   using IB = PanelImage<T, !BACK>;
   __shared__ __attribute__((aligned(16))) uint16_t lds[std::max(IA::kPlane + IB::kPlane, kOutbox)];
   uint16_t *const as = lds, *const bs = lds + IA::kPlane;
   RowsJob j;
-  if (!rows_job(offsets, experts, slots, kSide, nt, room, cols, slices != nullptr, j)) return;
+  if (!rows_job(offsets, experts, slots, kSide, nt, room, places, cols, j)) return;
   const int64_t m0 = j.g.lo + j.g.tile * kSide;
   const int n0 = j.n * kSide, here = (int)min<int64_t>(kSide, j.g.hi - m0), outs_here = min(kSide, outs - n0);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
@@ -244,12 +226,12 @@ template <class T, bool BACK, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void k_group_rows_fast(
     const Piece16<T>* __restrict__ x, int64_t xs, int64_t xp, const Piece16<T>* __restrict__ w, int64_t ws, int64_t wp,
     const T* __restrict__ b, const T* __restrict__ mask, const int32_t* __restrict__ offsets, T* __restrict__ y,
-    int64_t slots, int experts, int cols, int outs, bool relu, int nt, int room, f32x4* __restrict__ slices) {
+    int64_t slots, int experts, int cols, int outs, bool relu, int nt, int room, int places, f32x4* __restrict__ slices) {
   using E = Piece16<T>;
   using Tile = FastTile<E, kPieces<T>, true, !BACK, BM, BN, WM, WN, false>;
   __shared__ __attribute__((aligned(16))) uint16_t s0[Tile::kStage], s1[Tile::kStage];
   RowsJob j;
-  if (!rows_job(offsets, experts, slots, BM, nt, room, cols, slices != nullptr, j)) return;
+  if (!rows_job(offsets, experts, slots, BM, nt, room, places, cols, j)) return;
   const GroupTile& g = j.g;
   const int64_t m0 = g.lo + g.tile * BM;
   const int n0 = j.n * BN, here = (int)min<int64_t>(BM, g.hi - m0), outs_here = min(BN, outs - n0);
@@ -290,12 +272,12 @@ template <class T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void k_group_rows_join(const T* __restrict__ b, const T* __restrict__ mask,
                                                                   const int32_t* __restrict__ offsets,
                                                                   T* __restrict__ y, int64_t slots, int experts,
-                                                                  int depth, int outs, bool relu, int nt, int room,
+                                                                  int depth, int outs, bool relu, int nt, int room, int places,
                                                                   const f32x4* __restrict__ slices) {
   constexpr int kWaves = WM * WN, TN = BN / WN / 32;
   __shared__ __attribute__((aligned(16))) float room_of[kWaves][1024];
   const int64_t mt = group_tiles(offsets, experts, slots, BM, true);
-  const Turns turns = turns_of((uint32_t)(mt * nt), (uint32_t)room, depth, true);
+  const Turns turns = turns_of((uint32_t)(mt * nt), (uint32_t)room, (uint32_t)places, depth);
   if (turns.slices == 1 || blockIdx.x >= turns.left) return;
   int64_t m;
   int n;
@@ -330,12 +312,12 @@ __global__ __launch_bounds__(kWideThreads) void k_group_rows_wide(const float* _
                                                                   const float* __restrict__ mask,
                                                                   const int32_t* __restrict__ offsets,
                                                                   float* __restrict__ y, int64_t slots, int experts,
-                                                                  int cols, int outs, bool relu, int nt, int room,
+                                                                  int cols, int outs, bool relu, int nt, int room, int places,
                                                                   f32x4* __restrict__ slices) {
   using Tile = WideTile<true, !BACK, BM, BN, WM, WN>;
   __shared__ __attribute__((aligned(16))) float lds[Tile::kRoom];
   RowsJob j;
-  if (!rows_job(offsets, experts, slots, BM, nt, room, cols, slices != nullptr, j)) return;
+  if (!rows_job(offsets, experts, slots, BM, nt, room, places, cols, j)) return;
   const GroupTile& g = j.g;
   const int64_t m0 = g.lo + g.tile * BM;
   const int n0 = j.n * BN, here = (int)min<int64_t>(BM, g.hi - m0), outs_here = min(BN, outs - n0);
@@ -452,11 +434,10 @@ __global__ __launch_bounds__(kTokenThreads) void k_group_tokens(const T* __restr
                                                                 int outs, bool relu) {
   __shared__ Tokens<T> tokens;
   const int e = (int)blockIdx.y, n0 = (int)blockIdx.x * 16;
-  const int64_t lo = e == 0 ? 0 : min<int64_t>(max(offsets[e], 0), slots);
-  const int64_t hi = e == experts ? slots : max<int64_t>(lo, min<int64_t>(offsets[e + 1], slots));
-  const int64_t m0 = lo + (int64_t)blockIdx.z * kTokenRows;
-  if (m0 >= hi) return;
-  const int here = (int)min<int64_t>(kTokenRows, hi - m0);
+  const GroupRows g = group_rows(offsets, experts, slots, e);
+  const int64_t m0 = g.lo + (int64_t)blockIdx.z * kTokenRows;
+  if (m0 >= g.hi) return;
+  const int here = (int)min<int64_t>(kTokenRows, g.hi - m0);
   if (e == experts) {
     zero_rows(y, m0, here, n0, 16, outs);
     return;
@@ -492,8 +473,8 @@ __device__ __forceinline__ GroupTile grad_rows(const int32_t* __restrict__ offse
     const int e = (int)(threadIdx.x & 63);
     int mine = -1;
     if (e < experts) {
-      const int64_t lo = e == 0 ? 0 : min<int64_t>(max(offsets[e], 0), slots);
-      mine = (int)(max<int64_t>(lo, min<int64_t>(offsets[e + 1], slots)) - lo);
+      const GroupRows r = group_rows(offsets, experts, slots, e);
+      mine = (int)(r.hi - r.lo);
     }
     int before = 0;
     for (int i = 0; i < experts; ++i) {
@@ -503,9 +484,9 @@ __device__ __forceinline__ GroupTile grad_rows(const int32_t* __restrict__ offse
     const uint64_t at = __ballot(e < experts && before == (int)piece);
     g.group = __ffsll((unsigned long long)at) - 1;
   }
-  const int e = g.group;
-  g.lo = e == 0 ? 0 : min<int64_t>(max(offsets[e], 0), slots);
-  g.hi = max<int64_t>(g.lo, min<int64_t>(offsets[e + 1], slots));
+  const GroupRows r = group_rows(offsets, experts, slots, g.group);
+  g.lo = r.lo;
+  g.hi = r.hi;
   return g;
 }
 
@@ -734,11 +715,6 @@ __global__ __launch_bounds__(256) void k_group_chunk_sum(const float* __restrict
 
 int64_t tiles_of(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
 
-// Tiles of `size` rows that the groups can have between them.
-int64_t most_tiles(int64_t slots, int64_t groups, int64_t size) {
-  return slots / size + std::min(groups, slots);
-}
-
 // Rows of a weight gradient's chunk: as many chunks as fill the card, of 256
 // rows at least and of kMaxGroupChunk at most.
 constexpr int64_t kMaxGroupChunk = 8192;
@@ -876,7 +852,8 @@ struct RowsPlan {
   int bm, bn, room;
   bool cut;
   int64_t tiles = 0;  // the most that there can be
-  int64_t slices_bytes() const { return cut ? std::min<int64_t>(room, tiles * kMaxSlices) * bm * bn * 4 : 0; }
+  int places() const { return cut ? (int)slice_places(tiles, room) : 0; }
+  int64_t slices_bytes() const { return (int64_t)places() * bm * bn * 4; }
 };
 RowsPlan rows_plan(int type, bool fast, int64_t slots, int experts, int64_t cols, int64_t outs) {
   RowsPlan p{128, 128, 512, cols >= 2 * kSliceDepth, 0};
@@ -906,7 +883,7 @@ void launch_rows(const RowsPlan& p, Layouts& l, const T* b, const T* mask, const
   hipLaunchKernelGGL((k_group_rows_join<T, BM, BN, WM, WN>),
                      dim3((uint32_t)std::min<int64_t>(p.room / 2, p.tiles), BM / WM / 32 * (BN / WN / 32)),
                      dim3(64 * WM * WN), 0, st, b, mask, offsets, y, slots, experts, (int)cols, (int)outs, relu, nt,
-                     p.room, slices);
+                     p.room, p.places(), slices);
   SPHOPS_LAUNCHED();
 }
 
@@ -921,7 +898,7 @@ void rows_fast(Layouts& l, const Laid& x, const Laid& w, const T* b, const T* ma
                                    [&](dim3 grid, dim3 block, int nt, f32x4* slices) {
       hipLaunchKernelGGL((k_group_rows_fast<T, BACK, BM, BN, WM, WN>), grid, block, 0, st, static_cast<const E*>(x.base),
                          x.stride, x.plane, static_cast<const E*>(w.base), w.stride, w.plane, b, mask, offsets, y, slots,
-                         experts, (int)cols, (int)outs, relu, nt, p.room, slices);
+                         experts, (int)cols, (int)outs, relu, nt, p.room, p.places(), slices);
     });
   };
 #define SPHOPS_N(n) std::integral_constant<int, n>{}
@@ -945,10 +922,10 @@ void rows_plain(Layouts& l, const T* x, int64_t xs, const T* w, const T* b, cons
                                    [&](dim3 grid, dim3 block, int nt, f32x4* slices) {
       if constexpr (std::is_same_v<T, float>)
         hipLaunchKernelGGL((k_group_rows_wide<BACK, BM, BN, WM, WN>), grid, block, 0, st, x, xs, w, b, mask, offsets, y,
-                           slots, experts, (int)cols, (int)outs, relu, nt, p.room, slices);
+                           slots, experts, (int)cols, (int)outs, relu, nt, p.room, p.places(), slices);
       else
         hipLaunchKernelGGL((k_group_rows<T, BACK>), grid, block, 0, st, x, xs, w, b, mask, offsets, y, slots, experts,
-                           (int)cols, (int)outs, relu, nt, p.room, slices);
+                           (int)cols, (int)outs, relu, nt, p.room, p.places(), slices);
     });
   };
   if constexpr (std::is_same_v<T, float>) {

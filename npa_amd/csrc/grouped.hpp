@@ -5,6 +5,7 @@
 
 #include "rows8.hpp"
 #include "split16.hpp"
+#include "turns.hpp"
 
 #include <algorithm>
 #include <type_traits>
@@ -15,10 +16,9 @@ namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-// Tile `id` of the groups' rows in tiles of `size`: group e's rows are
-// offsets[e] to offsets[e + 1], the group after the last expert's the rows
-// behind them all.  Offsets are clamped to the rows there are, so that no tile
-// leaves them whatever they hold.  Every wave finds it for itself.
+// Tile `id` of the groups' rows (group_rows) in tiles of `size`.  No tile leaves
+// the rows, whatever the offsets hold; how many there are is bounded by most_tiles
+// only where offsets do not decrease.  Every wave finds it for itself.
 struct GroupTile {
   int group;        // -1: no such tile
   int64_t tile;     // within the group
@@ -30,12 +30,9 @@ __device__ __forceinline__ GroupTile group_tile(const int32_t* __restrict__ offs
   GroupTile g{-1, 0, 0, 0};
   for (int base = 0; base < groups; base += 64) {
     const int e = base + lane;
-    int64_t lo = 0, hi = 0;
-    if (e < groups) {
-      lo = e == 0 ? 0 : min<int64_t>(max(offsets[e], 0), slots);
-      hi = e == experts ? slots : max<int64_t>(lo, min<int64_t>(offsets[e + 1], slots));
-    }
-    const int64_t mine = (hi - lo + size - 1) / size;
+    GroupRows r{0, 0};
+    if (e < groups) r = group_rows(offsets, experts, slots, e);
+    const int64_t mine = (r.hi - r.lo + size - 1) / size;
     int64_t upto = mine;
 #pragma unroll
     for (int s = 1; s < 64; s *= 2) {
@@ -47,8 +44,8 @@ __device__ __forceinline__ GroupTile group_tile(const int32_t* __restrict__ offs
       const int at = __ffsll((unsigned long long)past) - 1;
       g.group = base + at;
       g.tile = id - __shfl(upto - mine, at);
-      g.lo = __shfl(lo, at);
-      g.hi = __shfl(hi, at);
+      g.lo = __shfl(r.lo, at);
+      g.hi = __shfl(r.hi, at);
       break;
     }
     id -= __shfl(upto, 63);
@@ -65,9 +62,8 @@ __device__ __forceinline__ int64_t group_tiles(const int32_t* __restrict__ offse
   for (int base = 0; base < groups; base += 64) {
     const int e = base + lane;
     if (e < groups) {
-      const int64_t lo = e == 0 ? 0 : min<int64_t>(max(offsets[e], 0), slots);
-      const int64_t hi = e == experts ? slots : max<int64_t>(lo, min<int64_t>(offsets[e + 1], slots));
-      all += (hi - lo + size - 1) / size;
+      const GroupRows r = group_rows(offsets, experts, slots, e);
+      all += (r.hi - r.lo + size - 1) / size;
     }
   }
 #pragma unroll
@@ -87,8 +83,8 @@ __device__ __forceinline__ GroupSpan group_span(const int32_t* __restrict__ offs
     const int i = base + lane;
     int64_t mine = 0;
     if (i < experts) {
-      const int64_t lo = i == 0 ? 0 : min<int64_t>(max(offsets[i], 0), slots);
-      mine = (max<int64_t>(lo, min<int64_t>(offsets[i + 1], slots)) - lo + size - 1) / size;
+      const GroupRows r = group_rows(offsets, experts, slots, i);
+      mine = (r.hi - r.lo + size - 1) / size;
     }
     int64_t before = i < e ? mine : 0;
     if (e >= base && e < base + 64) g.tiles = __shfl(mine, e - base);
