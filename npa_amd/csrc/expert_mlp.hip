@@ -462,7 +462,7 @@ __global__ __launch_bounds__(kGradThreads, grad_waves(KS, OS)) void k_expert_mlp
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
       float x0 = v[0], x1 = v[1], x2 = v[2], x3 = v[3];
-      const u32x2 x = {bf16_pair(x0, x1), bf16_pair(x2, x3)};
+      const u32x2 x = p == 0 ? u32x2{bf16_pair_top(x0, x1), bf16_pair_top(x2, x3)} : u32x2{bf16_pair(x0, x1), bf16_pair(x2, x3)};
       v = f32x4{x0, x1, x2, x3};
       *reinterpret_cast<u32x2*>(&image[p][row][at(row, k)]) = x;
     }
@@ -523,7 +523,7 @@ __global__ __launch_bounds__(kGradThreads, grad_waves(KS, OS)) void k_expert_mlp
     sb1 += tb1;
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const Thirds hs = split3<false>(hv[p]), gs = split3<false>(gv[p]);
+      const Thirds hs = split3(hv[p]), gs = split3(gv[p]);
       auto columns = [&](auto& image, int col) {
         Thirds d;
 #pragma unroll

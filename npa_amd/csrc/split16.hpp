@@ -54,11 +54,19 @@ __device__ __forceinline__ uint32_t bf16_pair(float& a, float& b) {
   b -= __builtin_bit_cast(float, w & 0xffff0000u);
   return w;
 }
-// TOP: the first piece is at most the largest bfloat16, past which float32's
-// largest values (from 3.396e38 on) would round up to infinity.
+// The first piece at most the largest bfloat16, past which float32's largest
+// values (from 3.396e38 on) would round up to infinity.
+__device__ __forceinline__ uint32_t bf16_pair_top(float& a, float& b) {
+  constexpr float kTop = 0x1.fep127f;
+  float p = __builtin_amdgcn_fmed3f(a, -kTop, kTop), q = __builtin_amdgcn_fmed3f(b, -kTop, kTop);
+  const uint32_t w = bf16_pair(p, q);
+  a -= __builtin_bit_cast(float, w << 16);
+  b -= __builtin_bit_cast(float, w & 0xffff0000u);
+  return w;
+}
+// TOP: values may be that large.
 template <bool TOP = true>
 __device__ __forceinline__ Thirds split3(f32x8 v) {
-  constexpr float kTop = 0x1.fep127f;
   Thirds r;
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
@@ -66,14 +74,7 @@ __device__ __forceinline__ Thirds split3(f32x8 v) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float x = v[2 * j], y = v[2 * j + 1];
-      if (TOP && i == 0) {
-        float p = __builtin_amdgcn_fmed3f(x, -kTop, kTop), q = __builtin_amdgcn_fmed3f(y, -kTop, kTop);
-        w[j] = bf16_pair(p, q);
-        x -= __builtin_bit_cast(float, w[j] << 16);
-        y -= __builtin_bit_cast(float, w[j] & 0xffff0000u);
-      } else {
-        w[j] = bf16_pair(x, y);
-      }
+      w[j] = TOP && i == 0 ? bf16_pair_top(x, y) : bf16_pair(x, y);
       v[2 * j] = x;
       v[2 * j + 1] = y;
     }
