@@ -1,6 +1,7 @@
 """What the operators over rows of several types share (``norm``, ``experts``):
 calls of the library on a tensor's device, and their checks."""
 import torch
+from torch.autograd import forward_ad
 
 from . import int8
 from .sphops import _native
@@ -23,7 +24,11 @@ def call(function, device, *args):
 
 
 def wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a call goes through its autograd function: for gradients, and
+    wherever tensors may hold tangents (whatever the grad mode), which the function
+    refuses and a kernel would lose."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+            or forward_ad._current_level >= 0)
 
 
 def check_weight(t, shape, types, device, what):

@@ -18,7 +18,8 @@ A row has k entries, each of which names an expert, or none: any number outside
 Everything stays on the device: no count is read on the host, so all of it can be
 captured into a HIP graph.  Rows are float32, bfloat16 or float16; sums are
 float32, in a fixed order, and each result is rounded once.  float32 factors keep
-their 24 bits.  Gradients throughout; a second derivative raises.
+their 24 bits.  Gradients throughout; a second derivative raises, and so does a
+forward-mode one.
 """
 import math
 from typing import NamedTuple

@@ -26,6 +26,7 @@ import functools
 from typing import NamedTuple, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .sphops import _native
 
@@ -98,6 +99,8 @@ def _check_bias(b, outs, device, what):
 def _no_backward(x, what):
     if torch.is_grad_enabled() and x.requires_grad:
         raise RuntimeError(f"{what} is for inference and has no backward: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+        raise RuntimeError(f"{what} is for inference and has no forward-mode derivative")
 
 
 def _rows_view(x):

@@ -62,7 +62,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer norm over x's last dimension, of x's type (float32, bfloat16 or
     float16; autocast changes nothing).  ``weight`` and ``bias`` have its length
     and are both float32 or both of x's type; either may be None.  Gradients of
-    all three; a second derivative raises.  Deviations from the mean whose squares pass
+    all three; a second derivative and a forward-mode one raise.  Deviations from the mean whose squares pass
     float32's range (about 1e19) give the bias."""
     _rows.check_rows(x, "x")
     types = (torch.float32,) if x.dtype == torch.float32 else (torch.float32, x.dtype)
