@@ -334,7 +334,9 @@ def mlp(x, w1, b1, w2, b2, offsets):
 class ExpertMlp(torch.nn.Module):
     """Linear, ReLU, Linear of ``experts`` experts, of which a router (a linear
     layer and a softmax) chooses ``choices`` for each row; the row's result is the
-    sum of theirs, weighted with the router's probabilities."""
+    sum of theirs, weighted with the router's probabilities.  Rows are of the
+    parameters' type; under autocast they may be of any, the router runs as autocast
+    runs a ``torch.nn.Linear`` and the experts in the parameters' type."""
 
     def __init__(self, in_features, hidden, out_features, experts, choices=1, bias=True, device=None, dtype=None):
         super().__init__()
@@ -358,7 +360,10 @@ class ExpertMlp(torch.nn.Module):
                     torch.nn.init.uniform_(t, -1 / math.sqrt(w.shape[2]), 1 / math.sqrt(w.shape[2]))
 
     def forward(self, x):
-        logits = _mlp.linear(x, self.router) if x.dtype == torch.float32 else self.router(x)
+        if torch.is_autocast_enabled("cuda"):
+            logits, x = self.router(x), x.to(self.w1.dtype)
+        else:
+            logits = _mlp.linear(x, self.router) if x.dtype == torch.float32 else self.router(x)
         weight, index = torch.softmax(logits.float(), -1).topk(self.choices, dim=-1)
         routing = sort_rows(index, self.experts)
         results = mlp(dispatch(x, routing), self.w1, self.b1, self.w2, self.b2, routing.offsets)
