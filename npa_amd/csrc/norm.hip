@@ -8,6 +8,12 @@
 // where rows lie far from zero: d = x - c is summed again and its mean e taken
 // off (v = mean d^2 - e^2, h = (d - e) r).  The backward is given c and r and
 // finds e beside its other two sums.
+//
+// c, d and e are halves and r is doubled, and c is summed in units of 2^17, which
+// changes no rounding: nothing of a finite row but the sums over d overflows, a
+// mask's lowest values and the difference of the largest ones included.  Where the
+// squares' sum does (the sum of d does not before), r and e are 0: y is the bias,
+// and no gradient reaches x.  A row that is not finite has a c that is not.
 #include "rows_out.hpp"
 
 #include <type_traits>
@@ -15,6 +21,28 @@
 namespace sphops {
 
 namespace {
+
+constexpr float kSumUnit = 0x1p-17f, kHalfUnit = 0x1p16f;  // of c: up to 2^16 values
+static_assert(kMaxRows8Cols <= 65536, "a row's sum stays in range");
+
+// e and twice 1 / sqrt(v + eps) from a row's sums of d and of its squares.
+struct Deviations {
+  float e, twice;
+  __device__ __forceinline__ Deviations(const float (&q)[2], float inv, float eps) {
+    e = q[0] * inv;
+    const float var = q[1] < __builtin_inff() ? fmaxf(q[1] * inv - e * e, 0.0f) : q[1];  // NaN stays
+    twice = 1.0f / sqrtf(var + 0.25f * eps);
+    if (twice == 0.0f) e = 0.0f;
+  }
+};
+
+// What the backward makes halved deviations with, and r: all 0 where the squares
+// overflowed, so that nothing of the row counts.
+struct RowStats {
+  float half, c, twice, r;
+  __device__ __forceinline__ RowStats(float2 st)
+      : half(st.y == 0.0f ? 0.0f : 0.5f), c(st.y == 0.0f ? 0.0f : st.x), twice(st.y), r(0.5f * st.y) {}
+};
 
 // A value of the weights, which are float32 or of the rows' type.
 template <class T>
@@ -120,24 +148,24 @@ __global__ __launch_bounds__(TH) void k_norm_forward(const T* __restrict__ x, in
 #pragma unroll
     for (int n = 0; n < N; ++n) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) s[0] += p[n].get(j);
+      for (int j = 0; j < V; ++j) s[0] += p[n].get(j) * kSumUnit;
     }
     sum1(s, turn1);
-    const float c = s[0] * inv;
+    const float c = s[0] * (inv * kHalfUnit);
     float q[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int n = 0; n < N; ++n) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         // only the last pieces reach past the row's end (with_lanes)
-        const float d = n < N - 1 || (n * L + l) * V + j < cols ? p[n].get(j) - c : 0.0f;
+        const float d = n < N - 1 || (n * L + l) * V + j < cols ? p[n].get(j) * 0.5f - c : 0.0f;
         q[0] += d;
         q[1] += d * d;
       }
     }
     sum2(q, turn2);
-    const float e = q[0] * inv, var = fmaxf(q[1] * inv - e * e, 0.0f);
-    const float rstd = 1.0f / sqrtf((q[1] != q[1] ? q[1] : var) + eps);  // fmaxf drops a NaN
+    const Deviations dev(q, inv, eps);
+    const float e = dev.e, rstd = dev.twice;
     if (stats != nullptr && l == 0) stats[r] = float2{c, rstd};
     const float er = e * rstd;
     Piece<T> o[N];
@@ -145,7 +173,7 @@ __global__ __launch_bounds__(TH) void k_norm_forward(const T* __restrict__ x, in
     for (int n = 0; n < N; ++n) {
       float v[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = ((p[n].get(j) - c) * rstd - er) * ww[n][j] + bb[n][j];
+      for (int j = 0; j < V; ++j) v[j] = ((p[n].get(j) * 0.5f - c) * rstd - er) * ww[n][j] + bb[n][j];
       o[n] = piece_of<T>(v);
     }
     const int wave = (int)threadIdx.x / 64;
@@ -174,24 +202,24 @@ __global__ __launch_bounds__(kLongThreads) void k_norm_forward_long(const T* __r
       Piece<T> p;
       p.load(row, k, cols);
 #pragma unroll
-      for (int j = 0; j < V; ++j) s[0] += p.get(j);
+      for (int j = 0; j < V; ++j) s[0] += p.get(j) * kSumUnit;
     }
     sum1(s, turn1);
-    const float c = s[0] * inv;
+    const float c = s[0] * (inv * kHalfUnit);
     float q[2] = {0.0f, 0.0f};
     for (int k = threadIdx.x * V; k < cols; k += TH * V) {
       Piece<T> p;
       p.load(row, k, cols);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = k + j < cols ? p.get(j) - c : 0.0f;
+        const float d = k + j < cols ? p.get(j) * 0.5f - c : 0.0f;
         q[0] += d;
         q[1] += d * d;
       }
     }
     sum2(q, turn2);
-    const float e = q[0] * inv, var = fmaxf(q[1] * inv - e * e, 0.0f);
-    const float rstd = 1.0f / sqrtf((q[1] != q[1] ? q[1] : var) + eps);
+    const Deviations dev(q, inv, eps);
+    const float e = dev.e, rstd = dev.twice;
     if (stats != nullptr && threadIdx.x == 0) stats[r] = float2{c, rstd};
     for (int k = threadIdx.x * V; k < cols; k += TH * V) {
       Piece<T> p;
@@ -201,7 +229,7 @@ __global__ __launch_bounds__(kLongThreads) void k_norm_forward_long(const T* __r
         const int kk = min(k + j, cols - 1);
         const float ww = w != nullptr ? weight_at<T>(w, wide, kk) : 1.0f;
         const float bb = b != nullptr ? weight_at<T>(b, wide, kk) : 0.0f;
-        p.set(j, from_f32<T>((p.get(j) - c - e) * rstd * ww + bb));
+        p.set(j, from_f32<T>((p.get(j) * 0.5f - c - e) * rstd * ww + bb));
       }
       p.store(y + r * cols, k, cols);
     }
@@ -253,14 +281,14 @@ __global__ __launch_bounds__(TH, N * Piece<T>::V <= 12 ? 4 : 2) void k_norm_back
       p[n] = pn[n];
       u[n] = un[n];
     }
-    const float2 st = sn;
+    const RowStats st(sn);
     load(r0 + step);  // in flight under this turn's sums
     float s[3] = {0.0f, 0.0f, 0.0f};  // of d, g and g d
 #pragma unroll
     for (int n = 0; n < N; ++n) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = n < N - 1 || (n * L + l) * V + j < cols ? p[n].get(j) - st.x : 0.0f;
+        const float d = n < N - 1 || (n * L + l) * V + j < cols ? p[n].get(j) * st.half - st.c : 0.0f;
         const float g = u[n].get(j) * ww[n][j];
         s[0] += d;
         s[1] += g;
@@ -268,16 +296,16 @@ __global__ __launch_bounds__(TH, N * Piece<T>::V <= 12 ? 4 : 2) void k_norm_back
       }
     }
     sums(s, turn);
-    const float e = s[0] * inv, mg = s[1] * inv, mgh = (s[2] - e * s[1]) * inv * st.y;
-    const float er = e * st.y, mgr = mg * st.y, mghr = mgh * st.y;
+    const float e = s[0] * inv, mg = s[1] * inv, mgh = (s[2] - e * s[1]) * inv * st.twice;
+    const float er = e * st.twice, mgr = mg * st.r, mghr = mgh * st.r;
     Piece<T> o[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       float v[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float h = (p[n].get(j) - st.x) * st.y - er, up = u[n].get(j);
-        v[j] = (up * ww[n][j]) * st.y - mgr - h * mghr;
+        const float h = (p[n].get(j) * st.half - st.c) * st.twice - er, up = u[n].get(j);
+        v[j] = (up * ww[n][j]) * st.r - mgr - h * mghr;
         if (live) {
           dw[n][j] += up * h;
           db[n][j] += up;
@@ -340,7 +368,7 @@ __global__ __launch_bounds__(kLongThreads) void k_norm_backward_long(const T* __
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* __restrict__ row = x + r * stride;
     const T* __restrict__ up = dy + r * dy_stride;
-    const float2 st = stats[r];
+    const RowStats st(stats[r]);
     float s[3] = {0.0f, 0.0f, 0.0f};
     for (int k = threadIdx.x * V; k < cols; k += TH * V) {
       Piece<T> p, u;
@@ -348,7 +376,7 @@ __global__ __launch_bounds__(kLongThreads) void k_norm_backward_long(const T* __
       u.load(up, k, cols);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = k + j < cols ? p.get(j) - st.x : 0.0f;
+        const float d = k + j < cols ? p.get(j) * st.half - st.c : 0.0f;
         const float g = u.get(j) * (w != nullptr ? weight_at<T>(w, wide, min(k + j, cols - 1)) : 1.0f);
         s[0] += d;
         s[1] += g;
@@ -356,7 +384,7 @@ __global__ __launch_bounds__(kLongThreads) void k_norm_backward_long(const T* __
       }
     }
     sums(s, turn);
-    const float e = s[0] * inv, mg = s[1] * inv, mgh = (s[2] - e * s[1]) * inv * st.y;
+    const float e = s[0] * inv, mg = s[1] * inv, mgh = (s[2] - e * s[1]) * inv * st.twice;
     if (low != nullptr && threadIdx.x == 0) low[r] = e;
     if (dx == nullptr) continue;
     for (int k = threadIdx.x * V; k < cols; k += TH * V) {
@@ -366,8 +394,8 @@ __global__ __launch_bounds__(kLongThreads) void k_norm_backward_long(const T* __
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float g = u.get(j) * (w != nullptr ? weight_at<T>(w, wide, min(k + j, cols - 1)) : 1.0f);
-        const float h = (p.get(j) - st.x - e) * st.y;
-        p.set(j, from_f32<T>(st.y * (g - mg - h * mgh)));
+        const float h = (p.get(j) * st.half - st.c - e) * st.twice;
+        p.set(j, from_f32<T>(st.r * (g - mg - h * mgh)));
       }
       p.store(dx + r * cols, k, cols);
     }
@@ -388,7 +416,8 @@ __global__ __launch_bounds__(256) void k_norm_columns_long(const T* __restrict__
 #pragma unroll 4
   for (int64_t r = r0; r < r1; ++r) {
     const float u = to_f32(dy[r * dy_stride + k]);
-    dw += u * ((to_f32(x[r * stride + k]) - stats[r].x - low[r]) * stats[r].y);
+    const RowStats st(stats[r]);
+    dw += u * ((to_f32(x[r * stride + k]) * st.half - st.c - low[r]) * st.twice);
     db += u;
   }
   float* __restrict__ to = part + (int64_t)blockIdx.x * 2 * cols;

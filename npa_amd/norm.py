@@ -62,8 +62,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer norm over x's last dimension, of x's type (float32, bfloat16 or
     float16; autocast changes nothing).  ``weight`` and ``bias`` have its length
     and are both float32 or both of x's type; either may be None.  Gradients of
-    all three; a second derivative and a forward-mode one raise.  Deviations from the mean whose squares pass
-    float32's range (about 1e19) give the bias."""
+    all three; a second derivative and a forward-mode one raise.  A finite row the
+    squares of whose deviations pass float32's range (deviations of about 1e19, masks
+    of the lowest value among them) gives the bias, and no gradient to x."""
     _rows.check_rows(x, "x")
     types = (torch.float32,) if x.dtype == torch.float32 else (torch.float32, x.dtype)
     weight = _rows.check_weight(weight, x.shape[-1:], types, x.device, "weight")
