@@ -665,8 +665,10 @@ int sphops_combine_rows_backward(const void* dy, int type, int64_t row_stride, c
  * rows behind the last expert's.  All of `type`; w (experts, out_features,
  * in_features) and b (experts, out_features, or NULL) dense, x's rows
  * row_stride elements apart, y dense.  relu: y = max(y, 0).  Sums are float32, and
- * float32 factors keep their 24 bits.  workspace:
- * sphops_expert_linear_workspace_bytes bytes (-1: not supported), 16-byte aligned.
+ * float32 factors keep their 24 bits.  slots times in_features or out_features, each
+ * rounded up to a multiple of 128, stays below about 2^37 (float32 2^38), for a launch
+ * of fewer than 2^32 threads.  workspace: sphops_expert_linear_workspace_bytes bytes
+ * (-1: not supported), 16-byte aligned.
  */
 int sphops_expert_linear(const void* x, int type, int64_t row_stride, const void* w, const void* b,
                          const int32_t* offsets, void* y, int64_t slots, int experts, int in_features,

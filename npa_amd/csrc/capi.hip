@@ -1501,7 +1501,7 @@ bool expert_linear_fits(int type, int64_t slots, int experts, int in_features, i
   return type >= SPHOPS_F32 && type <= SPHOPS_F16 && slots >= 0 && slots <= sphops::kMaxSlots && experts >= 1 && experts <= sphops::kMaxExperts &&
          in_features >= 1 && in_features <= sphops::kMaxGroupCols && out_features >= 1 &&
          out_features <= sphops::kMaxGroupCols &&
-         sphops::group_linear_fits(slots, experts, in_features, out_features);
+         sphops::group_linear_fits(type, slots, experts, in_features, out_features);
 }
 void require_weight_type(const void* w, const void* b, bool wide, int type) {
   const uintptr_t align = wide || type == SPHOPS_F32 ? 4 : 2;

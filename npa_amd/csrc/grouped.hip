@@ -783,23 +783,6 @@ GradPlan laid_plan(int64_t slots, int experts, int64_t cols, int64_t outs) {
   return grad_plan(slots, experts, cols, outs, tall ? 256 : 128, 128);
 }
 
-}  // namespace
-
-bool group_linear_fits(int64_t slots, int experts, int64_t cols, int64_t outs) {
-  const int64_t limit = (int64_t(1) << 32) / kGroupThreads - 512;  // threads a launch
-  for (const int64_t n : {outs, cols}) {
-    if (most_tiles(slots, experts + 1, kSide) * tiles_of(n, 32) >= limit) return false;
-    if (slots <= 32 * (int64_t)experts && most_tiles(slots, experts + 1, 32) * tiles_of(n, kSide) >= limit) return false;
-  }
-  for (const bool wide : {false, true}) {
-    const GradPlan p = chosen_plan(slots, experts, cols, outs, wide, false);
-    if ((int64_t)p.mt * p.nt * std::max<int64_t>(p.chunks, experts) >= limit) return false;
-  }
-  return tiles_of(cols * outs + outs, 256) * experts < limit;
-}
-
-namespace {
-
 // A matrix as the fast kernels read it.
 struct Laid {
   const void* base;
@@ -958,6 +941,23 @@ bool fast_as_is(const void* x, int64_t xs, int64_t cols, const void* w, int64_t 
 }
 
 }  // namespace
+
+// Whether every launch of a layer, forward and backward and at either alignment, stays
+// below the 2^32 threads that one can have along x.
+bool group_linear_fits(int type, int64_t slots, int experts, int64_t cols, int64_t outs) {
+  const auto threads = [](int64_t groups, int size) { return groups < (int64_t(1) << 32) / size; };
+  const bool wide = type == SPHOPS_F32;
+  for (const bool fast : {false, true}) {
+    for (const bool back : {false, true}) {
+      const RowsPlan p = rows_plan(type, fast, slots, experts, back ? outs : cols, back ? cols : outs);
+      const int size = wide ? (p.bm == 256 ? 512 : 256) : fast && p.bm == 128 ? 256 : 512;
+      if (!threads(p.tiles + p.room, size)) return false;
+    }
+    const GradPlan p = wide && fast ? laid_plan(slots, experts, cols, outs) : chosen_plan(slots, experts, cols, outs, wide, fast);
+    if (!threads(std::max<int64_t>(p.chunks, experts) * p.mt * p.nt, wide && !fast ? kWideThreads : kGroupThreads)) return false;
+  }
+  return threads(tiles_of(cols * outs + outs, 256), 256);
+}
 
 int64_t group_linear_workspace_bytes(int type, int64_t slots, int experts, int64_t cols, int64_t outs) {
   Layouts l{nullptr};

@@ -426,7 +426,7 @@ void run_combine_rows_backward(const void* dy, int type, int64_t stride, const v
                                int choices, int64_t cols, hipStream_t st);
 // grouped.hip: linear layers of experts over sorted rows
 constexpr int64_t kMaxGroupCols = 65536;
-bool group_linear_fits(int64_t slots, int experts, int64_t cols, int64_t outs);
+bool group_linear_fits(int type, int64_t slots, int experts, int64_t cols, int64_t outs);
 int64_t group_linear_workspace_bytes(int type, int64_t slots, int experts, int64_t cols, int64_t outs);
 void run_group_linear(const void* x, int type, int64_t xs, const void* w, const void* b, const int32_t* offsets,
                       void* y, int64_t slots, int experts, int64_t cols, int64_t outs, bool relu, void* work,

@@ -299,7 +299,8 @@ def linear(x, weight, bias, offsets):
     last expert's zeros.  ``weight`` (experts, out, in) and ``bias`` (experts,
     out; may be None) are of x's type; ``offsets`` (int32, as in a ``Routing``)
     starts at 0 and does not decrease.  The gradients of an expert without rows
-    are zeros.
+    are zeros.  A layer whose launch would pass 2^32 threads raises (from about 2^37,
+    float32 2^38, of places times inputs or outputs).
 
     Large float32 products run on bfloat16 pieces of their factors: there a value
     that is not finite may give NaN where float32 gives an infinity, and factors below
