@@ -929,10 +929,18 @@ int64_t rows_bytes(int type, int64_t slots, int experts, int64_t cols, int64_t o
                   rows_plan(type, false, slots, experts, cols, outs).slices_bytes());
 }
 
-// Few rows an expert: k_group_tokens.
-constexpr int64_t kTokenSlots = 1024;
-bool few_rows(int64_t slots, int experts) {
-  return slots <= kTokenSlots && slots <= 16 * (int64_t)experts;
+// Few rows an expert: k_group_tokens, which reads x again for every 16 outputs and has a
+// workgroup for each expert, its rows or not: as long as the products are few (for
+// float32, whose matrix cores are slower, a quarter), and the workgroups.  us on the
+// GPU, it and the tiles.  bfloat16, 4096 -> 2048: 32 rows of 16 experts 36 and 44, 64
+// 50 and 46, 256 82 and 59; 1024 -> 1024: 256 of 16 16 and 24, 128 of 64 23 and 26,
+// 512 of 64 37 and 28; 83 -> 128: 1024 of 64 6 and 9, of 256 19 and 11.  float32, 1024 ->
+// 1024: 64 of 16 23 and 23, 256 of 16 35 and 28, 64 of 64 34 and 51.
+constexpr int64_t kTokenSlots = 1024, kTokenProducts = int64_t(5) << 26, kTokenGroups = 1 << 15;
+bool few_rows(int type, int64_t slots, int experts, int64_t cols, int64_t outs) {
+  return slots <= kTokenSlots && slots <= 16 * (int64_t)experts &&
+         slots * cols * outs <= (type == SPHOPS_F32 ? kTokenProducts / 4 : kTokenProducts) &&
+         tiles_of(outs, 16) * (experts + 1) * tiles_of(slots, kTokenRows) <= kTokenGroups;
 }
 
 template <class T>
@@ -966,7 +974,7 @@ int64_t group_linear_workspace_bytes(int type, int64_t slots, int experts, int64
     l.take(Layouts::bytes_of(type, slots, cols));
     l.take(Layouts::bytes_of(type, experts * outs, cols));
   }
-  if (!few_rows(slots, experts)) l.take(rows_bytes(type, slots, experts, cols, outs, laid));
+  if (!few_rows(type, slots, experts, cols, outs)) l.take(rows_bytes(type, slots, experts, cols, outs, laid));
   return l.used;
 }
 
@@ -980,7 +988,7 @@ void run_group_linear(const void* x, int type, int64_t xs, const void* w, const 
     T* const py = static_cast<T*>(y);
     const bool as_is = fast_as_is<T>(x, xs, cols, w, cols);
     Layouts l{static_cast<char*>(work)};
-    if (few_rows(slots, experts)) {
+    if (few_rows(type, slots, experts, cols, outs)) {
       const dim3 grid((uint32_t)tiles_of(outs, 16), (uint32_t)(experts + 1), (uint32_t)tiles_of(slots, kTokenRows));
       hipLaunchKernelGGL((k_group_tokens<T>), grid, dim3(kTokenThreads), 0, st, px, xs, pw, pb, offsets, py, slots,
                          experts, (int)cols, (int)outs, relu);
