@@ -717,7 +717,17 @@ int64_t tiles_of(int64_t n, int64_t tile) { return (n + tile - 1) / tile; }
 
 // Rows of a weight gradient's chunk: as many chunks as fill the card, of 256
 // rows at least and of kMaxGroupChunk at most.
-constexpr int64_t kMaxGroupChunk = 8192;
+//
+// None where the experts' tiles fill the card: the chunks' float32 sums go to memory
+// and back.  But up to kMaxWhole places only, which one expert may have all of: its
+// sum is then that long, and its few workgroups work alone.  us with gradients, whole
+// and in chunks (in brackets all places of one expert): bfloat16, 2048 -> 4096, 16384 of
+// 8 909 and 1269 (1017, 1057), 32768 of 8 1703 and 2083 (1959, 1824), 65536 of 8 3290 and
+// 3648 (4070, 3572); 1024 -> 1024, 16384 of 64 268 and 650 (548, 407), 65536 of 64 709 and
+// 995 (2145, 796); 2048 -> 2048, 32768 of 64 1182 and 2557 (1535, 1667), 131072 of 8 4504
+// and 3751; float32, 1024 -> 1024, 32768 of 64 1887 and 2204 (2976, 1997); on the wrong
+// side 32768 of 16, 1536 -> 1536 bfloat16, 937 and 847.
+constexpr int64_t kMaxGroupChunk = 8192, kMaxWhole = 32768;
 struct GradPlan {
   int bm, bn, mt, nt;     // tiles of dW
   int64_t chunk, chunks;  // chunks 0: a workgroup takes all of an expert's rows
@@ -732,7 +742,7 @@ GradPlan grad_plan(int64_t slots, int experts, int64_t cols, int64_t outs, int b
   const int64_t want = std::max<int64_t>(1, 512 / tiles);  // chunks in all
   p.chunk = std::min(kMaxGroupChunk, std::max<int64_t>(256, tiles_of(tiles_of(slots, want), 64) * 64));
   p.chunks = most_tiles(slots, experts, p.chunk);
-  if (slots <= p.chunk || (tiles * experts >= 512 && slots <= 2 * kMaxGroupChunk)) {
+  if (slots <= p.chunk || (tiles * experts >= 512 && slots <= kMaxWhole)) {
     p.chunk = std::max<int64_t>(slots, 1);
     p.chunks = 0;
   }

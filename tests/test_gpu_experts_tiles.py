@@ -32,3 +32,13 @@ def test_both_kernels_of_few_rows_agree(dtype):
     half = torch.finfo(dtype).eps / 2 if dtype != F32 else 0.0
     limit = 2 * 1032 * 2 * 2.0 ** -24 * size + 2 * half * (few.double().abs() + 1032 * 2 * 2.0 ** -24 * size)
     assert ((y[:60].double() - few.double()).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_weight_gradients_whole_and_in_chunks(dtype):
+    """Weight tiles that fill the card, up to 32768 places and past them, rows laid out or as they are."""
+    for rows in (32768, 32769):
+        _check_linear([rows // 2, 0, *[rows // 32] * 14, 100], rows - rows // 2 - 14 * (rows // 32) - 100, 776, 760, dtype)
+    counts = [500] * 36 + [0, 7, 333]
+    _check_linear(counts, 5, 513, 520, dtype, bias=False)
+    _check_linear(counts + [14600], 5, 513, 520, dtype)
