@@ -755,15 +755,23 @@ bool whole_pieces(const void* p, int64_t stride) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0 && stride <= (1 << 22);
 }
 
-// 16-bit tiles: 256 where there are enough of them, else 128: 16384 rows of 8
-// experts, 2048 -> 4096 bfloat16, 390 us with the first and 435 with the second.  A
-// weight gradient's where no chunks are needed: the same with gradients 1085 and
-// 1220; 4096 rows of 4, 2048 -> 2048 (256 tiles of 256, in chunks) 305 and 192.
+// 16-bit tiles: 256 where there are enough of them, else 128.  us, bfloat16, tiles of
+// 256 and 128.  Over rows, 128 tiles of 256 (8192 rows of 4 experts, 2048 -> 1024) 73 and
+// 59, 192 (8192 of 4, 2048 -> 1536; 12288 of 8, 4096 -> 1024) 74 and 83, 122 and 142, 1024
+// (16384 of 8, 2048 -> 4096) 310 and 345; between them whole turns of the card decide:
+// 256 (8192 of 8, 2048 -> 2048; 16384 of 8, 2048 -> 1024) 103 and 103, 97 and 87, 512 (16384
+// of 8, 2048 -> 2048) 168 and 162.  Weight gradients, whole or in chunks, with the rest of
+// the pass: 256 tiles (4096 of 4, 2048 -> 2048) 293 and 180, 512 (16384 of 8, 2048 -> 2048;
+// 8192 of 32, 1024 -> 1024; 8192 of 8, 2048 -> 2048) 586 and 517, 156 and 148, 302 and 311,
+// 640 (16384 of 10, 2048 -> 2048) 556 and 528, 768 (16384 of 16, 1536 -> 2048; of 12, 2048 ->
+// 2048) 420 and 441, 563 and 548, 1024 (16384 of 8, 2048 -> 4096; of 64, 1024 -> 1024) 916
+// and 949, 266 and 282; in chunks (65536 of 8, 2048 -> 4096; of 64, 1024 -> 1024) 3662 and
+// 3901, 994 and 1014.
 int rows_side(int64_t slots, int64_t outs) {
   return outs > 128 && slots / 256 * tiles_of(outs, 256) >= 192 ? 256 : 128;
 }
 int grad_side(int experts, int64_t cols, int64_t outs) {
-  return outs > 128 && cols > 128 && tiles_of(outs, 256) * tiles_of(cols, 256) * experts >= 512 ? 256 : 128;
+  return outs > 128 && cols > 128 && tiles_of(outs, 256) * tiles_of(cols, 256) * experts >= 768 ? 256 : 128;
 }
 // Float32 tiles: 32, 64 or 128 outputs, as few as hold them; 32 rows where an expert
 // has no more on average (2048 rows of 128 experts, 512 -> 512, 48 us, with 128 91).

@@ -42,3 +42,10 @@ def test_weight_gradients_whole_and_in_chunks(dtype):
     counts = [500] * 36 + [0, 7, 333]
     _check_linear(counts, 5, 513, 520, dtype, bias=False)
     _check_linear(counts + [14600], 5, 513, 520, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("counts", [[4095, 9, 700], [33000, 9, 700]])
+def test_large_weight_tiles(counts, dtype):
+    """16-bit weight gradients in tiles of 256: whole, and in chunks."""
+    _check_linear(counts, 5, 4000, 4080, dtype)
