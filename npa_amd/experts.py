@@ -361,10 +361,9 @@ class ExpertMlp(torch.nn.Module):
                     torch.nn.init.uniform_(t, -1 / math.sqrt(w.shape[2]), 1 / math.sqrt(w.shape[2]))
 
     def forward(self, x):
-        if torch.is_autocast_enabled("cuda"):
-            logits, x = self.router(x), x.to(self.w1.dtype)
-        else:
-            logits = _mlp.linear(x, self.router) if x.dtype == torch.float32 else self.router(x)
+        logits = _mlp.linear(x, self.router) if x.dtype == torch.float32 else self.router(x)
+        if torch.is_autocast_enabled():
+            x = x.to(self.w1.dtype)
         weight, index = torch.softmax(logits.float(), -1).topk(self.choices, dim=-1)
         routing = sort_rows(index, self.experts)
         results = mlp(dispatch(x, routing), self.w1, self.b1, self.w2, self.b2, routing.offsets)

@@ -91,8 +91,7 @@ class ReluLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, weight, bias):
         out_f, in_f = weight.shape
-        fused = (a.is_cuda and a.dtype == torch.float32 and weight.dtype == torch.float32
-                 and in_f % 4 == 0 and 4 <= in_f <= RELU_LINEAR_MAX_IN and out_f <= RELU_LINEAR_MAX_OUT)
+        fused = _relu_linear_fused(a, weight)
         ctx.has_bias = bias is not None
         ctx.pre = fused
         if not fused:
@@ -270,6 +269,12 @@ class ReluLinear8(torch.autograd.Function):
         return da, (dw if need_w else None), (db if need_b else None)
 
 
+def _relu_linear_fused(a, weight):
+    out_f, in_f = weight.shape
+    return (a.is_cuda and a.dtype == torch.float32 and weight.dtype == torch.float32
+            and in_f % 4 == 0 and 4 <= in_f <= RELU_LINEAR_MAX_IN and out_f <= RELU_LINEAR_MAX_OUT)
+
+
 def _dense(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
@@ -346,8 +351,11 @@ def _check_checkpoint(checkpoint):
 
 
 def linear(x, layer, checkpoint=None):
-    """``layer(x)``; with checkpoint="int8" x is kept in 8 bits for dW."""
+    """``layer(x)``; with checkpoint="int8" x is kept in 8 bits for dW.  Under
+    autocast, which runs the product in 16 bits, the layer itself."""
     _check_checkpoint(checkpoint)
+    if torch.is_autocast_enabled():
+        return layer(x)
     if checkpoint and _rows8_ok(x, layer):
         return LinearRows8.apply(x, layer.weight, layer.bias)
     return LinearRows.apply(x, layer.weight, layer.bias)
@@ -355,8 +363,11 @@ def linear(x, layer, checkpoint=None):
 
 def relu_linear(a, layer, checkpoint=None):
     """``layer(torch.relu(a))`` with the fused backward; with checkpoint="int8"
-    relu(a) is kept in 8 bits and its mask exactly."""
+    relu(a) is kept in 8 bits and its mask exactly.  Under autocast the layer
+    itself, but where one kernel takes both in float32."""
     _check_checkpoint(checkpoint)
+    if torch.is_autocast_enabled() and not _relu_linear_fused(a, layer.weight):
+        return layer(torch.relu(a))
     if checkpoint and _rows8_ok(a, layer):
         return ReluLinear8.apply(a, layer.weight, layer.bias)
     return ReluLinear.apply(a, layer.weight, layer.bias)
