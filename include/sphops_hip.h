@@ -697,8 +697,9 @@ int64_t sphops_expert_linear_backward_workspace_bytes(int type, int64_t slots, i
  * sphops_expert_linear.  y is zero behind the last expert's rows.  mask (4 words a
  * row, 8-byte aligned, or NULL) keeps where the hidden values are above 0 for the
  * input gradient, which writes dz (zero behind the last expert's rows).  The
- * weight gradients (each may be NULL) compute the hidden values again and are
- * summed in a fixed order.  workspace: sphops_expert_mlp_workspace_bytes bytes
+ * weight gradients (each may be NULL) compute the hidden values again, in another
+ * order of sums (where one lies within rounding of 0 they may take the ReLU's other
+ * side than y and dz), and are summed in a fixed order.  workspace: sphops_expert_mlp_workspace_bytes bytes
  * (-1: not supported), 4-byte aligned.
  */
 int sphops_expert_mlp_forward(const float* z, const float* w1, const float* b1, const float* w2, const float* b2,

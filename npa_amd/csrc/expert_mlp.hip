@@ -74,8 +74,8 @@ __device__ __forceinline__ void zero_part(float* __restrict__ to, int64_t lo, in
 // parts have sums of their own, rounded once a step.
 // mask (slots x 4 words, or null): the lane's bit 16 t + r of its half's two words
 // says that register r of hidden tile t is above 0 (or NaN).
-// Bound: matrix and vector work, which add up: 2^20 rows of 8 experts, 83 -> 19, in 259
-// us (193 + 188 thousand cycles of a SIMD; a CU counts 386 busy of 467).
+// Bound: matrix and vector work, which add up: 2^20 rows of 8 experts, 83 -> 19, in 239
+// us (193 + 188 thousand cycles of a SIMD; a CU counts 389 busy of 468).
 template <int CT, int OT, int kThreads>
 __global__ __launch_bounds__(kThreads, kThreads / 256) void k_expert_mlp_forward(
     const float* __restrict__ z, const float* __restrict__ w1, const float* __restrict__ b1,
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(kThreads, kThreads / 256) void k_expert_mlp_forward
 // One wave a tile of 32 rows, rows as the columns n: hidden tile by hidden tile
 // dh = W2^T dy masked by the forward's bits; then dz += dh W1 with W1's image read
 // down its columns, dh's result registers as they stand being the first operand.
-// Bound: as the forward's; 221 us (193 + 160 thousand cycles, 314 busy of 385).
+// Bound: as the forward's; 205 us (193 + 160 thousand cycles, 318 busy of 388).
 template <int CT, int OT, int kThreads>
 __global__ __launch_bounds__(kThreads, kThreads / 256) void k_expert_mlp_input_grad(
     const float* __restrict__ dy, const float* __restrict__ w1, const float* __restrict__ w2,
@@ -381,8 +381,12 @@ constexpr int grad_waves(int ks, int os) { return ks > 6 || os > 2 ? 1 : 2; }
 // whose other operands come in a's and dh's result layout.  The next tile is
 // loaded under this one's products.  The sums of workgroup i stand at
 // place i of `part`: dW1 (128 x nin), db1 (128), dW2 (nout x 128), db2 (nout).
-// Bound: as the forward's; 379 us (385 + 247 thousand cycles, 581 busy of 639), more than a
+// Bound: as the forward's; 354 us (385 + 272 thousand cycles, 589 busy of 650), more than a
 // third of the products for hidden values that the forward had.
+//
+// The ReLU's side is taken from these values, which are summed in another order than
+// the forward's: where one lies within its rounding of 0, they may be on either side,
+// and so may dz and the weights' gradients, each of which is then right by itself.
 template <int KS, int OS>
 __global__ __launch_bounds__(kGradThreads, grad_waves(KS, OS)) void k_expert_mlp_weight_grad(
     const float* __restrict__ z, const float* __restrict__ dy, const float* __restrict__ w1,

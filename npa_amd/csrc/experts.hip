@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;
 // Entries a thread takes of a tile: few while tiles are few, whose steps follow one
-// another (16384 entries, 64 experts: three launches of 9, 5 and 9 us with eight, of 4, 3
+// another (16384 entries, 64 experts: three launches of 9, 5 and 9 us with eight, of 4, 2
 // and 5 with two).
 constexpr int kFewItems = 2, kManyItems = 8;
 constexpr int64_t kManyEntries = 1 << 18;
@@ -99,8 +99,8 @@ __device__ __forceinline__ void scan_experts(uint32_t* __restrict__ total, int e
 }
 
 // hist[key * tiles + tile]: the tile's entries of each key.
-// Bound (this, the scan and the places): latency; 2^20 entries of 4 experts in 9 + 5
-// + 9 us, 16384 of 64 in 5 + 5 + 5, one launch of 3 for a few.
+// Bound (this, the scan and the places): latency; 2^20 entries of 4 experts in 8 + 5
+// + 9 us, 16384 of 64 in 4 + 2 + 5, one launch of 3 for a few.
 template <int ITEMS>
 __global__ __launch_bounds__(kSortThreads) void k_sort_count(const void* __restrict__ index, bool wide, int64_t n,
                                                              int experts, int bits, uint32_t* __restrict__ hist) {
@@ -202,7 +202,7 @@ __device__ __forceinline__ Piece<T> scaled(const Piece<T>& p, float w) {
 }
 
 // out[slot[r, j]] = x[r], zeros for an entry without an expert.  L lanes a row's
-// block of L x N pieces.  Bound: HBM; 8192 x 4096 bfloat16, two entries each, in 34 us
+// block of L x N pieces.  Bound: HBM; 8192 x 4096 bfloat16, two entries each, in 35 us
 // (201 MB, part of them in cache).
 template <class T, int L, int N>
 __global__ __launch_bounds__(kMoveThreads) void k_rows_out(const T* __restrict__ x, int64_t stride,
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(kMoveThreads) void k_rows_in_backward(
 
 // y[r] = the sum over its entries, in their order, of w[r, j] result[slot[r,
 // j]] (w null: 1), in float32; entries without an expert are left out.  Bound: HBM;
-// 2^20 x 83 float32, one entry each, in 155 us (4.5 TB/s), 8192 x 4096 bfloat16, two, in
+// 2^20 x 83 float32, one entry each, in 154 us (4.5 TB/s), 8192 x 4096 bfloat16, two, in
 // 46.
 template <class T, int L, int N>
 __global__ __launch_bounds__(kMoveThreads) void k_rows_in(const T* __restrict__ results, int64_t stride,
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(kMoveThreads) void k_rows_in(const T* __restrict__ 
 // each and few values: out[p] = w[r] x[r] for the row r = source[p] (w null: 1; zeros
 // without an expert) and dw[r] = results[p] . x[r] (dw null: not wanted).  What is
 // written lies in order and leaves in whole runs: 2^20 x 83 float32 out 175 us row by
-// row, 165 so.
+// row, 167 so; combine's gradients 249.
 template <class T, int L, int N>
 __global__ __launch_bounds__(kMoveThreads) void k_places_out(const T* __restrict__ x, int64_t stride,
                                                              const T* __restrict__ results,

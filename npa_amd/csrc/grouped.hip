@@ -29,9 +29,8 @@ constexpr int kPieces = std::is_same_v<T, float> ? 3 : 1;
 __host__ __device__ __forceinline__ constexpr int64_t whole8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // Rows laid out for the kernels that load whole 16-byte pieces (HBM: 8192 x 2048
-// float32 in 29 us, 4.0 TB/s): out (rows x ld, ld
-// a multiple of 8, zeros past cols) as they are, or as three planes of bfloat16
-// pieces.
+// float32 in 28 us, 6.0 TB/s, part of them in cache): out (rows x ld, ld a multiple
+// of 8, zeros past cols) as they are, or as three planes of bfloat16 pieces.
 constexpr int kLayThreads = 256;
 template <class T>
 __global__ __launch_bounds__(kLayThreads) void k_lay_out(const T* __restrict__ x, int64_t stride,
@@ -217,9 +216,9 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_rows(const T* __restric
 // from memory to LDS.  A slice's sums go to `slices` (null: no tile is cut) as
 // they stand in registers.
 // Bound: the matrix cores and what stands between two steps (one barrier, then the
-// operands' first reads): 16384 rows of 8 experts, 2048 -> 4096 bfloat16 in 404 us
-// (0.68 PFLOP/s, its fastest run 326; the library's one product of that size without experts 242), 41% of
-// the cycles matrix-busy; 8192 rows of 4, 1024 -> 2048 float32 in 249 us (138
+// operands' first reads): 16384 rows of 8 experts, 2048 -> 4096 bfloat16 in 339 us
+// (0.81 PFLOP/s; the library's one product of that size without experts 242), 41% of
+// the cycles matrix-busy; 8192 rows of 4, 1024 -> 2048 float32 in 227 us (152
 // TFLOP/s, the library's float32 135), 46%.  Reading the operands of the next 16 of
 // the sum under the products of these changed nothing.
 template <class T, bool BACK, int BM, int BN, int WM, int WN>
@@ -585,7 +584,7 @@ __global__ __launch_bounds__(kGroupThreads) void k_group_weight_grad(const T* __
 // The same for 16-bit rows in whole 16-byte pieces, or float32 rows laid out in
 // bfloat16 pieces, straight from memory to LDS; db from products with ones.
 // Bound: as k_group_rows_fast; 16384 rows of 8 experts, 2048 and 4096 wide, bfloat16
-// in 356 us (0.77 PFLOP/s), 8192 rows of 4, 1024 and 2048, float32 in 293.
+// in 308 us (0.89 PFLOP/s), 8192 rows of 4, 1024 and 2048, float32 in 262.
 template <class T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void k_group_weight_grad_fast(
     const Piece16<T>* __restrict__ dy, int64_t dys, int64_t dyp, const Piece16<T>* __restrict__ x, int64_t xs, int64_t xp,

@@ -111,8 +111,8 @@ struct RowSums {
 // L lanes a row, which they hold in N pieces of 16 bytes each: the row is read
 // once, the next one under this one's sums.  A lane keeps its columns' weights over
 // all of its rows.
-// Bound: HBM: 2^20 x 83 float32 in 156 us (4.5 TB/s; 182 with a row's pieces stored as
-// they are), 8191 x 4097 bfloat16, at odd places, in 38 (3.6 TB/s), one row of 4096 in 3.
+// Bound: HBM: 2^20 x 83 float32 in 161 us (4.3 TB/s; 20 us more with a row's pieces stored
+// as they are), 8191 x 4097 bfloat16, at odd places, in 32 (4.2 TB/s), one row of 4096 in 3.
 template <class T, int L, int N, int TH>
 __global__ __launch_bounds__(TH) void k_norm_forward(const T* __restrict__ x, int64_t stride,
                                                      const void* __restrict__ w, const void* __restrict__ b,
@@ -239,9 +239,9 @@ __global__ __launch_bounds__(kLongThreads) void k_norm_forward_long(const T* __r
 // As the forward, with dy beside x; a lane sums its columns of dw and db over
 // its rows, the workgroup's rows meet in LDS and leave as one row of `part`
 // (2 x cols: dw, then db), in a fixed order.
-// Bound: HBM for short rows (2^20 x 83 float32 in 244 us, 4.3 TB/s), vector work and
+// Bound: HBM for short rows (2^20 x 83 float32 in 248 us, 4.2 TB/s), vector work and
 // the sums' latency for long ones, whose registers leave room for two waves a SIMD
-// (8191 x 4097 bfloat16 in 72 us, 2.8 TB/s).
+// (8191 x 4097 bfloat16 in 66 us, 3.1 TB/s).
 template <class T, int L, int N, int TH>
 __global__ __launch_bounds__(TH, N * Piece<T>::V <= 12 ? 4 : 2) void k_norm_backward(const T* __restrict__ x, int64_t stride,
                                                       const T* __restrict__ dy, int64_t dy_stride,

@@ -316,7 +316,9 @@ def mlp(x, w1, b1, w2, b2, offsets):
     """``linear(relu(linear(x, w1, b1, offsets)), w2, b2, offsets)``.  float32 rows
     of 4 to 168 values with 128 hidden units and 4 to 64 outputs, the shapes of an
     automaton's update rule, take one kernel each way, which keeps the hidden
-    values in registers.  Elsewhere the ReLU is in the first layer's kernel and its
+    values in registers; the weights' gradients compute them again, and where one
+    lies within rounding of 0 they may take the ReLU's other side than y and x's
+    gradient.  Elsewhere the ReLU is in the first layer's kernel and its
     mask in the second one's input gradient, and the hidden values, and their
     gradient, are kept in x's type.  float32 as in ``linear``."""
     slots, experts, cols = _check_sorted(x, offsets)
